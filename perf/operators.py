@@ -301,7 +301,7 @@ def _encode_m(m):
     b = m.view(-1, BLOCK)
     top = b.abs().amax(1, keepdim=True)
     c = torch.sqrt(b.abs() * _factor(top, 16129.0)).round().clamp(max=127.0)
-    scale = torch.where(top >= 2.0 ** -100, top / 16129.0, 0.0)
+    scale = torch.where(top >= 2.0 ** -100, top * (1 / 16129), 0.0)
     return torch.where(b < 0, -c, c).to(torch.int8).view(-1), scale.view(-1)
 
 
@@ -315,7 +315,7 @@ def _encode_v(v):
     top = b.amax(1, keepdim=True)
     c = torch.sqrt(b * _factor(top, 65025.0)).round().clamp(max=255.0)
     c = torch.where((b > 0) & (top >= 2.0 ** -100), c.clamp(min=1.0), c)
-    scale = torch.where(top >= 2.0 ** -100, top / 65025.0, 0.0)
+    scale = torch.where(top >= 2.0 ** -100, top * (1 / 65025), 0.0)
     return c.to(torch.uint8).view(-1), scale.view(-1)
 
 
