@@ -232,7 +232,9 @@ def _run_own(s):
         opt.step(s["grads"])
         m, v = opt.state_values()
         return dict(params=s["params"], m=m, v=v)
-    return encoder.fp8_linear(s["x"], encoder.Fp8Blocks(s["codes"], s["scales"], s["K"]), s["bias"])
+    # results of 16 bits take the 8-bit matrix instruction's sums, float32 ones float32 sums
+    return encoder.fp8_linear(s["x"], encoder.Fp8Blocks(s["codes"], s["scales"], s["K"]), s["bias"],
+                              fast_accum=s["x"].dtype != torch.float32)
 
 
 def _run_plain(s):
@@ -294,7 +296,7 @@ def _adamw_plain(s):
 
 def _factor(top, levels):
     """What maps a block's largest value to `levels`; 0 for a block without one."""
-    return torch.where(top >= 2.0 ** -100, levels / top, 0.0)
+    return torch.where(top >= 2.0 ** -100, top.reciprocal() * levels, 0.0)
 
 
 def _encode_m(m):
