@@ -279,6 +279,93 @@ int trident_host_alloc_mapped(size_t bytes, void** host_ptr);
 int trident_host_free(void* host_ptr);
 int trident_host_device_pointer(void* host_ptr, void** device_ptr);
 
+/* -----------------------------------------------------------------------------------------------
+ * The encoder: the operators that make and train the vectors an index holds.  No counterpart in the
+ * reference (its vectors come from data sets).  Matrices are row-major with a row pitch in elements;
+ * any element address will do unless said otherwise.  Sums and statistics are float32, results are
+ * rounded once.  Asynchronous on `stream`; nothing is allocated.  The results of a call do not depend
+ * on the order in which its workgroups run (no float atomics).
+ */
+enum TridentDtype { TRIDENT_F32 = 0, TRIDENT_F16 = 1, TRIDENT_BF16 = 2 };
+
+/* out[t, :] = scale * weight[ids[t], :] for n tokens.  ids: int32, or int64 where ids64 is not 0.  A
+ * negative id is an empty slot: a row of zeros.  An id >= V gives a row of NaN. */
+int trident_embedding(const void* weight, int32_t dtype, int64_t V, int64_t D, int64_t ld_weight, const void* ids,
+                      int32_t ids64, int64_t n, double scale, void* out, int64_t ld_out, void* stream);
+
+/* out[v, :] = scale * sum of grad[t, :] over the tokens with ids[t] == v, in token order; all V rows
+ * are written.  Ids outside [0, V) and padding_idx (-1: none) add nothing. */
+size_t trident_embedding_grad_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, const void* ids, int32_t ids64,
+                           int64_t n, int64_t V, int64_t D, double scale, int64_t padding_idx, void* out,
+                           int64_t ld_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* y = (x - mean) * rstd * weight + bias over rows of D.  weight / bias: [D] of the rows' type or
+ * float32, or NULL (ones / zeros).  mean, rstd: [rows] for the backward pass, or both NULL. */
+int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, int64_t ld_x, const void* weight,
+                       const void* bias, int32_t weight_dtype, double eps, void* y, int64_t ld_y, float* mean,
+                       float* rstd, void* stream);
+
+/* The backward pass: dx [rows, D], dweight and dbias [D] of weight_dtype (either may be NULL). */
+size_t trident_layer_norm_grad_workspace_bytes(int64_t rows, int64_t D);
+int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype, int64_t rows,
+                            int64_t D, const void* weight, int32_t weight_dtype, const float* mean, const float* rstd,
+                            void* dx, int64_t ld_dx, void* dweight, void* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* One AdamW step over `count` tensors (contiguous), updated in place with their states.  The states of
+ * all tensors lie in one flat buffer per moment; a tensor's begin at state_offset, a multiple of 256
+ * elements, and the rest of its last block of 256 is its own.  bits 32: m, v float32.  bits 8: m int8,
+ * v uint8 codes and m_scale, v_scale [len / 256] float32, with m = c |c| m_scale and
+ * v = (c^2 v_scale)^2.  step: the step being taken, from 1.  Gradients are multiplied by grad_scale. */
+typedef struct TridentAdamTensor {
+    void* param;
+    const void* grad;
+    int64_t numel;
+    int64_t state_offset;
+    int32_t dtype;       /* of param */
+    int32_t grad_dtype;
+} TridentAdamTensor;
+
+typedef struct TridentAdamState {
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t len;         /* elements, a multiple of 256 */
+    int32_t bits;        /* 32 or 8 */
+} TridentAdamState;
+
+typedef struct TridentAdamParams {
+    double lr, beta1, beta2, eps, weight_decay, grad_scale;
+    int64_t step;
+} TridentAdamParams;
+
+int trident_adamw(const TridentAdamTensor* tensors, int32_t count, const TridentAdamState* state,
+                  const TridentAdamParams* params, void* stream);
+
+/* The float32 values [len] that 8-bit states stand for. */
+int trident_adamw_state_values(const TridentAdamState* state, float* m, float* v, void* stream);
+
+/* 8-bit floating point (e4m3) with a scale 2^(e - 127) for each row and 128 columns.  Codes:
+ * [rows, 128 ceil(K / 128)], 16-byte aligned, zeros past K.  Scales e: [rows, 4 ceil(K / 512)] bytes,
+ * 127 past the last block.  A value that is not finite becomes NaN and leaves its block's scale alone. */
+int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x, uint8_t* codes,
+                         uint8_t* scales, void* stream);
+
+/* out [M, N] = A B^T + bias; bias [N] of out's type or float32, or NULL.  Sums are float32; with
+ * fast_accum they come from the 8-bit matrix instruction, twice as fast, which keeps 13 bits below the
+ * largest of each 8 products (the sums are then off by up to about 5e-5 of their size). */
+int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
+                       const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
+                       int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream);
+
+/* The same with A quantised in the call from x [M, K]; out has x's type. */
+size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t K);
+int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* w_codes,
+                       const uint8_t* w_scales, int64_t N, const void* bias, int32_t bias_dtype, void* out,
+                       int64_t ld_out, int32_t fast_accum, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* trident_last_error(void);
 int trident_abi_version(void);
 

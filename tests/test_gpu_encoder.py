@@ -1,0 +1,763 @@
+"""The encoder's operators against float64 implementations of their formulas.
+
+Tolerances are bounds, derived here from the arithmetic: u = 2^-24 is a float32 operation's rounding,
+``U[dtype]`` a result's, and a sum of n float32 terms is off by at most n u times the sum of their
+magnitudes, in whatever order.
+"""
+import math
+
+import pytest
+import torch
+
+from trident_amd import _lib, encoder
+
+pytestmark = pytest.mark.gpu
+
+F64 = torch.float64
+u = 2.0 ** -24
+U = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+TINY = {torch.float32: 2.0 ** -149, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -133}
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def gen(seed):
+    return torch.Generator(device="cuda:0").manual_seed(seed)
+
+
+def randn(g, *shape, dtype=torch.float32):
+    return torch.randn(shape, generator=g, device="cuda:0").to(dtype)
+
+
+def within(got, ref, bound, what=""):
+    """|got - ref| <= bound; where ref rounds to an infinity of got's type, that infinity."""
+    past = ref.to(got.dtype).isinf() & ref.isfinite()
+    off = torch.where(past & (got.to(F64) == ref.to(got.dtype).to(F64)), 0.0, (got.to(F64) - ref).abs())
+    bad = ~(off <= bound)
+    assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} values past their bound, worst by "
+                           f"{float((off / bound.clamp(min=1e-300))[bad].max()):.3g}x")
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding
+
+
+def token_ids(g, n, V, wide=True):
+    """Frequencies falling as one over the rank, a few empty slots."""
+    r = torch.rand(n, generator=g, device="cuda:0", dtype=F64)
+    ids = (torch.exp(r * math.log(V + 1)).long() - 1).clamp(0, V - 1)
+    ids[torch.rand(n, generator=g, device="cuda:0") < 0.1] = -1
+    return ids if wide else ids.int()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,D,n,wide", [(1, 1, 1, True), (5, 3, 7, False), (100, 7, 64, True), (1000, 8, 1, True),
+                                        (777, 33, 129, False), (300, 100, 1000, True), (2000, 960, 513, False),
+                                        (50, 2049, 300, True)])
+def test_embedding(dev, dtype, V, D, n, wide):
+    g = gen(V + D)
+    w, ids = randn(g, V, D, dtype=dtype), token_ids(g, n, V, wide)
+    y = encoder.embedding(ids, w, scale=math.sqrt(D))
+    ref = torch.where((ids >= 0)[:, None], w.to(F64)[ids.long().clamp(min=0)] * math.sqrt(D), 0.0)
+    assert y.dtype == dtype and y.shape == (n, D)
+    within(y, ref, (U[dtype] + 3 * u) * ref.abs() + TINY[dtype])
+
+
+def test_embedding_slots_outside_the_table(dev):
+    g = gen(1)
+    w = randn(g, 10, 24)
+    ids = torch.tensor([[3, -1, 10], [2 ** 40, -(2 ** 40), 9]], device=dev)
+    y = encoder.embedding(ids, w)
+    assert y.shape == (2, 3, 24)
+    assert torch.equal(y[0, 0], w[3]) and torch.equal(y[1, 2], w[9])
+    assert (y[0, 1] == 0).all() and (y[1, 1] == 0).all()
+    assert y[0, 2].isnan().all() and y[1, 0].isnan().all()
+    grad = torch.ones_like(y)
+    out = encoder.embedding_grad(grad, ids, 10)
+    assert out[3].eq(1).all() and out[9].eq(1).all() and out.sum() == 48
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_strided_table_and_unaligned_rows(dev, dtype):
+    g = gen(2)
+    big = randn(g, 40, 77, dtype=dtype)
+    ids = token_ids(g, 50, 40).reshape(5, 10).t()  # not contiguous
+    for w in (big[:, 1:38], big[::2, 3:40], big.t()[:40].contiguous().t()):
+        y = encoder.embedding(ids.clamp(max=w.shape[0] - 1), w)
+        ref = torch.where((ids >= 0)[..., None], w[ids.clamp(min=0, max=w.shape[0] - 1)], 0.0)
+        assert torch.equal(y, ref)
+
+
+def grad_ref(grad, ids, V, scale, skip=None):
+    """(sum, sum of magnitudes, number) of each row's tokens in float64."""
+    D = grad.shape[-1]
+    ids, g = ids.reshape(-1).long(), grad.reshape(-1, D).to(F64)
+    live = (ids >= 0) & (ids < V)
+    if skip is not None:
+        live &= ids != skip
+    ids, g = ids[live], g[live]
+    zero = torch.zeros((V, D), dtype=F64, device=grad.device)
+    count = torch.bincount(ids, minlength=V).to(F64)[:, None]
+    return zero.index_add(0, ids, g) * scale, zero.index_add(0, ids, g.abs()) * abs(scale), count
+
+
+def check_embedding_grad(grad, ids, V, scale=1.0, skip=None, out=None):
+    got = encoder.embedding_grad(grad, ids, V, scale=scale, padding_idx=skip, out=out)
+    ref, mag, count = grad_ref(grad, ids, V, scale, skip)
+    within(got, ref, U[grad.dtype] * ref.abs() + (count + 4) * u * mag + TINY[grad.dtype])
+    assert (got[count[:, 0] == 0] == 0).all()
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V,D,n", [(1, 1, 1), (1, 8, 1000), (3, 5, 64), (3, 9, 65), (700, 100, 1), (257, 33, 3000),
+                                   (1000, 128, 5000), (60, 960, 2000), (131, 2049, 700), (9, 4100, 200)])
+def test_embedding_grad(dev, dtype, V, D, n):
+    g = gen(V + n)
+    check_embedding_grad(randn(g, n, D, dtype=dtype), token_ids(g, n, V, wide=n % 2 == 0), V, scale=0.37)
+
+
+@pytest.mark.parametrize("counts", [[64, 65], [63, 1, 64, 128, 129], [0, 200, 0, 64, 0, 1000, 0], [4096], [1] * 130,
+                                    [65] * 9, [20, 300, 20]])
+def test_embedding_grad_long_rows(dev, counts):
+    """Rows at and around the length from which a row is summed in parts, in shuffled token order."""
+    g = gen(len(counts))
+    ids = torch.repeat_interleave(torch.arange(len(counts), device=dev), torch.tensor(counts, device=dev))
+    ids = ids[torch.randperm(ids.numel(), generator=g, device=dev)]
+    for D in (3, 72, 600):
+        check_embedding_grad(randn(g, ids.numel(), D), ids, len(counts))
+
+
+def test_embedding_grad_without_tokens(dev):
+    out = encoder.embedding_grad(torch.empty((0, 20), device=dev), torch.empty(0, dtype=torch.int64, device=dev), 300)
+    assert out.shape == (300, 20) and (out == 0).all()
+    ids = torch.full((500,), -1, device=dev)
+    assert (encoder.embedding_grad(torch.ones((500, 20), device=dev), ids, 300) == 0).all()
+
+
+def test_embedding_grad_padding_strides_and_out(dev):
+    g = gen(5)
+    ids = token_ids(g, 900, 50)
+    wide = randn(g, 900, 131, dtype=torch.bfloat16)
+    buf = torch.full((50, 140), 7.0, dtype=torch.bfloat16, device=dev)
+    out = check_embedding_grad(wide[:, 5:105], ids, 50, skip=0, out=buf[:, 9:109])
+    assert out.data_ptr() == buf[:, 9:109].data_ptr()
+    assert (buf[:, :9] == 7).all() and (buf[:, 109:] == 7).all() and (out[0] == 0).all()
+    # an expanded gradient (a broadcast input's) and a transposed one
+    check_embedding_grad(randn(g, 1, 40).expand(900, 40), ids, 50)
+    check_embedding_grad(randn(g, 40, 900).t(), ids, 50)
+
+
+def test_embedding_grad_is_the_same_every_time(dev):
+    g = gen(6)
+    ids, grad = token_ids(g, 30_000, 5000), randn(g, 30_000, 96)
+    a = encoder.embedding_grad(grad, ids, 5000)
+    for _ in range(3):
+        assert torch.equal(encoder.embedding_grad(grad, ids, 5000), a)
+
+
+def test_embedding_grad_keeps_nan_to_its_row(dev):
+    g = gen(7)
+    ids, grad = token_ids(g, 4000, 100), randn(g, 4000, 33)
+    ids[17] = 42
+    grad[17, 5] = float("nan")
+    out = encoder.embedding_grad(grad, ids, 100)
+    bad = out.isnan()
+    assert bad[42, 5] and int(bad.sum()) == 1
+
+
+def test_embedding_autograd_against_differences(dev):
+    """The loss is a quadratic, so its central difference has no error but rounding."""
+    g = gen(8)
+    w = randn(g, 30, 12).requires_grad_()
+    ids, t = token_ids(g, 60, 30), randn(g, 60, 12)
+    loss = lambda table: ((encoder.embedding(ids, table, scale=1.5).double() - t.double()) ** 2).sum()  # noqa: E731
+    loss(w).backward()
+    for _ in range(8):
+        d = randn(g, 30, 12)
+        h = 2.0 ** -4
+        with torch.no_grad():
+            diff = (loss(w + h * d) - loss(w - h * d)) / (2 * h)
+        want = (w.grad.double() * d.double()).sum()
+        # each y is off by a few u of its size, the loss by 2 |y - t| of that
+        assert abs(diff - want) <= 1e-4 * max(1.0, float(w.grad.double().norm() * d.double().norm()))
+
+
+def test_embedding_offsets_past_32_bits(dev):
+    """A table and a batch of more than 2^31 elements each."""
+    g = gen(9)
+    V, D = 2_200_000, 1000
+    w = torch.empty((V, D), dtype=torch.bfloat16, device=dev)
+    w[-5000:] = randn(g, 5000, D, dtype=torch.bfloat16)
+    ids = torch.randint(V - 5000, V, (2_200_000,), generator=g, device=dev)
+    y = encoder.embedding(ids, w)
+    for s in (0, 1_000_000, 2_199_000):
+        assert torch.equal(y[s:s + 1000], w[ids[s:s + 1000]])
+    del w
+    ids = ids - (V - 5000)
+    ids[:2_190_000] = -1
+    got = encoder.embedding_grad(y, ids, 5000)
+    ref, mag, count = grad_ref(y[2_190_000:], ids[2_190_000:], 5000, 1.0)
+    within(got, ref, U[torch.bfloat16] * ref.abs() + (count + 4) * u * mag)
+
+
+# ---------------------------------------------------------------------------------------------
+# layer norm
+
+
+def norm_ref(x, w, b, eps):
+    """y, dh (the bound on the normalised value's error), and what the backward pass needs, in float64."""
+    x = x.to(F64)
+    D = x.shape[-1]
+    mean = x.mean(-1, keepdim=True)
+    c = x - mean
+    r = 1 / torch.sqrt((c * c).mean(-1, keepdim=True) + eps)
+    h = c * r
+    e = (D + 2) * u * x.abs().mean(-1, keepdim=True) * r  # the mean's error, in units of the deviation
+    rel = (D + 8) * u + e * e                              # the deviation's relative error
+    dh = e + 2 * u * h.abs() + h.abs() * rel
+    y = h * (1 if w is None else w.to(F64)) + (0 if b is None else b.to(F64))
+    return y, h, r, dh, rel
+
+
+SHAPES = [(1, 1), (3, 2), (5, 7), (1, 8), (4, 33), (9, 64), (2, 100), (37, 128), (130, 960), (6, 1000), (3, 1537),
+          (2, 2048), (3, 2049), (2, 4099), (2, 8192), (1, 8200), (2, 20001)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D", SHAPES)
+def test_layer_norm(dev, dtype, rows, D):
+    g = gen(rows + D)
+    x = (2.0 * randn(g, rows, D) + 3.0).to(dtype)
+    w, b = randn(g, D, dtype=dtype), randn(g, D, dtype=dtype)
+    w32 = randn(g, D)
+    eps = 1e-3  # one element: the deviation is zero
+    for wt, bs in ((w, b), (None, None), (w, None), (None, b), (w32, None)):
+        y = encoder.layer_norm(x, wt, bs, eps=eps)
+        ref, h, _, dh, _ = norm_ref(x, wt, bs, eps)
+        size = (1.0 if wt is None else wt.to(F64).abs()) * dh + 4 * u * (ref.abs() + (0 if bs is None else bs.to(F64).abs()))
+        within(y, ref, U[dtype] * ref.abs() + size + TINY[dtype], f"weight {wt is not None} bias {bs is not None}")
+        assert y.dtype == dtype
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D", SHAPES + [(700, 96), (3000, 24)])
+def test_layer_norm_grad(dev, dtype, rows, D):
+    g = gen(rows * 3 + D)
+    x = (2.0 * randn(g, rows, D) + 1.0).to(dtype)
+    dy, w = randn(g, rows, D, dtype=dtype), randn(g, D, dtype=dtype)
+    eps = 1e-3
+    _, mean, rstd = encoder.layer_norm_forward(x, w, None, eps=eps)
+    for wt in (w, None):
+        dx, dw, db = encoder.layer_norm_grad(dy, x, wt, mean, rstd)
+        _, h, r, dh, rel = norm_ref(x, wt, None, eps)
+        d = dy.to(F64)
+        a = d * (1 if wt is None else wt.to(F64))
+        avg = lambda t: t.mean(-1, keepdim=True)  # noqa: E731
+        ma, mh = avg(a), avg(a * h)
+        ref = r * (a - ma - h * mh)
+        bound = r * (2 * u * a.abs() + (D + 2) * u * avg(a.abs()) + dh * mh.abs() +
+                     h.abs() * (avg(a.abs() * dh) + (D + 4) * u * avg((a * h).abs())))
+        bound = bound + (rel + 8 * u) * r * (a.abs() + ma.abs() + (h * mh).abs())
+        within(dx, ref, bound + U[dtype] * ref.abs() + TINY[dtype], "dx")
+        ref = (d * h).sum(0)
+        if wt is None:
+            assert dw is None
+        else:
+            within(dw, ref, (d.abs() * dh).sum(0) + (rows + 4) * u * (d * h).abs().sum(0) + U[dtype] * ref.abs() +
+                   TINY[dtype], "dw")
+        within(db, d.sum(0), (rows + 4) * u * d.abs().sum(0) + U[dtype] * d.sum(0).abs() + TINY[dtype], "db")
+
+
+def test_layer_norm_strides_and_shapes(dev):
+    g = gen(3)
+    big = randn(g, 12, 150, dtype=torch.float16)
+    w, b = randn(g, 100, dtype=torch.float16), randn(g, 100, dtype=torch.float16)
+    for x in (big[:, 3:103], big[::3, 50:150], randn(g, 100, 12, dtype=torch.float16).t(),
+              randn(g, 1, 100, dtype=torch.float16).expand(12, 100), randn(g, 2, 3, 100, dtype=torch.float16),
+              randn(g, 3, 2, 100, dtype=torch.float16).transpose(0, 1), randn(g, 100, dtype=torch.float16)):
+        flat = x.contiguous()
+        assert torch.equal(encoder.layer_norm(x, w, b), encoder.layer_norm(flat, w, b))
+        _, mean, rstd = encoder.layer_norm_forward(x, w, b)
+        dy = randn(g, *x.shape, dtype=torch.float16)
+        for got, want in zip(encoder.layer_norm_grad(dy, x, w, mean, rstd),
+                             encoder.layer_norm_grad(dy, flat, w, mean, rstd)):
+            assert torch.equal(got, want)
+    empty = torch.empty((0, 100), device=dev)
+    y, mean, rstd = encoder.layer_norm_forward(empty, None, None)
+    dx, dw, db = encoder.layer_norm_grad(y, empty, torch.ones(100, device=dev), mean, rstd)
+    assert dx.shape == (0, 100) and (dw == 0).all() and (db == 0).all()
+    empty = torch.empty((0, 9000), device=dev)
+    y, mean, rstd = encoder.layer_norm_forward(empty, None, None)
+    assert (encoder.layer_norm_grad(y, empty, None, mean, rstd)[2] == 0).all()
+
+
+def test_layer_norm_far_from_zero(dev):
+    """A mean a thousand times the deviation: the variance is that of the centred values."""
+    g = gen(4)
+    x = randn(g, 50, 512) + 1000.0
+    ref, _, _, dh, _ = norm_ref(x, None, None, 1e-5)
+    within(encoder.layer_norm(x), ref, dh + 8 * u * ref.abs())
+
+
+def test_layer_norm_keeps_nan_to_its_row(dev):
+    g = gen(5)
+    x = randn(g, 9, 200)
+    x[3, 7], x[5, 1] = float("nan"), float("inf")
+    y = encoder.layer_norm(x)
+    assert y[3].isnan().all() and y[5].isnan().all()
+    assert y[[0, 1, 2, 4, 6, 7, 8]].isfinite().all()
+
+
+def test_layer_norm_autograd(dev):
+    """Through autograd the same bits as the passes; and against central differences of a smooth loss,
+    whose error is of the third order in the step."""
+    g = gen(6)
+    x, w, b = (randn(g, *s).requires_grad_() for s in ((7, 30), (30,), (30,)))
+    t = randn(g, 7, 30)
+    encoder.layer_norm(x, w, b).backward(t)
+    _, mean, rstd = encoder.layer_norm_forward(x.detach(), w.detach(), b.detach())
+    for got, want in zip((x.grad, w.grad, b.grad), encoder.layer_norm_grad(t, x.detach(), w.detach(), mean, rstd)):
+        assert torch.equal(got, want)
+    loss = lambda *p: (encoder.layer_norm(*p).double() * t.double()).sum()  # noqa: E731
+    h = 2.0 ** -6
+    for i, p in enumerate((x, w, b)):
+        for _ in range(4):
+            d = randn(g, *p.shape)
+            at = lambda s: loss(*[(q + s * d).detach() if j == i else q.detach()  # noqa: E731, B023
+                                  for j, q in enumerate((x, w, b))])
+            diff = float((at(h) - at(-h)) / (2 * h))
+            want = float((p.grad.double() * d.double()).sum())
+            # the third derivative along d is a few |d|^3 |t|; float32 results are off by u |t| / h
+            assert abs(diff - want) <= 20 * h * h * float(t.norm()) * max(1.0, float(d.norm()) / 3), (i, diff, want)
+
+
+def test_layer_norm_bias_only_autograd(dev):
+    g = gen(7)
+    x, b = randn(g, 5, 40), randn(g, 40).requires_grad_()
+    encoder.layer_norm(x, None, b).sum().backward()
+    assert torch.equal(b.grad, torch.full((40,), 5.0, device=dev))
+
+
+# ---------------------------------------------------------------------------------------------
+# AdamW
+
+SIZES = [1, 255, 256, 257, 4096, 4097, 3, 10_001]
+
+
+def adam_case(seed, dtype, gdtype, sizes=SIZES, unaligned=True):
+    g = gen(seed)
+    params = [randn(g, n + 1, dtype=dtype)[1:] if unaligned else randn(g, n, dtype=dtype) for n in sizes]
+    grads = [randn(g, n + 3, dtype=gdtype)[3:] * (10.0 ** -(i % 4)) for i, n in enumerate(sizes)]
+    return g, params, grads
+
+
+def adam_steps(opt, p, g, m, v, t):
+    """One step in float64 from the state (p, m, v) of one tensor."""
+    b1, b2 = opt.betas
+    g = g.to(F64)
+    m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+    move = opt.lr / (1 - b1 ** t) * m / (torch.sqrt(v) / math.sqrt(1 - b2 ** t) + opt.eps)
+    return p.to(F64) * (1 - opt.lr * opt.weight_decay) - move, m, v, move
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("gdtype", TYPES)
+def test_adamw_32(dev, dtype, gdtype):
+    g, params, grads = adam_case(1, dtype, gdtype)
+    opt = encoder.AdamW(params, lr=1e-2, weight_decay=0.1)
+    for t in range(1, 4):
+        old = [p.clone() for p in params]
+        om, ov = opt.exp_avg.clone(), opt.exp_avg_sq.clone()
+        grads = [(x * 0.5).contiguous() if t == 2 else x for x in grads]
+        opt.step(grads)
+        assert opt.step_count == t
+        for i, (p, q, x) in enumerate(zip(params, old, grads)):
+            s = slice(opt.offsets[i], opt.offsets[i] + p.numel())
+            ref, m, v, move = adam_steps(opt, q, x, om[s].to(F64), ov[s].to(F64), t)
+            mag = 0.9 * om[s].to(F64).abs() + 0.1 * x.to(F64).abs()
+            within(opt.exp_avg[s], m, 4 * u * mag + 1e-44, "m")
+            within(opt.exp_avg_sq[s], v, 6 * u * v + 1e-44, "v")
+            # the move: m off by 4 u of its terms, the root by 4 u, eight more operations
+            near = 12 * u * move.abs() + 4 * u * opt.lr * 10 * mag / (v.sqrt() + opt.eps)
+            within(p, ref, (U[dtype] + 4 * u) * ref.abs() + 4 * u * q.to(F64).abs() + near + TINY[dtype], "p")
+    gaps = torch.ones_like(opt.exp_avg, dtype=torch.bool)
+    for o, p in zip(opt.offsets, params):
+        gaps[o:o + p.numel()] = False
+    assert (opt.exp_avg[gaps] == 0).all() and (opt.exp_avg_sq[gaps] == 0).all()
+
+
+def codes32(m, v):
+    """The 8-bit codes and scales of float32 moments [blocks, 256], one float32 operation at a time (CPU)."""
+    m, v = m.cpu(), v.cpu()
+    tiny = 2.0 ** -100
+    root32 = lambda x: torch.sqrt(x.double()).float()  # noqa: E731  (the CPU's float32 root is an ulp off)
+
+    def encode(x, levels, most):
+        top = x.amax(1, keepdim=True)
+        factor = torch.where(top >= tiny, levels / top, torch.zeros(()))
+        c = root32(x * factor).round().clamp(max=most)
+        return c, torch.where(top >= tiny, top * (1 / levels), torch.zeros(()))
+
+    cm, sm = encode(m.abs(), 16129.0, 127.0)
+    root = root32(v)
+    cv, sv = encode(root, 65025.0, 255.0)
+    cv = torch.where((root > 0) & (sv > 0), cv.clamp(min=1.0), cv)
+    return torch.where(m < 0, -cm, cm).to(torch.int8), cv.to(torch.uint8), sm[:, 0], sv[:, 0]
+
+
+@pytest.mark.parametrize("gdtype", TYPES)
+def test_adamw_8_codes_are_those_of_the_formula(dev, gdtype):
+    """Codes and scales equal the formula's bit for bit; each code is the nearest; the parameters move as
+    with the moments before they are stored."""
+    g, params, grads = adam_case(2, torch.float32, gdtype)
+    grads[4][100:200] = 0
+    opt = encoder.AdamW(params, lr=1e-2, weight_decay=0.1, state_bits=8)
+    for t in range(1, 4):
+        om, ov = opt.state_values()
+        old = [p.clone() for p in params]
+        opt.step(grads)
+        b1, b2 = torch.tensor(0.9), torch.tensor(0.999)
+        for i, (p, q, x) in enumerate(zip(params, old, grads)):
+            n = p.numel()
+            blocks = -(-n // 256)
+            s = slice(opt.offsets[i], opt.offsets[i] + blocks * 256)
+            gf = torch.zeros(blocks * 256)
+            gf[:n] = x.float().cpu()
+            m = om[s].cpu() * b1 + gf * torch.tensor(1 - 0.9)
+            v = ov[s].cpu() * b2 + (gf * gf) * torch.tensor(1 - 0.999)
+            cm, cv, sm, sv = codes32(m.view(-1, 256), v.view(-1, 256))
+            k = slice(opt.offsets[i] // 256, opt.offsets[i] // 256 + blocks)
+            assert torch.equal(opt.exp_avg[s].cpu(), cm.view(-1)), (t, i)
+            assert torch.equal(opt.exp_avg_sq[s].cpu(), cv.view(-1)), (t, i)
+            assert torch.equal(opt.exp_avg_scale[k].cpu(), sm) and torch.equal(opt.exp_avg_sq_scale[k].cpu(), sv)
+            live = sm[:, None].expand(-1, 256) > 0
+            exact = torch.sqrt(m.view(-1, 256).double().abs() / sm.double()[:, None])
+            assert ((exact - cm.double().abs()).abs()[live] <= 0.5 + 1e-4).all()
+            ref, m64, v64, move = adam_steps(opt, q, x, om[s][:n].to(F64), ov[s][:n].to(F64), t)
+            mag = 0.9 * om[s][:n].to(F64).abs() + 0.1 * x.to(F64).abs()
+            near = 12 * u * move.abs() + 4 * u * opt.lr * 10 * mag / (v64.sqrt() + opt.eps)
+            within(p, ref, 8 * u * (ref.abs() + q.to(F64).abs()) + near, "p")
+        m, v = opt.state_values()
+        sm, sv = opt.exp_avg_scale.repeat_interleave(256), opt.exp_avg_sq_scale.repeat_interleave(256)
+        cm, cv = opt.exp_avg.float(), opt.exp_avg_sq.float()
+        assert torch.equal(m, cm * cm.abs() * sm) and torch.equal(v, (cv * cv * sv) ** 2)
+
+
+def test_adamw_8_follows_32(dev):
+    """Over 50 steps on a quadratic the 8-bit states reach what the 32-bit ones do."""
+    g = gen(3)
+    target = randn(g, 5000)
+    ends = []
+    for bits in (32, 8):
+        p = torch.zeros(5000, device=dev)
+        opt = encoder.AdamW([p], lr=0.05, weight_decay=0.0, state_bits=bits)
+        for _ in range(120):
+            opt.step([p - target])
+        ends.append(float((p - target).norm() / target.norm()))
+    assert ends[0] < 0.05 and ends[1] < 0.06, ends
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_tensors_and_missing_gradients(dev, bits):
+    """More tensors than one launch takes, some without a gradient, one empty: those stay as they are."""
+    g = gen(4)
+    sizes = [(7 * i) % 900 + 1 for i in range(200)]
+    sizes[50] = 0
+    params = [randn(g, n) for n in sizes]
+    grads = [None if i % 7 == 3 else randn(g, n) for i, n in enumerate(sizes)]
+    old = [p.clone() for p in params]
+    opt = encoder.AdamW(params, lr=1e-2, state_bits=bits)
+    opt.step(grads)
+    for i, (p, q, x) in enumerate(zip(params, old, grads)):
+        if x is None:
+            assert torch.equal(p, q), i
+        elif p.numel():
+            ref, _, _, move = adam_steps(opt, q, x, torch.zeros_like(q, dtype=F64), torch.zeros_like(q, dtype=F64), 1)
+            within(p, ref, 32 * u * (q.to(F64).abs() + move.abs()), f"tensor {i}")
+
+
+def test_adamw_grad_attribute_scale_and_strides(dev):
+    g = gen(5)
+    a, b = randn(g, 30, 40).requires_grad_(), randn(g, 30, 40).requires_grad_()
+    with torch.no_grad():
+        b.copy_(a)
+    x = randn(g, 40, 30)
+    a.grad, b.grad = x.t(), x.t().contiguous() * 4.0
+    version = a._version
+    encoder.AdamW([a]).step()
+    encoder.AdamW([b]).step(grad_scale=0.25)
+    assert torch.equal(a, b) and a._version > version
+    opt = encoder.AdamW([a])
+    opt.zero_grad()
+    assert a.grad is None
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_not_finite_and_tiny(dev, bits):
+    p = torch.ones(1000, device=dev)
+    grad = torch.full((1000,), 0.5, device=dev)
+    grad[300], grad[700] = float("nan"), float("inf")
+    opt = encoder.AdamW([p], lr=1e-2, state_bits=bits)
+    opt.step([grad])
+    m, v = opt.state_values()
+    assert p[300].isnan() and m[300].isnan() and v[300].isnan()
+    assert not m[700].isfinite() and not v[700].isfinite()
+    others = torch.ones(1000, dtype=torch.bool, device=dev)
+    others[[300, 700]] = False
+    assert p[others].isfinite().all()
+    if bits == 8:
+        others[256:768] = False  # the two values' blocks
+    assert m[:1000][others].isfinite().all() and v[:1000][others].isfinite().all()
+    p = torch.ones(256, device=dev)
+    opt = encoder.AdamW([p], lr=1e-2, weight_decay=0.0, state_bits=bits)
+    opt.step([torch.full((256,), 1e-38, device=dev)])
+    m, v = opt.state_values()
+    assert p.isfinite().all() and m.isfinite().all() and (v == 0).all() and (m.abs() <= 1e-38).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_state_survives_saving(dev, bits):
+    _, params, grads = adam_case(6, torch.float32, torch.float32, unaligned=False)
+    opt = encoder.AdamW(params, state_bits=bits)
+    opt.step(grads)
+    twin_p = [p.clone() for p in params]
+    twin = encoder.AdamW(twin_p, state_bits=bits)
+    twin.load_state_dict(opt.state_dict())
+    opt.step(grads)
+    twin.step(grads)
+    assert twin.step_count == 2 and all(torch.equal(p, q) for p, q in zip(params, twin_p))
+    assert all(torch.equal(x, y) for x, y in zip(opt.state_values(), twin.state_values()))
+
+
+# ---------------------------------------------------------------------------------------------
+# 8-bit floating point
+
+
+def fp8_ref(x):
+    """(codes' values, scale exponents) of x [rows, K] in float64, blocks padded with zeros."""
+    rows, K = x.shape
+    kb = -(-K // 128)
+    b = torch.zeros((rows, kb * 128), dtype=F64, device=x.device)
+    b[:, :K] = x.to(F64)
+    b = b.view(rows, kb, 128)
+    top = b.abs().amax(2, keepdim=True)
+    e = torch.where(top > 0, torch.ceil(torch.log2(torch.where(top > 0, top, 1.0) / 448)), 0.0).clamp(min=-126)
+    q = b * torch.exp2(-e)
+    step = torch.exp2(torch.floor(torch.log2(q.abs().clamp(min=2.0 ** -6))) - 3)
+    return (torch.round(q / step) * step).view(rows, -1), e[..., 0]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,K", [(1, 1), (3, 7), (2, 127), (5, 128), (4, 129), (33, 333), (7, 960), (1, 4096),
+                                    (100, 513)])
+def test_quantize_fp8(dev, dtype, rows, K):
+    g = gen(rows + K)
+    x = (randn(g, rows, K) * torch.exp(3 * randn(g, rows, 1))).to(dtype)
+    x[0, 0] = 0
+    if K > 8:
+        x[:, 1:4] = torch.tensor([448.0, -449.0, 2.0 ** -9], device=dev).to(dtype)
+    q = encoder.quantize_fp8(x)
+    codes, e = fp8_ref(x)
+    assert torch.equal(q.codes.to(F64), codes)
+    assert torch.equal(q.scales[:, :e.shape[1]].to(F64) - 127, e)
+    assert (q.scales[:, e.shape[1]:] == 127).all()
+    # half a step of the code, which has four significant bits, or of the smallest one
+    bound = 2.0 ** -4 * x.to(F64).abs() + torch.exp2(e - 10).repeat_interleave(128, 1)[:, :K]
+    within((codes * torch.exp2(e).repeat_interleave(128, 1))[:, :K], x.to(F64), bound)
+
+
+def test_quantize_fp8_extremes(dev):
+    x = torch.zeros((6, 256))
+    x[0] = 0.0
+    x[1, :128] = 3.4e38
+    x[2, :128] = 1e-45
+    x[3, 5], x[3, 200] = float("nan"), 1.0
+    x[4, 5], x[4, 6], x[4, 7] = float("inf"), -float("inf"), 2.0
+    x[5, :128] = 1e-37
+    q = encoder.quantize_fp8(x.to(dev))
+    v = q.codes.float().cpu()
+    s = q.scales.cpu().int() - 127
+    assert (v[0] == 0).all() and (s[0] == 0).all()
+    assert torch.allclose(v[1, :128].double() * 2.0 ** int(s[1, 0]), torch.full((128,), 3.4e38).double(), rtol=0.07)
+    assert (v[2] == 0).all() and int(s[2, 0]) == -126
+    assert v[3, 5].isnan() and v[3].isnan().sum() == 1 and v[3, 200] * 2.0 ** int(s[3, 1]) == 1.0
+    assert v[4].isnan().sum() == 2 and v[4, 7] * 2.0 ** int(s[4, 0]) == 2.0
+    assert torch.allclose(v[5, :128].double() * 2.0 ** int(s[5, 0]), torch.full((128,), 1e-37).double(), rtol=0.07)
+
+
+def blocks_ref(q):
+    e = q.scales.to(F64)[:, :q.codes.shape[1] // 128] - 127
+    return q.codes.to(F64) * torch.exp2(e).repeat_interleave(128, 1)
+
+
+def check_product(got, a, b, bias, ctx="", fast=False):
+    """K + 4 float32 operations.  The 8-bit instruction (fast) drops up to 2^-13 of the largest of each 8
+    products from the other seven; and as a whole its sums are off by less than 1e-4 of their size (5e-5
+    measured for codes of all magnitudes)."""
+    ra, rb = blocks_ref(a), blocks_ref(b)
+    ref, mag = ra @ rb.t(), ra.abs() @ rb.abs().t()
+    if bias is not None:
+        ref, mag = ref + bias.to(F64), mag + bias.to(F64).abs()
+    K, t = a.codes.shape[1], got.dtype
+    bound = ((K + 4) * u + (7 * 2.0 ** -13 if fast else 0.0)) * mag
+    within(got, ref, bound + U[t] * ref.abs() + TINY[t], ctx)
+    if fast and ref.numel() > 1000 and got.isfinite().all():
+        off = float((got.to(F64) - ref).norm() / ref.norm())
+        assert off <= 1e-4 + U[t], (ctx, off)
+
+
+PRODUCTS = [(1, 1, 1), (1, 64, 128), (3, 5, 130), (1, 1024, 960), (2, 777, 1000), (15, 33, 64), (16, 128, 256),
+            (17, 129, 700), (40, 300, 512), (64, 96, 128), (65, 100, 96), (129, 130, 131), (200, 257, 640),
+            (333, 777, 960), (300, 64, 4224)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", PRODUCTS)
+def test_fp8_matmul_and_linear(dev, dtype, M, N, K):
+    g = gen(M + N + K)
+    x = (randn(g, M, K) * torch.exp(2 * randn(g, M, 1))).to(dtype)
+    w = encoder.quantize_fp8(randn(g, N, K) * torch.exp(2 * randn(g, N, 1)))
+    a = encoder.quantize_fp8(x)
+    bias = randn(g, N, dtype=dtype)
+    for bs in (None, bias, bias.float()):
+        check_product(encoder.fp8_matmul(a, w, bs, out_dtype=dtype), a, w, bs, "matmul")
+        y = encoder.fp8_linear(x, w, bs)
+        assert y.dtype == dtype and y.shape == (M, N)
+        check_product(y, a, w, bs, "linear")
+        check_product(encoder.fp8_matmul(a, w, bs, out_dtype=dtype, fast_accum=True), a, w, bs, "matmul", True)
+        check_product(encoder.fp8_linear(x, w, bs, fast_accum=True), a, w, bs, "linear", True)
+
+
+def test_fp8_linear_shapes_strides_and_empty(dev):
+    g = gen(11)
+    w, bias = encoder.quantize_fp8(randn(g, 70, 100)), randn(g, 70)
+    for x in (randn(g, 3, 4, 100), randn(g, 9, 160)[:, 30:130], randn(g, 100, 9).t(), randn(g, 100),
+              randn(g, 1, 100).expand(9, 100)):
+        y = encoder.fp8_linear(x, w, bias)
+        assert y.shape == (*x.shape[:-1], 70)
+        check_product(y.reshape(-1, 70), encoder.quantize_fp8(x.reshape(-1, 100)), w, bias)
+    assert encoder.fp8_linear(torch.empty((0, 100), device=dev), w).shape == (0, 70)
+    assert encoder.fp8_matmul(w, encoder.quantize_fp8(torch.empty((0, 100), device=dev))).shape == (70, 0)
+
+
+def test_fp8_linear_keeps_nan_to_its_row(dev):
+    g = gen(12)
+    for M in (1, 5, 40, 300):
+        for dtype in TYPES:
+            x = randn(g, M, 300, dtype=dtype)
+            x[M // 2, 131] = float("inf")
+            w = encoder.quantize_fp8(randn(g, 200, 300))
+            for fast in (False, True):
+                y = encoder.fp8_linear(x, w, fast_accum=fast)
+                assert y[M // 2].isnan().all() and int(y.isnan().sum()) == 200
+
+
+def test_fp8_codes_of_all_magnitudes(dev):
+    """Every code but NaN, scales across their range: products far above and below one another."""
+    g = gen(13)
+    for M, N, K in ((40, 50, 640), (3, 70, 640), (300, 200, 256)):
+        q = []
+        for rows in (M, N):
+            c = torch.randint(0, 256, (rows, K), generator=g, device=dev).to(torch.uint8)
+            c[(c & 127) == 127] = 0
+            s = torch.full((rows, -(-K // 512) * 4), 127, dtype=torch.uint8, device=dev)
+            s[:, :K // 128] = torch.randint(112, 140, (rows, K // 128), generator=g, device=dev).to(torch.uint8)
+            q.append(encoder.Fp8Blocks(c.view(torch.float8_e4m3fn), s, K))
+        for dtype in (torch.float32, torch.bfloat16):
+            for fast in (False, True):
+                check_product(encoder.fp8_matmul(*q, out_dtype=dtype, fast_accum=fast), *q, None,
+                              f"{M} {N} {K} {dtype} {fast}", fast)
+
+
+# ---------------------------------------------------------------------------------------------
+# streams and refusals
+
+
+def test_on_another_stream(dev):
+    """Calls follow the current stream, and its workspace is its own."""
+    g = gen(14)
+    ids, grad = token_ids(g, 20_000, 3000), randn(g, 20_000, 64)
+    x, w = randn(g, 500, 256), encoder.quantize_fp8(randn(g, 300, 256))
+    want = encoder.embedding_grad(grad, ids, 3000), encoder.fp8_linear(x, w), encoder.layer_norm(x)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        late = grad * 0
+        for _ in range(20):  # the operands are made on this stream, after the call is enqueued they change
+            late = late * 0 + grad
+        got = encoder.embedding_grad(late, ids, 3000), encoder.fp8_linear(x, w), encoder.layer_norm(x)
+        late.zero_()
+    here = encoder.embedding_grad(grad, ids, 3000)
+    st.synchronize()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and torch.equal(here, want[0])
+
+
+def test_in_a_graph(dev):
+    """A captured sequence gives the eager results on every replay, with eager work between."""
+    g = gen(15)
+    ids, w = token_ids(g, 700, 400), randn(g, 400, 96)
+    wq, grad = encoder.quantize_fp8(randn(g, 80, 96)), randn(g, 700, 96)
+    gamma = randn(g, 96)
+
+    def sequence():
+        e = encoder.embedding(ids, w)
+        y, mean, rstd = encoder.layer_norm_forward(e, gamma)
+        dx, dw, db = encoder.layer_norm_grad(grad, e, gamma, mean, rstd)
+        return encoder.fp8_linear(y, wq), encoder.embedding_grad(dx, ids, 400), dw, db
+
+    st = torch.cuda.Stream()
+    st.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(st):
+        sequence()
+    torch.cuda.current_stream().wait_stream(st)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=st):
+        out = sequence()
+    for i in range(4):
+        w.copy_(randn(g, 400, 96))
+        ids.copy_(token_ids(g, 700, 400))
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in out]
+        assert all(torch.equal(a, b) for a, b in zip(got, sequence())), i
+
+
+def test_refusals(dev):
+    f, i64 = torch.zeros((4, 8), device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
+    q = encoder.quantize_fp8(f)
+    bad = [
+        (lambda: encoder.embedding(i64.short(), f), "int64 or int32"),
+        (lambda: encoder.embedding(i64, f.double()), "float32, float16 or bfloat16"),
+        (lambda: encoder.embedding(i64.cpu(), f), "must be on"),
+        (lambda: encoder.embedding(i64, f[0]), r"\[V, D\]"),
+        (lambda: encoder.embedding_grad(f, i64[:3], 10), "ids.shape"),
+        (lambda: encoder.embedding_grad(f, i64, 0), "num_rows"),
+        (lambda: encoder.embedding_grad(f, i64, 10, padding_idx=10), "padding_idx"),
+        (lambda: encoder.embedding_grad(f, i64, 10, out=f), "out must be"),
+        (lambda: encoder.layer_norm(f, torch.ones(7, device=dev)), "weight must be"),
+        (lambda: encoder.layer_norm(f, torch.ones(8, device=dev).half()), "or float32"),
+        (lambda: encoder.layer_norm(f, eps=-1.0), "eps"),
+        (lambda: encoder.layer_norm_grad(f, f[:2], None, i64.float(), i64.float()), "grad must be"),
+        (lambda: encoder.layer_norm_grad(f, f, None, i64[:3].float(), i64.float()), "mean must be"),
+        (lambda: encoder.AdamW([]), "at least one"),
+        (lambda: encoder.AdamW([f, f]), "twice"),
+        (lambda: encoder.AdamW([f.t()]), "contiguous"),
+        (lambda: encoder.AdamW([f], state_bits=16), "state_bits"),
+        (lambda: encoder.AdamW([f], betas=(1.0, 0.9)), "betas"),
+        (lambda: encoder.AdamW([f]).step([f, f]), "gradients are needed"),
+        (lambda: encoder.AdamW([f]).step([f[:2]]), "gradient 0"),
+        (lambda: encoder.AdamW([f], state_bits=8).load_state(1, f, f), "exp_avg must be"),
+        (lambda: encoder.AdamW([f]).load_state_dict(dict(state_bits=8)), "8 bits"),
+        (lambda: encoder.quantize_fp8(f[0]), r"\[rows, K\]"),
+        (lambda: encoder.fp8_linear(f[:, :7], q), r"\[..., 8\]"),
+        (lambda: encoder.fp8_linear(f, q, torch.zeros(5, device=dev)), "bias must be"),
+        (lambda: encoder.fp8_linear(f, f), "Fp8Blocks"),
+        (lambda: encoder.fp8_matmul(q, encoder.quantize_fp8(f[:, :7])), "columns"),
+        (lambda: encoder.fp8_matmul(q, encoder.Fp8Blocks(q.codes[:, :64], q.scales, 8)), "codes must be"),
+        (lambda: encoder.fp8_matmul(q, q, out_dtype=torch.float64), "out_dtype"),
+    ]
+    for call, text in bad:
+        with pytest.raises(_lib.TridentError, match=text):
+            call()

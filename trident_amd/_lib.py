@@ -19,6 +19,8 @@ MODE_TRIBASE = 11
 
 _P = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
+_size = ctypes.c_size_t
 _f64 = ctypes.c_double
 
 NOALLOC_SCRATCH_BYTES = 64 << 20  # TRIDENT_NOALLOC_SCRATCH_BYTES
@@ -56,6 +58,24 @@ class TridentSearchOutputs(ctypes.Structure):
                 ("events", ctypes.POINTER(_P)), ("host_rows", _P), ("host_rows_seed", _P)]
 
 
+# enum TridentDtype
+F32, F16, BF16 = range(3)
+
+
+class TridentAdamTensor(ctypes.Structure):
+    _fields_ = [("param", _P), ("grad", _P), ("numel", _i64), ("state_offset", _i64), ("dtype", _i32),
+                ("grad_dtype", _i32)]
+
+
+class TridentAdamState(ctypes.Structure):
+    _fields_ = [("m", _P), ("v", _P), ("m_scale", _P), ("v_scale", _P), ("len", _i64), ("bits", _i32)]
+
+
+class TridentAdamParams(ctypes.Structure):
+    _fields_ = [("lr", _f64), ("beta1", _f64), ("beta2", _f64), ("eps", _f64), ("weight_decay", _f64),
+                ("grad_scale", _f64), ("step", _i64)]
+
+
 # Stage boundaries recorded into TridentSearchOutputs.events (enum TridentStageEvent).
 EV_START, EV_PROBED, EV_GROUPED, EV_P1_SCAN, EV_P1_MERGE, EV_P2_SCAN, EV_END, EV_COUNT = range(8)
 
@@ -83,6 +103,22 @@ EXPORTS = {
     "trident_event_create": (ctypes.c_int, [ctypes.POINTER(_P)]),
     "trident_event_destroy": (ctypes.c_int, [_P]),
     "trident_event_elapsed_ms": (ctypes.c_int, [_P, _P, ctypes.POINTER(ctypes.c_float)]),
+    "trident_embedding": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _i32, _i64, _f64, _P, _i64, _P]),
+    "trident_embedding_grad_workspace_bytes": (_size, [_i64, _i64, _i64]),
+    "trident_embedding_grad": (ctypes.c_int, [_P, _i32, _i64, _P, _i32, _i64, _i64, _i64, _f64, _i64, _P, _i64, _P,
+                                              _size, _P]),
+    "trident_layer_norm": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _i32, _f64, _P, _i64, _P, _P, _P]),
+    "trident_layer_norm_grad_workspace_bytes": (_size, [_i64, _i64]),
+    "trident_layer_norm_grad": (ctypes.c_int, [_P, _i64, _P, _i64, _i32, _i64, _i64, _P, _i32, _P, _P, _P, _i64, _P,
+                                               _P, _P, _size, _P]),
+    "trident_adamw": (ctypes.c_int, [ctypes.POINTER(TridentAdamTensor), _i32, ctypes.POINTER(TridentAdamState),
+                                     ctypes.POINTER(TridentAdamParams), _P]),
+    "trident_adamw_state_values": (ctypes.c_int, [ctypes.POINTER(TridentAdamState), _P, _P, _P]),
+    "trident_fp8_quantize": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _P]),
+    "trident_fp8_matmul": (ctypes.c_int, [_P, _P, _i64, _P, _P, _i64, _i64, _P, _i32, _P, _i32, _i64, _i32, _P]),
+    "trident_fp8_linear_workspace_bytes": (_size, [_i64, _i64]),
+    "trident_fp8_linear": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _i64, _P, _i32, _P, _i64, _i32, _P,
+                                          _size, _P]),
     "trident_last_error": (ctypes.c_char_p, []),
     "trident_abi_version": (ctypes.c_int, []),
 }

@@ -27,6 +27,7 @@
 
 #include "../../include/trident_hip.h"
 #include "common.hpp"
+#include "encoder.hpp"
 #include "kernels.hpp"
 
 using namespace trident;
@@ -1032,6 +1033,18 @@ int group_units(const TridentIndexView* ix, const Workspace& w, int B, int nprob
 }
 
 }  // namespace
+
+// The same for the encoder's entry points, which live in their kernels' files.
+int trident::capi_fail(int code, const char* fmt, ...) {
+    char buf[512];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof(buf), fmt, ap);
+    va_end(ap);
+    return fail(code, "%s", buf);
+}
+
+int trident::capi_check_launch(const char* what) { return check_launch(what); }
 
 extern "C" {
 

@@ -1,0 +1,98 @@
+// Shared by the encoder's kernels (embedding.hip, layernorm.hip, adamw.hip, fp8mm.hip): element
+// types, 16-byte loads and stores through float, wave reductions, and the C entry points' errors.
+//
+// Every sum is held in float32 and every result is rounded to its type once.  Rows may start at any
+// element: gfx950 takes 16-byte accesses at any element's address, so one vector form serves every
+// row pitch, and a row's last vector is shifted back to end with the row (it overlaps the one before).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../include/trident_hip.h"
+#include "common.hpp"
+
+namespace trident {
+
+// Records the calling thread's last error (trident_last_error) and returns `code`; never throws.
+int capi_fail(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
+int capi_check_launch(const char* what);
+
+using f16_t = _Float16;
+using bf16_t = __bf16;
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+constexpr int kVec = 16 / (int)sizeof(T);  // elements of one 16-byte access
+
+inline bool dtype_ok(int32_t t) { return t == TRIDENT_F32 || t == TRIDENT_F16 || t == TRIDENT_BF16; }
+
+// Calls f with a value of the element type that `t` names.
+template <typename F>
+inline void with_dtype(int32_t t, F&& f) {
+    if (t == TRIDENT_F32) f(float{});
+    else if (t == TRIDENT_F16) f(f16_t{});
+    else f(bf16_t{});
+}
+
+// N elements from any element's address: one element, or whole 16-byte accesses.
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[N]) {
+    if constexpr (N == 1) {
+        f[0] = (float)p[0];
+    } else {
+        constexpr int V = kVec<T>;
+        static_assert(N % V == 0, "whole 16-byte accesses");
+#pragma unroll
+        for (int k = 0; k < N; k += V) {
+            u32x4 v;
+            __builtin_memcpy(&v, p + k, 16);
+            if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) f[k + i] = __uint_as_float(v[i]);
+            } else if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    f[k + 2 * i] = __uint_as_float(v[i] << 16);
+                    f[k + 2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+                }
+            } else {
+                typedef f16_t h8 __attribute__((ext_vector_type(8)));
+                const h8 h = __builtin_bit_cast(h8, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) f[k + i] = (float)h[i];
+            }
+        }
+    }
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[N]) {
+    if constexpr (N == 1) {
+        p[0] = (T)f[0];
+    } else {
+        static_assert(N == kVec<T>, "one 16-byte access");
+        typedef T tv __attribute__((ext_vector_type(N)));
+        tv t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = (T)f[i];
+        __builtin_memcpy(p, &t, 16);
+    }
+}
+
+// Sum over the 64 lanes of a wave, the same in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
+    return v;
+}
+
+}  // namespace trident

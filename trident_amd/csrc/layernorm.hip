@@ -1,0 +1,410 @@
+// Layer norm of rows of D elements, and its backward pass.
+//
+//   m = mean(x)   r = 1 / sqrt(mean((x - m)^2) + eps)   h = (x - m) r   y = w h + b
+//   a = w dy      dx = r (a - mean(a) - h mean(a h))    dw = sum_rows dy h   db = sum_rows dy
+//
+// The variance is that of the centred values (a second pass over registers, no further read), sums and
+// statistics are float32.  The weight's gradient is summed without atomics: each workgroup keeps its
+// rows' share in registers, and a second launch adds the workgroups' shares in order.
+#include <algorithm>
+
+#include "encoder.hpp"
+
+namespace trident {
+namespace {
+
+struct NormArgs {
+    const void* x;        // [rows, ldx]
+    const void* dy;       // [rows, lddy]
+    const void* weight;   // [D] or null: ones
+    const void* bias;     // [D] or null: zeros
+    void* y;              // [rows, ldy]
+    void* dx;             // [rows, lddx]
+    float* mean;          // [rows] or null
+    float* rstd;
+    float* part;          // [workgroups, 2, D]
+    int64_t rows, ldx, lddy, ldy, lddx;
+    int D, nv;            // nv: vectors of a row
+    float eps, inv_D;
+};
+
+// The vectors of a row that this lane holds: W waves share a row, lane l of them holds the vectors
+// l + 64 W c.  The last vector of a row ends with the row; its first `dup` elements are also the
+// vector before's and count there.
+template <int VEC, int NV, int W>
+struct Columns {
+    int col[NV], dup[NV];
+    bool on[NV];
+    __device__ __forceinline__ void init(const NormArgs& a, int l) {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int v = l + kWave * W * c;
+            on[c] = v < a.nv;
+            col[c] = min(v * VEC, a.D - VEC);
+            dup[c] = v * VEC - col[c];
+        }
+    }
+};
+
+template <typename T, int VEC, int NV, int W>
+__device__ __forceinline__ void load_row(const T* p, const Columns<VEC, NV, W>& k, float (&f)[NV][VEC]) {
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        if (k.on[c]) load_vec(p + k.col[c], f[c]);
+        else
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[c][i] = 0.0f;
+    }
+}
+
+// Sum over the W waves that share a row; with W > 1 every thread of the workgroup calls it.
+template <int W>
+__device__ __forceinline__ float row_sum(float v, float* s_red) {
+    v = wave_sum(v);
+    if constexpr (W > 1) {
+        __syncthreads();
+        if (lane_id() == 0) s_red[threadIdx.x / kWave] = v;
+        __syncthreads();
+        v = s_red[0];
+#pragma unroll
+        for (int i = 1; i < W; ++i) v += s_red[i];
+    }
+    return v;
+}
+
+// One wave per row up to NV * 64 vectors, else one workgroup of W = 4 waves.
+template <typename T, typename TW, int VEC, int NV, int W>
+__global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
+    __shared__ float s_red[W];
+    constexpr int kRows = kWavesPerBlock / W;
+    const int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? threadIdx.x / kWave : 0);
+    if (row >= a.rows) return;
+    Columns<VEC, NV, W> k;
+    k.init(a, W == 1 ? lane_id() : threadIdx.x);
+    float x[NV][VEC];
+    load_row<T>(static_cast<const T*>(a.x) + row * a.ldx, k, x);
+    float s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+            if (i >= k.dup[c]) s += x[c][i];
+    const float mean = row_sum<W>(s, s_red) * a.inv_D;
+    s = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            x[c][i] -= mean;
+            if (k.on[c] && i >= k.dup[c]) s += x[c][i] * x[c][i];
+        }
+    const float rstd = 1.0f / sqrtf(row_sum<W>(s, s_red) * a.inv_D + a.eps);
+    T* y = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        if (!k.on[c]) continue;
+        float w[VEC], b[VEC];
+        if (a.weight) load_vec(static_cast<const TW*>(a.weight) + k.col[c], w);
+        if (a.bias) load_vec(static_cast<const TW*>(a.bias) + k.col[c], b);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float v = x[c][i] * rstd;
+            if (a.weight) v *= w[i];
+            if (a.bias) v += b[i];
+            x[c][i] = v;
+        }
+        store_vec(y + k.col[c], x[c]);
+    }
+    if (a.mean && (W == 1 ? lane_id() : (int)threadIdx.x) == 0) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+}
+
+// Rows too long for a workgroup's registers: the row is read three times (from L2 after the first).
+template <typename T, typename TW>
+__global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
+    __shared__ float s_red[kWavesPerBlock];
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+    T* y = static_cast<T*>(a.y) + row * a.ldy;
+    float s = 0.0f;
+    for (int d = threadIdx.x; d < a.D; d += kBlock) s += (float)x[d];
+    const float mean = row_sum<kWavesPerBlock>(s, s_red) * a.inv_D;
+    s = 0.0f;
+    for (int d = threadIdx.x; d < a.D; d += kBlock) s += ((float)x[d] - mean) * ((float)x[d] - mean);
+    const float rstd = 1.0f / sqrtf(row_sum<kWavesPerBlock>(s, s_red) * a.inv_D + a.eps);
+    for (int d = threadIdx.x; d < a.D; d += kBlock) {
+        float v = ((float)x[d] - mean) * rstd;
+        if (a.weight) v *= (float)static_cast<const TW*>(a.weight)[d];
+        if (a.bias) v += (float)static_cast<const TW*>(a.bias)[d];
+        y[d] = (T)v;
+    }
+    if (a.mean && threadIdx.x == 0) {
+        a.mean[row] = mean;
+        a.rstd[row] = rstd;
+    }
+}
+
+// A wave (or a workgroup, W = 4) takes every gridDim-th row: dx from the row's two means, and dy h and
+// dy added to the columns' sums, which stay in registers until the last row.
+template <typename T, typename TW, int VEC, int NV, int W>
+__global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
+    extern __shared__ float s_part[];  // [kWavesPerBlock][D], W = 1 only
+    __shared__ float s_red[W];
+    constexpr int kRows = kWavesPerBlock / W;
+    const int wave = threadIdx.x / kWave;
+    Columns<VEC, NV, W> k;
+    k.init(a, W == 1 ? lane_id() : threadIdx.x);
+    float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            w[c][i] = 1.0f;
+            dw[c][i] = db[c][i] = 0.0f;
+        }
+    if (a.weight) load_row<TW>(static_cast<const TW*>(a.weight), k, w);
+    for (int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0); row < a.rows;
+         row += (int64_t)gridDim.x * kRows) {
+        float h[NV][VEC], g[NV][VEC];
+        load_row<T>(static_cast<const T*>(a.x) + row * a.ldx, k, h);
+        load_row<T>(static_cast<const T*>(a.dy) + row * a.lddy, k, g);
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        float sa = 0.0f, sh = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                h[c][i] = (h[c][i] - mean) * rstd;
+                const float dy = g[c][i];
+                dw[c][i] += dy * h[c][i];
+                db[c][i] += dy;
+                g[c][i] = dy * w[c][i];
+                if (k.on[c] && i >= k.dup[c]) {
+                    sa += g[c][i];
+                    sh += g[c][i] * h[c][i];
+                }
+            }
+        sa = row_sum<W>(sa, s_red) * a.inv_D;
+        sh = row_sum<W>(sh, s_red) * a.inv_D;
+        T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            if (!k.on[c]) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) g[c][i] = rstd * (g[c][i] - sa - h[c][i] * sh);
+            store_vec(dx + k.col[c], g[c]);
+        }
+    }
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
+    if constexpr (W == 1) {
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            __syncthreads();
+#pragma unroll
+            for (int c = 0; c < NV; ++c)
+                if (k.on[c])
+#pragma unroll
+                    for (int i = 0; i < VEC; ++i)
+                        s_part[wave * a.D + k.col[c] + i] = which ? db[c][i] : dw[c][i];
+            __syncthreads();
+            for (int d = threadIdx.x; d < a.D; d += kBlock) {
+                float s = s_part[d];
+#pragma unroll
+                for (int i = 1; i < kWavesPerBlock; ++i) s += s_part[i * a.D + d];
+                part[which * a.D + d] = s;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int c = 0; c < NV; ++c)
+            if (k.on[c])
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) {
+                    part[k.col[c] + i] = dw[c][i];
+                    part[a.D + k.col[c] + i] = db[c][i];
+                }
+    }
+}
+
+template <typename T, typename TW>
+__global__ __launch_bounds__(kBlock) void norm_grad_long_kernel(NormArgs a) {
+    __shared__ float s_red[kWavesPerBlock];
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
+    if ((int64_t)blockIdx.x >= a.rows)  // no row: a share of zeros
+        for (int d = threadIdx.x; d < 2 * a.D; d += kBlock) part[d] = 0.0f;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.ldx;
+        const T* dy = static_cast<const T*>(a.dy) + row * a.lddy;
+        T* dx = static_cast<T*>(a.dx) + row * a.lddx;
+        const float mean = a.mean[row], rstd = a.rstd[row];
+        const bool first = row == (int64_t)blockIdx.x;
+        float sa = 0.0f, sh = 0.0f;
+        for (int d = threadIdx.x; d < a.D; d += kBlock) {
+            const float h = ((float)x[d] - mean) * rstd, g = (float)dy[d];
+            const float v = a.weight ? g * (float)static_cast<const TW*>(a.weight)[d] : g;
+            sa += v;
+            sh += v * h;
+            // a column is always this thread's: its sums need no lock
+            part[d] = (first ? 0.0f : part[d]) + g * h;
+            part[a.D + d] = (first ? 0.0f : part[a.D + d]) + g;
+        }
+        sa = row_sum<kWavesPerBlock>(sa, s_red) * a.inv_D;
+        sh = row_sum<kWavesPerBlock>(sh, s_red) * a.inv_D;
+        for (int d = threadIdx.x; d < a.D; d += kBlock) {
+            const float h = ((float)x[d] - mean) * rstd, g = (float)dy[d];
+            const float v = a.weight ? g * (float)static_cast<const TW*>(a.weight)[d] : g;
+            dx[d] = (T)(rstd * (v - sa - h * sh));
+        }
+    }
+}
+
+constexpr int kJoinBlock = 1024;
+
+// dw and db from the workgroups' shares: 64 columns a workgroup, its 16 waves each every 16th share,
+// then the waves' sums in order.
+template <typename TW>
+__global__ __launch_bounds__(kJoinBlock) void norm_join_kernel(const float* __restrict__ part, int parts, int D,
+                                                               TW* __restrict__ dw, TW* __restrict__ db) {
+    __shared__ float s_sum[kJoinBlock / kWave][kWave];
+    const int wave = threadIdx.x / kWave;
+    const int64_t col = (int64_t)blockIdx.x * kWave + lane_id();
+    float s = 0.0f;
+    if (col < 2 * (int64_t)D) {
+#pragma unroll 8
+        for (int p = wave; p < parts; p += kJoinBlock / kWave) s += part[(int64_t)p * 2 * D + col];
+    }
+    s_sum[wave][lane_id()] = s;
+    __syncthreads();
+    if (wave == 0 && col < 2 * (int64_t)D) {
+        for (int i = 1; i < kJoinBlock / kWave; ++i) s += s_sum[i][lane_id()];
+        if (col < D) {
+            if (dw) dw[col] = (TW)s;
+        } else if (db) {
+            db[col - D] = (TW)s;
+        }
+    }
+}
+
+// Calls f<VEC, NV, W> for rows of D elements of type T; false if they are too long for registers.
+template <typename T, typename F>
+bool with_shape(int64_t D, F&& f) {
+    constexpr int V = kVec<T>;
+    using std::integral_constant;
+    const int64_t nv = D < V ? D : (D + V - 1) / V;
+    const auto go = [&](auto vec, auto n, auto w) { f(vec, n, w); return true; };
+    integral_constant<int, 1> i1;
+    integral_constant<int, 2> i2;
+    integral_constant<int, 3> i3;
+    integral_constant<int, 4> i4;
+    integral_constant<int, V> v;
+    if (D < V) return go(i1, i1, i1);
+    if (nv <= 64) return go(v, i1, i1);
+    if (nv <= 128) return go(v, i2, i1);
+    if (nv <= 192) return go(v, i3, i1);
+    if (nv <= 256) return go(v, i4, i1);
+    if (nv <= 512) return go(v, i2, i4);
+    if (nv <= 1024) return go(v, i4, i4);
+    return false;
+}
+
+constexpr int kGradBlocks = 512;  // workgroups that share the rows of a backward pass
+
+int64_t grad_parts(int64_t rows) {
+    return std::max<int64_t>(1, std::min<int64_t>(kGradBlocks, (rows + kWavesPerBlock - 1) / kWavesPerBlock));
+}
+
+bool sizes_ok(int64_t rows, int64_t D) { return rows >= 0 && rows <= 0x7fffffff && D >= 1 && D <= (1 << 29); }
+
+}  // namespace
+}  // namespace trident
+
+using namespace trident;
+
+extern "C" {
+
+int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, int64_t ld_x, const void* weight,
+                       const void* bias, int32_t weight_dtype, double eps, void* y, int64_t ld_y, float* mean,
+                       float* rstd, void* stream) {
+    if (!dtype_ok(dtype) || (weight_dtype != dtype && weight_dtype != TRIDENT_F32))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm: dtype=%d weight_dtype=%d", dtype, weight_dtype);
+    if (!sizes_ok(rows, D) || ld_x < D || ld_y < D || !(eps >= 0.0))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm: bad sizes rows=%lld D=%lld ld=%lld, %lld eps=%g",
+                         (long long)rows, (long long)D, (long long)ld_x, (long long)ld_y, eps);
+    if (rows == 0) return TRIDENT_OK;
+    if (!x || !y || !mean != !rstd) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm: NULL pointer");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        with_dtype(weight_dtype, [&](auto u) {
+            using TW = decltype(u);
+            if constexpr (std::is_same<T, TW>::value || std::is_same<TW, float>::value) {
+                NormArgs a{x, nullptr, weight, bias, y, nullptr, mean, rstd, nullptr, rows, ld_x, 0, ld_y, 0, (int)D, 0,
+                           (float)eps, (float)(1.0 / (double)D)};
+                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
+                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
+                    a.nv = (int)((D + VEC - 1) / VEC);
+                    const int64_t per = kWavesPerBlock / W;
+                    norm_kernel<T, TW, VEC, NV, W><<<(unsigned)((rows + per - 1) / per), kBlock, 0, st>>>(a);
+                });
+                if (!ok) norm_long_kernel<T, TW><<<(unsigned)rows, kBlock, 0, st>>>(a);
+            }
+        });
+    });
+    return capi_check_launch("norm_kernel");
+}
+
+size_t trident_layer_norm_grad_workspace_bytes(int64_t rows, int64_t D) {
+    if (!sizes_ok(rows, D)) return 0;
+    return (size_t)grad_parts(rows) * 2 * (size_t)D * sizeof(float);
+}
+
+int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype, int64_t rows,
+                            int64_t D, const void* weight, int32_t weight_dtype, const float* mean, const float* rstd,
+                            void* dx, int64_t ld_dx, void* dweight, void* dbias, void* workspace,
+                            size_t workspace_bytes, void* stream) {
+    if (!dtype_ok(dtype) || (weight_dtype != dtype && weight_dtype != TRIDENT_F32))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm_grad: dtype=%d weight_dtype=%d", dtype,
+                         weight_dtype);
+    if (!sizes_ok(rows, D) || ld_x < D || ld_dy < D || ld_dx < D)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "layer_norm_grad: bad sizes rows=%lld D=%lld ld=%lld, %lld, %lld", (long long)rows,
+                         (long long)D, (long long)ld_dy, (long long)ld_x, (long long)ld_dx);
+    if (rows > 0 && (!dy || !x || !mean || !rstd || !dx))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm_grad: NULL pointer");
+    const int64_t parts = grad_parts(rows);
+    const size_t need = trident_layer_norm_grad_workspace_bytes(rows, D);
+    if (!workspace || workspace_bytes < need)
+        return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "layer_norm_grad: workspace %zu < %zu bytes",
+                         workspace_bytes, need);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    int rc = TRIDENT_OK;
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        with_dtype(weight_dtype, [&](auto u) {
+            using TW = decltype(u);
+            if constexpr (std::is_same<T, TW>::value || std::is_same<TW, float>::value) {
+                NormArgs a{x, dy, weight, nullptr, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd),
+                           static_cast<float*>(workspace), rows, ld_x, ld_dy, 0, ld_dx, (int)D, 0, 0.0f,
+                           (float)(1.0 / (double)D)};
+                // with no rows every share is zero: the kernels' loops are empty
+                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
+                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
+                    a.nv = (int)((D + VEC - 1) / VEC);
+                    const size_t lds = W == 1 ? kWavesPerBlock * (size_t)D * sizeof(float) : 0;
+                    norm_grad_kernel<T, TW, VEC, NV, W><<<(unsigned)parts, kBlock, lds, st>>>(a);
+                });
+                if (!ok) norm_grad_long_kernel<T, TW><<<(unsigned)parts, kBlock, 0, st>>>(a);
+                if ((rc = capi_check_launch("norm_grad_kernel")) || (!dweight && !dbias)) return;
+                norm_join_kernel<TW><<<(unsigned)((2 * D + kWave - 1) / kWave), kJoinBlock, 0, st>>>(
+                    static_cast<const float*>(workspace), (int)parts, (int)D, static_cast<TW*>(dweight),
+                    static_cast<TW*>(dbias));
+                rc = capi_check_launch("norm_join_kernel");
+            }
+        });
+    });
+    return rc;
+}
+
+}  // extern "C"

@@ -1,0 +1,463 @@
+"""The operators of the encoder that makes and trains the vectors an index holds.
+
+  embedding, embedding_grad            rows of a table for token ids, scaled; the table's gradient
+  layer_norm, layer_norm_forward / _grad
+  AdamW                                one launch per step for up to 88 tensors, states in 32 or 8 bits
+  quantize_fp8, fp8_matmul, fp8_linear products in 8-bit floating point, one scale per row and 128 columns
+
+``embedding`` and ``layer_norm`` take part in autograd; the ``*_forward`` / ``*_grad`` functions are the
+bare passes.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics and states are
+float32 and every result is rounded once.  Each call runs on the current stream of its tensors' device,
+with the library's workspace of that stream (``trident_amd.ext.workspace``); results are the same bits
+every time.  Wrong arguments raise ``TridentError``.
+
+The reference has no counterpart: its vectors come from data sets.  The kernels are in libtrident_hip.so
+(include/trident_hip.h); there is no fallback.
+"""
+from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
+
+import ctypes
+
+import numpy as np
+import torch
+
+from . import _lib, ext
+from .ext import _need
+
+_DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+STATE_BLOCK = 256  # elements of an 8-bit state that share a scale
+
+
+def _dtype(name: str, t: torch.Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    _need(code is not None, f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _on(device: torch.device, **tensors) -> None:
+    _need(device.type == "cuda", "the encoder's operators need device tensors")
+    for name, t in tensors.items():
+        _need(t is None or t.device == device, f"{name} must be on {device}, got {t.device if t is not None else None}")
+
+
+def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """(t, or a copy, with the elements of its last dimension next to each other and one pitch between
+    its rows; that pitch)."""
+    D = t.shape[-1]
+    if not t.is_contiguous():
+        if t.dim() != 2:
+            t = t.reshape(-1, D)
+        if (t.stride(1) != 1 and D != 1) or t.stride(0) < D:
+            t = t.contiguous()
+        elif t.shape[0] > 1:
+            return t, t.stride(0)
+    return t, max(D, 1)
+
+
+def _call(device: torch.device, name: str, *args) -> None:
+    fn = getattr(_lib.lib(), name)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+    _lib.check(rc, name)
+
+
+def _call_ws(device: torch.device, name: str, nbytes: int, *args) -> None:
+    """_call with this stream's workspace of at least ``nbytes`` as the last two arguments."""
+    st = torch.cuda.current_stream(device)
+    slot = ext._workspace_slot(device, st)
+    with slot.lock:
+        ws = ext._grow(slot, device, nbytes, st)
+        _call(device, name, *args, ws.data_ptr(), ws.numel())
+
+
+# ---------------------------------------------------------------------------------------------
+# embedding
+
+
+def _ids(ids: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    _need(ids.dtype in (torch.int64, torch.int32), f"ids must be int64 or int32, got {ids.dtype}")
+    return (ids if ids.is_contiguous() else ids.contiguous()), int(ids.dtype == torch.int64)
+
+
+def _embed(ids, weight, scale):
+    _need(weight.dim() == 2 and weight.shape[0] > 0 and weight.shape[1] > 0,
+          f"weight must be [V, D], got {tuple(weight.shape)}")
+    code = _dtype("weight", weight)
+    _on(weight.device, ids=ids)
+    _need(weight.device.type == "cuda", "weight must be a device tensor")
+    idc, wide = _ids(ids)
+    V, D = weight.shape
+    w, ld = _rows(weight)
+    out = torch.empty((*ids.shape, D), dtype=weight.dtype, device=weight.device)
+    _call(weight.device, "trident_embedding", w.data_ptr(), code, V, D, ld, idc.data_ptr(), wide, idc.numel(),
+          float(scale), out.data_ptr(), D)
+    return out
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, padding_idx):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
+        return _embed(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        (ids,) = ctx.saved_tensors
+        return None, embedding_grad(grad, ids, ctx.rows, ctx.scale, ctx.padding_idx), None, None
+
+
+def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
+              padding_idx: Optional[int] = None) -> torch.Tensor:
+    """``scale * weight[ids]``, shape ``[*ids.shape, D]`` in the table's type.
+
+    A negative id is an empty slot of a padded batch and gives zeros; an id past the table gives NaN
+    (the ids stay on the device, so no call can refuse them).  Neither has a gradient, nor has
+    ``padding_idx``, whose row is looked up like any other.
+    """
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(ids, weight, float(scale), padding_idx)
+    return _embed(ids, weight, scale)
+
+
+def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float = 1.0,
+                   padding_idx: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """The table's gradient ``[num_rows, D]`` in the type of ``grad`` (``[*ids.shape, D]``): row v is
+    ``scale`` times the sum of the gradients of the tokens with id v, in their order.  ``out`` (rows of
+    any pitch) is written whole."""
+    code = _dtype("grad", grad)
+    _on(grad.device, ids=ids, out=out)
+    _need(grad.device.type == "cuda", "grad must be a device tensor")
+    _need(grad.dim() >= 1 and grad.shape[:-1] == ids.shape and grad.shape[-1] > 0,
+          f"grad must be [*ids.shape, D], got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
+    num_rows = int(num_rows)
+    _need(num_rows > 0, f"num_rows must be positive, got {num_rows}")
+    _need(padding_idx is None or 0 <= padding_idx < num_rows, f"padding_idx={padding_idx} outside [0, {num_rows})")
+    idc, wide = _ids(ids)
+    D = grad.shape[-1]
+    g, ld = _rows(grad)
+    if out is None:
+        out = torch.empty((num_rows, D), dtype=grad.dtype, device=grad.device)
+    else:
+        _need(out.dtype == grad.dtype and tuple(out.shape) == (num_rows, D) and (out.stride(1) == 1 or D == 1) and
+              (out.stride(0) >= D or num_rows == 1), f"out must be [{num_rows}, {D}] {grad.dtype} with whole rows")
+    nbytes = _lib.lib().trident_embedding_grad_workspace_bytes(idc.numel(), num_rows, D)
+    _call_ws(grad.device, "trident_embedding_grad", nbytes, g.data_ptr(), code, ld, idc.data_ptr(), wide, idc.numel(),
+             num_rows, D, float(scale), -1 if padding_idx is None else int(padding_idx), out.data_ptr(),
+             out.stride(0) if num_rows > 1 else D)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# layer norm
+
+
+def _affine(x, weight, bias) -> int:
+    """The type code of weight and bias, which is x's or float32."""
+    D, code = x.shape[-1], None
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is None:
+            continue
+        _need(t.dim() == 1 and t.shape[0] == D and t.is_contiguous(), f"{name} must be a contiguous [{D}]")
+        _need(t.dtype in (x.dtype, torch.float32), f"{name} must be {x.dtype} or float32, got {t.dtype}")
+        _need(code is None or _DTYPES[t.dtype] == code, "weight and bias must have one type")
+        code = _DTYPES[t.dtype]
+    return _DTYPES[x.dtype] if code is None else code
+
+
+def _norm(x, weight, bias, eps, keep):
+    code = _dtype("x", x)
+    _need(x.dim() >= 1 and x.shape[-1] > 0, f"x must be [..., D], got {tuple(x.shape)}")
+    _on(x.device, weight=weight, bias=bias)
+    wcode = _affine(x, weight, bias)
+    D = x.shape[-1]
+    rows = x.numel() // D
+    xr, ld = _rows(x)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if keep:
+        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
+    _call(x.device, "trident_layer_norm", xr.data_ptr(), code, rows, D, ld, ext._ptr(weight), ext._ptr(bias), wcode,
+          float(eps), y.data_ptr(), D, ext._ptr(mean), ext._ptr(rstd))
+    return y, mean, rstd
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _norm(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        x, weight, mean, rstd = ctx.saved_tensors
+        dx, dw, db = _norm_grad(grad, x, weight, mean, rstd, ctx.needs_input_grad[1], ctx.needs_input_grad[2],
+                                ctx.bias_dtype if weight is None else weight.dtype)
+        return (dx if ctx.needs_input_grad[0] else None), dw, db, None
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of ``x``; ``weight`` and ``bias`` ([D], of x's type or
+    float32) may be left out."""
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
+                                    (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _norm(x, weight, bias, eps, False)[0]
+
+
+def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                       eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(y, mean, rstd): layer norm and the rows' float32 statistics, which the backward pass takes."""
+    return _norm(x, weight, bias, eps, True)
+
+
+def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor,
+                    rstd: torch.Tensor):
+    """(dx, dweight, dbias) from the gradient of y and what ``layer_norm_forward`` kept; the last two in
+    the weight's type (x's without a weight, and then no dweight)."""
+    return _norm_grad(grad, x, weight, mean, rstd, weight is not None, True, x.dtype if weight is None else weight.dtype)
+
+
+def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
+    code = _dtype("x", x)
+    _need(grad.shape == x.shape and grad.dtype == x.dtype,
+          f"grad must be {tuple(x.shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
+    _on(x.device, grad=grad, weight=weight, mean=mean, rstd=rstd)
+    for name, t in (("mean", mean), ("rstd", rstd)):
+        _need(t.dtype == torch.float32 and t.shape == x.shape[:-1] and t.is_contiguous(),
+              f"{name} must be a contiguous float32 {tuple(x.shape[:-1])}")
+    _affine(x, weight, None)
+    D = x.shape[-1]
+    rows = x.numel() // D
+    wdtype = x.dtype if wdtype is None else wdtype
+    xr, ldx = _rows(x)
+    gr, ldg = _rows(grad)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dw = torch.empty(D, dtype=wdtype, device=x.device) if need_w else None
+    db = torch.empty(D, dtype=wdtype, device=x.device) if need_b else None
+    nbytes = _lib.lib().trident_layer_norm_grad_workspace_bytes(rows, D)
+    _call_ws(x.device, "trident_layer_norm_grad", nbytes, gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D,
+             ext._ptr(weight), _DTYPES[wdtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, ext._ptr(dw),
+             ext._ptr(db))
+    return dx, dw, db
+
+
+# ---------------------------------------------------------------------------------------------
+# AdamW
+
+_TABLE = np.dtype([("param", "u8"), ("grad", "u8"), ("numel", "i8"), ("offset", "i8"), ("dtype", "i4"),
+                   ("grad_dtype", "i4")])  # TridentAdamTensor
+
+
+class AdamW:
+    """AdamW (decoupled weight decay) over a list of tensors of float32, float16 or bfloat16.
+
+    ``step()`` updates the parameters in place from their ``.grad`` (or from a list of gradients, each of
+    any of the three types); a parameter without one is left alone.  ``grad_scale`` multiplies the
+    gradients (one over a loss scale).  ``lr``, ``weight_decay`` and ``step_count`` may be set between
+    steps; groups with other settings are other optimizers.
+
+    The moments are float32 (``state_bits=32``) or 8-bit codes with a float32 scale for every 256
+    (``state_bits=8``: 2.03 bytes a parameter instead of 8); the arithmetic is float32 either way.  They
+    lie in flat buffers ``exp_avg`` and ``exp_avg_sq`` (with ``exp_avg_scale`` and ``exp_avg_sq_scale``),
+    tensor i's from ``offsets[i]``, a multiple of 256, zeros up to the next tensor's.  A gradient that is
+    not finite shows in its parameter and state; in 8 bits in the state of its block of 256.
+    """
+
+    def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, state_bits: int = 32):
+        self.params: List[torch.Tensor] = list(params)
+        _need(len(self.params) > 0, "AdamW needs at least one parameter")
+        _need(state_bits in (8, 32), f"state_bits must be 8 or 32, got {state_bits}")
+        _need(0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0, f"betas must lie in [0, 1), got {betas}")
+        _need(lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0, "lr, eps and weight_decay must not be negative")
+        _need(len({id(p) for p in self.params}) == len(self.params), "a parameter is listed twice")
+        self.device = self.params[0].device
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(betas), float(eps), float(weight_decay)
+        self.state_bits, self.step_count = state_bits, 0
+        self._table = np.zeros(len(self.params), _TABLE)
+        self.offsets, total = [], 0
+        for i, p in enumerate(self.params):
+            self._table[i]["dtype"] = _dtype(f"parameter {i}", p)
+            _on(self.device, **{f"parameter {i}": p})
+            _need(p.is_contiguous(), f"parameter {i} must be contiguous")
+            self.offsets.append(total)
+            total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        self._numel = np.array([p.numel() for p in self.params], np.int64)
+        self._table["offset"] = self.offsets
+        kind = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
+        self.exp_avg = torch.zeros(total, dtype=kind[0], device=self.device)
+        self.exp_avg_sq = torch.zeros(total, dtype=kind[1], device=self.device)
+        self.exp_avg_scale = self.exp_avg_sq_scale = None
+        if state_bits == 8:
+            self.exp_avg_scale = torch.zeros(total // STATE_BLOCK, device=self.device)
+            self.exp_avg_sq_scale = torch.zeros(total // STATE_BLOCK, device=self.device)
+        self._state = _lib.TridentAdamState(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
+                                            ext._ptr(self.exp_avg_scale), ext._ptr(self.exp_avg_sq_scale), total,
+                                            state_bits)
+
+    def zero_grad(self) -> None:
+        for p in self.params:
+            p.grad = None
+
+    @torch.no_grad()
+    def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, grad_scale: float = 1.0) -> None:
+        grads = [p.grad for p in self.params] if grads is None else list(grads)
+        _need(len(grads) == len(self.params), f"{len(self.params)} gradients are needed, got {len(grads)}")
+        table = self._table
+        for i, (p, g) in enumerate(zip(self.params, grads)):
+            if g is None:
+                continue
+            _need(isinstance(g, torch.Tensor) and g.shape == p.shape and g.device == self.device and
+                  g.layout == torch.strided, f"gradient {i} must be a dense {tuple(p.shape)} on {self.device}")
+            if not g.is_contiguous():
+                grads[i] = g.contiguous()
+        table["numel"] = [0 if g is None else n for g, n in zip(grads, self._numel)]
+        table["param"] = [p.data_ptr() for p in self.params]
+        table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        table["grad_dtype"] = [0 if g is None else _dtype("gradient", g) for g in grads]
+        h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
+                                   float(grad_scale), self.step_count + 1)
+        _call(self.device, "trident_adamw",
+              ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.TridentAdamTensor)), len(table),
+              ctypes.byref(self._state), ctypes.byref(h))
+        self.step_count += 1
+        torch.autograd.graph.increment_version([p for p, g in zip(self.params, grads) if g is not None])
+
+    def state_values(self) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The moments as flat float32 tensors: the buffers themselves, or what the 8-bit codes stand for."""
+        if self.state_bits == 32:
+            return self.exp_avg, self.exp_avg_sq
+        m, v = torch.empty((2, self.exp_avg.numel()), device=self.device)
+        _call(self.device, "trident_adamw_state_values", ctypes.byref(self._state), m.data_ptr(), v.data_ptr())
+        return m, v
+
+    def load_state(self, step_count: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
+                   exp_avg_scale: Optional[torch.Tensor] = None,
+                   exp_avg_sq_scale: Optional[torch.Tensor] = None) -> None:
+        """Copies flat states (as the attributes of the same names hold them) and the steps taken."""
+        _need(step_count >= 0, f"step_count must not be negative, got {step_count}")
+        given = dict(exp_avg=exp_avg, exp_avg_sq=exp_avg_sq, exp_avg_scale=exp_avg_scale,
+                     exp_avg_sq_scale=exp_avg_sq_scale)
+        for name, t in given.items():
+            mine = getattr(self, name)
+            _need((t is None) == (mine is None), f"{name} does not go with states of {self.state_bits} bits")
+            _need(t is None or (t.dtype == mine.dtype and t.numel() == mine.numel()),
+                  f"{name} must be {None if mine is None else (mine.numel(), mine.dtype)}")
+        for name, t in given.items():
+            if t is not None:
+                getattr(self, name).copy_(t.reshape(-1))
+        self.step_count = int(step_count)
+
+    def state_dict(self) -> dict:
+        names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
+        return dict(step_count=self.step_count, state_bits=self.state_bits,
+                    **{n: getattr(self, n).clone() for n in names if getattr(self, n) is not None})
+
+    def load_state_dict(self, state: dict) -> None:
+        _need(state.get("state_bits") == self.state_bits,
+              f"the state has {state.get('state_bits')} bits, this optimizer {self.state_bits}")
+        self.load_state(state["step_count"], state["exp_avg"], state["exp_avg_sq"], state.get("exp_avg_scale"),
+                        state.get("exp_avg_sq_scale"))
+
+
+# ---------------------------------------------------------------------------------------------
+# 8-bit floating point
+
+
+class Fp8Blocks(NamedTuple):
+    """A matrix [rows, K] as e4m3 codes with one scale ``2**(scales - 127)`` per row and 128 columns:
+    ``codes`` [rows, 128 ceil(K / 128)] float8_e4m3fn (zeros past K), ``scales`` [rows, 4 ceil(K / 512)]
+    uint8 (127 past the last block)."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    K: int
+
+
+def _fp8_pitches(K: int) -> Tuple[int, int]:
+    return -(-K // 128) * 128, -(-K // 512) * 4
+
+
+def _check_blocks(name: str, b: Fp8Blocks, device: torch.device) -> int:
+    _need(isinstance(b, Fp8Blocks), f"{name} must be Fp8Blocks (quantize_fp8)")
+    _need(b.K > 0 and b.codes.dim() == 2, f"{name} must be a matrix")
+    kp, sp = _fp8_pitches(b.K)
+    rows = b.codes.shape[0]
+    _need(b.codes.dtype == torch.float8_e4m3fn and b.codes.shape[1] == kp and b.codes.is_contiguous(),
+          f"{name}.codes must be a contiguous [{rows}, {kp}] float8_e4m3fn")
+    _need(b.scales.dtype == torch.uint8 and tuple(b.scales.shape) == (rows, sp) and b.scales.is_contiguous(),
+          f"{name}.scales must be a contiguous [{rows}, {sp}] uint8")
+    _need(b.codes.device == device and b.scales.device == device, f"{name} must be on {device}")
+    return rows
+
+
+def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
+    """``x`` [rows, K] in 8-bit floating point: each row's 128 columns share the least power of two under
+    which their largest value is at most 448.  A value that is not finite becomes NaN."""
+    code = _dtype("x", x)
+    _on(x.device)
+    _need(x.dim() == 2 and x.shape[1] > 0, f"x must be [rows, K], got {tuple(x.shape)}")
+    rows, K = x.shape
+    xr, ld = _rows(x)
+    kp, sp = _fp8_pitches(K)
+    codes = torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((rows, sp), dtype=torch.uint8, device=x.device)
+    _call(x.device, "trident_fp8_quantize", xr.data_ptr(), code, rows, K, ld, codes.data_ptr(), scales.data_ptr())
+    return Fp8Blocks(codes, scales, K)
+
+
+def _bias(bias, N, dtype, device) -> int:
+    if bias is None:
+        return _DTYPES[dtype]
+    _need(bias.dim() == 1 and bias.shape[0] == N and bias.is_contiguous(), f"bias must be a contiguous [{N}]")
+    _need(bias.dtype in (dtype, torch.float32), f"bias must be {dtype} or float32, got {bias.dtype}")
+    _need(bias.device == device, f"bias must be on {device}")
+    return _DTYPES[bias.dtype]
+
+
+def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
+               out_dtype: torch.dtype = torch.bfloat16, fast_accum: bool = False) -> torch.Tensor:
+    """``a @ b.T + bias``: [M, N] from [M, K] and [N, K], summed in float32.
+
+    ``fast_accum`` takes the 8-bit matrix instruction, which is twice as fast and keeps 13 bits below the
+    largest of each 8 products: the sums are off by up to about 5e-5 of their size, which a bfloat16
+    result does not show."""
+    _need(isinstance(a, Fp8Blocks), "a must be Fp8Blocks (quantize_fp8)")
+    device = a.codes.device
+    _on(device)
+    M, N = _check_blocks("a", a, device), _check_blocks("b", b, device)
+    _need(a.K == b.K, f"a has {a.K} columns, b {b.K}")
+    _need(out_dtype in _DTYPES, f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    bcode = _bias(bias, N, out_dtype, device)
+    out = torch.empty((M, N), dtype=out_dtype, device=device)
+    _call(device, "trident_fp8_matmul", a.codes.data_ptr(), a.scales.data_ptr(), M, b.codes.data_ptr(),
+          b.scales.data_ptr(), N, a.K, ext._ptr(bias), bcode, out.data_ptr(), _DTYPES[out_dtype], max(N, 1), int(fast_accum))
+    return out
+
+
+def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] = None,
+               fast_accum: bool = False) -> torch.Tensor:
+    """``x @ weight.T + bias`` for ``x`` [..., K], quantised in the call, in x's type: the projection of a
+    query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``."""
+    code = _dtype("x", x)
+    device = x.device
+    _on(device)
+    N = _check_blocks("weight", weight, device)
+    K = weight.K
+    _need(x.dim() >= 1 and x.shape[-1] == K, f"x must be [..., {K}], got {tuple(x.shape)}")
+    M = x.numel() // K
+    bcode = _bias(bias, N, x.dtype, device)
+    xr, ld = _rows(x)
+    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=device)
+    nbytes = _lib.lib().trident_fp8_linear_workspace_bytes(M, K)
+    _call_ws(device, "trident_fp8_linear", nbytes, xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(),
+             weight.scales.data_ptr(), N, ext._ptr(bias), bcode, out.data_ptr(), max(N, 1), int(fast_accum))
+    return out
