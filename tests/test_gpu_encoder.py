@@ -127,6 +127,27 @@ def test_embedding_grad_long_rows(dev, counts):
         check_embedding_grad(randn(g, ids.numel(), D), ids, len(counts))
 
 
+@pytest.mark.parametrize("counts", [[8], [9], [7, 8, 9], [8] * 20, [1, 15, 16, 17, 1, 31, 32, 33, 1], [3, 5] * 40,
+                                    [100, 1, 1, 100], [0, 0, 9, 0]])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embedding_grad_rows_across_chunks(dev, dtype, counts):
+    """Rows that end at, before and past the ends of the parts that the ordered tokens are cut into."""
+    g = gen(sum(counts))
+    ids = torch.repeat_interleave(torch.arange(len(counts), device=dev), torch.tensor(counts, device=dev))
+    ids = ids[torch.randperm(ids.numel(), generator=g, device=dev)]
+    for D in (5, 40, 700):
+        check_embedding_grad(randn(g, ids.numel(), D, dtype=dtype), ids, len(counts), scale=2.0)
+
+
+@pytest.mark.parametrize("n,V,D", [(8192, 3000, 40), (8193, 3000, 40), (20_000, 513, 1000), (40_000, 70_000, 900),
+                                   (40_000, 2, 300), (30_000, 1, 17), (9000, 200_000, 24)])
+@pytest.mark.parametrize("wide", [True, False])
+def test_embedding_grad_many_tokens(dev, n, V, D, wide):
+    """Past the sizes at which the ordering and the parts change; ids with most of all tokens."""
+    g = gen(n + V)
+    check_embedding_grad(randn(g, n, D, dtype=torch.bfloat16), token_ids(g, n, V, wide), V, skip=0 if V > 2 else None)
+
+
 def test_embedding_grad_without_tokens(dev):
     out = encoder.embedding_grad(torch.empty((0, 20), device=dev), torch.empty(0, dtype=torch.int64, device=dev), 300)
     assert out.shape == (300, 20) and (out == 0).all()

@@ -111,7 +111,7 @@ EXPORTS = {
     "trident_layer_norm_grad_workspace_bytes": (_size, [_i64, _i64]),
     "trident_layer_norm_grad": (ctypes.c_int, [_P, _i64, _P, _i64, _i32, _i64, _i64, _P, _i32, _P, _P, _P, _i64, _P,
                                                _P, _P, _size, _P]),
-    "trident_adamw": (ctypes.c_int, [ctypes.POINTER(TridentAdamTensor), _i32, ctypes.POINTER(TridentAdamState),
+    "trident_adamw": (ctypes.c_int, [_P, _i32, ctypes.POINTER(TridentAdamState),
                                      ctypes.POINTER(TridentAdamParams), _P]),
     "trident_adamw_state_values": (ctypes.c_int, [ctypes.POINTER(TridentAdamState), _P, _P, _P]),
     "trident_fp8_quantize": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _P]),

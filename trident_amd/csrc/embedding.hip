@@ -66,190 +66,200 @@ __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
 // ---------------------------------------------------------------------------------------------
 // gradient
 
-constexpr int kSortBlock = 1024;
-constexpr int kSortWaves = kSortBlock / kWave;
-constexpr int kSortAhead = 8;   // groups of 64 ids a wave loads at once
-constexpr int kMaxOwned = 512;  // ids a sorting workgroup owns at most (32 KB of counters)
-constexpr int kChunk = 64;      // tokens of a part of a long row; longer rows are split
+constexpr int kMaxOwned = 512;  // ids of one sorting workgroup at most
 
-// Orders the tokens by id.  A workgroup owns `w` consecutive ids and reads all n ids twice: first it
-// counts the tokens of smaller ids and, per wave, those of each id it owns (each wave takes a
-// contiguous part of the tokens), which gives every (id, wave) its first place; then it places its
-// tokens in order.  row_off[v] .. row_off[v + 1] are the places of id v in pos.  One launch, no
-// workgroup waits for another.
-template <typename ID>
-__global__ __launch_bounds__(kSortBlock) void sort_ids_kernel(const ID* __restrict__ ids, int n, int V, int w,
-                                                              int64_t skip, int* __restrict__ row_off,
-                                                              int* __restrict__ pos) {
-    extern __shared__ int hist[];  // [kSortWaves][w]
-    __shared__ int s_sum[kSortWaves];
+struct RowInfo {
+    int beg, count;  // a row's places among the ordered tokens
+};
+
+struct Token {
+    int t, row;
+};
+
+// Ids of one sorting workgroup and what of them each of its waves keeps in LDS.
+template <int WAVES>
+struct SortShape {
+    static constexpr int kAheadIds = 16;                    // groups of 64 ids a wave loads at once
+    static constexpr int kList = WAVES == 4 ? 2048 : 1024;  // tokens a wave keeps in LDS
+    static constexpr size_t lds(int w) {
+        return (size_t)WAVES * w * sizeof(int) + (size_t)WAVES * kList * (sizeof(int) + sizeof(uint16_t));
+    }
+};
+constexpr int kSmallTokens = 4 * 2048;  // four waves keep all of them
+
+struct SortArgs {
+    const void* ids;
+    int n, V, owned, shift, chunk;
+    uint32_t skip;     // an id without a gradient; 2^32 - 1: none
+    RowInfo* row;      // [V + 1]
+    Token* token;      // [n]
+    int* long_count;   // [2^shift]
+    int* long_rows;    // [2^shift, owned]
+};
+
+// An id's low half if it is a row's that takes part, else 2^32 - 1.
+__device__ __forceinline__ uint32_t row_id(const int64_t* ids, int t, uint32_t V, uint32_t skip) {
+    const uint2 id = reinterpret_cast<const uint2*>(ids)[t];
+    return id.y == 0 && id.x < V && id.x != skip ? id.x : ~0u;
+}
+__device__ __forceinline__ uint32_t row_id(const int32_t* ids, int t, uint32_t V, uint32_t skip) {
+    const uint32_t id = (uint32_t)ids[t];
+    return id < V && id != skip ? id : ~0u;
+}
+
+// Orders the tokens by id: row[v] says where in `token` the tokens of id v lie, in their own order;
+// row[V] holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power of two): the
+// most frequent ids of a vocabulary are neighbours, so a range of them would be one workgroup's work.
+// Each wave reads a contiguous part of the ids, keeps the tokens its workgroup owns in a list in LDS,
+// and counts them by id and those of lower workgroups; the counts give every (id, wave) its first
+// place, and the lists are placed in order.  A wave whose list overflows (an id with a large share of
+// many tokens) reads its part again instead.  One launch, and no workgroup waits for another; the price
+// is that every one reads all ids.
+template <typename ID, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
+    using Shape = SortShape<WAVES>;
+    constexpr int A = Shape::kAheadIds, kList = Shape::kList;
+    extern __shared__ int lds[];
+    __shared__ int s_sum[WAVES], s_long;
+    const int w = a.owned, n = a.n;
+    int* hist = lds;                // [WAVES][w]
+    int* list = lds + WAVES * w;    // [WAVES][kList]
+    uint16_t* list_id = reinterpret_cast<uint16_t*>(list + WAVES * kList);
+    const ID* ids = static_cast<const ID*>(a.ids);
     const int lane = lane_id(), wave = threadIdx.x / kWave;
-    const int lo = blockIdx.x * w, owned = min(w, V - lo);
-    const int seg = (n + kSortBlock - 1) / kSortBlock * kWave;
+    const uint32_t b = blockIdx.x, mask = (1u << a.shift) - 1;
+    const int seg = (n + WAVES * kWave - 1) / (WAVES * kWave) * kWave;
     const int beg = (int)min((int64_t)n, (int64_t)wave * seg), end = (int)min((int64_t)n, (int64_t)beg + seg);
-    for (int i = threadIdx.x; i < kSortWaves * w; i += kSortBlock) hist[i] = 0;
+    for (int i = threadIdx.x; i < WAVES * w; i += WAVES * kWave) hist[i] = 0;
+    if (threadIdx.x == 0) s_long = 0;
     __syncthreads();
     int* mine = hist + wave * w;
-    int lower = 0;
-    for (int t0 = beg; t0 < end; t0 += kWave * kSortAhead) {
-        int64_t id[kSortAhead];
+    int* kept = list + wave * kList;
+    uint16_t* kept_id = list_id + wave * kList;
+    int lower = 0, found = 0;
+    for (int t0 = beg; t0 < end; t0 += kWave * A) {
+        uint32_t id[A];
+        if (t0 + kWave * A <= end) {
 #pragma unroll
-        for (int u = 0; u < kSortAhead; ++u) {
-            const int t = t0 + u * kWave + lane;
-            id[u] = t < end ? (int64_t)ids[t] : -1;
+            for (int u = 0; u < A; ++u) id[u] = row_id(ids, t0 + u * kWave + lane, (uint32_t)a.V, a.skip);
+        } else {
+#pragma unroll
+            for (int u = 0; u < A; ++u) {
+                const int t = t0 + u * kWave + lane;
+                id[u] = t < end ? row_id(ids, t, (uint32_t)a.V, a.skip) : ~0u;
+            }
         }
 #pragma unroll
-        for (int u = 0; u < kSortAhead; ++u) {
-            if (id[u] < 0 || id[u] == skip) continue;
-            const int64_t rel = id[u] - lo;
-            if (rel < 0) ++lower;
-            else if (rel < owned) atomicAdd(&mine[rel], 1);
+        for (int u = 0; u < A; ++u) {
+            const uint32_t owner = id[u] == ~0u ? ~0u : id[u] & mask;
+            lower += __popcll((unsigned long long)__ballot(owner < b));
+            const uint64_t m = __ballot(owner == b);
+            if (m) {
+                const int at = found + mask_rank(m);
+                if (owner == b) {
+                    const int rel = (int)(id[u] >> a.shift);
+                    atomicAdd(&mine[rel], 1);
+                    if (at < kList) {
+                        kept[at] = t0 + u * kWave + lane;
+                        kept_id[at] = (uint16_t)rel;
+                    }
+                }
+                found += __popcll((unsigned long long)m);
+            }
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) lower += __shfl_xor(lower, o, kWave);
     if (lane == 0) s_sum[wave] = lower;
     __syncthreads();
     int place = 0;
-    for (int i = 0; i < kSortWaves; ++i) place += s_sum[i];
-    __syncthreads();
-    // thread j: the first place of id lo + j
-    const int j = threadIdx.x;
-    int count = 0;
-    if (j < owned)
-        for (int i = 0; i < kSortWaves; ++i) count += hist[i * w + j];
-    int inc = count;
+    for (int i = 0; i < WAVES; ++i) place += s_sum[i];
+    // the first place of each owned id, a workgroup's threads of them at a time
+    for (int j0 = 0; j0 < w; j0 += WAVES * kWave) {
+        const int j = j0 + threadIdx.x;
+        const int64_t v = ((int64_t)j << a.shift) + b;
+        const bool live = j < w && v < a.V;
+        int count = 0;
+        if (live)
+            for (int i = 0; i < WAVES; ++i) count += hist[i * w + j];
+        int inc = count;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const int t = __shfl_up(inc, o, kWave);
-        if (lane >= o) inc += t;
-    }
-    if (lane == kWave - 1) s_sum[wave] = inc;
-    __syncthreads();
-    for (int i = 0; i < wave; ++i) place += s_sum[i];
-    place += inc - count;
-    if (j < owned) {
-        row_off[lo + j] = place;
-        if (lo + j == V - 1) row_off[V] = place + count;
-        for (int i = 0; i < kSortWaves; ++i) {
-            const int c = hist[i * w + j];
-            hist[i * w + j] = place;
-            place += c;
+        for (int o = 1; o < kWave; o <<= 1) {
+            const int t = __shfl_up(inc, o, kWave);
+            if (lane >= o) inc += t;
         }
-    }
-    __syncthreads();
-    for (int t0 = beg; t0 < end; t0 += kWave * kSortAhead) {
-        int rel[kSortAhead];
-#pragma unroll
-        for (int u = 0; u < kSortAhead; ++u) {
-            const int t = t0 + u * kWave + lane;
-            const int64_t id = t < end ? (int64_t)ids[t] : -1;
-            const int64_t r = id - lo;
-            rel[u] = id >= 0 && id != skip && r >= 0 && r < owned ? (int)r : -1;
+        __syncthreads();
+        if (lane == kWave - 1) s_sum[wave] = inc;
+        __syncthreads();
+        int at = place + inc - count;
+        for (int i = 0; i < WAVES; ++i) {
+            if (i < wave) at += s_sum[i];
+            place += s_sum[i];
         }
-#pragma unroll
-        for (int u = 0; u < kSortAhead; ++u) {
-            const int t = t0 + u * kWave + lane;
-            uint64_t left = __ballot(rel[u] >= 0);
-            while (left) {  // one turn per id among these 64 tokens
-                const int first = __ffsll((unsigned long long)left) - 1;
-                const int r = __builtin_amdgcn_readlane(rel[u], first);
-                const uint64_t same = __ballot(rel[u] == r);
-                const int at = mine[r];
-                if (rel[u] == r) pos[at + mask_rank(same)] = t;
-                wave_sync();
-                if (lane == first) mine[r] = at + __popcll((unsigned long long)same);
-                wave_sync();
-                left &= ~same;
+        if (live) {
+            a.row[v] = RowInfo{at, count};
+            if (count > a.chunk) a.long_rows[(int64_t)b * w + atomicAdd(&s_long, 1)] = (int)v;  // in any order
+            for (int i = 0; i < WAVES; ++i) {
+                const int c = hist[i * w + j];
+                hist[i * w + j] = at;
+                at += c;
             }
+        }
+    }
+    if (b == mask && threadIdx.x == 0) a.row[a.V] = RowInfo{place, 0};
+    __syncthreads();
+    if (threadIdx.x == 0) a.long_count[b] = s_long;
+    const auto put = [&](int t, int rel) {  // rel < 0: no token in this lane
+        uint64_t left = __ballot(rel >= 0);
+        while (left) {  // one turn per id among these 64 tokens
+            const int first = __ffsll((unsigned long long)left) - 1;
+            const int r = __builtin_amdgcn_readlane(rel, first);
+            const uint64_t same = __ballot(rel == r);
+            const int at = mine[r];
+            if (rel == r) a.token[at + mask_rank(same)] = Token{t, (int)(((uint32_t)r << a.shift) + b)};
+            wave_sync();
+            if (lane == first) mine[r] = at + __popcll((unsigned long long)same);
+            wave_sync();
+            left &= ~same;
+        }
+    };
+    if (found <= kList) {
+        for (int k = lane; k - lane < found; k += kWave) put(k < found ? kept[k] : 0, k < found ? (int)kept_id[k] : -1);
+    } else {
+        for (int t0 = beg; t0 < end; t0 += kWave) {
+            const int t = t0 + lane;
+            const uint32_t id = t < end ? row_id(ids, t, (uint32_t)a.V, a.skip) : ~0u;
+            put(t, id != ~0u && (id & mask) == b ? (int)(id >> a.shift) : -1);
         }
     }
 }
 
 struct EmbedGradArgs {
-    const void* grad;     // [n, ld]
-    const void* ids;      // [n]
-    const int* row_off;   // [V + 1]
-    const int* pos;       // tokens by id
-    float* part;          // [2 chunks, D]: sums of the parts of long rows
-    void* out;            // [V, ldo]
+    const void* grad;       // [n, ld]
+    const RowInfo* row;     // [V + 1]
+    const Token* token;     // tokens by id
+    float* part;            // [2 chunks, D]: sums of the parts of long rows
+    const int* long_count;  // [owners]: long rows of each sorting workgroup
+    const int* long_rows;   // [owners, owned]
+    void* out;              // [V, ldo]
     int64_t ld, ldo;
-    int V, D, nv;
-    int lanes;            // lanes of a row: a power of two, 64 where a row has more vectors
-    int row_blocks;       // workgroups that take whole rows; the others take chunks
+    int V, D, nv, owned;
+    int lanes;              // lanes of a row: a power of two, 64 where a row has more vectors
+    int chunk;              // tokens of a group of lanes
+    int chunk_blocks;       // workgroups that take tokens; the others clear the rows without any
     float scale;
 };
 
-// Sums the gradient rows of the tokens pos[beg .. end), every `step`-th, into acc; four rows are in
-// flight, added in order.
+constexpr int kClear = 16;  // rows of a wave that clears
+
+// Bound by bytes.  The ordered tokens are cut into chunks, a group of lanes each, every lane the same
+// columns of all of its tokens, kAhead of them in flight.  A row of up to a chunk's tokens belongs to
+// the chunk that it begins in, which sums it to its end and writes it.  A longer row (a frequent token)
+// is summed chunk by chunk into `part`, of which a chunk needs two: for the row it begins in and the
+// row it ends in; join_long_kernel adds a row's parts in order.  So every group has between one and two
+// chunks of work, whatever the frequencies.
 template <typename T, int VEC, int NVL>
-__device__ __forceinline__ void sum_rows(const EmbedGradArgs& a, int beg, int end, int step, const int (&col)[NVL],
-                                         const bool (&on)[NVL], float (&acc)[NVL][VEC]) {
-    const T* g = static_cast<const T*>(a.grad);
-    int k = beg;
-    for (; k + 3 * step < end; k += 4 * step) {
-        float f[4][NVL][VEC];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const T* row = g + (int64_t)a.pos[k + u * step] * a.ld;
-#pragma unroll
-            for (int c = 0; c < NVL; ++c)
-                if (on[c]) load_vec(row + col[c], f[u][c]);
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int c = 0; c < NVL; ++c)
-                if (on[c])
-#pragma unroll
-                    for (int i = 0; i < VEC; ++i) acc[c][i] += f[u][c][i];
-    }
-    for (; k < end; k += step) {
-        const T* row = g + (int64_t)a.pos[k] * a.ld;
-#pragma unroll
-        for (int c = 0; c < NVL; ++c)
-            if (on[c]) {
-                float f[VEC];
-                load_vec(row + col[c], f);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[c][i] += f[i];
-            }
-    }
-}
-
-// The two rows that a chunk of kChunk ordered tokens can hold a part of a long row of: the row of its
-// first token and that of its last.
-template <typename ID>
-struct ChunkRows {
-    int beg, end;       // the chunk's places
-    int row[2], lo[2], hi[2];
-    bool is_long[2];
-    __device__ __forceinline__ bool init(const EmbedGradArgs& a, int chunk) {
-        const int live = a.row_off[a.V];
-        beg = chunk * kChunk;
-        if (beg >= live) return false;
-        end = min(live, beg + kChunk);
-        const ID* ids = static_cast<const ID*>(a.ids);
-        row[0] = (int)ids[a.pos[beg]];
-        row[1] = (int)ids[a.pos[end - 1]];
-        for (int i = 0; i < 2; ++i) {
-            lo[i] = a.row_off[row[i]];
-            hi[i] = a.row_off[row[i] + 1];
-            is_long[i] = hi[i] - lo[i] > kChunk && (i == 0 || row[1] != row[0]);
-        }
-        return is_long[0] || is_long[1];
-    }
-};
-
-// Bound by bytes.  Rows of up to kChunk tokens: a group of lanes per row, each lane the same columns
-// of every token.  Longer rows (frequent tokens): the ordered tokens are cut into chunks of kChunk, a
-// workgroup sums what its chunk holds of long rows into `part` (at most two: the row it begins in and
-// the row it ends in), and join_long_kernel adds a row's parts in order.
-template <typename T, int VEC, int NVL, typename ID>
 __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
-    extern __shared__ float sums[];  // [groups][lanes * NVL * VEC]
-    const int groups = kBlock / a.lanes;
-    const int group = threadIdx.x / a.lanes, l = threadIdx.x % a.lanes;
+    constexpr int kAhead = NVL > 2 ? 4 : 8;
+    const int l = threadIdx.x % a.lanes;
     int col[NVL];
     bool on[NVL];
     float acc[NVL][VEC];
@@ -261,70 +271,108 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
     }
-    if ((int)blockIdx.x < a.row_blocks) {
-        const int row = blockIdx.x * groups + group;
-        if (row >= a.V) return;
-        const int beg = a.row_off[row], end = a.row_off[row + 1];
-        if (end - beg > kChunk) return;
-        sum_rows<T, VEC, NVL>(a, beg, end, 1, col, on, acc);
-        T* out = static_cast<T*>(a.out) + (int64_t)row * a.ldo;
+    T* out = static_cast<T*>(a.out);
+    if ((int)blockIdx.x >= a.chunk_blocks) {
+        const int per = kClear * (kWave / a.lanes);  // of this wave's rows, its groups take turns
+        const int64_t r0 = ((int64_t)(blockIdx.x - a.chunk_blocks) * kWavesPerBlock + threadIdx.x / kWave) * per;
+        for (int i = lane_id() / a.lanes; i < per && r0 + i < a.V; i += kWave / a.lanes) {
+            if (a.row[r0 + i].count) continue;
 #pragma unroll
-        for (int c = 0; c < NVL; ++c)
-            if (on[c]) {
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) acc[c][i] *= a.scale;
-                store_vec(out + col[c], acc[c]);
-            }
+            for (int c = 0; c < NVL; ++c)
+                if (on[c]) store_vec(out + (r0 + i) * a.ldo + col[c], acc[c]);
+        }
         return;
     }
-    const int chunk = blockIdx.x - a.row_blocks;
-    ChunkRows<ID> rows;
-    if (!rows.init(a, chunk)) return;
-    for (int i = 0; i < 2; ++i) {
-        if (!rows.is_long[i]) continue;  // the same in every lane
-        const int beg = max(rows.beg, rows.lo[i]), end = min(rows.end, rows.hi[i]);
+    const int chunk = blockIdx.x * (kBlock / a.lanes) + threadIdx.x / a.lanes;
+    const int live = a.row[a.V].beg;
+    const int64_t first = (int64_t)chunk * a.chunk;
+    if (first >= live) return;
+    int beg = (int)first, end = min(live, beg + a.chunk);
+    const int row0 = a.token[beg].row, row1 = a.token[end - 1].row;
+    const RowInfo i0 = a.row[row0], i1 = a.row[row1];
+    const bool long0 = i0.count > a.chunk, long1 = i1.count > a.chunk;
+    if (!long0 && i0.beg < beg) beg = i0.beg + i0.count;  // the chunk before has it
+    if (!long1) end = i1.beg + i1.count;
+    if (beg >= end) return;
+    const T* g = static_cast<const T*>(a.grad);
+    const auto flush = [&](int row) {
+        const bool is0 = long0 && row == row0, is1 = long1 && row == row1;
+        float* part = a.part + (int64_t)(2 * chunk + (is0 ? 0 : 1)) * a.D;
 #pragma unroll
-        for (int c = 0; c < NVL; ++c)
+        for (int c = 0; c < NVL; ++c) {
+            if (on[c]) {
+                if (is0 || is1) {
+                    __builtin_memcpy(part + col[c], acc[c], sizeof(acc[c]));
+                } else {
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) acc[c][e] = 0.0f;
-        sum_rows<T, VEC, NVL>(a, beg + group, end, groups, col, on, acc);
-        __syncthreads();
+                    for (int i = 0; i < VEC; ++i) acc[c][i] *= a.scale;
+                    store_vec(out + (int64_t)row * a.ldo + col[c], acc[c]);
+                }
+            }
 #pragma unroll
-        for (int c = 0; c < NVL; ++c)
+            for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
+        }
+    };
+    Token next[kAhead];
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) sums[(c * VEC + e) * kBlock + threadIdx.x] = acc[c][e];
-        __syncthreads();
-        if (group == 0) {
+    for (int u = 0; u < kAhead; ++u) next[u] = beg + u < end ? a.token[beg + u] : Token{-1, -1};
+    int row = next[0].row;
+    for (int k = beg; k < end; k += kAhead) {
+        Vec<T, VEC> f[kAhead][NVL];
+        Token now[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            now[u] = next[u];
+            if (now[u].t >= 0)
+#pragma unroll
+                for (int c = 0; c < NVL; ++c)
+                    if (on[c]) f[u][c].load(g + (int64_t)now[u].t * a.ld + col[c]);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            next[u] = k + kAhead + u < end ? a.token[k + kAhead + u] : Token{-1, -1};
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            if (now[u].t < 0) break;
+            if (now[u].row != row) {
+                flush(row);
+                row = now[u].row;
+            }
 #pragma unroll
             for (int c = 0; c < NVL; ++c) {
-                if (!on[c]) continue;
+                float x[VEC];
+                f[u][c].get(x);
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) {
-                    float s = 0.0f;
-                    for (int g = 0; g < groups; ++g) s += sums[(c * VEC + e) * kBlock + g * a.lanes + l];
-                    a.part[(int64_t)(2 * chunk + i) * a.D + col[c] + e] = s;
-                }
+                for (int i = 0; i < VEC; ++i) acc[c][i] += x[i];
             }
         }
     }
+    flush(row);
 }
 
-// Adds the parts of the long row that begins in this chunk (at most one does: a long row reaches into
-// the next chunk).
-template <typename T, typename ID>
+// Adds the parts of the long rows, those of one sorting workgroup's ids here: 64 columns a workgroup,
+// each of its waves a quarter of a row's parts, then the waves' sums in order.
+template <typename T>
 __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
-    ChunkRows<ID> rows;
-    const int chunk = blockIdx.x;
-    if (!rows.init(a, chunk)) return;
-    for (int i = 0; i < 2; ++i) {
-        if (!rows.is_long[i] || rows.lo[i] < rows.beg) continue;
-        const int last = (rows.hi[i] - 1) / kChunk;
-        T* out = static_cast<T*>(a.out) + (int64_t)rows.row[i] * a.ldo;
-        for (int d = blockIdx.y * kBlock + threadIdx.x; d < a.D; d += gridDim.y * kBlock) {
-            float s = a.part[(int64_t)(2 * chunk + i) * a.D + d];
-#pragma unroll 8
-            for (int c = chunk + 1; c <= last; ++c) s += a.part[(int64_t)(2 * c) * a.D + d];
-            out[d] = (T)(s * a.scale);
+    __shared__ float s_sum[kWavesPerBlock][kWave];
+    const int lane = lane_id(), wave = threadIdx.x / kWave, d = blockIdx.y * kWave + lane;
+    const int count = a.long_count[blockIdx.x];
+    for (int i = 0; i < count; ++i) {
+        const int v = a.long_rows[(int64_t)blockIdx.x * a.owned + i];
+        const RowInfo r = a.row[v];
+        const int first = r.beg / a.chunk, parts = (r.beg + r.count - 1) / a.chunk - first + 1;
+        const int per = (parts + kWavesPerBlock - 1) / kWavesPerBlock;
+        const float* part = a.part + min(d, a.D - 1);
+        float s = 0.0f;
+#pragma unroll 16
+        for (int c = wave * per; c < min(parts, (wave + 1) * per); ++c)  // in its first chunk a row is the last one,
+            s += part[(int64_t)(2 * (first + c) + (c == 0 && r.beg % a.chunk)) * a.D];  // unless it begins the chunk
+        __syncthreads();
+        s_sum[wave][lane] = s;
+        __syncthreads();
+        if (wave == 0 && d < a.D) {
+            for (int k = 1; k < kWavesPerBlock; ++k) s += s_sum[k][lane];
+            static_cast<T*>(a.out)[(int64_t)v * a.ldo + d] = (T)(s * a.scale);
         }
     }
 }
@@ -336,9 +384,12 @@ void with_ids(int32_t ids64, F&& f) {
 }
 
 struct GradSpace {
-    int* row_off;
-    int* pos;
+    RowInfo* row;
+    Token* token;
     float* part;
+    int *long_count, *long_rows;
+    int shift, owned;  // sorting workgroups: 2^shift, of `owned` ids each
+    int64_t chunk, chunks;
     size_t bytes;
 };
 
@@ -346,17 +397,45 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 GradSpace grad_space(void* base, int64_t n, int64_t V, int64_t D) {
     GradSpace s;
-    const size_t chunks = (size_t)((n + kChunk - 1) / kChunk);
-    const size_t off = up256((size_t)(V + 1) * 4), pos = up256((size_t)n * 4);
+    // Chunks as long as leave about 2,000 waves (8 on each CU): the parts of long rows cost a write and
+    // a read of four bytes a column each.
+    s.chunk = n * D <= (16 << 20) ? 8 : n * D <= (32 << 20) ? 16 : 32;
+    s.chunks = (n + s.chunk - 1) / s.chunk;
+    // Sorting workgroups: few tokens, one a CU, since the counting of its ids is most of its time; many
+    // tokens, as few as their ids allow, since each reads all of them.
+    s.shift = n <= kSmallTokens ? 8 : 6;
+    while (((int64_t)kMaxOwned << s.shift) < V) ++s.shift;
+    s.owned = (int)((V + ((int64_t)1 << s.shift) - 1) >> s.shift);
     char* p = static_cast<char*>(base);
-    s.row_off = reinterpret_cast<int*>(p);
-    s.pos = reinterpret_cast<int*>(p + off);
-    s.part = reinterpret_cast<float*>(p + off + pos);
-    s.bytes = off + pos + up256(2 * chunks * (size_t)D * 4);
+    size_t off = 0;
+    const auto take = [&](size_t bytes) {
+        char* at = p ? p + off : nullptr;
+        off += up256(bytes);
+        return at;
+    };
+    s.row = reinterpret_cast<RowInfo*>(take((size_t)(V + 1) * sizeof(RowInfo)));
+    s.token = reinterpret_cast<Token*>(take((size_t)n * sizeof(Token)));
+    s.part = reinterpret_cast<float*>(take(2 * (size_t)s.chunks * (size_t)D * sizeof(float)));
+    s.long_count = reinterpret_cast<int*>(take(sizeof(int) << s.shift));
+    s.long_rows = reinterpret_cast<int*>(take(((size_t)s.owned << s.shift) * sizeof(int)));
+    s.bytes = off;
     return s;
 }
 
-constexpr int64_t kMaxCount = 0x7fffffff - 4 * kSortBlock;  // tokens, rows and columns count in 32 bits
+template <typename ID, int WAVES>
+int sort_ids(const SortArgs& a, hipStream_t st) {
+    const size_t lds = SortShape<WAVES>::lds(a.owned);
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_ids_kernel<ID, WAVES>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess)
+            return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(sort_ids): %s", hipGetErrorString(e));
+    }
+    sort_ids_kernel<ID, WAVES><<<1u << a.shift, WAVES * kWave, lds, st>>>(a);
+    return capi_check_launch("sort_ids_kernel");
+}
+
+constexpr int64_t kMaxCount = 0x7fffffff - 4096;  // tokens, rows and columns count in 32 bits
 
 }  // namespace
 }  // namespace trident
@@ -409,6 +488,8 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
                          (long long)V, (long long)D, (long long)n, (long long)ld_grad, (long long)ld_out);
     if (!out || (n > 0 && (!grad || !ids)))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "embedding_grad: NULL pointer");
+    if (D > 65535 * (int64_t)kWave)
+        return capi_fail(TRIDENT_ERR_UNSUPPORTED, "embedding_grad: D=%lld is too large", (long long)D);
     const GradSpace s = grad_space(workspace, n, V, D);
     if (!workspace || workspace_bytes < s.bytes)
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "embedding_grad: workspace %zu < %zu bytes", workspace_bytes,
@@ -417,40 +498,34 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
     int rc = TRIDENT_OK;
     with_ids(ids64, [&](auto i) {
         using ID = decltype(i);
-        // one workgroup per CU where the ids they own allow it
-        const int w = (int)std::min<int64_t>(kMaxOwned, (V + 255) / 256);
-        sort_ids_kernel<ID><<<(unsigned)((V + w - 1) / w), kSortBlock, sizeof(int) * kSortWaves * w, st>>>(
-            static_cast<const ID*>(ids), (int)n, (int)V, w, padding_idx, s.row_off, s.pos);
-        if ((rc = capi_check_launch("sort_ids_kernel"))) return;
-        with_dtype(dtype, [&](auto t) {
-            using T = decltype(t);
-            EmbedGradArgs a{grad, ids, s.row_off, s.pos, s.part, out, ld_grad, ld_out, (int)V, (int)D, 0, 0, 0,
-                            (float)scale};
-            const int vec = D >= kVec<T> ? kVec<T> : 1;
-            a.nv = (int)((D + vec - 1) / vec);
-            a.lanes = 1;
-            while (a.lanes < a.nv && a.lanes < kWave) a.lanes *= 2;
-            const int nvl = std::min(4, (a.nv + kWave - 1) / kWave);
-            const int groups = kBlock / a.lanes;
-            a.row_blocks = (int)((V + groups - 1) / groups);
-            const int64_t chunks = (n + kChunk - 1) / kChunk;
-            const unsigned tiles = (unsigned)((a.nv + nvl * a.lanes - 1) / (nvl * a.lanes));
-            if (tiles > 65535) {
-                rc = capi_fail(TRIDENT_ERR_UNSUPPORTED, "embedding_grad: D=%lld is too large", (long long)D);
-                return;
-            }
-            const dim3 grid((unsigned)(a.row_blocks + chunks), tiles);
-            const size_t lds = (size_t)kBlock * nvl * vec * sizeof(float);
-            if (vec == 1) embed_grad_kernel<T, 1, 1, ID><<<grid, kBlock, lds, st>>>(a);
-            else if (nvl == 1) embed_grad_kernel<T, kVec<T>, 1, ID><<<grid, kBlock, lds, st>>>(a);
-            else if (nvl == 2) embed_grad_kernel<T, kVec<T>, 2, ID><<<grid, kBlock, lds, st>>>(a);
-            else if (nvl == 3) embed_grad_kernel<T, kVec<T>, 3, ID><<<grid, kBlock, lds, st>>>(a);
-            else embed_grad_kernel<T, kVec<T>, 4, ID><<<grid, kBlock, lds, st>>>(a);
-            if ((rc = capi_check_launch("embed_grad_kernel")) || n <= kChunk) return;
-            const dim3 join((unsigned)chunks, (unsigned)std::min<int64_t>(64, (D + kBlock - 1) / kBlock));
-            join_long_kernel<T, ID><<<join, kBlock, 0, st>>>(a);
-            rc = capi_check_launch("join_long_kernel");
-        });
+        const SortArgs order{ids, (int)n, (int)V, s.owned, s.shift, (int)s.chunk,
+                             padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : ~0u, s.row, s.token,
+                             s.long_count, s.long_rows};
+        rc = n <= kSmallTokens ? sort_ids<ID, 4>(order, st) : sort_ids<ID, 16>(order, st);
+    });
+    if (rc) return rc;
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        EmbedGradArgs a{grad,   s.row,  s.token, s.part, s.long_count, s.long_rows, out, ld_grad,
+                        ld_out, (int)V, (int)D,  0,      s.owned,      0,           (int)s.chunk, 0, (float)scale};
+        const int vec = D >= kVec<T> ? kVec<T> : 1;
+        a.nv = (int)((D + vec - 1) / vec);
+        a.lanes = 1;
+        while (a.lanes < a.nv && a.lanes < kWave) a.lanes *= 2;
+        const int nvl = std::min(4, (a.nv + kWave - 1) / kWave);
+        const int groups = kBlock / a.lanes;
+        const int64_t clear = kClear * (int64_t)groups;
+        a.chunk_blocks = (int)((s.chunks + groups - 1) / groups);
+        const dim3 grid((unsigned)(a.chunk_blocks + (V + clear - 1) / clear),
+                        (unsigned)((a.nv + nvl * a.lanes - 1) / (nvl * a.lanes)));
+        if (vec == 1) embed_grad_kernel<T, 1, 1><<<grid, kBlock, 0, st>>>(a);
+        else if (nvl == 1) embed_grad_kernel<T, kVec<T>, 1><<<grid, kBlock, 0, st>>>(a);
+        else if (nvl == 2) embed_grad_kernel<T, kVec<T>, 2><<<grid, kBlock, 0, st>>>(a);
+        else if (nvl == 3) embed_grad_kernel<T, kVec<T>, 3><<<grid, kBlock, 0, st>>>(a);
+        else embed_grad_kernel<T, kVec<T>, 4><<<grid, kBlock, 0, st>>>(a);
+        if ((rc = capi_check_launch("embed_grad_kernel")) || n <= s.chunk) return;
+        join_long_kernel<T><<<dim3(1u << s.shift, (unsigned)((D + kWave - 1) / kWave)), kBlock, 0, st>>>(a);
+        rc = capi_check_launch("join_long_kernel");
     });
     return rc;
 }

@@ -37,35 +37,53 @@ inline void with_dtype(int32_t t, F&& f) {
     else f(bf16_t{});
 }
 
-// N elements from any element's address: one element, or whole 16-byte accesses.
+// N elements from any element's address, held as they are stored: one element, or whole 16-byte
+// accesses.
 template <typename T, int N>
-__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[N]) {
-    if constexpr (N == 1) {
-        f[0] = (float)p[0];
-    } else {
-        constexpr int V = kVec<T>;
-        static_assert(N % V == 0, "whole 16-byte accesses");
+struct Vec {
+    static constexpr int kWords = N == 1 ? 1 : N / kVec<T>;
+    u32x4 raw[kWords];
+    T one;
+    __device__ __forceinline__ void load(const T* __restrict__ p) {
+        if constexpr (N == 1) {
+            one = *p;
+        } else {
+            static_assert(N % kVec<T> == 0, "whole 16-byte accesses");
 #pragma unroll
-        for (int k = 0; k < N; k += V) {
-            u32x4 v;
-            __builtin_memcpy(&v, p + k, 16);
-            if constexpr (sizeof(T) == 4) {
+            for (int k = 0; k < kWords; ++k) __builtin_memcpy(&raw[k], p + k * kVec<T>, 16);
+        }
+    }
+    __device__ __forceinline__ void get(float (&f)[N]) const {
+        if constexpr (N == 1) {
+            f[0] = (float)one;
+        } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) f[k + i] = __uint_as_float(v[i]);
-            } else if constexpr (std::is_same<T, bf16_t>::value) {
+            for (int k = 0; k < kWords; ++k) {
+                if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    f[k + 2 * i] = __uint_as_float(v[i] << 16);
-                    f[k + 2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u);
+                    for (int i = 0; i < 4; ++i) f[4 * k + i] = __uint_as_float(raw[k][i]);
+                } else if constexpr (std::is_same<T, bf16_t>::value) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        f[8 * k + 2 * i] = __uint_as_float(raw[k][i] << 16);
+                        f[8 * k + 2 * i + 1] = __uint_as_float(raw[k][i] & 0xffff0000u);
+                    }
+                } else {
+                    typedef f16_t h8 __attribute__((ext_vector_type(8)));
+                    const h8 h = __builtin_bit_cast(h8, raw[k]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) f[8 * k + i] = (float)h[i];
                 }
-            } else {
-                typedef f16_t h8 __attribute__((ext_vector_type(8)));
-                const h8 h = __builtin_bit_cast(h8, v);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) f[k + i] = (float)h[i];
             }
         }
     }
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void load_vec(const T* __restrict__ p, float (&f)[N]) {
+    Vec<T, N> v;
+    v.load(p);
+    v.get(f);
 }
 
 template <typename T, int N>

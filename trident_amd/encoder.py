@@ -25,19 +25,38 @@ from . import _lib, ext
 from .ext import _need
 
 _DTYPES = {torch.float32: _lib.F32, torch.float16: _lib.F16, torch.bfloat16: _lib.BF16}
+_ID_TYPES = {torch.int32: 0, torch.int64: 1}
 STATE_BLOCK = 256  # elements of an 8-bit state that share a scale
+
+# A call on one query takes a few microseconds on the GPU, so the path to the library is kept short: the
+# conditions are plain expressions, and messages are only made for a call that is refused.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_fns = {}
+
+
+def _refuse(message: str) -> None:
+    raise _lib.TridentError(message)
 
 
 def _dtype(name: str, t: torch.Tensor) -> int:
     code = _DTYPES.get(t.dtype)
-    _need(code is not None, f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    if code is None:
+        _refuse(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
     return code
 
 
-def _on(device: torch.device, **tensors) -> None:
-    _need(device.type == "cuda", "the encoder's operators need device tensors")
-    for name, t in tensors.items():
-        _need(t is None or t.device == device, f"{name} must be on {device}, got {t.device if t is not None else None}")
+def _gpu(name: str, t: torch.Tensor) -> int:
+    """The index of the GPU that holds ``t``."""
+    index = t.get_device()
+    if index < 0:
+        _refuse(f"{name} must be a device tensor, got one on {t.device}")
+    return index
+
+
+def _same(index: int, name: str, t: Optional[torch.Tensor]) -> None:
+    if t is not None and t.get_device() != index:
+        _refuse(f"{name} must be on cuda:{index}, got {t.device}")
 
 
 def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -54,46 +73,57 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, max(D, 1)
 
 
-def _call(device: torch.device, name: str, *args) -> None:
-    fn = getattr(_lib.lib(), name)
-    if device.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
+def _fn(name: str):
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_lib.lib(), name)
+    return fn
+
+
+def _call(index: int, name: str, *args) -> None:
+    if index == _current_device():
+        rc = _fn(name)(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream(device).cuda_stream)
-    _lib.check(rc, name)
+        with torch.cuda.device(index):
+            rc = _fn(name)(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
 
 
-def _call_ws(device: torch.device, name: str, nbytes: int, *args) -> None:
+def _call_ws(device: torch.device, index: int, name: str, nbytes: int, *args) -> None:
     """_call with this stream's workspace of at least ``nbytes`` as the last two arguments."""
-    st = torch.cuda.current_stream(device)
-    slot = ext._workspace_slot(device, st)
+    slot = ext._ws_cache.get((device, _raw_stream(index)))
+    if slot is None:
+        slot = ext._workspace_slot(device, torch.cuda.current_stream(device))
     with slot.lock:
-        ws = ext._grow(slot, device, nbytes, st)
-        _call(device, name, *args, ws.data_ptr(), ws.numel())
+        ws = slot.buf
+        if ws is None or ws.numel() < nbytes:
+            ws = ext._grow(slot, device, nbytes, torch.cuda.current_stream(device))
+        _call(index, name, *args, ws.data_ptr(), ws.numel())
 
 
 # ---------------------------------------------------------------------------------------------
 # embedding
 
 
-def _ids(ids: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    _need(ids.dtype in (torch.int64, torch.int32), f"ids must be int64 or int32, got {ids.dtype}")
-    return (ids if ids.is_contiguous() else ids.contiguous()), int(ids.dtype == torch.int64)
+def _ids(index: int, ids: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    wide = _ID_TYPES.get(ids.dtype)
+    if wide is None:
+        _refuse(f"ids must be int64 or int32, got {ids.dtype}")
+    _same(index, "ids", ids)
+    return (ids if ids.is_contiguous() else ids.contiguous()), wide
 
 
 def _embed(ids, weight, scale):
-    _need(weight.dim() == 2 and weight.shape[0] > 0 and weight.shape[1] > 0,
-          f"weight must be [V, D], got {tuple(weight.shape)}")
-    code = _dtype("weight", weight)
-    _on(weight.device, ids=ids)
-    _need(weight.device.type == "cuda", "weight must be a device tensor")
-    idc, wide = _ids(ids)
+    if weight.dim() != 2 or weight.numel() == 0:
+        _refuse(f"weight must be [V, D], got {tuple(weight.shape)}")
+    code, index = _dtype("weight", weight), _gpu("weight", weight)
+    idc, wide = _ids(index, ids)
     V, D = weight.shape
     w, ld = _rows(weight)
-    out = torch.empty((*ids.shape, D), dtype=weight.dtype, device=weight.device)
-    _call(weight.device, "trident_embedding", w.data_ptr(), code, V, D, ld, idc.data_ptr(), wide, idc.numel(),
-          float(scale), out.data_ptr(), D)
+    out = weight.new_empty((*ids.shape, D))
+    _call(index, "trident_embedding", w.data_ptr(), code, V, D, ld, idc.data_ptr(), wide, idc.numel(), scale,
+          out.data_ptr(), D)
     return out
 
 
@@ -120,7 +150,7 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     ``padding_idx``, whose row is looked up like any other.
     """
     if weight.requires_grad and torch.is_grad_enabled():
-        return _Embedding.apply(ids, weight, float(scale), padding_idx)
+        return _Embedding.apply(ids, weight, scale, padding_idx)
     return _embed(ids, weight, scale)
 
 
@@ -129,26 +159,29 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
     """The table's gradient ``[num_rows, D]`` in the type of ``grad`` (``[*ids.shape, D]``): row v is
     ``scale`` times the sum of the gradients of the tokens with id v, in their order.  ``out`` (rows of
     any pitch) is written whole."""
-    code = _dtype("grad", grad)
-    _on(grad.device, ids=ids, out=out)
-    _need(grad.device.type == "cuda", "grad must be a device tensor")
-    _need(grad.dim() >= 1 and grad.shape[:-1] == ids.shape and grad.shape[-1] > 0,
-          f"grad must be [*ids.shape, D], got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
-    num_rows = int(num_rows)
-    _need(num_rows > 0, f"num_rows must be positive, got {num_rows}")
-    _need(padding_idx is None or 0 <= padding_idx < num_rows, f"padding_idx={padding_idx} outside [0, {num_rows})")
-    idc, wide = _ids(ids)
-    D = grad.shape[-1]
+    code, index = _dtype("grad", grad), _gpu("grad", grad)
+    if grad.dim() < 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] == 0:
+        _refuse(f"grad must be [*ids.shape, D], got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
+    if num_rows < 1:
+        _refuse(f"num_rows must be positive, got {num_rows}")
+    if padding_idx is not None and not 0 <= padding_idx < num_rows:
+        _refuse(f"padding_idx={padding_idx} outside [0, {num_rows})")
+    idc, wide = _ids(index, ids)
+    n, D = idc.numel(), grad.shape[-1]
     g, ld = _rows(grad)
+    ld_out = D
     if out is None:
-        out = torch.empty((num_rows, D), dtype=grad.dtype, device=grad.device)
+        out = grad.new_empty((num_rows, D))
     else:
-        _need(out.dtype == grad.dtype and tuple(out.shape) == (num_rows, D) and (out.stride(1) == 1 or D == 1) and
-              (out.stride(0) >= D or num_rows == 1), f"out must be [{num_rows}, {D}] {grad.dtype} with whole rows")
-    nbytes = _lib.lib().trident_embedding_grad_workspace_bytes(idc.numel(), num_rows, D)
-    _call_ws(grad.device, "trident_embedding_grad", nbytes, g.data_ptr(), code, ld, idc.data_ptr(), wide, idc.numel(),
-             num_rows, D, float(scale), -1 if padding_idx is None else int(padding_idx), out.data_ptr(),
-             out.stride(0) if num_rows > 1 else D)
+        _same(index, "out", out)
+        if out.dtype != grad.dtype or tuple(out.shape) != (num_rows, D) or (out.stride(1) != 1 and D != 1) or \
+                (out.stride(0) < D and num_rows > 1):
+            _refuse(f"out must be [{num_rows}, {D}] {grad.dtype} with whole rows")
+        if num_rows > 1:
+            ld_out = out.stride(0)
+    nbytes = _fn("trident_embedding_grad_workspace_bytes")(n, num_rows, D)
+    _call_ws(grad.device, index, "trident_embedding_grad", nbytes, g.data_ptr(), code, ld, idc.data_ptr(), wide, n,
+             num_rows, D, scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ld_out)
     return out
 
 
@@ -156,33 +189,38 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
 # layer norm
 
 
-def _affine(x, weight, bias) -> int:
+def _affine(index, x, D, weight, bias) -> int:
     """The type code of weight and bias, which is x's or float32."""
-    D, code = x.shape[-1], None
+    dtype = None
     for name, t in (("weight", weight), ("bias", bias)):
         if t is None:
             continue
-        _need(t.dim() == 1 and t.shape[0] == D and t.is_contiguous(), f"{name} must be a contiguous [{D}]")
-        _need(t.dtype in (x.dtype, torch.float32), f"{name} must be {x.dtype} or float32, got {t.dtype}")
-        _need(code is None or _DTYPES[t.dtype] == code, "weight and bias must have one type")
-        code = _DTYPES[t.dtype]
-    return _DTYPES[x.dtype] if code is None else code
+        _same(index, name, t)
+        if t.dim() != 1 or t.shape[0] != D or not t.is_contiguous():
+            _refuse(f"{name} must be a contiguous [{D}]")
+        if dtype is None:
+            dtype = t.dtype
+            if dtype != x.dtype and dtype != torch.float32:
+                _refuse(f"{name} must be {x.dtype} or float32, got {dtype}")
+        elif t.dtype != dtype:
+            _refuse("weight and bias must have one type")
+    return _DTYPES[x.dtype if dtype is None else dtype]
 
 
 def _norm(x, weight, bias, eps, keep):
-    code = _dtype("x", x)
-    _need(x.dim() >= 1 and x.shape[-1] > 0, f"x must be [..., D], got {tuple(x.shape)}")
-    _on(x.device, weight=weight, bias=bias)
-    wcode = _affine(x, weight, bias)
-    D = x.shape[-1]
-    rows = x.numel() // D
+    code, index = _dtype("x", x), _gpu("x", x)
+    D = x.shape[-1] if x.dim() else 0
+    if D == 0:
+        _refuse(f"x must be [..., D], got {tuple(x.shape)}")
+    wcode = _affine(index, x, D, weight, bias)
     xr, ld = _rows(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     mean = rstd = None
     if keep:
-        mean, rstd = torch.empty((2, *x.shape[:-1]), dtype=torch.float32, device=x.device)
-    _call(x.device, "trident_layer_norm", xr.data_ptr(), code, rows, D, ld, ext._ptr(weight), ext._ptr(bias), wcode,
-          float(eps), y.data_ptr(), D, ext._ptr(mean), ext._ptr(rstd))
+        mean, rstd = x.new_empty((2, *x.shape[:-1]), dtype=torch.float32)
+    _call(index, "trident_layer_norm", xr.data_ptr(), code, x.numel() // D, D, ld,
+          None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), wcode, eps,
+          y.data_ptr(), D, mean.data_ptr() if keep else None, rstd.data_ptr() if keep else None)
     return y, mean, rstd
 
 
@@ -227,24 +265,25 @@ def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.
 
 
 def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
-    code = _dtype("x", x)
-    _need(grad.shape == x.shape and grad.dtype == x.dtype,
-          f"grad must be {tuple(x.shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
-    _on(x.device, grad=grad, weight=weight, mean=mean, rstd=rstd)
+    code, index = _dtype("x", x), _gpu("x", x)
+    if grad.shape != x.shape or grad.dtype != x.dtype:
+        _refuse(f"grad must be {tuple(x.shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
+    _same(index, "grad", grad)
     for name, t in (("mean", mean), ("rstd", rstd)):
-        _need(t.dtype == torch.float32 and t.shape == x.shape[:-1] and t.is_contiguous(),
-              f"{name} must be a contiguous float32 {tuple(x.shape[:-1])}")
-    _affine(x, weight, None)
+        _same(index, name, t)
+        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
+            _refuse(f"{name} must be a contiguous float32 {tuple(x.shape[:-1])}")
     D = x.shape[-1]
+    _affine(index, x, D, weight, None)
     rows = x.numel() // D
     wdtype = x.dtype if wdtype is None else wdtype
     xr, ldx = _rows(x)
     gr, ldg = _rows(grad)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty(D, dtype=wdtype, device=x.device) if need_w else None
-    db = torch.empty(D, dtype=wdtype, device=x.device) if need_b else None
-    nbytes = _lib.lib().trident_layer_norm_grad_workspace_bytes(rows, D)
-    _call_ws(x.device, "trident_layer_norm_grad", nbytes, gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D,
+    dx = x.new_empty(x.shape)
+    dw = x.new_empty(D, dtype=wdtype) if need_w else None
+    db = x.new_empty(D, dtype=wdtype) if need_b else None
+    nbytes = _fn("trident_layer_norm_grad_workspace_bytes")(rows, D)
+    _call_ws(x.device, index, "trident_layer_norm_grad", nbytes, gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D,
              ext._ptr(weight), _DTYPES[wdtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, ext._ptr(dw),
              ext._ptr(db))
     return dx, dw, db
@@ -280,19 +319,17 @@ class AdamW:
         _need(0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0, f"betas must lie in [0, 1), got {betas}")
         _need(lr >= 0.0 and eps >= 0.0 and weight_decay >= 0.0, "lr, eps and weight_decay must not be negative")
         _need(len({id(p) for p in self.params}) == len(self.params), "a parameter is listed twice")
-        self.device = self.params[0].device
+        self.device, self._index = self.params[0].device, _gpu("parameter 0", self.params[0])
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(betas), float(eps), float(weight_decay)
         self.state_bits, self.step_count = state_bits, 0
-        self._table = np.zeros(len(self.params), _TABLE)
         self.offsets, total = [], 0
         for i, p in enumerate(self.params):
-            self._table[i]["dtype"] = _dtype(f"parameter {i}", p)
-            _on(self.device, **{f"parameter {i}": p})
+            _dtype(f"parameter {i}", p)
+            _same(self._index, f"parameter {i}", p)
             _need(p.is_contiguous(), f"parameter {i} must be contiguous")
             self.offsets.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
-        self._numel = np.array([p.numel() for p in self.params], np.int64)
-        self._table["offset"] = self.offsets
+        self._numel = [p.numel() for p in self.params]
         kind = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
         self.exp_avg = torch.zeros(total, dtype=kind[0], device=self.device)
         self.exp_avg_sq = torch.zeros(total, dtype=kind[1], device=self.device)
@@ -311,33 +348,33 @@ class AdamW:
     @torch.no_grad()
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, grad_scale: float = 1.0) -> None:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
-        _need(len(grads) == len(self.params), f"{len(self.params)} gradients are needed, got {len(grads)}")
-        table = self._table
-        for i, (p, g) in enumerate(zip(self.params, grads)):
+        if len(grads) != len(self.params):
+            _refuse(f"{len(self.params)} gradients are needed, got {len(grads)}")
+        rows, moved = [], []
+        for i, (p, g, at) in enumerate(zip(self.params, grads, self.offsets)):
             if g is None:
                 continue
-            _need(isinstance(g, torch.Tensor) and g.shape == p.shape and g.device == self.device and
-                  g.layout == torch.strided, f"gradient {i} must be a dense {tuple(p.shape)} on {self.device}")
+            if g.shape != p.shape or g.get_device() != self._index or g.layout != torch.strided:
+                _refuse(f"gradient {i} must be a dense {tuple(p.shape)} on {self.device}")
+            if not p.is_contiguous() or p.get_device() != self._index or p.numel() != self._numel[i]:
+                _refuse(f"parameter {i} is no longer the {self._numel[i]} elements it was")
             if not g.is_contiguous():
-                grads[i] = g.contiguous()
-        table["numel"] = [0 if g is None else n for g, n in zip(grads, self._numel)]
-        table["param"] = [p.data_ptr() for p in self.params]
-        table["grad"] = [0 if g is None else g.data_ptr() for g in grads]
-        table["grad_dtype"] = [0 if g is None else _dtype("gradient", g) for g in grads]
-        h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay,
-                                   float(grad_scale), self.step_count + 1)
-        _call(self.device, "trident_adamw",
-              ctypes.cast(table.ctypes.data, ctypes.POINTER(_lib.TridentAdamTensor)), len(table),
-              ctypes.byref(self._state), ctypes.byref(h))
+                g = grads[i] = g.contiguous()
+            moved.append(p)
+            rows.append((p.data_ptr(), g.data_ptr(), self._numel[i], at, _dtype("parameter", p), _dtype("gradient", g)))
+        table = np.array(rows, _TABLE)
+        h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
+                                   self.step_count + 1)
+        _call(self._index, "trident_adamw", table.ctypes.data, len(rows), ctypes.byref(self._state), ctypes.byref(h))
         self.step_count += 1
-        torch.autograd.graph.increment_version([p for p, g in zip(self.params, grads) if g is not None])
+        torch.autograd.graph.increment_version(moved)
 
     def state_values(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The moments as flat float32 tensors: the buffers themselves, or what the 8-bit codes stand for."""
         if self.state_bits == 32:
             return self.exp_avg, self.exp_avg_sq
         m, v = torch.empty((2, self.exp_avg.numel()), device=self.device)
-        _call(self.device, "trident_adamw_state_values", ctypes.byref(self._state), m.data_ptr(), v.data_ptr())
+        _call(self._index, "trident_adamw_state_values", ctypes.byref(self._state), m.data_ptr(), v.data_ptr())
         return m, v
 
     def load_state(self, step_count: int, exp_avg: torch.Tensor, exp_avg_sq: torch.Tensor,
@@ -386,40 +423,45 @@ def _fp8_pitches(K: int) -> Tuple[int, int]:
     return -(-K // 128) * 128, -(-K // 512) * 4
 
 
-def _check_blocks(name: str, b: Fp8Blocks, device: torch.device) -> int:
-    _need(isinstance(b, Fp8Blocks), f"{name} must be Fp8Blocks (quantize_fp8)")
-    _need(b.K > 0 and b.codes.dim() == 2, f"{name} must be a matrix")
-    kp, sp = _fp8_pitches(b.K)
-    rows = b.codes.shape[0]
-    _need(b.codes.dtype == torch.float8_e4m3fn and b.codes.shape[1] == kp and b.codes.is_contiguous(),
-          f"{name}.codes must be a contiguous [{rows}, {kp}] float8_e4m3fn")
-    _need(b.scales.dtype == torch.uint8 and tuple(b.scales.shape) == (rows, sp) and b.scales.is_contiguous(),
-          f"{name}.scales must be a contiguous [{rows}, {sp}] uint8")
-    _need(b.codes.device == device and b.scales.device == device, f"{name} must be on {device}")
+def _check_blocks(name: str, b: Fp8Blocks, index: int) -> int:
+    if not isinstance(b, Fp8Blocks):
+        _refuse(f"{name} must be Fp8Blocks (quantize_fp8)")
+    codes, scales, K = b
+    if K < 1 or codes.dim() != 2 or scales.dim() != 2:
+        _refuse(f"{name} must be a matrix")
+    kp, sp = _fp8_pitches(K)
+    rows = codes.shape[0]
+    if codes.dtype != torch.float8_e4m3fn or codes.shape[1] != kp or not codes.is_contiguous():
+        _refuse(f"{name}.codes must be a contiguous [{rows}, {kp}] float8_e4m3fn")
+    if scales.dtype != torch.uint8 or scales.shape[0] != rows or scales.shape[1] != sp or not scales.is_contiguous():
+        _refuse(f"{name}.scales must be a contiguous [{rows}, {sp}] uint8")
+    if codes.get_device() != index or scales.get_device() != index:
+        _refuse(f"{name} must be on cuda:{index}")
     return rows
 
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
     """``x`` [rows, K] in 8-bit floating point: each row's 128 columns share the least power of two under
     which their largest value is at most 448.  A value that is not finite becomes NaN."""
-    code = _dtype("x", x)
-    _on(x.device)
-    _need(x.dim() == 2 and x.shape[1] > 0, f"x must be [rows, K], got {tuple(x.shape)}")
+    code, index = _dtype("x", x), _gpu("x", x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        _refuse(f"x must be [rows, K], got {tuple(x.shape)}")
     rows, K = x.shape
     xr, ld = _rows(x)
     kp, sp = _fp8_pitches(K)
-    codes = torch.empty((rows, kp), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((rows, sp), dtype=torch.uint8, device=x.device)
-    _call(x.device, "trident_fp8_quantize", xr.data_ptr(), code, rows, K, ld, codes.data_ptr(), scales.data_ptr())
+    codes, scales = x.new_empty((rows, kp), dtype=torch.float8_e4m3fn), x.new_empty((rows, sp), dtype=torch.uint8)
+    _call(index, "trident_fp8_quantize", xr.data_ptr(), code, rows, K, ld, codes.data_ptr(), scales.data_ptr())
     return Fp8Blocks(codes, scales, K)
 
 
-def _bias(bias, N, dtype, device) -> int:
+def _bias(bias, N, dtype, index) -> int:
     if bias is None:
         return _DTYPES[dtype]
-    _need(bias.dim() == 1 and bias.shape[0] == N and bias.is_contiguous(), f"bias must be a contiguous [{N}]")
-    _need(bias.dtype in (dtype, torch.float32), f"bias must be {dtype} or float32, got {bias.dtype}")
-    _need(bias.device == device, f"bias must be on {device}")
+    if bias.dim() != 1 or bias.shape[0] != N or not bias.is_contiguous():
+        _refuse(f"bias must be a contiguous [{N}]")
+    if bias.dtype != dtype and bias.dtype != torch.float32:
+        _refuse(f"bias must be {dtype} or float32, got {bias.dtype}")
+    _same(index, "bias", bias)
     return _DTYPES[bias.dtype]
 
 
@@ -430,16 +472,19 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
     ``fast_accum`` takes the 8-bit matrix instruction, which is twice as fast and keeps 13 bits below the
     largest of each 8 products: the sums are off by up to about 5e-5 of their size, which a bfloat16
     result does not show."""
-    _need(isinstance(a, Fp8Blocks), "a must be Fp8Blocks (quantize_fp8)")
-    device = a.codes.device
-    _on(device)
-    M, N = _check_blocks("a", a, device), _check_blocks("b", b, device)
-    _need(a.K == b.K, f"a has {a.K} columns, b {b.K}")
-    _need(out_dtype in _DTYPES, f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
-    bcode = _bias(bias, N, out_dtype, device)
-    out = torch.empty((M, N), dtype=out_dtype, device=device)
-    _call(device, "trident_fp8_matmul", a.codes.data_ptr(), a.scales.data_ptr(), M, b.codes.data_ptr(),
-          b.scales.data_ptr(), N, a.K, ext._ptr(bias), bcode, out.data_ptr(), _DTYPES[out_dtype], max(N, 1), int(fast_accum))
+    if not isinstance(a, Fp8Blocks):
+        _refuse("a must be Fp8Blocks (quantize_fp8)")
+    index = _gpu("a", a.codes)
+    M, N = _check_blocks("a", a, index), _check_blocks("b", b, index)
+    if a.K != b.K:
+        _refuse(f"a has {a.K} columns, b {b.K}")
+    if out_dtype not in _DTYPES:
+        _refuse(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
+    bcode = _bias(bias, N, out_dtype, index)
+    out = a.codes.new_empty((M, N), dtype=out_dtype)
+    _call(index, "trident_fp8_matmul", a.codes.data_ptr(), a.scales.data_ptr(), M, b.codes.data_ptr(),
+          b.scales.data_ptr(), N, a.K, None if bias is None else bias.data_ptr(), bcode, out.data_ptr(),
+          _DTYPES[out_dtype], max(N, 1), fast_accum)
     return out
 
 
@@ -447,17 +492,17 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
                fast_accum: bool = False) -> torch.Tensor:
     """``x @ weight.T + bias`` for ``x`` [..., K], quantised in the call, in x's type: the projection of a
     query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``."""
-    code = _dtype("x", x)
-    device = x.device
-    _on(device)
-    N = _check_blocks("weight", weight, device)
+    code, index = _dtype("x", x), _gpu("x", x)
+    N = _check_blocks("weight", weight, index)
     K = weight.K
-    _need(x.dim() >= 1 and x.shape[-1] == K, f"x must be [..., {K}], got {tuple(x.shape)}")
+    if x.dim() < 1 or x.shape[-1] != K:
+        _refuse(f"x must be [..., {K}], got {tuple(x.shape)}")
     M = x.numel() // K
-    bcode = _bias(bias, N, x.dtype, device)
+    bcode = _bias(bias, N, x.dtype, index)
     xr, ld = _rows(x)
-    out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=device)
-    nbytes = _lib.lib().trident_fp8_linear_workspace_bytes(M, K)
-    _call_ws(device, "trident_fp8_linear", nbytes, xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(),
-             weight.scales.data_ptr(), N, ext._ptr(bias), bcode, out.data_ptr(), max(N, 1), int(fast_accum))
+    out = x.new_empty((*x.shape[:-1], N))
+    nbytes = _fn("trident_fp8_linear_workspace_bytes")(M, K)
+    _call_ws(x.device, index, "trident_fp8_linear", nbytes, xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(),
+             weight.scales.data_ptr(), N, None if bias is None else bias.data_ptr(), bcode, out.data_ptr(),
+             max(N, 1), fast_accum)
     return out
