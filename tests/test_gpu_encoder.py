@@ -140,7 +140,7 @@ def test_embedding_grad_rows_across_chunks(dev, dtype, counts):
 
 
 @pytest.mark.parametrize("n,V,D", [(8192, 3000, 40), (8193, 3000, 40), (20_000, 513, 1000), (40_000, 70_000, 900),
-                                   (40_000, 2, 300), (30_000, 1, 17), (9000, 200_000, 24)])
+                                   (40_000, 2, 300), (30_000, 1, 17), (9000, 200_000, 24), (9000, 600_000, 16)])
 @pytest.mark.parametrize("wide", [True, False])
 def test_embedding_grad_many_tokens(dev, n, V, D, wide):
     """Past the sizes at which the ordering and the parts change; ids with most of all tokens."""

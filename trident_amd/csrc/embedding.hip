@@ -76,124 +76,249 @@ struct Token {
     int t, row;
 };
 
-// Ids of one sorting workgroup and what of them each of its waves keeps in LDS.
-template <int WAVES>
-struct SortShape {
-    static constexpr int kAheadIds = 16;                    // groups of 64 ids a wave loads at once
-    static constexpr int kList = WAVES == 4 ? 2048 : 1024;  // tokens a wave keeps in LDS
-    static constexpr size_t lds(int w) {
-        return (size_t)WAVES * w * sizeof(int) + (size_t)WAVES * kList * (sizeof(int) + sizeof(uint16_t));
-    }
-};
-constexpr int kSmallTokens = 4 * 2048;  // four waves keep all of them
+constexpr int kSmallTokens = 4 * 2048;  // ordered in one launch: four waves can keep all of them
+constexpr int kPartTokens = 1024;       // tokens that bucket_ids_kernel orders at a time
+constexpr int kMaxBuckets = 1024;
 
 struct SortArgs {
     const void* ids;
-    int n, V, owned, shift, chunk;
+    int n, V, owned, shift, chunk, parts;
     uint32_t skip;     // an id without a gradient; 2^32 - 1: none
     RowInfo* row;      // [V + 1]
     Token* token;      // [n]
     int* long_count;   // [2^shift]
     int* long_rows;    // [2^shift, owned]
+    Token* bucketed;   // [n]: each part's tokens by bucket (t, id)
+    uint16_t* starts;  // [parts, 2^shift + 1]: the buckets' first places in their part
 };
 
-// An id's low half if it is a row's that takes part, else 2^32 - 1.
-__device__ __forceinline__ uint32_t row_id(const int64_t* ids, int t, uint32_t V, uint32_t skip) {
-    const uint2 id = reinterpret_cast<const uint2*>(ids)[t];
-    return id.y == 0 && id.x < V && id.x != skip ? id.x : ~0u;
+// An id if it is a row's that takes part, else 2^32 - 1.
+template <bool SKIP>
+__device__ __forceinline__ uint32_t row_id(int64_t id, uint32_t V, uint32_t skip) {
+    return (uint64_t)id < V && !(SKIP && id == skip) ? (uint32_t)id : ~0u;
 }
-__device__ __forceinline__ uint32_t row_id(const int32_t* ids, int t, uint32_t V, uint32_t skip) {
-    const uint32_t id = (uint32_t)ids[t];
-    return id < V && id != skip ? id : ~0u;
+template <bool SKIP>
+__device__ __forceinline__ uint32_t row_id(int32_t id, uint32_t V, uint32_t skip) {
+    return (uint32_t)id < V && !(SKIP && (uint32_t)id == skip) ? (uint32_t)id : ~0u;
 }
+
+// The lanes whose key (of `bits` bits) equals this one's, among those with `in`: found bit by bit.
+__device__ __forceinline__ uint64_t lanes_with(bool in, uint32_t key, int bits) {
+    uint64_t same = __ballot(in);
+    for (int i = 0; i < bits; ++i) {
+        const bool set = (key >> i) & 1;
+        const uint64_t m = __ballot(set);
+        same &= set ? m : ~m;
+    }
+    return same;
+}
+
+// Inclusive sum over a workgroup of WAVES waves, and the total of all; two barriers.
+template <int WAVES>
+__device__ __forceinline__ int block_sum(int v, int* s_sum, int* total) {
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) {
+        const int t = __shfl_up(v, o, kWave);
+        if (lane >= o) v += t;
+    }
+    __syncthreads();
+    if (lane == kWave - 1) s_sum[wave] = v;
+    __syncthreads();
+    int all = 0;
+    for (int i = 0; i < WAVES; ++i) {
+        if (i < wave) v += s_sum[i];
+        all += s_sum[i];
+    }
+    *total = all;
+    return v;
+}
+
+// Many tokens, first step: a part of kPartTokens of them is ordered by bucket, id modulo 2^shift, and
+// the buckets' first places are written beside it.
+template <typename ID, bool SKIP>
+__global__ __launch_bounds__(kBlock) void bucket_ids_kernel(SortArgs a) {
+    constexpr int G = kPartTokens / kBlock;
+    __shared__ int hist[kWavesPerBlock * kMaxBuckets];
+    __shared__ Token sorted[kPartTokens];
+    __shared__ int s_sum[kWavesPerBlock];
+    const int lane = lane_id(), wave = threadIdx.x / kWave, buckets = 1 << a.shift;
+    const int t0 = blockIdx.x * kPartTokens + wave * (G * kWave) + lane;
+    const ID* ids = static_cast<const ID*>(a.ids);
+    uint32_t id[G];
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        const ID raw = ids[min(t0 + u * kWave, a.n - 1)];
+        id[u] = t0 + u * kWave < a.n ? row_id<SKIP>(raw, (uint32_t)a.V, a.skip) : ~0u;
+    }
+    for (int i = threadIdx.x; i < kWavesPerBlock * buckets; i += kBlock) hist[i] = 0;
+    __syncthreads();
+    int* mine = hist + wave * buckets;
+#pragma unroll
+    for (int u = 0; u < G; ++u)
+        if (id[u] != ~0u) atomicAdd(&mine[id[u] & (buckets - 1)], 1);
+    __syncthreads();
+    uint16_t* starts = a.starts + (int64_t)blockIdx.x * (buckets + 1);
+    int place = 0;
+    for (int j0 = 0; j0 < buckets; j0 += kBlock) {
+        const int j = j0 + threadIdx.x;
+        int count = 0, total;
+        if (j < buckets)
+            for (int i = 0; i < kWavesPerBlock; ++i) count += hist[i * buckets + j];
+        int at = place + block_sum<kWavesPerBlock>(count, s_sum, &total) - count;
+        place += total;
+        if (j < buckets) {
+            starts[j] = (uint16_t)at;
+            for (int i = 0; i < kWavesPerBlock; ++i) {
+                const int c = hist[i * buckets + j];
+                hist[i * buckets + j] = at;
+                at += c;
+            }
+        }
+    }
+    if (threadIdx.x == 0) starts[buckets] = (uint16_t)place;
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        const uint32_t key = id[u] & (buckets - 1);
+        const uint64_t same = lanes_with(id[u] != ~0u, key, a.shift);
+        if (id[u] != ~0u) {
+            const int rank = mask_rank(same), at = mine[key];
+            sorted[at + rank] = Token{t0 + u * kWave, (int)id[u]};
+            wave_sync();
+            if (rank == 0) mine[key] = at + __popcll((unsigned long long)same);
+        }
+        wave_sync();
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < place; i += kBlock) a.bucketed[(int64_t)blockIdx.x * kPartTokens + i] = sorted[i];
+}
+
+// What a sorting workgroup's waves read: all ids (FROM_PARTS false), or its bucket of every part.  A
+// wave takes a contiguous share, and calls f(t, rel) for 64 tokens at a time in their order, rel < 0 in
+// lanes without one; returns how many tokens of lower buckets its share has.
+template <typename ID, int WAVES, bool SKIP, bool FROM_PARTS>
+struct SortSource {
+    template <typename F>
+    static __device__ __forceinline__ int read(const SortArgs& a, F&& f) {
+        const int lane = lane_id(), wave = threadIdx.x / kWave;
+        const uint32_t b = blockIdx.x, mask = (1u << a.shift) - 1;
+        int lower = 0;
+        if constexpr (FROM_PARTS) {
+            constexpr int A = 4;
+            const int share = (a.parts + WAVES - 1) / WAVES, stride = (int)mask + 2;
+            const int p0 = min(a.parts, wave * share), p1 = min(a.parts, p0 + share);
+            for (int p = p0; p < p1; p += kWave) {
+                const int mine = min(p + lane, p1 - 1);
+                const int beg = a.starts[(int64_t)mine * stride + b];
+                const int num = p + lane < p1 ? a.starts[(int64_t)mine * stride + b + 1] - beg : 0;
+                lower += p + lane < p1 ? beg : 0;
+                for (int q = 0; q < min(kWave, p1 - p); q += A) {
+                    Token tok[A];
+                    int n[A], s[A];
+#pragma unroll
+                    for (int u = 0; u < A; ++u) {
+                        n[u] = __builtin_amdgcn_readlane(num, q + u);  // 0 past the share's end
+                        s[u] = (p + q + u) * kPartTokens + __builtin_amdgcn_readlane(beg, q + u);
+                        if (lane < n[u]) tok[u] = a.bucketed[s[u] + lane];
+                    }
+#pragma unroll
+                    for (int u = 0; u < A; ++u) {
+                        if (n[u] == 0) continue;
+                        f(tok[u].t, lane < n[u] ? tok[u].row >> a.shift : -1);
+                        for (int k = kWave; k < n[u]; k += kWave) {
+                            const bool in = k + lane < n[u];
+                            const Token more = in ? a.bucketed[s[u] + k + lane] : Token{0, 0};
+                            f(more.t, in ? more.row >> a.shift : -1);
+                        }
+                    }
+                }
+            }
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) lower += __shfl_xor(lower, o, kWave);
+        } else {
+            constexpr int A = 16;
+            const int n = a.n, seg = (n + WAVES * kWave - 1) / (WAVES * kWave) * kWave;
+            const int beg = (int)min((int64_t)n, (int64_t)wave * seg), end = (int)min((int64_t)n, (int64_t)beg + seg);
+            const ID* ids = static_cast<const ID*>(a.ids);
+            for (int t0 = beg; t0 < end; t0 += kWave * A) {
+                ID raw[A];
+#pragma unroll
+                for (int u = 0; u < A; ++u) raw[u] = ids[min(t0 + u * kWave + lane, n - 1)];
+#pragma unroll
+                for (int u = 0; u < A; ++u) {
+                    const int t = t0 + u * kWave + lane;
+                    const uint32_t id = t < end ? row_id<SKIP>(raw[u], (uint32_t)a.V, a.skip) : ~0u;
+                    const uint32_t owner = id == ~0u ? ~0u : id & mask;
+                    lower += __popcll((unsigned long long)__ballot(owner < b));
+                    if (__ballot(owner == b)) f(t, owner == b ? (int)(id >> a.shift) : -1);
+                }
+            }
+        }
+        return lower;
+    }
+};
+
+template <int WAVES>
+struct SortShape {
+    static constexpr int kList = WAVES == 4 ? 2048 : 1024;  // tokens a wave keeps in LDS
+    static constexpr size_t lds(int w) {
+        return (size_t)WAVES * w * sizeof(int) + (size_t)WAVES * kList * (sizeof(int) + sizeof(uint16_t));
+    }
+};
 
 // Orders the tokens by id: row[v] says where in `token` the tokens of id v lie, in their own order;
 // row[V] holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power of two): the
 // most frequent ids of a vocabulary are neighbours, so a range of them would be one workgroup's work.
-// Each wave reads a contiguous part of the ids, keeps the tokens its workgroup owns in a list in LDS,
-// and counts them by id and those of lower workgroups; the counts give every (id, wave) its first
-// place, and the lists are placed in order.  A wave whose list overflows (an id with a large share of
-// many tokens) reads its part again instead.  One launch, and no workgroup waits for another; the price
-// is that every one reads all ids.
-template <typename ID, int WAVES>
+// Each wave goes through its share of the tokens, keeps those its workgroup owns in a list in LDS, and
+// counts them by id; the counts, and the number of tokens of lower workgroups, give every (id, wave)
+// its first place, and the lists are placed in order.  A wave whose list overflows (an id with a large
+// share of many tokens) goes through its share again instead.  No workgroup waits for another.
+//
+// Few tokens are read by every workgroup.  For many that is most of the time (131,072: 35 us), so they
+// are bucketed first, which leaves each workgroup its own (4 + 8 us).
+template <typename ID, int WAVES, bool SKIP, bool FROM_PARTS>
 __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
-    using Shape = SortShape<WAVES>;
-    constexpr int A = Shape::kAheadIds, kList = Shape::kList;
+    using Source = SortSource<ID, WAVES, SKIP, FROM_PARTS>;
+    constexpr int kList = SortShape<WAVES>::kList;
     extern __shared__ int lds[];
     __shared__ int s_sum[WAVES], s_long;
-    const int w = a.owned, n = a.n;
-    int* hist = lds;                // [WAVES][w]
-    int* list = lds + WAVES * w;    // [WAVES][kList]
+    const int w = a.owned, lane = lane_id(), wave = threadIdx.x / kWave;
+    const uint32_t b = blockIdx.x;
+    int* hist = lds;              // [WAVES][w]
+    int* list = lds + WAVES * w;  // [WAVES][kList]
     uint16_t* list_id = reinterpret_cast<uint16_t*>(list + WAVES * kList);
-    const ID* ids = static_cast<const ID*>(a.ids);
-    const int lane = lane_id(), wave = threadIdx.x / kWave;
-    const uint32_t b = blockIdx.x, mask = (1u << a.shift) - 1;
-    const int seg = (n + WAVES * kWave - 1) / (WAVES * kWave) * kWave;
-    const int beg = (int)min((int64_t)n, (int64_t)wave * seg), end = (int)min((int64_t)n, (int64_t)beg + seg);
     for (int i = threadIdx.x; i < WAVES * w; i += WAVES * kWave) hist[i] = 0;
     if (threadIdx.x == 0) s_long = 0;
     __syncthreads();
     int* mine = hist + wave * w;
     int* kept = list + wave * kList;
     uint16_t* kept_id = list_id + wave * kList;
-    int lower = 0, found = 0;
-    for (int t0 = beg; t0 < end; t0 += kWave * A) {
-        uint32_t id[A];
-        if (t0 + kWave * A <= end) {
-#pragma unroll
-            for (int u = 0; u < A; ++u) id[u] = row_id(ids, t0 + u * kWave + lane, (uint32_t)a.V, a.skip);
-        } else {
-#pragma unroll
-            for (int u = 0; u < A; ++u) {
-                const int t = t0 + u * kWave + lane;
-                id[u] = t < end ? row_id(ids, t, (uint32_t)a.V, a.skip) : ~0u;
+    int found = 0;
+    const int lower = Source::read(a, [&](int t, int rel) {
+        const uint64_t m = __ballot(rel >= 0);
+        if (rel >= 0) {
+            const int at = found + mask_rank(m);
+            atomicAdd(&mine[rel], 1);
+            if (at < kList) {
+                kept[at] = t;
+                kept_id[at] = (uint16_t)rel;
             }
         }
-#pragma unroll
-        for (int u = 0; u < A; ++u) {
-            const uint32_t owner = id[u] == ~0u ? ~0u : id[u] & mask;
-            lower += __popcll((unsigned long long)__ballot(owner < b));
-            const uint64_t m = __ballot(owner == b);
-            if (m) {
-                const int at = found + mask_rank(m);
-                if (owner == b) {
-                    const int rel = (int)(id[u] >> a.shift);
-                    atomicAdd(&mine[rel], 1);
-                    if (at < kList) {
-                        kept[at] = t0 + u * kWave + lane;
-                        kept_id[at] = (uint16_t)rel;
-                    }
-                }
-                found += __popcll((unsigned long long)m);
-            }
-        }
-    }
-    if (lane == 0) s_sum[wave] = lower;
-    __syncthreads();
-    int place = 0;
-    for (int i = 0; i < WAVES; ++i) place += s_sum[i];
+        found += __popcll((unsigned long long)m);
+    });
+    int place;
+    block_sum<WAVES>(lane == 0 ? lower : 0, s_sum, &place);
     // the first place of each owned id, a workgroup's threads of them at a time
     for (int j0 = 0; j0 < w; j0 += WAVES * kWave) {
         const int j = j0 + threadIdx.x;
         const int64_t v = ((int64_t)j << a.shift) + b;
         const bool live = j < w && v < a.V;
-        int count = 0;
+        int count = 0, total;
         if (live)
             for (int i = 0; i < WAVES; ++i) count += hist[i * w + j];
-        int inc = count;
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const int t = __shfl_up(inc, o, kWave);
-            if (lane >= o) inc += t;
-        }
-        __syncthreads();
-        if (lane == kWave - 1) s_sum[wave] = inc;
-        __syncthreads();
-        int at = place + inc - count;
-        for (int i = 0; i < WAVES; ++i) {
-            if (i < wave) at += s_sum[i];
-            place += s_sum[i];
-        }
+        int at = place + block_sum<WAVES>(count, s_sum, &total) - count;
+        place += total;
         if (live) {
             a.row[v] = RowInfo{at, count};
             if (count > a.chunk) a.long_rows[(int64_t)b * w + atomicAdd(&s_long, 1)] = (int)v;  // in any order
@@ -204,31 +329,25 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
             }
         }
     }
-    if (b == mask && threadIdx.x == 0) a.row[a.V] = RowInfo{place, 0};
+    if (b == gridDim.x - 1 && threadIdx.x == 0) a.row[a.V] = RowInfo{place, 0};
     __syncthreads();
     if (threadIdx.x == 0) a.long_count[b] = s_long;
-    const auto put = [&](int t, int rel) {  // rel < 0: no token in this lane
-        uint64_t left = __ballot(rel >= 0);
-        while (left) {  // one turn per id among these 64 tokens
-            const int first = __ffsll((unsigned long long)left) - 1;
-            const int r = __builtin_amdgcn_readlane(rel, first);
-            const uint64_t same = __ballot(rel == r);
-            const int at = mine[r];
-            if (rel == r) a.token[at + mask_rank(same)] = Token{t, (int)(((uint32_t)r << a.shift) + b)};
+    int bits = 0;
+    while ((1 << bits) < w) ++bits;
+    const auto put = [&](int t, int rel) {
+        const uint64_t same = lanes_with(rel >= 0, (uint32_t)rel, bits);
+        if (rel >= 0) {
+            const int rank = mask_rank(same), at = mine[rel];
+            a.token[at + rank] = Token{t, (int)(((uint32_t)rel << a.shift) + b)};
             wave_sync();
-            if (lane == first) mine[r] = at + __popcll((unsigned long long)same);
-            wave_sync();
-            left &= ~same;
+            if (rank == 0) mine[rel] = at + __popcll((unsigned long long)same);
         }
+        wave_sync();
     };
     if (found <= kList) {
         for (int k = lane; k - lane < found; k += kWave) put(k < found ? kept[k] : 0, k < found ? (int)kept_id[k] : -1);
     } else {
-        for (int t0 = beg; t0 < end; t0 += kWave) {
-            const int t = t0 + lane;
-            const uint32_t id = t < end ? row_id(ids, t, (uint32_t)a.V, a.skip) : ~0u;
-            put(t, id != ~0u && (id & mask) == b ? (int)(id >> a.shift) : -1);
-        }
+        Source::read(a, put);
     }
 }
 
@@ -388,7 +507,10 @@ struct GradSpace {
     Token* token;
     float* part;
     int *long_count, *long_rows;
+    Token* bucketed;
+    uint16_t* starts;
     int shift, owned;  // sorting workgroups: 2^shift, of `owned` ids each
+    int parts;         // of the bucketing step; 0: none
     int64_t chunk, chunks;
     size_t bytes;
 };
@@ -401,10 +523,9 @@ GradSpace grad_space(void* base, int64_t n, int64_t V, int64_t D) {
     // a read of four bytes a column each.
     s.chunk = n * D <= (16 << 20) ? 8 : n * D <= (32 << 20) ? 16 : 32;
     s.chunks = (n + s.chunk - 1) / s.chunk;
-    // Sorting workgroups: few tokens, one a CU, since the counting of its ids is most of its time; many
-    // tokens, as few as their ids allow, since each reads all of them.
-    s.shift = n <= kSmallTokens ? 8 : 6;
+    s.shift = 8;  // one sorting workgroup per CU, more where they would own too many ids
     while (((int64_t)kMaxOwned << s.shift) < V) ++s.shift;
+    s.parts = n > kSmallTokens && (1 << s.shift) <= kMaxBuckets ? (int)((n + kPartTokens - 1) / kPartTokens) : 0;
     s.owned = (int)((V + ((int64_t)1 << s.shift) - 1) >> s.shift);
     char* p = static_cast<char*>(base);
     size_t off = 0;
@@ -418,21 +539,33 @@ GradSpace grad_space(void* base, int64_t n, int64_t V, int64_t D) {
     s.part = reinterpret_cast<float*>(take(2 * (size_t)s.chunks * (size_t)D * sizeof(float)));
     s.long_count = reinterpret_cast<int*>(take(sizeof(int) << s.shift));
     s.long_rows = reinterpret_cast<int*>(take(((size_t)s.owned << s.shift) * sizeof(int)));
+    s.bucketed = reinterpret_cast<Token*>(take(s.parts ? (size_t)n * sizeof(Token) : 0));
+    s.starts = reinterpret_cast<uint16_t*>(take((size_t)s.parts * ((1 << s.shift) + 1) * sizeof(uint16_t)));
     s.bytes = off;
     return s;
 }
 
-template <typename ID, int WAVES>
+template <typename ID, int WAVES, bool SKIP, bool FROM_PARTS>
 int sort_ids(const SortArgs& a, hipStream_t st) {
+    const auto kernel = sort_ids_kernel<ID, WAVES, SKIP, FROM_PARTS>;
     const size_t lds = SortShape<WAVES>::lds(a.owned);
     if (lds > 65536) {
-        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(sort_ids_kernel<ID, WAVES>),
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
         if (e != hipSuccess)
             return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(sort_ids): %s", hipGetErrorString(e));
     }
-    sort_ids_kernel<ID, WAVES><<<1u << a.shift, WAVES * kWave, lds, st>>>(a);
+    kernel<<<1u << a.shift, WAVES * kWave, lds, st>>>(a);
     return capi_check_launch("sort_ids_kernel");
+}
+
+template <typename ID, bool SKIP>
+int order_tokens(const SortArgs& a, hipStream_t st) {
+    if (a.n <= kSmallTokens) return sort_ids<ID, 4, SKIP, false>(a, st);
+    if (a.parts == 0) return sort_ids<ID, 16, SKIP, false>(a, st);  // a table of more than 2^19 rows
+    bucket_ids_kernel<ID, SKIP><<<(unsigned)a.parts, kBlock, 0, st>>>(a);
+    const int rc = capi_check_launch("bucket_ids_kernel");
+    return rc ? rc : sort_ids<ID, 16, SKIP, true>(a, st);
 }
 
 constexpr int64_t kMaxCount = 0x7fffffff - 4096;  // tokens, rows and columns count in 32 bits
@@ -498,10 +631,10 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
     int rc = TRIDENT_OK;
     with_ids(ids64, [&](auto i) {
         using ID = decltype(i);
-        const SortArgs order{ids, (int)n, (int)V, s.owned, s.shift, (int)s.chunk,
+        const SortArgs order{ids, (int)n, (int)V, s.owned, s.shift, (int)s.chunk, s.parts,
                              padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : ~0u, s.row, s.token,
-                             s.long_count, s.long_rows};
-        rc = n <= kSmallTokens ? sort_ids<ID, 4>(order, st) : sort_ids<ID, 16>(order, st);
+                             s.long_count, s.long_rows, s.bucketed, s.starts};
+        rc = order.skip == ~0u ? order_tokens<ID, false>(order, st) : order_tokens<ID, true>(order, st);
     });
     if (rc) return rc;
     with_dtype(dtype, [&](auto t) {
