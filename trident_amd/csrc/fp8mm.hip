@@ -110,6 +110,7 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(QuantArgs a) {
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x8 __attribute__((ext_vector_type(8)));
 typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 struct MatmulArgs {
     const uint8_t *a, *b;    // codes [M, pitch], [N, pitch]
@@ -117,7 +118,7 @@ struct MatmulArgs {
     const void* bias;        // [N] or null
     void* out;               // [M, ldo]
     int64_t pitch, ldo;
-    int M, N, kb, spitch, bias_f32;
+    int M, N, kb, spitch, bias_f32, tiles_m, tiles_n;
 };
 
 __device__ __forceinline__ float scale_value(uint32_t e) {
@@ -139,90 +140,237 @@ __device__ __forceinline__ void to_bf16(const i32x8& codes, float scale, bf16x8 
         }
 }
 
-constexpr int kTile = 128;
+// One of a grid of workgroups in an order that keeps neighbouring tiles on one XCD (workgroups go to the
+// eight XCDs in turn, each with its own L2): each XCD takes a contiguous eighth, in bands of `band` tile
+// rows, so that the tiles it works on at a time share their rows and columns.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int band, int* tm, int* tn) {
+    const int total = tiles_m * tiles_n, each = total / 8, more = total % 8;
+    const int xcd = id % 8, k = id / 8;
+    const int t = xcd * each + min(xcd, more) + k;
+    const int first = t / (band * tiles_n) * band, rows = min(band, tiles_m - first);
+    const int in = t - first * tiles_n;
+    *tm = first + in % rows;
+    *tn = in / rows;
+}
 
-// A workgroup's 128 x 128 tile, 64 x 64 a wave.  The weight is the instruction's first operand, so a
-// lane holds four neighbouring columns of a result row.
-template <typename T, bool FAST>
-__global__ __launch_bounds__(kBlock) void matmul_kernel(MatmulArgs g) {
-    __shared__ __align__(16) uint8_t sA[kTile * kBlockK], sB[kTile * kBlockK];
-    const int lane = lane_id(), wave = threadIdx.x / kWave, r = lane & 15, q = lane >> 4;
-    const int m0 = blockIdx.y * kTile, n0 = blockIdx.x * kTile;
-    const int wm = (wave >> 1) * 64, wn = (wave & 1) * 64;
-    f32x4 acc[4][4] = {};
-    for (int kb = 0; kb < g.kb; ++kb) {
-        __syncthreads();
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+// A buffer that begins at p.  Offsets are 32 bits; the caller keeps them inside.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0xffffffffu, 0x00027000);
+}
+
+// A workgroup of WM x WN waves computes a tile of WM MT x WN NT blocks of 32 x 32, a wave MT x NT of
+// them.  128 columns of both operands at a time go straight from memory to LDS (no registers between),
+// the next ones while these are multiplied.  16-byte pieces of a row are stored exchanged by the row's
+// last three bits, so that the eight lanes that LDS serves at a time read from all of its banks.  The
+// weight is the instruction's first operand, so a lane holds four neighbouring columns of a result row.
+// A block of 128 columns is two instructions of 64 each with the same scale; in both operands a lane
+// passes the same columns, in whatever order the instruction takes them.  The rows' scales of four
+// blocks, one word a row, go to LDS with the first of them: no register waits for memory in the loop, so
+// the only wait for the loads in flight is the one at the barrier.
+template <typename T, bool FAST, int WM, int WN, int MT, int NT>
+__global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
+    constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, kStage = (BM + BN) * kBlockK;
+    constexpr int kLoads = (BM + BN) / 8 / kWaves;  // a wave's loads of eight rows each
+    static_assert((BM + BN) / 8 % kWaves == 0, "whole loads");
+    constexpr int kScaleLoads = (BM + BN + kWaves * kWave - 1) / (kWaves * kWave);
+    constexpr int kScaleStage = kScaleLoads * kWaves * kWave * 4;
+    extern __shared__ __align__(16) uint8_t lds[];  // [2][BM + BN][128], [2][BM + BN] words of scales
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r = lane & 31, q = lane >> 5;
+    int tm, tn;
+    tile_of(blockIdx.x, g.tiles_m, g.tiles_n, 8, &tm, &tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int wm = (wave / WN) * MT * 32, wn = (wave % WN) * NT * 32;
+
+    // rows of the tile: BM of a, then BN of b; those past an operand's end read its last row
+    const auto row_of = [&](int row) { return row < BM ? min(row, g.M - 1 - m0) : min(row - BM, g.N - 1 - n0); };
+    const __amdgpu_buffer_rsrc_t buf_a = buffer_at(g.a + (int64_t)m0 * g.pitch);
+    const __amdgpu_buffer_rsrc_t buf_b = buffer_at(g.b + (int64_t)n0 * g.pitch);
+    const __amdgpu_buffer_rsrc_t buf_sa = buffer_at(g.sa + (int64_t)m0 * g.spitch);
+    const __amdgpu_buffer_rsrc_t buf_sb = buffer_at(g.sb + (int64_t)n0 * g.spitch);
+    // This lane's part of each load: row l / 8 of it, piece l % 8.  The offsets are made anew for each
+    // block (`sub` is hidden from the compiler, which would keep them all in registers, and spill).
+    int sub = lane / 8;
+    const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    const auto fetch = [&](int kb) {
+        asm volatile("" : "+v"(sub));
+        uint8_t* to = lds + (kb & 1) * kStage + wave * kLoads * 1024;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int c = i * kBlock + threadIdx.x, row = c / 8, slot = (c % 8) ^ (row & 7);
-            const int64_t k = (int64_t)kb * kBlockK + slot * 16;
-            const uint4 va = *reinterpret_cast<const uint4*>(g.a + min(m0 + row, g.M - 1) * g.pitch + k);
-            const uint4 vb = *reinterpret_cast<const uint4*>(g.b + min(n0 + row, g.N - 1) * g.pitch + k);
-            *reinterpret_cast<uint4*>(sA + c * 16) = va;
-            *reinterpret_cast<uint4*>(sB + c * 16) = vb;
+        for (int i = 0; i < kLoads; ++i) {
+            const int first = (wave * kLoads + i) * 8;  // the same operand for the whole wave
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16,
+                                                     (uint32_t)row_of(first + sub) * (uint32_t)g.pitch + piece,
+                                                     kb * kBlockK, 0, 0);
         }
-        __syncthreads();
-        i32x8 fa[4], fb[4];
-        int ea[4], eb[4];
+        if (kb % 4 == 0) {
+            uint8_t* st = lds + 2 * kStage + (kb / 4 & 1) * kScaleStage + wave * kWave * 4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int ra = wm + i * 16 + r, rb = wn + i * 16 + r;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 va = *reinterpret_cast<const u32x4*>(sA + ra * kBlockK + ((2 * q + h) ^ (ra & 7)) * 16);
-                const u32x4 vb = *reinterpret_cast<const u32x4*>(sB + rb * kBlockK + ((2 * q + h) ^ (rb & 7)) * 16);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    fa[i][4 * h + j] = (int)va[j];
-                    fb[i][4 * h + j] = (int)vb[j];
-                }
+            for (int i = 0; i < kScaleLoads; ++i) {
+                const int first = (i * kWaves + wave) * kWave;
+                const int row = min(first + (sub * 8 + (lane & 7)), BM + BN - 1);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_sa : buf_sb,
+                                                         (lds_ptr)(st + i * kWaves * kWave * 4), 4,
+                                                         (uint32_t)row_of(row) * (uint32_t)g.spitch, kb, 0, 0);
             }
-            ea[i] = g.sa[(int64_t)min(m0 + ra, g.M - 1) * g.spitch + kb];
-            eb[i] = g.sb[(int64_t)min(n0 + rb, g.N - 1) * g.spitch + kb];
         }
-        if constexpr (!FAST) {
-            bf16x8 ha[4];
+    };
+    // where this lane reads the four pieces of its first row of either operand; the other rows are 32
+    // rows on, the other stage is the next bit
+    static_assert((kStage & (kStage - 1)) == 0, "a stage is a bit of the address");
+    const uint32_t origin = (uint32_t)(uintptr_t)(lds_ptr)lds;
+    uint32_t at_a[4], at_b[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                to_bf16(fa[i], scale_value(ea[i]), ha);
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t p = (uint32_t)((4 * (c / 2) + 2 * q + c % 2) ^ (r & 7)) * 16;
+        at_a[c] = (uint32_t)(wm + r) * kBlockK + p;
+        at_b[c] = (uint32_t)(BM + wn + r) * kBlockK + p;
+    }
+    const auto read = [&](const uint32_t (&at)[4], int half, int block) {
+        typedef const __attribute__((address_space(3))) u32x4* piece_ptr;
+        const u32x4 lo = *(piece_ptr)(uintptr_t)(origin + at[2 * half] + block * 32 * kBlockK);
+        const u32x4 hi = *(piece_ptr)(uintptr_t)(origin + at[2 * half + 1] + block * 32 * kBlockK);
+        i32x8 f;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    bf16x8 hb[4];
-                    to_bf16(fb[j], scale_value(eb[j]), hb);
+        for (int e = 0; e < 4; ++e) {
+            f[e] = (int)lo[e];
+            f[4 + e] = (int)hi[e];
+        }
+        return f;
+    };
+
+    f32x16 acc[MT][NT] = {};
+    fetch(0);
+    uint32_t ea[MT], eb[NT];  // the scale of the current block in the lowest byte
+    for (int kb = 0; kb < g.kb; ++kb) {
+        // this block has arrived, every wave's part of it, and the other stage is no longer read
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (kb + 1 < g.kb) fetch(kb + 1);
+        if (kb % 4 == 0) {
+            const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + 2 * kStage + (kb / 4 & 1) * kScaleStage);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) eb[j] = st[BM + wn + j * 32 + r];
+        }
+        i32x8 fa[2][MT], fb[2][NT];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j) fb[half][j] = read(at_b, half, j);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) fa[half][i] = read(at_a, half, i);
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            if constexpr (FAST) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                            fb[half][j], fa[half][i], acc[i][j], 0, 0, 0, (int)eb[j], 0, (int)ea[i]);
+            } else {
+                bf16x8 hb[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) to_bf16(fb[half][j], scale_value(eb[j] & 255u), hb[j]);
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    bf16x8 ha[4];
+                    to_bf16(fa[half][i], scale_value(ea[i] & 255u), ha);
 #pragma unroll
                     for (int k = 0; k < 4; ++k)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[k], ha[k], acc[i][j], 0, 0, 0);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hb[j][k], ha[k], acc[i][j], 0, 0, 0);
                 }
             }
-        } else {
+        }
+        if constexpr (FAST) {
+            // the first half's reads, the second half's among the first half's products, the rest
+            constexpr int kReads = 2 * (MT + NT), kProducts = MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < kProducts; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
+        }
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa[i], acc[i][j], 0, 0, 0,
-                                                                                 eb[j], 0, ea[i]);
+        for (int i = 0; i < MT; ++i) ea[i] >>= 8;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) eb[j] >>= 8;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            at_a[c] ^= kStage;
+            at_b[c] ^= kStage;
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int n = n0 + wn + j * 16 + q * 4;
-        float bias[4] = {};
-        if (g.bias)
+    for (int j = 0; j < NT; ++j) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < g.N)
-                    bias[e] = g.bias_f32 ? static_cast<const float*>(g.bias)[n + e]
-                                         : (float)static_cast<const T*>(g.bias)[n + e];
+        for (int p = 0; p < 4; ++p) {
+            const int n = n0 + wn + j * 32 + p * 8 + q * 4, left = g.N - n;
+            if (left <= 0) continue;
+            float bias[4] = {};
+            if (g.bias)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int m = m0 + wm + i * 16 + r;
-            if (m >= g.M) continue;
-            T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + n;
+                for (int e = 0; e < 4; ++e)
+                    if (e < left)
+                        bias[e] = g.bias_f32 ? static_cast<const float*>(g.bias)[n + e]
+                                             : (float)static_cast<const T*>(g.bias)[n + e];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (n + e < g.N) out[e] = (T)(acc[i][j][e] + bias[e]);
+            for (int i = 0; i < MT; ++i) {
+                const int m = m0 + wm + i * 32 + r;
+                if (m >= g.M) continue;
+                T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + n;
+                T v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * p + e] + bias[e]);
+                if (left >= 4) {
+                    __builtin_memcpy(out, v, sizeof(v));
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (e < left) out[e] = v[e];
+                }
+            }
         }
     }
+}
+
+// Launches the kernel of one tile size.
+template <typename T, bool FAST, int WM, int WN, int MT, int NT>
+int launch_matmul(MatmulArgs g, hipStream_t st) {
+    constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
+    constexpr size_t scale_rows = (BM + BN + WM * WN * kWave - 1) / (WM * WN * kWave) * (WM * WN * kWave);
+    constexpr size_t lds = 2 * ((size_t)(BM + BN) * kBlockK + scale_rows * 4);
+    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(matmul): %s", hipGetErrorString(e));
+    }
+    g.tiles_m = (g.M + BM - 1) / BM;
+    g.tiles_n = (g.N + BN - 1) / BN;
+    if ((int64_t)g.tiles_m * g.tiles_n > 0x7fffffff)
+        return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: %d x %d is too large", g.M, g.N);
+    kernel<<<(unsigned)(g.tiles_m * g.tiles_n), WM * WN * kWave, lds, st>>>(g);
+    return capi_check_launch("matmul_kernel");
+}
+
+// The largest tile that still gives every CU one: a larger tile reads its operands less often (256 x
+// 256: 64 bytes of LDS for 8,192 products), but 256 CUs want 256 tiles.
+template <typename T, bool FAST>
+int matmul(const MatmulArgs& g, hipStream_t st) {
+    const auto tiles = [&](int64_t bm, int64_t bn) { return (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn); };
+    if constexpr (FAST)
+        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2>(g, st);
+    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2>(g, st);
+    return launch_matmul<T, FAST, 2, 2, 1, 1>(g, st);
 }
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
@@ -263,6 +411,7 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
                        int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
     if (!dtype_ok(dtype) || (bias && bias_dtype != dtype && bias_dtype != TRIDENT_F32))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: dtype=%d bias_dtype=%d", dtype, bias_dtype);
+    if (K > (1 << 22)) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: K=%lld is too large", (long long)K);
     if (!counts_ok(M, K) || !counts_ok(N, K) || ld_out < N)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: bad sizes M=%lld N=%lld K=%lld ld=%lld",
                          (long long)M, (long long)N, (long long)K, (long long)ld_out);
@@ -270,17 +419,14 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
     if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !aligned16(a_codes) || !aligned16(b_codes))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
     MatmulArgs g{a_codes, b_codes, a_scales, b_scales, bias, out, pitch_of(K), ld_out, (int)M, (int)N,
-                 (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32};
-    const int64_t gy = (M + kTile - 1) / kTile, gx = (N + kTile - 1) / kTile;
-    if (gy > 65535) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: M=%lld is too large", (long long)M);
+                 (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
+    int rc = TRIDENT_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        const dim3 grid((unsigned)gx, (unsigned)gy);
         hipStream_t st = static_cast<hipStream_t>(stream);
-        if (fast_accum) matmul_kernel<T, true><<<grid, kBlock, 0, st>>>(g);
-        else matmul_kernel<T, false><<<grid, kBlock, 0, st>>>(g);
+        rc = fast_accum ? matmul<T, true>(g, st) : matmul<T, false>(g, st);
     });
-    return capi_check_launch("matmul_kernel");
+    return rc;
 }
 
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t K) {
