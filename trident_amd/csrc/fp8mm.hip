@@ -31,9 +31,9 @@ inline int64_t scale_pitch_of(int64_t K) { return (blocks_of(K) + 3) / 4 * 4; } 
 
 struct QuantArgs {
     const void* x;   // [rows, ld]
-    uint8_t* codes;  // [rows, 128 kb]
+    uint8_t* codes;  // [rows, pitch]
     uint8_t* scales; // [rows, kbp]
-    int64_t rows, ld;
+    int64_t rows, ld, pitch;
     int K, kb, kbp;
 };
 
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(kBlock) void quantize_kernel(QuantArgs a) {
 #pragma unroll
     for (int o = kQuantLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o, kWave));
     const int e = scale_of(top);
-    *reinterpret_cast<uint2*>(a.codes + row * ((int64_t)a.kb * kBlockK) + col) = codes_of(f, e);
+    *reinterpret_cast<uint2*>(a.codes + row * a.pitch + col) = codes_of(f, e);
     if (l == 0) {
         uint8_t* s = a.scales + row * a.kbp;
         s[kb] = (uint8_t)e;
@@ -117,7 +117,7 @@ struct MatmulArgs {
     const uint8_t *sa, *sb;  // scales [M, spitch], [N, spitch]
     const void* bias;        // [N] or null
     void* out;               // [M, ldo]
-    int64_t pitch, ldo;
+    int64_t pitch_a, pitch_b, ldo;
     int M, N, kb, spitch, bias_f32, tiles_m, tiles_n;
 };
 
@@ -162,8 +162,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
 
 // A workgroup of WM x WN waves computes a tile of WM MT x WN NT blocks of 32 x 32, a wave MT x NT of
 // them.  128 columns of both operands at a time go straight from memory to LDS (no registers between),
-// the next ones while these are multiplied.  16-byte pieces of a row are stored exchanged by the row's
-// last three bits, so that the eight lanes that LDS serves at a time read from all of its banks.  The
+// the next ones while these are multiplied.  The eight 16-byte pieces of a row are stored exchanged by
+// bits 1 to 3 of its number: 16 lanes that read the same piece of as many rows then read from all of
+// LDS's 64 banks (a row is half of them, so rows that differ in bit 0 never meet).  The
 // weight is the instruction's first operand, so a lane holds four neighbouring columns of a result row.
 // A block of 128 columns is two instructions of 64 each with the same scale; in both operands a lane
 // passes the same columns, in whatever order the instruction takes them.  The rows' scales of four
@@ -173,7 +174,7 @@ template <typename T, bool FAST, int WM, int WN, int MT, int NT>
 __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, kStage = (BM + BN) * kBlockK;
     constexpr int kLoads = (BM + BN) / 8 / kWaves;  // a wave's loads of eight rows each
-    static_assert((BM + BN) / 8 % kWaves == 0, "whole loads");
+    static_assert((BM + BN) / 8 % kWaves == 0 && kLoads % 2 == 0, "whole loads, of either parity by turns");
     constexpr int kScaleLoads = (BM + BN + kWaves * kWave - 1) / (kWaves * kWave);
     constexpr int kScaleStage = kScaleLoads * kWaves * kWave * 4;
     extern __shared__ __align__(16) uint8_t lds[];  // [2][BM + BN][128], [2][BM + BN] words of scales
@@ -186,22 +187,24 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
 
     // rows of the tile: BM of a, then BN of b; those past an operand's end read its last row
     const auto row_of = [&](int row) { return row < BM ? min(row, g.M - 1 - m0) : min(row - BM, g.N - 1 - n0); };
-    const __amdgpu_buffer_rsrc_t buf_a = buffer_at(g.a + (int64_t)m0 * g.pitch);
-    const __amdgpu_buffer_rsrc_t buf_b = buffer_at(g.b + (int64_t)n0 * g.pitch);
+    const __amdgpu_buffer_rsrc_t buf_a = buffer_at(g.a + (int64_t)m0 * g.pitch_a);
+    const __amdgpu_buffer_rsrc_t buf_b = buffer_at(g.b + (int64_t)n0 * g.pitch_b);
     const __amdgpu_buffer_rsrc_t buf_sa = buffer_at(g.sa + (int64_t)m0 * g.spitch);
     const __amdgpu_buffer_rsrc_t buf_sb = buffer_at(g.sb + (int64_t)n0 * g.spitch);
-    // This lane's part of each load: row l / 8 of it, piece l % 8.  The offsets are made anew for each
+    // This lane's part of each load: row l / 8 of it, piece l % 8, exchanged by bits 1 to 3 of the row,
+    // of which the last is the load's parity.  The offsets are made anew for each
     // block (`sub` is hidden from the compiler, which would keep them all in registers, and spill).
     int sub = lane / 8;
-    const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 8)) * 16;
+    const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 16)) * 16;
     const auto fetch = [&](int kb) {
         asm volatile("" : "+v"(sub));
         uint8_t* to = lds + (kb & 1) * kStage + wave * kLoads * 1024;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int first = (wave * kLoads + i) * 8;  // the same operand for the whole wave
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16,
-                                                     (uint32_t)row_of(first + sub) * (uint32_t)g.pitch + piece,
+            const uint32_t pitch = (uint32_t)(first < BM ? g.pitch_a : g.pitch_b);
+            const uint32_t at = (uint32_t)row_of(first + sub) * pitch + (piece ^ (i % 2 * 64));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16, at,
                                                      kb * kBlockK, 0, 0);
         }
         if (kb % 4 == 0) {
@@ -223,7 +226,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     uint32_t at_a[4], at_b[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-        const uint32_t p = (uint32_t)((4 * (c / 2) + 2 * q + c % 2) ^ (r & 7)) * 16;
+        const uint32_t p = (uint32_t)((4 * (c / 2) + 2 * q + c % 2) ^ (r >> 1 & 7)) * 16;
         at_a[c] = (uint32_t)(wm + r) * kBlockK + p;
         at_b[c] = (uint32_t)(BM + wn + r) * kBlockK + p;
     }
@@ -309,36 +312,54 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
             at_b[c] ^= kStage;
         }
     }
+    // The results go through this wave's part of LDS, 32 rows at a time, so that it writes whole lines: a
+    // lane holds four columns, and rows a power of two apart would all meet in one channel of L2.
+    constexpr int kCols = NT * 32, kPitch = kCols * (int)sizeof(T) + 16, kPer = 16 / (int)sizeof(T);
+    constexpr int kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
+    static_assert(kWaves * 32 * kPitch <= 2 * kStage, "the results fit where the operands were");
+    __syncthreads();
+    uint8_t* mine = lds + wave * 32 * kPitch;
+    float bias[NT][4][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int p = 0; p < 4; ++p) {
-            const int n = n0 + wn + j * 32 + p * 8 + q * 4, left = g.N - n;
-            if (left <= 0) continue;
-            float bias[4] = {};
-            if (g.bias)
+        for (int p = 0; p < 4; ++p)
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (e < left)
-                        bias[e] = g.bias_f32 ? static_cast<const float*>(g.bias)[n + e]
-                                             : (float)static_cast<const T*>(g.bias)[n + e];
+            for (int e = 0; e < 4; ++e) {
+                const int n = min(n0 + wn + j * 32 + p * 8 + q * 4 + e, g.N - 1);
+                bias[j][p][e] = !g.bias ? 0.0f
+                                : g.bias_f32 ? static_cast<const float*>(g.bias)[n]
+                                             : (float)static_cast<const T*>(g.bias)[n];
+            }
+    const int piece_col = n0 + wn + lane % kRowPieces * kPer, left = g.N - piece_col;
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int m = m0 + wm + i * 32 + r;
-                if (m >= g.M) continue;
-                T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + n;
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
                 T v[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * p + e] + bias[e]);
-                if (left >= 4) {
-                    __builtin_memcpy(out, v, sizeof(v));
-                } else {
+                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * p + e] + bias[j][p][e]);
+                __builtin_memcpy(mine + r * kPitch + (j * 32 + p * 8 + q * 4) * (int)sizeof(T), v, sizeof(v));
+            }
+        wave_sync();
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (e < left) out[e] = v[e];
-                }
+        for (int k = 0; k < 32; k += kRowsAtOnce) {
+            const int row = k + lane / kRowPieces, m = m0 + wm + i * 32 + row;
+            T v[kPer];
+            __builtin_memcpy(v, mine + row * kPitch + lane % kRowPieces * 16, 16);
+            if (m >= g.M) continue;
+            T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + piece_col;
+            if (left >= kPer) {
+                __builtin_memcpy(out, v, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < kPer; ++e)
+                    if (e < left) out[e] = v[e];
             }
         }
+        wave_sync();
     }
 }
 
@@ -379,15 +400,12 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
-}  // namespace
-}  // namespace trident
+// The pitch of codes that only this library reads: rows that are not a power of two apart, so that the
+// same columns of neighbouring rows lie in different channels of L2.
+inline int64_t own_pitch_of(int64_t K) { return pitch_of(K) + (pitch_of(K) % 1024 == 0 ? kBlockK : 0); }
 
-using namespace trident;
-
-extern "C" {
-
-int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x, uint8_t* codes,
-                         uint8_t* scales, void* stream) {
+int quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x, uint8_t* codes, int64_t pitch,
+             uint8_t* scales, void* stream) {
     if (!dtype_ok(dtype)) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_quantize: dtype=%d", dtype);
     if (!counts_ok(rows, K) || ld_x < K)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_quantize: bad sizes rows=%lld K=%lld ld=%lld",
@@ -395,7 +413,7 @@ int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, 
     if (rows == 0) return TRIDENT_OK;
     if (!x || !codes || !scales || !aligned16(codes))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_quantize: NULL pointer, or codes not 16-byte aligned");
-    QuantArgs a{x, codes, scales, rows, ld_x, (int)K, (int)blocks_of(K), (int)scale_pitch_of(K)};
+    QuantArgs a{x, codes, scales, rows, ld_x, pitch, (int)K, (int)blocks_of(K), (int)scale_pitch_of(K)};
     constexpr int per = kBlock / kQuantLanes;
     const int64_t grid = (rows * a.kb + per - 1) / per;
     if (grid > 0x7fffffff)
@@ -406,9 +424,9 @@ int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, 
     return capi_check_launch("quantize_kernel");
 }
 
-int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
-                       const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
-                       int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
+int product(const uint8_t* a_codes, int64_t pitch_a, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
+            const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
+            int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
     if (!dtype_ok(dtype) || (bias && bias_dtype != dtype && bias_dtype != TRIDENT_F32))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: dtype=%d bias_dtype=%d", dtype, bias_dtype);
     if (K > (1 << 22)) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: K=%lld is too large", (long long)K);
@@ -418,8 +436,8 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
     if (M == 0 || N == 0) return TRIDENT_OK;
     if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !aligned16(a_codes) || !aligned16(b_codes))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
-    MatmulArgs g{a_codes, b_codes, a_scales, b_scales, bias, out, pitch_of(K), ld_out, (int)M, (int)N,
-                 (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
+    const MatmulArgs g{a_codes, b_codes, a_scales, b_scales, bias, out, pitch_a, pitch_of(K), ld_out, (int)M, (int)N,
+                       (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
     int rc = TRIDENT_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
@@ -429,9 +447,28 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
     return rc;
 }
 
+}  // namespace
+}  // namespace trident
+
+using namespace trident;
+
+extern "C" {
+
+int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x, uint8_t* codes,
+                         uint8_t* scales, void* stream) {
+    return quantize(x, dtype, rows, K, ld_x, codes, pitch_of(K), scales, stream);
+}
+
+int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
+                       const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
+                       int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
+    return product(a_codes, pitch_of(K), a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
+                   fast_accum, stream);
+}
+
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t K) {
     if (!counts_ok(M, K)) return 0;
-    return up256((size_t)(M * pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
+    return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
 }
 
 int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* w_codes,
@@ -442,11 +479,11 @@ int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "fp8_linear: workspace %zu < %zu bytes, or not 16-byte aligned",
                          workspace_bytes, need);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
-    uint8_t* scales = codes + up256((size_t)(M * pitch_of(K)));
-    const int rc = trident_fp8_quantize(x, dtype, M, K, ld_x, codes, scales, stream);
+    uint8_t* scales = codes + (counts_ok(M, K) ? up256((size_t)(M * own_pitch_of(K))) : 0);
+    const int rc = quantize(x, dtype, M, K, ld_x, codes, own_pitch_of(K), scales, stream);
     if (rc) return rc;
-    return trident_fp8_matmul(codes, scales, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
-                              fast_accum, stream);
+    return product(codes, own_pitch_of(K), scales, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
+                   fast_accum, stream);
 }
 
 }  // extern "C"
