@@ -100,17 +100,20 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[N]
     }
 }
 
-// Sum over the 64 lanes of a wave, the same in every lane.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, kWave);
-    return v;
+// Sum over the 64 lanes of a wave, the same in every lane: each step adds a neighbour's partial sum in
+// the vector unit itself (no trip through LDS), 16 lanes, then the rows of 16; lane 63 ends with all.
+template <int CTRL>
+__device__ __forceinline__ float add_from(float v) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
 }
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, kWave));
-    return v;
+__device__ __forceinline__ float wave_sum(float v) {
+    v = add_from<0x111>(v);  // one lane down
+    v = add_from<0x112>(v);  // two
+    v = add_from<0x114>(v);
+    v = add_from<0x118>(v);
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x142, 0xa, 0xf, true));  // row 0 to 1, 2 to 3
+    v += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x143, 0xc, 0xf, true));  // rows 0, 1 to 2, 3
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), kWave - 1));
 }
 
 }  // namespace trident

@@ -167,17 +167,18 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
 // LDS's 64 banks (a row is half of them, so rows that differ in bit 0 never meet).  The
 // weight is the instruction's first operand, so a lane holds four neighbouring columns of a result row.
 // A block of 128 columns is two instructions of 64 each with the same scale; in both operands a lane
-// passes the same columns, in whatever order the instruction takes them.  The rows' scales of four
-// blocks, one word a row, go to LDS with the first of them: no register waits for memory in the loop, so
-// the only wait for the loads in flight is the one at the barrier.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT>
+// passes the same columns, in whatever order the instruction takes them.  The rows' scales (a word a row,
+// that of four blocks) go to LDS as well: no register waits for memory in the loop, and every block is
+// the same number of loads, so the wait before a block leaves the later ones' in flight.
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int STAGES>
 __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, kStage = (BM + BN) * kBlockK;
     constexpr int kLoads = (BM + BN) / 8 / kWaves;  // a wave's loads of eight rows each
     static_assert((BM + BN) / 8 % kWaves == 0 && kLoads % 2 == 0, "whole loads, of either parity by turns");
     constexpr int kScaleLoads = (BM + BN + kWaves * kWave - 1) / (kWaves * kWave);
     constexpr int kScaleStage = kScaleLoads * kWaves * kWave * 4;
-    extern __shared__ __align__(16) uint8_t lds[];  // [2][BM + BN][128], [2][BM + BN] words of scales
+    constexpr int kFlight = kLoads + kScaleLoads;  // a wave's loads of one block
+    extern __shared__ __align__(16) uint8_t lds[];  // [STAGES][BM + BN][128], [STAGES][BM + BN] words of scales
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r = lane & 31, q = lane >> 5;
     int tm, tn;
@@ -198,7 +199,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 16)) * 16;
     const auto fetch = [&](int kb) {
         asm volatile("" : "+v"(sub));
-        uint8_t* to = lds + (kb & 1) * kStage + wave * kLoads * 1024;
+        uint8_t* to = lds + kb % STAGES * kStage + wave * kLoads * 1024;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
             const int first = (wave * kLoads + i) * 8;  // the same operand for the whole wave
@@ -207,21 +208,19 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
             __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16, at,
                                                      kb * kBlockK, 0, 0);
         }
-        if (kb % 4 == 0) {
-            uint8_t* st = lds + 2 * kStage + (kb / 4 & 1) * kScaleStage + wave * kWave * 4;
+        uint8_t* st = lds + STAGES * kStage + kb % STAGES * kScaleStage + wave * kWave * 4;
 #pragma unroll
-            for (int i = 0; i < kScaleLoads; ++i) {
-                const int first = (i * kWaves + wave) * kWave;
-                const int row = min(first + (sub * 8 + (lane & 7)), BM + BN - 1);
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_sa : buf_sb,
-                                                         (lds_ptr)(st + i * kWaves * kWave * 4), 4,
-                                                         (uint32_t)row_of(row) * (uint32_t)g.spitch, kb, 0, 0);
-            }
+        for (int i = 0; i < kScaleLoads; ++i) {
+            const int first = (i * kWaves + wave) * kWave;
+            const int row = min(first + (sub * 8 + (lane & 7)), BM + BN - 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_sa : buf_sb,
+                                                     (lds_ptr)(st + i * kWaves * kWave * 4), 4,
+                                                     (uint32_t)row_of(row) * (uint32_t)g.spitch, kb & ~3, 0, 0);
         }
     };
     // where this lane reads the four pieces of its first row of either operand; the other rows are 32
-    // rows on, the other stage is the next bit
-    static_assert((kStage & (kStage - 1)) == 0, "a stage is a bit of the address");
+    // rows on, the stages count in the bits above
+    static_assert((kStage & (kStage - 1)) == 0 && (STAGES & (STAGES - 1)) == 0, "stages are bits of the address");
     const uint32_t origin = (uint32_t)(uintptr_t)(lds_ptr)lds;
     uint32_t at_a[4], at_b[4];
 #pragma unroll
@@ -244,20 +243,26 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     };
 
     f32x16 acc[MT][NT] = {};
-    fetch(0);
-    uint32_t ea[MT], eb[NT];  // the scale of the current block in the lowest byte
+#pragma unroll
+    for (int kb = 0; kb < STAGES - 1; ++kb)
+        if (kb < g.kb) fetch(kb);
     for (int kb = 0; kb < g.kb; ++kb) {
-        // this block has arrived, every wave's part of it, and the other stage is no longer read
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (kb + 1 < g.kb) fetch(kb + 1);
-        if (kb % 4 == 0) {
-            const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + 2 * kStage + (kb / 4 & 1) * kScaleStage);
+        // Past the barrier this block has arrived, every wave's part of it, and every wave has read the one
+        // before, whose stage the next loads take.  Loads arrive in order; those of up to STAGES - 2 later
+        // blocks stay in flight.
+        const int later = min(STAGES - 2, g.kb - 1 - kb);
+        if (later <= 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        else if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(kFlight) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * kFlight) : "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (kb + STAGES - 1 < g.kb) fetch(kb + STAGES - 1);
+        uint32_t ea[MT], eb[NT];  // the scale of this block in the lowest byte
+        const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + STAGES * kStage + kb % STAGES * kScaleStage);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r];
+        for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r] >> (kb % 4 * 8);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) eb[j] = st[BM + wn + j * 32 + r];
-        }
+        for (int j = 0; j < NT; ++j) eb[j] = st[BM + wn + j * 32 + r] >> (kb % 4 * 8);
         i32x8 fa[2][MT], fb[2][NT];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -294,7 +299,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
         if constexpr (FAST) {
             // the first half's reads, the second half's among the first half's products, the rest
             constexpr int kReads = 2 * (MT + NT), kProducts = MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
-            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads + MT + NT, 0);  // with the scales'
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
@@ -302,21 +307,18 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
             }
             __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
         }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) ea[i] >>= 8;
-#pragma unroll
-        for (int j = 0; j < NT; ++j) eb[j] >>= 8;
+        const uint32_t next = (uint32_t)((kb + 1) % STAGES ^ kb % STAGES) * kStage;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            at_a[c] ^= kStage;
-            at_b[c] ^= kStage;
+            at_a[c] ^= next;
+            at_b[c] ^= next;
         }
     }
     // The results go through this wave's part of LDS, 32 rows at a time, so that it writes whole lines: a
     // lane holds four columns, and rows a power of two apart would all meet in one channel of L2.
     constexpr int kCols = NT * 32, kPitch = kCols * (int)sizeof(T) + 16, kPer = 16 / (int)sizeof(T);
     constexpr int kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
-    static_assert(kWaves * 32 * kPitch <= 2 * kStage, "the results fit where the operands were");
+    static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the results fit where the operands were");
     __syncthreads();
     uint8_t* mine = lds + wave * 32 * kPitch;
     float bias[NT][4][4];
@@ -363,13 +365,123 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     }
 }
 
+constexpr int kFew = 16;       // rows that one instruction takes
+constexpr int kFewWaves = 8;
+
+struct FewArgs {
+    const void* x;           // [M, ldx], or null: the codes of a
+    const uint8_t *a, *sa;
+    const uint8_t *b, *sb;
+    const void* bias;
+    void* out;
+    int64_t ldx, pitch_b, ldo;
+    int M, N, K, kb, spitch, bias_f32;
+};
+
+// Up to 16 rows, bound by the weight's bytes or, for one query, by the latency of a launch.  A workgroup
+// takes 16 columns; its eight waves take the blocks of 128 of K in turn, the weight straight from memory
+// to registers, and their sums are added in order at the end.  The rows are quantised on the way (QUANT):
+// a lane holds the 32 columns of its row that the instruction wants from it, and a block's largest value
+// is that of four lanes, so one launch does all and nothing is stored between.
+template <typename T, bool FAST, bool QUANT>
+__global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g) {
+    constexpr int U = sizeof(T) == 4 ? 2 : 4;  // blocks of a wave in flight
+    __shared__ f32x4 s_acc[kFewWaves][kWave];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
+    const int64_t n = min(n0 + r, g.N - 1), m = min(r, g.M - 1);
+    const uint8_t* b = g.b + n * g.pitch_b + q * 32;
+    const uint8_t* sb = g.sb + n * g.spitch;
+    f32x4 acc = {};
+    for (int k0 = wave; k0 < g.kb; k0 += kFewWaves * U) {
+        u32x4 wb[U][2], wa[U][2];
+        Vec<T, 8> x[U][4];
+        int eb[U], ea[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int kb = min(k0 + u * kFewWaves, g.kb - 1);  // past the end: read again, not multiplied
+            __builtin_memcpy(wb[u], b + (int64_t)kb * kBlockK, 32);
+            eb[u] = sb[kb];
+            if constexpr (QUANT) {
+                const T* row = static_cast<const T*>(g.x) + m * g.ldx;
+                const int col = kb * kBlockK + q * 32;
+                if (col + 32 <= g.K) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[u][e].load(row + col + e * 8);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        T v[8];
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = col + e * 8 + i < g.K ? row[col + e * 8 + i] : (T)0.0f;
+                        x[u][e].load(v);
+                    }
+                }
+            } else {
+                __builtin_memcpy(wa[u], g.a + m * ((int64_t)g.kb * kBlockK) + (int64_t)kb * kBlockK + q * 32, 32);
+                ea[u] = g.sa[m * g.spitch + kb];
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (k0 + u * kFewWaves >= g.kb) break;
+            i32x8 fa, fb;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) fb[e] = (int)wb[u][e / 4][e % 4];
+            if constexpr (QUANT) {
+                float v[4][8], top = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    x[u][e].get(v[e]);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[e][i]) < INFINITY ? fabsf(v[e][i]) : 0.0f);
+                }
+                top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                ea[u] = scale_of(top);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint2 c = codes_of(v[e], ea[u]);
+                    fa[2 * e] = (int)c.x;
+                    fa[2 * e + 1] = (int)c.y;
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) fa[e] = (int)wa[u][e / 4][e % 4];
+            }
+            if constexpr (FAST) {
+                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc, 0, 0, 0, eb[u], 0, ea[u]);
+            } else {
+                bf16x8 ha[4], hb[4];
+                to_bf16(fa, scale_value((uint32_t)ea[u]), ha);
+                to_bf16(fb, scale_value((uint32_t)eb[u]), hb);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[k], ha[k], acc, 0, 0, 0);
+            }
+        }
+    }
+    s_acc[wave][lane] = acc;
+    __syncthreads();
+    if (wave != 0 || r >= g.M) return;
+    for (int w = 1; w < kFewWaves; ++w) acc += s_acc[w][lane];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int c = n0 + q * 4 + e;
+        if (c >= g.N) break;
+        float v = acc[e];
+        if (g.bias) v += g.bias_f32 ? static_cast<const float*>(g.bias)[c] : (float)static_cast<const T*>(g.bias)[c];
+        static_cast<T*>(g.out)[(int64_t)r * g.ldo + c] = (T)v;
+    }
+}
+
 // Launches the kernel of one tile size.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT>
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int STAGES>
 int launch_matmul(MatmulArgs g, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
     constexpr size_t scale_rows = (BM + BN + WM * WN * kWave - 1) / (WM * WN * kWave) * (WM * WN * kWave);
-    constexpr size_t lds = 2 * ((size_t)(BM + BN) * kBlockK + scale_rows * 4);
-    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT>;
+    constexpr size_t lds = STAGES * ((size_t)(BM + BN) * kBlockK + scale_rows * 4);
+    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT, STAGES>;
+    static_assert(lds <= 163840 && STAGES <= 4, "LDS of a CU; the waits of the loop");
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -389,9 +501,9 @@ template <typename T, bool FAST>
 int matmul(const MatmulArgs& g, hipStream_t st) {
     const auto tiles = [&](int64_t bm, int64_t bn) { return (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn); };
     if constexpr (FAST)
-        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2>(g, st);
-    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2>(g, st);
-    return launch_matmul<T, FAST, 2, 2, 1, 1>(g, st);
+        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2, 2>(g, st);
+    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2, 2>(g, st);
+    return launch_matmul<T, FAST, 2, 2, 1, 1, 4>(g, st);
 }
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
@@ -424,27 +536,46 @@ int quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x
     return capi_check_launch("quantize_kernel");
 }
 
-int product(const uint8_t* a_codes, int64_t pitch_a, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
-            const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
-            int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
+int check_product(int64_t M, int64_t N, int64_t K, const void* a, const void* b_codes, const void* b_scales,
+                  const void* bias, int32_t bias_dtype, const void* out, int32_t dtype, int64_t ld_out) {
     if (!dtype_ok(dtype) || (bias && bias_dtype != dtype && bias_dtype != TRIDENT_F32))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: dtype=%d bias_dtype=%d", dtype, bias_dtype);
     if (K > (1 << 22)) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: K=%lld is too large", (long long)K);
     if (!counts_ok(M, K) || !counts_ok(N, K) || ld_out < N)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: bad sizes M=%lld N=%lld K=%lld ld=%lld",
                          (long long)M, (long long)N, (long long)K, (long long)ld_out);
-    if (M == 0 || N == 0) return TRIDENT_OK;
-    if (!a_codes || !a_scales || !b_codes || !b_scales || !out || !aligned16(a_codes) || !aligned16(b_codes))
+    if (M > 0 && N > 0 && (!a || !b_codes || !b_scales || !out || !aligned16(b_codes)))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
-    const MatmulArgs g{a_codes, b_codes, a_scales, b_scales, bias, out, pitch_a, pitch_of(K), ld_out, (int)M, (int)N,
+    return TRIDENT_OK;
+}
+
+// Codes and scales of A from `a`, or (few rows) A itself from x, of out's type.
+int product(const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M, const uint8_t* b, const uint8_t* sb,
+            int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out, int32_t dtype, int64_t ld_out,
+            int32_t fast_accum, hipStream_t st) {
+    const MatmulArgs g{a, b, sa, sb, bias, out, pitch_a, pitch_of(K), ld_out, (int)M, (int)N,
                        (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
     int rc = TRIDENT_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        hipStream_t st = static_cast<hipStream_t>(stream);
         rc = fast_accum ? matmul<T, true>(g, st) : matmul<T, false>(g, st);
     });
     return rc;
+}
+
+template <bool QUANT>
+int product_few(const void* x, int64_t ld_x, const uint8_t* a, const uint8_t* sa, int64_t M, const uint8_t* b,
+                const uint8_t* sb, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
+                int32_t dtype, int64_t ld_out, int32_t fast_accum, hipStream_t st) {
+    const FewArgs g{x, a, sa, b, sb, bias, out, ld_x, pitch_of(K), ld_out, (int)M, (int)N, (int)K,
+                    (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32};
+    const unsigned grid = (unsigned)((N + 15) / 16);
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        if (fast_accum) matmul_few_kernel<T, true, QUANT><<<grid, kFewWaves * kWave, 0, st>>>(g);
+        else matmul_few_kernel<T, false, QUANT><<<grid, kFewWaves * kWave, 0, st>>>(g);
+    });
+    return capi_check_launch("matmul_few_kernel");
 }
 
 }  // namespace
@@ -462,28 +593,44 @@ int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, 
 int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t M, const uint8_t* b_codes,
                        const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
                        int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
+    const int rc = check_product(M, N, K, a_codes, b_codes, b_scales, bias, bias_dtype, out, dtype, ld_out);
+    if (rc || M == 0 || N == 0) return rc;
+    if (!a_scales || !aligned16(a_codes))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (M <= kFew)
+        return product_few<false>(nullptr, 0, a_codes, a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out,
+                                  dtype, ld_out, fast_accum, st);
     return product(a_codes, pitch_of(K), a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
-                   fast_accum, stream);
+                   fast_accum, st);
 }
 
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t K) {
-    if (!counts_ok(M, K)) return 0;
+    if (!counts_ok(M, K) || M <= kFew) return 0;
     return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
 }
 
 int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* w_codes,
                        const uint8_t* w_scales, int64_t N, const void* bias, int32_t bias_dtype, void* out,
                        int64_t ld_out, int32_t fast_accum, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check_product(M, N, K, x, w_codes, w_scales, bias, bias_dtype, out, dtype, ld_out);
+    if (rc) return rc;
+    if (ld_x < K)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_linear: ld=%lld < K=%lld", (long long)ld_x, (long long)K);
+    if (M == 0 || N == 0) return TRIDENT_OK;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    if (M <= kFew)
+        return product_few<true>(x, ld_x, nullptr, nullptr, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype,
+                                 ld_out, fast_accum, st);
     const size_t need = trident_fp8_linear_workspace_bytes(M, K);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "fp8_linear: workspace %zu < %zu bytes, or not 16-byte aligned",
                          workspace_bytes, need);
     uint8_t* codes = static_cast<uint8_t*>(workspace);
-    uint8_t* scales = codes + (counts_ok(M, K) ? up256((size_t)(M * own_pitch_of(K))) : 0);
-    const int rc = quantize(x, dtype, M, K, ld_x, codes, own_pitch_of(K), scales, stream);
-    if (rc) return rc;
+    uint8_t* scales = codes + up256((size_t)(M * own_pitch_of(K)));
+    if ((rc = quantize(x, dtype, M, K, ld_x, codes, own_pitch_of(K), scales, stream))) return rc;
     return product(codes, own_pitch_of(K), scales, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
-                   fast_accum, stream);
+                   fast_accum, st);
 }
 
 }  // extern "C"

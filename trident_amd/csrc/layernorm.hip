@@ -46,16 +46,27 @@ struct Columns {
     }
 };
 
-template <typename T, int VEC, int NV, int W>
-__device__ __forceinline__ void load_row(const T* p, const Columns<VEC, NV, W>& k, float (&f)[NV][VEC]) {
+template <typename T, int VEC, int NV>
+struct Row {
+    Vec<T, VEC> v[NV];
+    template <int W>
+    __device__ __forceinline__ void load(const T* __restrict__ p, const Columns<VEC, NV, W>& k) {
 #pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        if (k.on[c]) load_vec(p + k.col[c], f[c]);
-        else
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) f[c][i] = 0.0f;
+        for (int c = 0; c < NV; ++c)
+            if (k.on[c]) v[c].load(p + k.col[c]);
     }
-}
+    // the values, zeros in a lane's vectors past the row
+    template <int W>
+    __device__ __forceinline__ void get(const Columns<VEC, NV, W>& k, float (&f)[NV][VEC]) const {
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            if (k.on[c]) v[c].get(f[c]);
+            else
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) f[c][i] = 0.0f;
+        }
+    }
+};
 
 // Sum over the W waves that share a row; with W > 1 every thread of the workgroup calls it.
 template <int W>
@@ -72,52 +83,68 @@ __device__ __forceinline__ float row_sum(float v, float* s_red) {
     return v;
 }
 
-// One wave per row up to NV * 64 vectors, else one workgroup of W = 4 waves.
+// Bound by bytes.  A wave (a workgroup of W = 4 waves for rows of more than 256 vectors) takes every
+// gridDim-th row and loads the next one while it works on this one.
 template <typename T, typename TW, int VEC, int NV, int W>
 __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
     __shared__ float s_red[W];
     constexpr int kRows = kWavesPerBlock / W;
-    const int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? threadIdx.x / kWave : 0);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0);
     if (row >= a.rows) return;
     Columns<VEC, NV, W> k;
     k.init(a, W == 1 ? lane_id() : threadIdx.x);
-    float x[NV][VEC];
-    load_row<T>(static_cast<const T*>(a.x) + row * a.ldx, k, x);
-    float s = 0.0f;
+    const T* X = static_cast<const T*>(a.x);
+    Row<T, VEC, NV> now, next;
+    Row<TW, VEC, NV> weight, bias;
+    now.load(X + row * a.ldx, k);
+    if (a.weight) weight.load(static_cast<const TW*>(a.weight), k);
+    if (a.bias) bias.load(static_cast<const TW*>(a.bias), k);
+    for (;;) {
+        const bool more = row + step < a.rows;
+        if (more) next.load(X + (row + step) * a.ldx, k);
+        float x[NV][VEC];
+        now.get(k, x);
+        float s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+        for (int c = 0; c < NV; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (i >= k.dup[c]) s += x[c][i];
-    const float mean = row_sum<W>(s, s_red) * a.inv_D;
-    s = 0.0f;
+            for (int i = 0; i < VEC; ++i)
+                if (i >= k.dup[c]) s += x[c][i];
+        const float mean = row_sum<W>(s, s_red) * a.inv_D;
+        s = 0.0f;
 #pragma unroll
-    for (int c = 0; c < NV; ++c)
+        for (int c = 0; c < NV; ++c)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            x[c][i] -= mean;
-            if (k.on[c] && i >= k.dup[c]) s += x[c][i] * x[c][i];
+            for (int i = 0; i < VEC; ++i) {
+                x[c][i] -= mean;
+                if (k.on[c] && i >= k.dup[c]) s += x[c][i] * x[c][i];
+            }
+        const float rstd = 1.0f / sqrtf(row_sum<W>(s, s_red) * a.inv_D + a.eps);
+        T* y = static_cast<T*>(a.y) + row * a.ldy;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            if (!k.on[c]) continue;
+            float w[VEC], b[VEC];
+            if (a.weight) weight.v[c].get(w);
+            if (a.bias) bias.v[c].get(b);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) {
+                float v = x[c][i] * rstd;
+                if (a.weight) v *= w[i];
+                if (a.bias) v += b[i];
+                x[c][i] = v;
+            }
+            store_vec(y + k.col[c], x[c]);
         }
-    const float rstd = 1.0f / sqrtf(row_sum<W>(s, s_red) * a.inv_D + a.eps);
-    T* y = static_cast<T*>(a.y) + row * a.ldy;
-#pragma unroll
-    for (int c = 0; c < NV; ++c) {
-        if (!k.on[c]) continue;
-        float w[VEC], b[VEC];
-        if (a.weight) load_vec(static_cast<const TW*>(a.weight) + k.col[c], w);
-        if (a.bias) load_vec(static_cast<const TW*>(a.bias) + k.col[c], b);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            float v = x[c][i] * rstd;
-            if (a.weight) v *= w[i];
-            if (a.bias) v += b[i];
-            x[c][i] = v;
+        if (a.mean && (W == 1 ? lane_id() : (int)threadIdx.x) == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
         }
-        store_vec(y + k.col[c], x[c]);
-    }
-    if (a.mean && (W == 1 ? lane_id() : (int)threadIdx.x) == 0) {
-        a.mean[row] = mean;
-        a.rstd[row] = rstd;
+        if (!more) return;
+        now = next;
+        row += step;
     }
 }
 
@@ -146,46 +173,56 @@ __global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
     }
 }
 
-// A wave (or a workgroup, W = 4) takes every gridDim-th row: dx from the row's two means, and dy h and
-// dy added to the columns' sums, which stay in registers until the last row.
+// Bound by bytes.  A wave (or a workgroup, W = 4) takes every gridDim-th row, the next one's loads ahead
+// of this one's work: dx from the row's two means, and dy h and dy added to the columns' sums, which stay
+// in registers until the last row.
 template <typename T, typename TW, int VEC, int NV, int W>
 __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
     extern __shared__ float s_part[];  // [kWavesPerBlock][D], W = 1 only
     __shared__ float s_red[W];
     constexpr int kRows = kWavesPerBlock / W;
-    const int wave = threadIdx.x / kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     Columns<VEC, NV, W> k;
     k.init(a, W == 1 ? lane_id() : threadIdx.x);
-    float w[NV][VEC], dw[NV][VEC], db[NV][VEC];
-#pragma unroll
-    for (int c = 0; c < NV; ++c)
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            w[c][i] = 1.0f;
-            dw[c][i] = db[c][i] = 0.0f;
+    float dw[NV][VEC] = {}, db[NV][VEC] = {};
+    Row<TW, VEC, NV> weight;
+    if (a.weight) weight.load(static_cast<const TW*>(a.weight), k);
+    const T* X = static_cast<const T*>(a.x);
+    const T* DY = static_cast<const T*>(a.dy);
+    const int64_t step = (int64_t)gridDim.x * kRows;
+    int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0);
+    Row<T, VEC, NV> now_x, now_dy, next_x, next_dy;
+    if (row < a.rows) {
+        now_x.load(X + row * a.ldx, k);
+        now_dy.load(DY + row * a.lddy, k);
+    }
+    for (; row < a.rows; row += step) {
+        if (row + step < a.rows) {
+            next_x.load(X + (row + step) * a.ldx, k);
+            next_dy.load(DY + (row + step) * a.lddy, k);
         }
-    if (a.weight) load_row<TW>(static_cast<const TW*>(a.weight), k, w);
-    for (int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0); row < a.rows;
-         row += (int64_t)gridDim.x * kRows) {
-        float h[NV][VEC], g[NV][VEC];
-        load_row<T>(static_cast<const T*>(a.x) + row * a.ldx, k, h);
-        load_row<T>(static_cast<const T*>(a.dy) + row * a.lddy, k, g);
         const float mean = a.mean[row], rstd = a.rstd[row];
+        float h[NV][VEC], g[NV][VEC];
+        now_x.get(k, h);
+        now_dy.get(k, g);
         float sa = 0.0f, sh = 0.0f;
 #pragma unroll
-        for (int c = 0; c < NV; ++c)
+        for (int c = 0; c < NV; ++c) {
+            float w[VEC];
+            if (a.weight) weight.v[c].get(w);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
                 h[c][i] = (h[c][i] - mean) * rstd;
                 const float dy = g[c][i];
                 dw[c][i] += dy * h[c][i];
                 db[c][i] += dy;
-                g[c][i] = dy * w[c][i];
+                if (a.weight) g[c][i] = dy * w[i];
                 if (k.on[c] && i >= k.dup[c]) {
                     sa += g[c][i];
                     sh += g[c][i] * h[c][i];
                 }
             }
+        }
         sa = row_sum<W>(sa, s_red) * a.inv_D;
         sh = row_sum<W>(sh, s_red) * a.inv_D;
         T* dx = static_cast<T*>(a.dx) + row * a.lddx;
@@ -196,6 +233,8 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
             for (int i = 0; i < VEC; ++i) g[c][i] = rstd * (g[c][i] - sa - h[c][i] * sh);
             store_vec(dx + k.col[c], g[c]);
         }
+        now_x = next_x;
+        now_dy = next_dy;
     }
     float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
     if constexpr (W == 1) {
@@ -309,7 +348,8 @@ bool with_shape(int64_t D, F&& f) {
     return false;
 }
 
-constexpr int kGradBlocks = 512;  // workgroups that share the rows of a backward pass
+constexpr int kNormBlocks = 2048;  // workgroups of a forward pass: all that 256 CUs hold
+constexpr int kGradBlocks = 1024;  // of a backward pass, each of which leaves a share of the weight's gradient
 
 int64_t grad_parts(int64_t rows) {
     return std::max<int64_t>(1, std::min<int64_t>(kGradBlocks, (rows + kWavesPerBlock - 1) / kWavesPerBlock));
@@ -346,7 +386,8 @@ int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, in
                     constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
                     const int64_t per = kWavesPerBlock / W;
-                    norm_kernel<T, TW, VEC, NV, W><<<(unsigned)((rows + per - 1) / per), kBlock, 0, st>>>(a);
+                    const unsigned grid = (unsigned)std::min<int64_t>(kNormBlocks, (rows + per - 1) / per);
+                    norm_kernel<T, TW, VEC, NV, W><<<grid, kBlock, 0, st>>>(a);
                 });
                 if (!ok) norm_long_kernel<T, TW><<<(unsigned)rows, kBlock, 0, st>>>(a);
             }

@@ -501,8 +501,11 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     bcode = _bias(bias, N, x.dtype, index)
     xr, ld = _rows(x)
     out = x.new_empty((*x.shape[:-1], N))
+    args = ("trident_fp8_linear", xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(), weight.scales.data_ptr(), N,
+            None if bias is None else bias.data_ptr(), bcode, out.data_ptr(), max(N, 1), fast_accum)
     nbytes = _fn("trident_fp8_linear_workspace_bytes")(M, K)
-    _call_ws(x.device, index, "trident_fp8_linear", nbytes, xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(),
-             weight.scales.data_ptr(), N, None if bias is None else bias.data_ptr(), bcode, out.data_ptr(),
-             max(N, 1), fast_accum)
+    if nbytes:
+        _call_ws(x.device, index, args[0], nbytes, *args[1:])
+    else:
+        _call(index, *args, None, 0)
     return out
