@@ -47,12 +47,13 @@ def test_embedding_arguments():
     refused(L.trident_embedding(P, 0, 10, 8, 8, P, 1, 1 << 31, 1.0, P, 8, None), 1, "bad sizes")
     refused(L.trident_embedding(None, 0, 10, 8, 8, P, 1, 4, 1.0, P, 8, None), 1, "NULL")
     assert L.trident_embedding(None, 0, 10, 8, 8, None, 1, 0, 1.0, None, 8, None) == 0
-    need = L.trident_embedding_grad_workspace_bytes(1000, 50, 64)
-    assert need >= 51 * 4 + 1000 * 4 + 2 * 16 * 64 * 4
+    assert L.trident_embedding_grad_workspace_bytes(1000, 50, 64) == 0
+    need = L.trident_embedding_grad_workspace_bytes(10_000, 50, 64)
+    assert need >= 51 * 8 + 10_000 * 8 + 2 * 313 * 64 * 4
     assert L.trident_embedding_grad_workspace_bytes(-1, 50, 64) == 0
-    refused(L.trident_embedding_grad(P, 0, 64, P, 1, 1000, 50, 64, 1.0, -1, P, 64, P, need - 1, None), 3, str(need))
-    refused(L.trident_embedding_grad(P, 0, 64, P, 1, 1000, 50, 64, 1.0, -1, None, 64, P, need, None), 1, "NULL")
-    refused(L.trident_embedding_grad(P, 0, 63, P, 1, 1000, 50, 64, 1.0, -1, P, 64, P, need, None), 1, "bad sizes")
+    refused(L.trident_embedding_grad(P, 0, 64, P, 1, 10_000, 50, 64, 1.0, -1, P, 64, P, need - 1, None), 3, str(need))
+    refused(L.trident_embedding_grad(P, 0, 64, P, 1, 10_000, 50, 64, 1.0, -1, None, 64, P, need, None), 1, "NULL")
+    refused(L.trident_embedding_grad(P, 0, 63, P, 1, 10_000, 50, 64, 1.0, -1, P, 64, P, need, None), 1, "bad sizes")
 
 
 def test_layer_norm_arguments():

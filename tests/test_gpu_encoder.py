@@ -123,7 +123,7 @@ def test_embedding_grad_long_rows(dev, counts):
     g = gen(len(counts))
     ids = torch.repeat_interleave(torch.arange(len(counts), device=dev), torch.tensor(counts, device=dev))
     ids = ids[torch.randperm(ids.numel(), generator=g, device=dev)]
-    for D in (3, 72, 600):
+    for D in (3, 72, 600, 1100):  # one launch; past 1024 columns the tokens are cut into parts
         check_embedding_grad(randn(g, ids.numel(), D), ids, len(counts))
 
 
@@ -135,7 +135,7 @@ def test_embedding_grad_rows_across_chunks(dev, dtype, counts):
     g = gen(sum(counts))
     ids = torch.repeat_interleave(torch.arange(len(counts), device=dev), torch.tensor(counts, device=dev))
     ids = ids[torch.randperm(ids.numel(), generator=g, device=dev)]
-    for D in (5, 40, 700):
+    for D in (5, 40, 700, 1100):
         check_embedding_grad(randn(g, ids.numel(), D, dtype=dtype), ids, len(counts), scale=2.0)
 
 
@@ -768,7 +768,10 @@ def test_refusals(dev):
         (lambda: encoder.AdamW([f], state_bits=16), "state_bits"),
         (lambda: encoder.AdamW([f], betas=(1.0, 0.9)), "betas"),
         (lambda: encoder.AdamW([f]).step([f, f]), "gradients are needed"),
-        (lambda: encoder.AdamW([f]).step([f[:2]]), "gradient 0"),
+        (lambda: encoder.AdamW([f]).step([f[:2]]), "shapes"),
+        (lambda: encoder.AdamW([f]).step([f.double()]), "got torch.float64"),
+        (lambda: encoder.AdamW([f]).step([f.cpu()]), "must be dense, on"),
+        (lambda: encoder.AdamW([f]).step([f.to_sparse()]), "must be dense"),
         (lambda: encoder.AdamW([f], state_bits=8).load_state(1, f, f), "exp_avg must be"),
         (lambda: encoder.AdamW([f]).load_state_dict(dict(state_bits=8)), "8 bits"),
         (lambda: encoder.quantize_fp8(f[0]), r"\[rows, K\]"),

@@ -496,6 +496,177 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
     }
 }
 
+// Few tokens, in one launch: the time is that of launches, not of bytes.  Workgroup b owns the ids = b
+// modulo gridDim.x as in sort_ids_kernel, orders its tokens in LDS, and sums and writes its own rows, so
+// nothing passes between workgroups: groups of lanes take the rows in turn; the rows of more than
+// kShared tokens are then summed by all groups together.
+constexpr int kFewThreads = 512;
+constexpr int kFewTokens = 8192;           // 16 a thread, held in registers
+constexpr int kFewElements = 512 * 1024;   // tokens * columns: past it one workgroup may have too much to sum
+constexpr int kShared = 8;
+
+struct FewArgs {
+    const void *grad, *ids;
+    void* out;
+    int64_t ld, ldo;
+    int n, V, D, nv, owned, shift, lanes;
+    uint32_t skip;
+    float scale;
+};
+
+inline size_t few_lds(int owned, int nvl, int vec) {
+    const size_t sums = (size_t)kFewThreads * nvl * vec * sizeof(float);
+    return ((size_t)kFewThreads / kWave * owned + 2 * owned + 1) * sizeof(int) + kFewTokens * sizeof(uint16_t) + sums;
+}
+
+template <typename T, int VEC, int NVL, typename ID>
+__global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) {
+    constexpr int WAVES = kFewThreads / kWave, A = kFewTokens / kFewThreads;
+    extern __shared__ __align__(16) float sums[];  // [NVL * VEC][kFewThreads]
+    __shared__ int s_sum[WAVES], s_shared;
+    const int w = a.owned, lane = lane_id(), wave = threadIdx.x / kWave;
+    int* hist = reinterpret_cast<int*>(sums + kFewThreads * NVL * VEC);    // [WAVES][w]
+    int* start = hist + WAVES * w;                                         // [w + 1]
+    int* shared_rows = start + w + 1;                                      // [w]
+    uint16_t* order = reinterpret_cast<uint16_t*>(shared_rows + w);        // tokens by id
+    const uint32_t b = blockIdx.x, mask = (1u << a.shift) - 1;
+    const ID* ids = static_cast<const ID*>(a.ids);
+    for (int i = threadIdx.x; i < WAVES * w; i += kFewThreads) hist[i] = 0;
+    if (threadIdx.x == 0) s_shared = 0;
+    const int per = (a.n + kFewThreads - 1) / kFewThreads;  // groups of 64 tokens of a wave
+    const int first = wave * per * kWave + lane;
+    uint32_t rel[A];
+#pragma unroll
+    for (int u = 0; u < A; ++u) {
+        const int t = first + u * kWave;
+        const bool in = u < per && t < a.n;
+        const ID raw = u < per ? ids[min(t, a.n - 1)] : (ID)-1;
+        const uint32_t id = in ? row_id<true>(raw, (uint32_t)a.V, a.skip) : ~0u;
+        rel[u] = id != ~0u && (id & mask) == b ? id >> a.shift : ~0u;
+    }
+    __syncthreads();
+    int* mine = hist + wave * w;
+#pragma unroll
+    for (int u = 0; u < A; ++u)
+        if (rel[u] != ~0u) atomicAdd(&mine[rel[u]], 1);
+    __syncthreads();
+    int place = 0;
+    for (int j0 = 0; j0 < w; j0 += kFewThreads) {
+        const int j = j0 + threadIdx.x;
+        int count = 0, total;
+        if (j < w)
+            for (int i = 0; i < WAVES; ++i) count += hist[i * w + j];
+        int at = place + block_sum<WAVES>(count, s_sum, &total) - count;
+        place += total;
+        if (j < w) {
+            start[j] = at;
+            if (count > kShared) shared_rows[atomicAdd(&s_shared, 1)] = j;  // in any order
+            for (int i = 0; i < WAVES; ++i) {
+                const int c = hist[i * w + j];
+                hist[i * w + j] = at;
+                at += c;
+            }
+        }
+    }
+    if (threadIdx.x == 0) start[w] = place;
+    __syncthreads();
+    int bits = 0;
+    while ((1 << bits) < w) ++bits;
+#pragma unroll
+    for (int u = 0; u < A; ++u) {
+        if (!__ballot(rel[u] != ~0u)) continue;
+        const uint64_t same = lanes_with(rel[u] != ~0u, rel[u], bits);
+        if (rel[u] != ~0u) {
+            const int rank = mask_rank(same), at = mine[rel[u]];
+            order[at + rank] = (uint16_t)(first + u * kWave);
+            wave_sync();
+            if (rank == 0) mine[rel[u]] = at + __popcll((unsigned long long)same);
+        }
+        wave_sync();
+    }
+    __syncthreads();
+
+    const int groups = kFewThreads / a.lanes, group = threadIdx.x / a.lanes, l = threadIdx.x % a.lanes;
+    const T* g = static_cast<const T*>(a.grad);
+    int col[NVL];
+    bool on[NVL];
+    float acc[NVL][VEC];
+#pragma unroll
+    for (int c = 0; c < NVL; ++c) {
+        const int v = c * a.lanes + l;
+        on[c] = v < a.nv;
+        col[c] = min(v * VEC, a.D - VEC);
+    }
+    const auto clear = [&] {
+#pragma unroll
+        for (int c = 0; c < NVL; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
+    };
+    // adds the tokens order[beg], order[beg + step] .. below end, four in flight
+    const auto add = [&](int beg, int end, int step) {
+        for (int k = beg; k < end; k += 4 * step) {
+            Vec<T, VEC> f[4][NVL];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + u * step < end) {
+                    const T* row = g + (int64_t)order[k + u * step] * a.ld;
+#pragma unroll
+                    for (int c = 0; c < NVL; ++c)
+                        if (on[c]) f[u][c].load(row + col[c]);
+                }
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (k + u * step < end)
+#pragma unroll
+                    for (int c = 0; c < NVL; ++c) {
+                        float x[VEC];
+                        f[u][c].get(x);
+#pragma unroll
+                        for (int i = 0; i < VEC; ++i) acc[c][i] += x[i];
+                    }
+        }
+    };
+    const auto write = [&](int j) {
+        T* out = static_cast<T*>(a.out) + (((int64_t)j << a.shift) + b) * a.ldo;
+#pragma unroll
+        for (int c = 0; c < NVL; ++c)
+            if (on[c]) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) acc[c][i] *= a.scale;
+                store_vec(out + col[c], acc[c]);
+            }
+    };
+    const int rows = (int)(((int64_t)a.V - b + mask) >> a.shift);  // owned ids below V
+    for (int j = group; j < rows; j += groups) {
+        const int beg = start[j], end = start[j + 1];
+        if (end - beg > kShared) continue;
+        clear();
+        add(beg, end, 1);
+        write(j);
+    }
+    for (int i = 0; i < s_shared; ++i) {  // the same in every thread
+        const int j = shared_rows[i], beg = start[j], end = start[j + 1];
+        clear();
+        add(beg + group, end, groups);
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < NVL; ++c)
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) sums[(c * VEC + i) * kFewThreads + threadIdx.x] = acc[c][i];
+        __syncthreads();
+        if (group == 0) {
+            const int used = min(groups, end - beg);
+#pragma unroll
+            for (int c = 0; c < NVL; ++c)
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    for (int k = 1; k < used; ++k) acc[c][i] += sums[(c * VEC + i) * kFewThreads + k * a.lanes + l];
+            write(j);
+        }
+    }
+}
+
 template <typename F>
 void with_ids(int32_t ids64, F&& f) {
     if (ids64) f(int64_t{});
@@ -568,6 +739,43 @@ int order_tokens(const SortArgs& a, hipStream_t st) {
     return rc ? rc : sort_ids<ID, 16, SKIP, true>(a, st);
 }
 
+// Which calls take one launch (of about 5 us) instead of three: at most kFewTokens and kFewElements, rows
+// within one group's registers, and ids within the 256 workgroups' counters.
+bool few_ok(int64_t n, int64_t V, int64_t D) {
+    return n > 0 && n <= kFewTokens && n * D <= kFewElements && D <= 1024 && V <= (int64_t)kMaxOwned << 8;
+}
+
+template <typename T, typename ID>
+int embed_grad_few(const void* grad, int64_t ld, const void* ids, int64_t n, int64_t V, int64_t D, double scale,
+                   int64_t padding_idx, void* out, int64_t ldo, hipStream_t st) {
+    FewArgs a{grad, ids, out, ld, ldo, (int)n, (int)V, (int)D, 0, (int)((V + 255) >> 8), 8, 1,
+              padding_idx >= 0 && padding_idx < V ? (uint32_t)padding_idx : ~0u, (float)scale};
+    const int vec = D >= kVec<T> ? kVec<T> : 1;
+    a.nv = (int)((D + vec - 1) / vec);
+    while (a.lanes < a.nv && a.lanes < kWave) a.lanes *= 2;
+    const int nvl = vec == 1 ? 1 : (a.nv + kWave - 1) / kWave;
+    const unsigned grid = (unsigned)std::min<int64_t>(256, V);
+    const auto go = [&](auto v, auto c) {
+        constexpr int VEC = decltype(v)::value, NVL = decltype(c)::value;
+        const auto kernel = embed_grad_few_kernel<T, VEC, NVL, ID>;
+        const size_t lds = few_lds(a.owned, NVL, VEC);
+        if (lds > 65536) {
+            const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                     hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+            if (e != hipSuccess)
+                return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(embed_grad): %s", hipGetErrorString(e));
+        }
+        kernel<<<grid, kFewThreads, lds, st>>>(a);
+        return capi_check_launch("embed_grad_few_kernel");
+    };
+    using std::integral_constant;
+    integral_constant<int, kVec<T>> v;
+    if (vec == 1) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+    if (nvl == 1) return go(v, integral_constant<int, 1>{});
+    if (nvl == 2) return go(v, integral_constant<int, 2>{});
+    return go(v, integral_constant<int, 4>{});
+}
+
 constexpr int64_t kMaxCount = 0x7fffffff - 4096;  // tokens, rows and columns count in 32 bits
 
 }  // namespace
@@ -609,7 +817,7 @@ int trident_embedding(const void* weight, int32_t dtype, int64_t V, int64_t D, i
 
 size_t trident_embedding_grad_workspace_bytes(int64_t n, int64_t V, int64_t D) {
     if (n < 0 || V < 1 || D < 1 || n > kMaxCount || V > kMaxCount || D > kMaxCount) return 0;
-    return grad_space(nullptr, n, V, D).bytes;
+    return few_ok(n, V, D) ? 0 : grad_space(nullptr, n, V, D).bytes;
 }
 
 int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, const void* ids, int32_t ids64,
@@ -623,12 +831,21 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "embedding_grad: NULL pointer");
     if (D > 65535 * (int64_t)kWave)
         return capi_fail(TRIDENT_ERR_UNSUPPORTED, "embedding_grad: D=%lld is too large", (long long)D);
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    int rc = TRIDENT_OK;
+    if (few_ok(n, V, D)) {
+        with_ids(ids64, [&](auto i) {
+            using ID = decltype(i);
+            with_dtype(dtype, [&](auto t) {
+                rc = embed_grad_few<decltype(t), ID>(grad, ld_grad, ids, n, V, D, scale, padding_idx, out, ld_out, st);
+            });
+        });
+        return rc;
+    }
     const GradSpace s = grad_space(workspace, n, V, D);
     if (!workspace || workspace_bytes < s.bytes)
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "embedding_grad: workspace %zu < %zu bytes", workspace_bytes,
                          s.bytes);
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    int rc = TRIDENT_OK;
     with_ids(ids64, [&](auto i) {
         using ID = decltype(i);
         const SortArgs order{ids, (int)n, (int)V, s.owned, s.shift, (int)s.chunk, s.parts,

@@ -23,6 +23,7 @@ struct NormArgs {
     float* mean;          // [rows] or null
     float* rstd;
     float* part;          // [workgroups, 2, D]
+    void *dw, *db;        // [D] or null: written by the only workgroup of a pass over few rows
     int64_t rows, ldx, lddy, ldy, lddx;
     int D, nv;            // nv: vectors of a row
     float eps, inv_D;
@@ -238,8 +239,10 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
     }
     float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
     if constexpr (W == 1) {
+        const bool only = gridDim.x == 1;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
+            TW* out = static_cast<TW*>(which ? a.db : a.dw);
             __syncthreads();
 #pragma unroll
             for (int c = 0; c < NV; ++c)
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
                 float s = s_part[d];
 #pragma unroll
                 for (int i = 1; i < kWavesPerBlock; ++i) s += s_part[i * a.D + d];
-                part[which * a.D + d] = s;
+                if (!only) part[which * a.D + d] = s;
+                else if (out) out[d] = (TW)s;
             }
         }
     } else {
@@ -349,10 +353,11 @@ bool with_shape(int64_t D, F&& f) {
 }
 
 constexpr int kNormBlocks = 2048;  // workgroups of a forward pass: all that 256 CUs hold
-constexpr int kGradBlocks = 1024;  // of a backward pass, each of which leaves a share of the weight's gradient
+constexpr int kGradBlocks = 512;   // of a backward pass, each of which leaves a share of the weight's gradient
+constexpr int kFewRows = 32;       // one workgroup takes these, and its share is the gradient
 
 int64_t grad_parts(int64_t rows) {
-    return std::max<int64_t>(1, std::min<int64_t>(kGradBlocks, (rows + kWavesPerBlock - 1) / kWavesPerBlock));
+    return rows <= kFewRows ? 1 : std::min<int64_t>(kGradBlocks, (rows + kWavesPerBlock - 1) / kWavesPerBlock);
 }
 
 bool sizes_ok(int64_t rows, int64_t D) { return rows >= 0 && rows <= 0x7fffffff && D >= 1 && D <= (1 << 29); }
@@ -380,8 +385,8 @@ int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, in
         with_dtype(weight_dtype, [&](auto u) {
             using TW = decltype(u);
             if constexpr (std::is_same<T, TW>::value || std::is_same<TW, float>::value) {
-                NormArgs a{x, nullptr, weight, bias, y, nullptr, mean, rstd, nullptr, rows, ld_x, 0, ld_y, 0, (int)D, 0,
-                           (float)eps, (float)(1.0 / (double)D)};
+                NormArgs a{x, nullptr, weight, bias, y, nullptr, mean, rstd, nullptr, nullptr, nullptr, rows, ld_x, 0, ld_y,
+                           0, (int)D, 0, (float)eps, (float)(1.0 / (double)D)};
                 const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
                     constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
@@ -427,17 +432,19 @@ int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_
             using TW = decltype(u);
             if constexpr (std::is_same<T, TW>::value || std::is_same<TW, float>::value) {
                 NormArgs a{x, dy, weight, nullptr, nullptr, dx, const_cast<float*>(mean), const_cast<float*>(rstd),
-                           static_cast<float*>(workspace), rows, ld_x, ld_dy, 0, ld_dx, (int)D, 0, 0.0f,
-                           (float)(1.0 / (double)D)};
+                           static_cast<float*>(workspace), dweight, dbias, rows, ld_x, ld_dy, 0, ld_dx, (int)D, 0,
+                           0.0f, (float)(1.0 / (double)D)};
                 // with no rows every share is zero: the kernels' loops are empty
+                bool joined = !dweight && !dbias;
                 const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
                     constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
                     const size_t lds = W == 1 ? kWavesPerBlock * (size_t)D * sizeof(float) : 0;
                     norm_grad_kernel<T, TW, VEC, NV, W><<<(unsigned)parts, kBlock, lds, st>>>(a);
+                    joined = joined || (W == 1 && parts == 1);
                 });
                 if (!ok) norm_grad_long_kernel<T, TW><<<(unsigned)parts, kBlock, 0, st>>>(a);
-                if ((rc = capi_check_launch("norm_grad_kernel")) || (!dweight && !dbias)) return;
+                if ((rc = capi_check_launch("norm_grad_kernel")) || joined) return;
                 norm_join_kernel<TW><<<(unsigned)((2 * D + kWave - 1) / kWave), kJoinBlock, 0, st>>>(
                     static_cast<const float*>(workspace), (int)parts, (int)D, static_cast<TW*>(dweight),
                     static_cast<TW*>(dbias));

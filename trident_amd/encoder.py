@@ -91,7 +91,10 @@ def _call(index: int, name: str, *args) -> None:
 
 
 def _call_ws(device: torch.device, index: int, name: str, nbytes: int, *args) -> None:
-    """_call with this stream's workspace of at least ``nbytes`` as the last two arguments."""
+    """_call with this stream's workspace of at least ``nbytes`` as the last two arguments, or, for none,
+    without one."""
+    if nbytes == 0:
+        return _call(index, name, *args, None, 0)
     slot = ext._ws_cache.get((device, _raw_stream(index)))
     if slot is None:
         slot = ext._workspace_slot(device, torch.cuda.current_stream(device))
@@ -179,9 +182,9 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
             _refuse(f"out must be [{num_rows}, {D}] {grad.dtype} with whole rows")
         if num_rows > 1:
             ld_out = out.stride(0)
-    nbytes = _fn("trident_embedding_grad_workspace_bytes")(n, num_rows, D)
-    _call_ws(grad.device, index, "trident_embedding_grad", nbytes, g.data_ptr(), code, ld, idc.data_ptr(), wide, n,
-             num_rows, D, scale, -1 if padding_idx is None else padding_idx, out.data_ptr(), ld_out)
+    _call_ws(grad.device, index, "trident_embedding_grad", _fn("trident_embedding_grad_workspace_bytes")(n, num_rows, D),
+             g.data_ptr(), code, ld, idc.data_ptr(), wide, n, num_rows, D, scale,
+             -1 if padding_idx is None else padding_idx, out.data_ptr(), ld_out)
     return out
 
 
@@ -214,7 +217,7 @@ def _norm(x, weight, bias, eps, keep):
         _refuse(f"x must be [..., D], got {tuple(x.shape)}")
     wcode = _affine(index, x, D, weight, bias)
     xr, ld = _rows(x)
-    y = x.new_empty(x.shape)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = None
     if keep:
         mean, rstd = x.new_empty((2, *x.shape[:-1]), dtype=torch.float32)
@@ -279,7 +282,7 @@ def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
     wdtype = x.dtype if wdtype is None else wdtype
     xr, ldx = _rows(x)
     gr, ldg = _rows(grad)
-    dx = x.new_empty(x.shape)
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = x.new_empty(D, dtype=wdtype) if need_w else None
     db = x.new_empty(D, dtype=wdtype) if need_b else None
     nbytes = _fn("trident_layer_norm_grad_workspace_bytes")(rows, D)
@@ -329,7 +332,10 @@ class AdamW:
             _need(p.is_contiguous(), f"parameter {i} must be contiguous")
             self.offsets.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
-        self._numel = [p.numel() for p in self.params]
+        self._shapes = [p.shape for p in self.params]
+        self._table = np.zeros(len(self.params), _TABLE)
+        self._table["numel"] = [p.numel() for p in self.params]
+        self._table["offset"] = self.offsets
         kind = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
         self.exp_avg = torch.zeros(total, dtype=kind[0], device=self.device)
         self.exp_avg_sq = torch.zeros(total, dtype=kind[1], device=self.device)
@@ -350,24 +356,30 @@ class AdamW:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
             _refuse(f"{len(self.params)} gradients are needed, got {len(grads)}")
-        rows, moved = [], []
-        for i, (p, g, at) in enumerate(zip(self.params, grads, self.offsets)):
-            if g is None:
-                continue
-            if g.shape != p.shape or g.get_device() != self._index or g.layout != torch.strided:
-                _refuse(f"gradient {i} must be a dense {tuple(p.shape)} on {self.device}")
-            if not p.is_contiguous() or p.get_device() != self._index or p.numel() != self._numel[i]:
-                _refuse(f"parameter {i} is no longer the {self._numel[i]} elements it was")
-            if not g.is_contiguous():
-                g = grads[i] = g.contiguous()
-            moved.append(p)
-            rows.append((p.data_ptr(), g.data_ptr(), self._numel[i], at, _dtype("parameter", p), _dtype("gradient", g)))
-        table = np.array(rows, _TABLE)
+        params, shapes, table = self.params, self._shapes, self._table
+        if any(g is None for g in grads):
+            at = [i for i, g in enumerate(grads) if g is not None]
+            params, shapes, grads = [params[i] for i in at], [shapes[i] for i in at], [grads[i] for i in at]
+            table = table[at]
+        if [g.shape for g in grads] != shapes or any(g.get_device() != self._index or g.is_sparse for g in grads):
+            _refuse(f"gradients must be dense, on {self.device} and of their parameters' shapes "
+                    f"{[tuple(s) for s in shapes]}, got {[tuple(g.shape) for g in grads]}")
+        if [p.shape for p in params] != shapes or not all([p.is_contiguous() for p in params]):
+            _refuse("a parameter is no longer the contiguous tensor it was")
+        if not all([g.is_contiguous() for g in grads]):
+            grads = [g.contiguous() for g in grads]
+        try:
+            table["dtype"] = [_DTYPES[p.dtype] for p in params]
+            table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
+        except KeyError as e:
+            _refuse(f"parameters and gradients must be float32, float16 or bfloat16, got {e}")
+        table["param"] = [p.data_ptr() for p in params]
+        table["grad"] = [g.data_ptr() for g in grads]
         h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
                                    self.step_count + 1)
-        _call(self._index, "trident_adamw", table.ctypes.data, len(rows), ctypes.byref(self._state), ctypes.byref(h))
+        _call(self._index, "trident_adamw", table.ctypes.data, len(params), ctypes.byref(self._state), ctypes.byref(h))
         self.step_count += 1
-        torch.autograd.graph.increment_version(moved)
+        torch.autograd.graph.increment_version(params)
 
     def state_values(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The moments as flat float32 tensors: the buffers themselves, or what the 8-bit codes stand for."""
@@ -427,14 +439,14 @@ def _check_blocks(name: str, b: Fp8Blocks, index: int) -> int:
     if not isinstance(b, Fp8Blocks):
         _refuse(f"{name} must be Fp8Blocks (quantize_fp8)")
     codes, scales, K = b
-    if K < 1 or codes.dim() != 2 or scales.dim() != 2:
-        _refuse(f"{name} must be a matrix")
+    if K < 1 or codes.dim() != 2 or codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
+        _refuse(f"{name} must be a matrix of float8_e4m3fn codes with uint8 scales")
+    rows, width = codes.shape
     kp, sp = _fp8_pitches(K)
-    rows = codes.shape[0]
-    if codes.dtype != torch.float8_e4m3fn or codes.shape[1] != kp or not codes.is_contiguous():
-        _refuse(f"{name}.codes must be a contiguous [{rows}, {kp}] float8_e4m3fn")
-    if scales.dtype != torch.uint8 or scales.shape[0] != rows or scales.shape[1] != sp or not scales.is_contiguous():
-        _refuse(f"{name}.scales must be a contiguous [{rows}, {sp}] uint8")
+    if width != kp or not codes.is_contiguous():
+        _refuse(f"{name}.codes must be a contiguous [{rows}, {kp}]")
+    if scales.shape != (rows, sp) or not scales.is_contiguous():
+        _refuse(f"{name}.scales must be a contiguous [{rows}, {sp}]")
     if codes.get_device() != index or scales.get_device() != index:
         _refuse(f"{name} must be on cuda:{index}")
     return rows
@@ -501,11 +513,7 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     bcode = _bias(bias, N, x.dtype, index)
     xr, ld = _rows(x)
     out = x.new_empty((*x.shape[:-1], N))
-    args = ("trident_fp8_linear", xr.data_ptr(), code, M, K, ld, weight.codes.data_ptr(), weight.scales.data_ptr(), N,
-            None if bias is None else bias.data_ptr(), bcode, out.data_ptr(), max(N, 1), fast_accum)
-    nbytes = _fn("trident_fp8_linear_workspace_bytes")(M, K)
-    if nbytes:
-        _call_ws(x.device, index, args[0], nbytes, *args[1:])
-    else:
-        _call(index, *args, None, 0)
+    _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, K), xr.data_ptr(),
+             code, M, K, ld, weight.codes.data_ptr(), weight.scales.data_ptr(), N,
+             None if bias is None else bias.data_ptr(), bcode, out.data_ptr(), max(N, 1), fast_accum)
     return out
