@@ -498,8 +498,8 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
 
 // Few tokens, in one launch: the time is that of launches, not of bytes.  Workgroup b owns the ids = b
 // modulo gridDim.x as in sort_ids_kernel, orders its tokens in LDS, and sums and writes its own rows, so
-// nothing passes between workgroups: groups of lanes take the rows in turn; the rows of more than
-// kShared tokens are then summed by all groups together.
+// nothing passes between workgroups: groups of lanes clear the rows without tokens, take those with up to
+// kShared of them in turn, and sum the others together.
 constexpr int kFewThreads = 512;
 constexpr int kFewTokens = 8192;           // 16 a thread, held in registers
 constexpr int kFewElements = 512 * 1024;   // tokens * columns: past it one workgroup may have too much to sum
@@ -523,16 +523,16 @@ template <typename T, int VEC, int NVL, typename ID>
 __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) {
     constexpr int WAVES = kFewThreads / kWave, A = kFewTokens / kFewThreads;
     extern __shared__ __align__(16) float sums[];  // [NVL * VEC][kFewThreads]
-    __shared__ int s_sum[WAVES], s_shared;
+    __shared__ int s_sum[WAVES], s_shared, s_single;
     const int w = a.owned, lane = lane_id(), wave = threadIdx.x / kWave;
     int* hist = reinterpret_cast<int*>(sums + kFewThreads * NVL * VEC);    // [WAVES][w]
     int* start = hist + WAVES * w;                                         // [w + 1]
-    int* shared_rows = start + w + 1;                                      // [w]
-    uint16_t* order = reinterpret_cast<uint16_t*>(shared_rows + w);        // tokens by id
+    int* busy = start + w + 1;  // [w]: rows with tokens, those of all groups from the front, of one from the back
+    uint16_t* order = reinterpret_cast<uint16_t*>(busy + w);  // tokens by id
     const uint32_t b = blockIdx.x, mask = (1u << a.shift) - 1;
     const ID* ids = static_cast<const ID*>(a.ids);
     for (int i = threadIdx.x; i < WAVES * w; i += kFewThreads) hist[i] = 0;
-    if (threadIdx.x == 0) s_shared = 0;
+    if (threadIdx.x == 0) s_shared = s_single = 0;
     const int per = (a.n + kFewThreads - 1) / kFewThreads;  // groups of 64 tokens of a wave
     const int first = wave * per * kWave + lane;
     uint32_t rel[A];
@@ -560,7 +560,8 @@ __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) 
         place += total;
         if (j < w) {
             start[j] = at;
-            if (count > kShared) shared_rows[atomicAdd(&s_shared, 1)] = j;  // in any order
+            if (count > kShared) busy[atomicAdd(&s_shared, 1)] = j;  // in any order
+            else if (count > 0) busy[w - 1 - atomicAdd(&s_single, 1)] = j;
             for (int i = 0; i < WAVES; ++i) {
                 const int c = hist[i * w + j];
                 hist[i * w + j] = at;
@@ -638,15 +639,17 @@ __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) 
             }
     };
     const int rows = (int)(((int64_t)a.V - b + mask) >> a.shift);  // owned ids below V
-    for (int j = group; j < rows; j += groups) {
-        const int beg = start[j], end = start[j + 1];
-        if (end - beg > kShared) continue;
+    clear();
+    for (int j = group; j < rows; j += groups)
+        if (start[j] == start[j + 1]) write(j);
+    for (int i = group; i < s_single; i += groups) {
+        const int j = busy[w - 1 - i];
         clear();
-        add(beg, end, 1);
+        add(start[j], start[j + 1], 1);
         write(j);
     }
     for (int i = 0; i < s_shared; ++i) {  // the same in every thread
-        const int j = shared_rows[i], beg = start[j], end = start[j + 1];
+        const int j = busy[i], beg = start[j], end = start[j + 1];
         clear();
         add(beg + group, end, groups);
         __syncthreads();

@@ -160,6 +160,16 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, 0xffffffffu, 0x00027000);
 }
 
+// The bias of columns first .. first + N - 1; those past the last one repeat it.
+template <typename T, int N>
+__device__ __forceinline__ void load_bias(const void* bias, int f32, int first, int columns, float (&out)[N]) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+        const int n = min(first + e, columns - 1);
+        out[e] = !bias ? 0.0f : f32 ? static_cast<const float*>(bias)[n] : (float)static_cast<const T*>(bias)[n];
+    }
+}
+
 // A workgroup of WM x WN waves computes a tile of WM MT x WN NT blocks of 32 x 32, a wave MT x NT of
 // them.  128 columns of both operands at a time go straight from memory to LDS (no registers between),
 // the next ones while these are multiplied.  The eight 16-byte pieces of a row are stored exchanged by
@@ -242,6 +252,14 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
         return f;
     };
 
+    // at the end this lane writes kPer columns of every kRowsAtOnce-th row: their bias, early
+    constexpr int kCols = NT * 32, kPitch = kCols * 4 + 16, kPer = 16 / (int)sizeof(T);
+    constexpr int kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
+    static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the results fit where the operands were");
+    const int piece_col = n0 + wn + lane % kRowPieces * kPer, left = g.N - piece_col;
+    float bias[kPer];
+    load_bias<T, kPer>(g.bias, g.bias_f32, piece_col, g.N, bias);
+
     f32x16 acc[MT][NT] = {};
 #pragma unroll
     for (int kb = 0; kb < STAGES - 1; ++kb)
@@ -316,41 +334,27 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     }
     // The results go through this wave's part of LDS, 32 rows at a time, so that it writes whole lines: a
     // lane holds four columns, and rows a power of two apart would all meet in one channel of L2.
-    constexpr int kCols = NT * 32, kPitch = kCols * (int)sizeof(T) + 16, kPer = 16 / (int)sizeof(T);
-    constexpr int kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
-    static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the results fit where the operands were");
     __syncthreads();
-    uint8_t* mine = lds + wave * 32 * kPitch;
-    float bias[NT][4][4];
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = min(n0 + wn + j * 32 + p * 8 + q * 4 + e, g.N - 1);
-                bias[j][p][e] = !g.bias ? 0.0f
-                                : g.bias_f32 ? static_cast<const float*>(g.bias)[n]
-                                             : (float)static_cast<const T*>(g.bias)[n];
-            }
-    const int piece_col = n0 + wn + lane % kRowPieces * kPer, left = g.N - piece_col;
+    float* mine = reinterpret_cast<float*>(lds + wave * 32 * kPitch);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-                T v[4];
+                f32x4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = (T)(acc[i][j][4 * p + e] + bias[j][p][e]);
-                __builtin_memcpy(mine + r * kPitch + (j * 32 + p * 8 + q * 4) * (int)sizeof(T), v, sizeof(v));
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * p + e];
+                *reinterpret_cast<f32x4*>(mine + r * (kPitch / 4) + j * 32 + p * 8 + q * 4) = v;
             }
         wave_sync();
 #pragma unroll
         for (int k = 0; k < 32; k += kRowsAtOnce) {
             const int row = k + lane / kRowPieces, m = m0 + wm + i * 32 + row;
+            const f32x4* from = reinterpret_cast<const f32x4*>(mine + row * (kPitch / 4) + lane % kRowPieces * kPer);
             T v[kPer];
-            __builtin_memcpy(v, mine + row * kPitch + lane % kRowPieces * 16, 16);
+#pragma unroll
+            for (int e = 0; e < kPer; ++e) v[e] = (T)(from[e / 4][e % 4] + bias[e]);
             if (m >= g.M) continue;
             T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + piece_col;
             if (left >= kPer) {
@@ -392,6 +396,8 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
     const int64_t n = min(n0 + r, g.N - 1), m = min(r, g.M - 1);
     const uint8_t* b = g.b + n * g.pitch_b + q * 32;
     const uint8_t* sb = g.sb + n * g.spitch;
+    float bias[4];
+    load_bias<T, 4>(g.bias, g.bias_f32, n0 + q * 4, g.N, bias);
     f32x4 acc = {};
     for (int k0 = wave; k0 < g.kb; k0 += kFewWaves * U) {
         u32x4 wb[U][2], wa[U][2];
@@ -399,7 +405,8 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
         int eb[U], ea[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = min(k0 + u * kFewWaves, g.kb - 1);  // past the end: read again, not multiplied
+            const int kb = k0 + u * kFewWaves;
+            if (kb >= g.kb) break;
             __builtin_memcpy(wb[u], b + (int64_t)kb * kBlockK, 32);
             eb[u] = sb[kb];
             if constexpr (QUANT) {
@@ -468,9 +475,7 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
     for (int e = 0; e < 4; ++e) {
         const int c = n0 + q * 4 + e;
         if (c >= g.N) break;
-        float v = acc[e];
-        if (g.bias) v += g.bias_f32 ? static_cast<const float*>(g.bias)[c] : (float)static_cast<const T*>(g.bias)[c];
-        static_cast<T*>(g.out)[(int64_t)r * g.ldo + c] = (T)v;
+        static_cast<T*>(g.out)[(int64_t)r * g.ldo + c] = (T)(acc[e] + bias[e]);
     }
 }
 
