@@ -102,7 +102,7 @@ def test_fp8_arguments():
     refused(L.trident_fp8_matmul(P, P, 4, P, P, 4, 100, None, 0, P, 2, 3, 0, None), 1, "bad sizes")
     refused(L.trident_fp8_matmul(P, None, 4, P, P, 4, 100, None, 0, P, 2, 4, 0, None), 1, "NULL")
     assert L.trident_fp8_matmul(P, P, 0, P, P, 4, 100, None, 0, P, 2, 4, 0, None) == 0
-    need = L.trident_fp8_linear_workspace_bytes(100, 1000)
+    need = L.trident_fp8_linear_workspace_bytes(100, 4, 1000)
     assert need >= 100 * 1024 + 100 * 8
     refused(L.trident_fp8_linear(P, 0, 100, 1000, 1000, P, P, 4, None, 0, P, 4, 0, P, need - 1, None), 3, str(need))
 

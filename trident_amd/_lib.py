@@ -116,7 +116,7 @@ EXPORTS = {
     "trident_adamw_state_values": (ctypes.c_int, [ctypes.POINTER(TridentAdamState), _P, _P, _P]),
     "trident_fp8_quantize": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _P]),
     "trident_fp8_matmul": (ctypes.c_int, [_P, _P, _i64, _P, _P, _i64, _i64, _P, _i32, _P, _i32, _i64, _i32, _P]),
-    "trident_fp8_linear_workspace_bytes": (_size, [_i64, _i64]),
+    "trident_fp8_linear_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "trident_fp8_linear": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _i64, _P, _i32, _P, _i64, _i32, _P,
                                           _size, _P]),
     "trident_last_error": (ctypes.c_char_p, []),

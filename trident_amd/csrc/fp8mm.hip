@@ -369,8 +369,9 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     }
 }
 
-constexpr int kFew = 16;       // rows that one instruction takes
 constexpr int kFewWaves = 8;
+constexpr int kFewRows = 16;    // rows that one instruction takes
+constexpr int kFewBlocks = 24;  // blocks of 16 rows by 128 columns that a CU quantises, past 16 rows
 
 struct FewArgs {
     const void* x;           // [M, ldx], or null: the codes of a
@@ -382,101 +383,126 @@ struct FewArgs {
     int M, N, K, kb, spitch, bias_f32;
 };
 
-// Up to 16 rows, bound by the weight's bytes or, for one query, by the latency of a launch.  A workgroup
+// Up to 64 rows, bound by the weight's bytes or, for one query, by the latency of a launch.  A workgroup
 // takes 16 columns; its eight waves take the blocks of 128 of K in turn, the weight straight from memory
 // to registers, and their sums are added in order at the end.  The rows are quantised on the way (QUANT):
 // a lane holds the 32 columns of its row that the instruction wants from it, and a block's largest value
 // is that of four lanes, so one launch does all and nothing is stored between.
-template <typename T, bool FAST, bool QUANT>
+template <typename T, bool FAST, bool QUANT, int MT>
 __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g) {
-    constexpr int U = sizeof(T) == 4 ? 2 : 4;  // blocks of a wave in flight
-    __shared__ f32x4 s_acc[kFewWaves][kWave];
+    constexpr int U = MT > 1 ? 1 : sizeof(T) == 4 ? 2 : 4;  // blocks of a wave in flight
+    __shared__ f32x4 s_acc[kFewWaves][MT][kWave];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
-    const int64_t n = min(n0 + r, g.N - 1), m = min(r, g.M - 1);
+    const int64_t n = min(n0 + r, g.N - 1);
     const uint8_t* b = g.b + n * g.pitch_b + q * 32;
     const uint8_t* sb = g.sb + n * g.spitch;
     float bias[4];
     load_bias<T, 4>(g.bias, g.bias_f32, n0 + q * 4, g.N, bias);
-    f32x4 acc = {};
+    f32x4 acc[MT] = {};
     for (int k0 = wave; k0 < g.kb; k0 += kFewWaves * U) {
-        u32x4 wb[U][2], wa[U][2];
-        Vec<T, 8> x[U][4];
-        int eb[U], ea[U];
+        u32x4 wb[U][2], wa[U][MT][2];
+        Vec<T, 8> x[U][MT][4];
+        int eb[U], ea[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int kb = k0 + u * kFewWaves;
             if (kb >= g.kb) break;
             __builtin_memcpy(wb[u], b + (int64_t)kb * kBlockK, 32);
             eb[u] = sb[kb];
-            if constexpr (QUANT) {
-                const T* row = static_cast<const T*>(g.x) + m * g.ldx;
-                const int col = kb * kBlockK + q * 32;
-                if (col + 32 <= g.K) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[u][e].load(row + col + e * 8);
-                } else {
+            for (int i = 0; i < MT; ++i) {
+                const int64_t m = min(i * kFewRows + r, g.M - 1);
+                if constexpr (QUANT) {
+                    const T* row = static_cast<const T*>(g.x) + m * g.ldx;
+                    const int col = kb * kBlockK + q * 32;
+                    if (col + 32 <= g.K) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        T v[8];
+                        for (int e = 0; e < 4; ++e) x[u][i][e].load(row + col + e * 8);
+                    } else {
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) v[i] = col + e * 8 + i < g.K ? row[col + e * 8 + i] : (T)0.0f;
-                        x[u][e].load(v);
+                        for (int e = 0; e < 4; ++e) {
+                            T v[8];
+#pragma unroll
+                            for (int c = 0; c < 8; ++c)
+                                v[c] = col + e * 8 + c < g.K ? row[col + e * 8 + c] : (T)0.0f;
+                            x[u][i][e].load(v);
+                        }
                     }
+                } else {
+                    __builtin_memcpy(wa[u][i], g.a + m * ((int64_t)g.kb * kBlockK) + (int64_t)kb * kBlockK + q * 32,
+                                     32);
+                    ea[u][i] = g.sa[m * g.spitch + kb];
                 }
-            } else {
-                __builtin_memcpy(wa[u], g.a + m * ((int64_t)g.kb * kBlockK) + (int64_t)kb * kBlockK + q * 32, 32);
-                ea[u] = g.sa[m * g.spitch + kb];
             }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (k0 + u * kFewWaves >= g.kb) break;
-            i32x8 fa, fb;
+            i32x8 fb;
 #pragma unroll
             for (int e = 0; e < 8; ++e) fb[e] = (int)wb[u][e / 4][e % 4];
-            if constexpr (QUANT) {
-                float v[4][8], top = 0.0f;
+            bf16x8 hb[4];
+            if constexpr (!FAST) to_bf16(fb, scale_value((uint32_t)eb[u]), hb);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    x[u][e].get(v[e]);
+            for (int i = 0; i < MT; ++i) {
+                i32x8 fa;
+                if constexpr (QUANT) {
+                    float v[4][8], top = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[e][i]) < INFINITY ? fabsf(v[e][i]) : 0.0f);
+                    for (int e = 0; e < 4; ++e) {
+                        x[u][i][e].get(v[e]);
+#pragma unroll
+                        for (int c = 0; c < 8; ++c) top = fmaxf(top, fabsf(v[e][c]) < INFINITY ? fabsf(v[e][c]) : 0.0f);
+                    }
+                    top = fmaxf(top, __shfl_xor(top, 16, kWave));
+                    top = fmaxf(top, __shfl_xor(top, 32, kWave));
+                    ea[u][i] = scale_of(top);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const uint2 c = codes_of(v[e], ea[u][i]);
+                        fa[2 * e] = (int)c.x;
+                        fa[2 * e + 1] = (int)c.y;
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) fa[e] = (int)wa[u][i][e / 4][e % 4];
                 }
-                top = fmaxf(top, __shfl_xor(top, 16, kWave));
-                top = fmaxf(top, __shfl_xor(top, 32, kWave));
-                ea[u] = scale_of(top);
+                if constexpr (FAST) {
+                    acc[i] =
+                        __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc[i], 0, 0, 0, eb[u], 0, ea[u][i]);
+                } else {
+                    bf16x8 ha[4];
+                    to_bf16(fa, scale_value((uint32_t)ea[u][i]), ha);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const uint2 c = codes_of(v[e], ea[u]);
-                    fa[2 * e] = (int)c.x;
-                    fa[2 * e + 1] = (int)c.y;
+                    for (int k = 0; k < 4; ++k)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[k], ha[k], acc[i], 0, 0, 0);
                 }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) fa[e] = (int)wa[u][e / 4][e % 4];
-            }
-            if constexpr (FAST) {
-                acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc, 0, 0, 0, eb[u], 0, ea[u]);
-            } else {
-                bf16x8 ha[4], hb[4];
-                to_bf16(fa, scale_value((uint32_t)ea[u]), ha);
-                to_bf16(fb, scale_value((uint32_t)eb[u]), hb);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[k], ha[k], acc, 0, 0, 0);
             }
         }
     }
-    s_acc[wave][lane] = acc;
+#pragma unroll
+    for (int i = 0; i < MT; ++i) s_acc[wave][i][lane] = acc[i];
     __syncthreads();
-    if (wave != 0 || r >= g.M) return;
-    for (int w = 1; w < kFewWaves; ++w) acc += s_acc[w][lane];
+    const int m = wave * kFewRows + r;  // a wave for 16 rows
+    if (wave >= MT || m >= g.M) return;
+    f32x4 sum = s_acc[0][wave][lane];
+    for (int w = 1; w < kFewWaves; ++w) sum += s_acc[w][wave][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         const int c = n0 + q * 4 + e;
         if (c >= g.N) break;
-        static_cast<T*>(g.out)[(int64_t)r * g.ldo + c] = (T)(acc[e] + bias[e]);
+        static_cast<T*>(g.out)[(int64_t)m * g.ldo + c] = (T)(sum[e] + bias[e]);
     }
+}
+
+// Whether the kernel for few rows takes a projection: 16 rows always; up to 64 where what a CU's
+// workgroups quantise again (all of them quantise all rows) costs less than a launch.  Measured with
+// float32 rows, against 11 to 13 us for two launches: 24 blocks 8.9 us, 32 11.6 (N = 1024); 16 blocks of
+// N = 8192, two workgroups a CU, 15.4.
+inline bool few_rows(int64_t M, int64_t N, int64_t K) {
+    return M <= kFewRows || (M <= 4 * kFewRows && (M + kFewRows - 1) / kFewRows * blocks_of(K) *
+                                                          ((N + 4095) / 4096) <= kFewBlocks);
 }
 
 // Launches the kernel of one tile size.
@@ -577,8 +603,17 @@ int product_few(const void* x, int64_t ld_x, const uint8_t* a, const uint8_t* sa
     const unsigned grid = (unsigned)((N + 15) / 16);
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (fast_accum) matmul_few_kernel<T, true, QUANT><<<grid, kFewWaves * kWave, 0, st>>>(g);
-        else matmul_few_kernel<T, false, QUANT><<<grid, kFewWaves * kWave, 0, st>>>(g);
+        const auto go = [&](auto fast, auto mt) {
+            matmul_few_kernel<T, decltype(fast)::value, QUANT, decltype(mt)::value>
+                <<<grid, kFewWaves * kWave, 0, st>>>(g);
+        };
+        const auto rows = [&](auto fast) {
+            if (M <= kFewRows) go(fast, std::integral_constant<int, 1>{});
+            else if (M <= 2 * kFewRows) go(fast, std::integral_constant<int, 2>{});
+            else go(fast, std::integral_constant<int, 4>{});
+        };
+        if (fast_accum) rows(std::true_type{});
+        else rows(std::false_type{});
     });
     return capi_check_launch("matmul_few_kernel");
 }
@@ -603,15 +638,15 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
     if (!a_scales || !aligned16(a_codes))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= kFew)
+    if (M <= kFewRows)
         return product_few<false>(nullptr, 0, a_codes, a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out,
                                   dtype, ld_out, fast_accum, st);
     return product(a_codes, pitch_of(K), a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
                    fast_accum, st);
 }
 
-size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t K) {
-    if (!counts_ok(M, K) || M <= kFew) return 0;
+size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+    if (!counts_ok(M, K) || !counts_ok(N, K) || few_rows(M, N, K)) return 0;
     return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
 }
 
@@ -624,10 +659,10 @@ int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_linear: ld=%lld < K=%lld", (long long)ld_x, (long long)K);
     if (M == 0 || N == 0) return TRIDENT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= kFew)
+    if (few_rows(M, N, K))
         return product_few<true>(x, ld_x, nullptr, nullptr, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype,
                                  ld_out, fast_accum, st);
-    const size_t need = trident_fp8_linear_workspace_bytes(M, K);
+    const size_t need = trident_fp8_linear_workspace_bytes(M, N, K);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "fp8_linear: workspace %zu < %zu bytes, or not 16-byte aligned",
                          workspace_bytes, need);

@@ -439,14 +439,13 @@ def _check_blocks(name: str, b: Fp8Blocks, index: int) -> int:
     if not isinstance(b, Fp8Blocks):
         _refuse(f"{name} must be Fp8Blocks (quantize_fp8)")
     codes, scales, K = b
-    if K < 1 or codes.dim() != 2 or codes.dtype != torch.float8_e4m3fn or scales.dtype != torch.uint8:
-        _refuse(f"{name} must be a matrix of float8_e4m3fn codes with uint8 scales")
-    rows, width = codes.shape
-    kp, sp = _fp8_pitches(K)
-    if width != kp or not codes.is_contiguous():
-        _refuse(f"{name}.codes must be a contiguous [{rows}, {kp}]")
-    if scales.shape != (rows, sp) or not scales.is_contiguous():
-        _refuse(f"{name}.scales must be a contiguous [{rows}, {sp}]")
+    rows = codes.shape[0]
+    if codes.dtype is not torch.float8_e4m3fn or scales.dtype is not torch.uint8 or K < 1 or \
+            codes.shape != (rows, -(-K // 128) * 128) or scales.shape != (rows, -(-K // 512) * 4) or \
+            not codes.is_contiguous() or not scales.is_contiguous():
+        _refuse(f"{name} must hold contiguous float8_e4m3fn codes {(rows,) + _fp8_pitches(K)[:1]} and uint8 scales "
+                f"{(rows,) + _fp8_pitches(K)[1:]} for K={K}, got {codes.dtype} {tuple(codes.shape)} and "
+                f"{scales.dtype} {tuple(scales.shape)}")
     if codes.get_device() != index or scales.get_device() != index:
         _refuse(f"{name} must be on cuda:{index}")
     return rows
@@ -469,9 +468,9 @@ def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
 def _bias(bias, N, dtype, index) -> int:
     if bias is None:
         return _DTYPES[dtype]
-    if bias.dim() != 1 or bias.shape[0] != N or not bias.is_contiguous():
+    if bias.shape != (N,) or not bias.is_contiguous():
         _refuse(f"bias must be a contiguous [{N}]")
-    if bias.dtype != dtype and bias.dtype != torch.float32:
+    if bias.dtype is not dtype and bias.dtype is not torch.float32:
         _refuse(f"bias must be {dtype} or float32, got {bias.dtype}")
     _same(index, "bias", bias)
     return _DTYPES[bias.dtype]
@@ -506,14 +505,16 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``."""
     code, index = _dtype("x", x), _gpu("x", x)
     N = _check_blocks("weight", weight, index)
-    K = weight.K
-    if x.dim() < 1 or x.shape[-1] != K:
-        _refuse(f"x must be [..., {K}], got {tuple(x.shape)}")
+    codes, scales, K = weight
+    shape = x.shape
+    if not shape or shape[-1] != K:
+        _refuse(f"x must be [..., {K}], got {tuple(shape)}")
     M = x.numel() // K
-    bcode = _bias(bias, N, x.dtype, index)
-    xr, ld = _rows(x)
-    out = x.new_empty((*x.shape[:-1], N))
-    _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, K), xr.data_ptr(),
-             code, M, K, ld, weight.codes.data_ptr(), weight.scales.data_ptr(), N,
-             None if bias is None else bias.data_ptr(), bcode, out.data_ptr(), max(N, 1), fast_accum)
+    bcode, bptr = code, None
+    if bias is not None:
+        bcode, bptr = _bias(bias, N, x.dtype, index), bias.data_ptr()
+    xr, ld = (x, K) if x.is_contiguous() else _rows(x)
+    out = x.new_empty((M, N) if len(shape) == 2 else (*shape[:-1], N))
+    _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, N, K), xr.data_ptr(),
+             code, M, K, ld, codes.data_ptr(), scales.data_ptr(), N, bptr, bcode, out.data_ptr(), N or 1, fast_accum)
     return out
