@@ -163,10 +163,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_at(const void* p) {
 // The bias of columns first .. first + N - 1; those past the last one repeat it.
 template <typename T, int N>
 __device__ __forceinline__ void load_bias(const void* bias, int f32, int first, int columns, float (&out)[N]) {
+    if (!bias) {
 #pragma unroll
-    for (int e = 0; e < N; ++e) {
-        const int n = min(first + e, columns - 1);
-        out[e] = !bias ? 0.0f : f32 ? static_cast<const float*>(bias)[n] : (float)static_cast<const T*>(bias)[n];
+        for (int e = 0; e < N; ++e) out[e] = 0.0f;
+    } else if (f32) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = static_cast<const float*>(bias)[min(first + e, columns - 1)];
+    } else {
+#pragma unroll
+        for (int e = 0; e < N; ++e) out[e] = (float)static_cast<const T*>(bias)[min(first + e, columns - 1)];
     }
 }
 
@@ -177,24 +182,27 @@ __device__ __forceinline__ void load_bias(const void* bias, int f32, int first, 
 // LDS's 64 banks (a row is half of them, so rows that differ in bit 0 never meet).  The
 // weight is the instruction's first operand, so a lane holds four neighbouring columns of a result row.
 // A block of 128 columns is two instructions of 64 each with the same scale; in both operands a lane
-// passes the same columns, in whatever order the instruction takes them.  The rows' scales (a word a row,
-// that of four blocks) go to LDS as well: no register waits for memory in the loop, and every block is
-// the same number of loads, so the wait before a block leaves the later ones' in flight.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT, int STAGES>
-__global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
-    constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32, kStage = (BM + BN) * kBlockK;
-    constexpr int kLoads = (BM + BN) / 8 / kWaves;  // a wave's loads of eight rows each
-    static_assert((BM + BN) / 8 % kWaves == 0 && kLoads % 2 == 0, "whole loads, of either parity by turns");
-    constexpr int kScaleLoads = (BM + BN + kWaves * kWave - 1) / (kWaves * kWave);
+// passes the same columns, in whatever order the instruction takes them.  WK teams of such waves take
+// WK blocks at a time, where a CU has one small tile and the length of K is what it waits for.  The rows'
+// scales (a word a row, that of four blocks) go to LDS as well: no register waits for memory in the loop,
+// and every stage is the same number of loads, so the wait for one leaves the next one's in flight.
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
+__global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g) {
+    constexpr int kTeam = WM * WN, kWaves = kTeam * WK, BM = WM * MT * 32, BN = WN * NT * 32, kRows = BM + BN;
+    constexpr int kStage = WK * kRows * kBlockK;
+    constexpr int kLoads = WK * kRows / 8 / kWaves;  // a wave's loads of eight rows each
+    static_assert(WK * kRows / 8 % kWaves == 0 && kLoads % 2 == 0, "whole loads, of either parity by turns");
+    static_assert(BM % kWave == 0 && BN % kWave == 0, "a load of scales is of one operand and block");
+    constexpr int kScaleLoads = (WK * kRows + kWaves * kWave - 1) / (kWaves * kWave);
     constexpr int kScaleStage = kScaleLoads * kWaves * kWave * 4;
-    constexpr int kFlight = kLoads + kScaleLoads;  // a wave's loads of one block
-    extern __shared__ __align__(16) uint8_t lds[];  // [STAGES][BM + BN][128], [STAGES][BM + BN] words of scales
+    constexpr int kFlight = kLoads + kScaleLoads;  // a wave's loads of one stage
+    extern __shared__ __align__(16) uint8_t lds[];  // [2][WK][BM + BN][128], [2][WK][BM + BN] words of scales
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int r = lane & 31, q = lane >> 5;
     int tm, tn;
     tile_of(blockIdx.x, g.tiles_m, g.tiles_n, 8, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
-    const int wm = (wave / WN) * MT * 32, wn = (wave % WN) * NT * 32;
+    const int team = wave / kTeam, wm = wave % kTeam / WN * MT * 32, wn = wave % WN * NT * 32;
 
     // rows of the tile: BM of a, then BN of b; those past an operand's end read its last row
     const auto row_of = [&](int row) { return row < BM ? min(row, g.M - 1 - m0) : min(row - BM, g.N - 1 - n0); };
@@ -207,37 +215,38 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
     // block (`sub` is hidden from the compiler, which would keep them all in registers, and spill).
     int sub = lane / 8;
     const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 16)) * 16;
-    const auto fetch = [&](int kb) {
+    const auto fetch = [&](int step) {
         asm volatile("" : "+v"(sub));
-        uint8_t* to = lds + kb % STAGES * kStage + wave * kLoads * 1024;
+        uint8_t* to = lds + step % 2 * kStage + wave * kLoads * 1024;
 #pragma unroll
         for (int i = 0; i < kLoads; ++i) {
-            const int first = (wave * kLoads + i) * 8;  // the same operand for the whole wave
+            const int at = (wave * kLoads + i) * 8, first = at % kRows;  // the same operand for the whole wave
+            const int kb = min(step * WK + at / kRows, g.kb - 1);
             const uint32_t pitch = (uint32_t)(first < BM ? g.pitch_a : g.pitch_b);
-            const uint32_t at = (uint32_t)row_of(first + sub) * pitch + (piece ^ (i % 2 * 64));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16, at,
+            const uint32_t from = (uint32_t)row_of(first + sub) * pitch + (piece ^ (i % 2 * 64));
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16, from,
                                                      kb * kBlockK, 0, 0);
         }
-        uint8_t* st = lds + STAGES * kStage + kb % STAGES * kScaleStage + wave * kWave * 4;
+        uint8_t* st = lds + 2 * kStage + step % 2 * kScaleStage + wave * kWave * 4;
 #pragma unroll
         for (int i = 0; i < kScaleLoads; ++i) {
-            const int first = (i * kWaves + wave) * kWave;
-            const int row = min(first + (sub * 8 + (lane & 7)), BM + BN - 1);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_sa : buf_sb,
-                                                     (lds_ptr)(st + i * kWaves * kWave * 4), 4,
-                                                     (uint32_t)row_of(row) * (uint32_t)g.spitch, kb & ~3, 0, 0);
+            const int at = min((i * kWaves + wave) * kWave, WK * kRows - kWave), first = at % kRows;
+            const int kb = min(step * WK + at / kRows, g.kb - 1);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                first < BM ? buf_sa : buf_sb, (lds_ptr)(st + i * kWaves * kWave * 4), 4,
+                (uint32_t)row_of(first + sub * 8 + (lane & 7)) * (uint32_t)g.spitch, kb & ~3, 0, 0);
         }
     };
     // where this lane reads the four pieces of its first row of either operand; the other rows are 32
-    // rows on, the stages count in the bits above
-    static_assert((kStage & (kStage - 1)) == 0 && (STAGES & (STAGES - 1)) == 0, "stages are bits of the address");
+    // rows on, the other stage is the next bit
+    static_assert((kStage & (kStage - 1)) == 0, "a stage is a bit of the address");
     const uint32_t origin = (uint32_t)(uintptr_t)(lds_ptr)lds;
     uint32_t at_a[4], at_b[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const uint32_t p = (uint32_t)((4 * (c / 2) + 2 * q + c % 2) ^ (r >> 1 & 7)) * 16;
-        at_a[c] = (uint32_t)(wm + r) * kBlockK + p;
-        at_b[c] = (uint32_t)(BM + wn + r) * kBlockK + p;
+        at_a[c] = (uint32_t)(team * kRows + wm + r) * kBlockK + p;
+        at_b[c] = (uint32_t)(team * kRows + BM + wn + r) * kBlockK + p;
     }
     const auto read = [&](const uint32_t (&at)[4], int half, int block) {
         typedef const __attribute__((address_space(3))) u32x4* piece_ptr;
@@ -252,31 +261,32 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
         return f;
     };
 
-    // at the end this lane writes kPer columns of every kRowsAtOnce-th row: their bias, early
+    // at the end this lane writes kPer columns of every kRowsAtOnce-th row: their bias, early where
+    // registers are left
+    constexpr bool kEarly = MT * NT < 8;
     constexpr int kCols = NT * 32, kPitch = kCols * 4 + 16, kPer = 16 / (int)sizeof(T);
     constexpr int kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
-    static_assert(kWaves * 32 * kPitch <= STAGES * kStage, "the results fit where the operands were");
+    static_assert(kTeam * 32 * kPitch <= 2 * kStage, "the results fit where the operands were");
     const int piece_col = n0 + wn + lane % kRowPieces * kPer, left = g.N - piece_col;
     float bias[kPer];
-    load_bias<T, kPer>(g.bias, g.bias_f32, piece_col, g.N, bias);
+    if constexpr (kEarly) load_bias<T, kPer>(g.bias, g.bias_f32, piece_col, g.N, bias);
 
     f32x16 acc[MT][NT] = {};
-#pragma unroll
-    for (int kb = 0; kb < STAGES - 1; ++kb)
-        if (kb < g.kb) fetch(kb);
-    for (int kb = 0; kb < g.kb; ++kb) {
-        // Past the barrier this block has arrived, every wave's part of it, and every wave has read the one
-        // before, whose stage the next loads take.  Loads arrive in order; those of up to STAGES - 2 later
-        // blocks stay in flight.
-        const int later = min(STAGES - 2, g.kb - 1 - kb);
-        if (later <= 0) asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-        else if (later == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(kFlight) : "memory");
-        else asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(2 * kFlight) : "memory");
+    // Two stages.  A stage's next loads are issued as soon as every wave holds its part of it in
+    // registers, halfway through its products, so they have a step and a half to arrive.
+    const int steps = (g.kb + WK - 1) / WK;
+    fetch(0);
+    if (steps > 1) fetch(1);
+    for (int step = 0; step < steps; ++step) {
+        // past the barrier this stage has arrived, every wave's part of it (loads arrive in order)
+        if (step + 1 < steps) asm volatile("s_waitcnt vmcnt(%0)" ::"i"(kFlight) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (kb + STAGES - 1 < g.kb) fetch(kb + STAGES - 1);
-        uint32_t ea[MT], eb[NT];  // the scale of this block in the lowest byte
-        const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + STAGES * kStage + kb % STAGES * kScaleStage);
+        const int kb = step * WK + team;
+        const bool live = WK == 1 || kb < g.kb;  // not in the last step of the last team of an odd number
+        uint32_t ea[MT], eb[NT];                 // the scale of this block in the lowest byte
+        const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + 2 * kStage + step % 2 * kScaleStage) + team * kRows;
 #pragma unroll
         for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r] >> (kb % 4 * 8);
 #pragma unroll
@@ -289,8 +299,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
 #pragma unroll
             for (int i = 0; i < MT; ++i) fa[half][i] = read(at_a, half, i);
         }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
+        const auto multiply = [&](int half) {
             if constexpr (FAST) {
 #pragma unroll
                 for (int i = 0; i < MT; ++i)
@@ -313,28 +322,54 @@ __global__ __launch_bounds__(WM* WN* kWave) void matmul_kernel(MatmulArgs g) {
                             acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hb[j][k], ha[k], acc[i][j], 0, 0, 0);
                 }
             }
-        }
+        };
+        if (live) multiply(0);
         if constexpr (FAST) {
-            // the first half's reads, the second half's among the first half's products, the rest
+            // the first half's reads with the scales', the second half's among the first half's products
             constexpr int kReads = 2 * (MT + NT), kProducts = MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
-            __builtin_amdgcn_sched_group_barrier(0x100, kReads + MT + NT, 0);  // with the scales'
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads + MT + NT, 0);
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
                 __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
             }
-            __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);
         }
-        const uint32_t next = (uint32_t)((kb + 1) % STAGES ^ kb % STAGES) * kStage;
+        // the first half's products stay before the wait (the compiler would sink them past it)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+        // past this barrier every wave has read the stage
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (step + 2 < steps) fetch(step + 2);
+        if (live) multiply(1);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-            at_a[c] ^= next;
-            at_b[c] ^= next;
+            at_a[c] ^= kStage;
+            at_b[c] ^= kStage;
         }
     }
     // The results go through this wave's part of LDS, 32 rows at a time, so that it writes whole lines: a
     // lane holds four columns, and rows a power of two apart would all meet in one channel of L2.
+    if constexpr (!kEarly) load_bias<T, kPer>(g.bias, g.bias_f32, piece_col, g.N, bias);
     __syncthreads();
+    if constexpr (WK > 1) {  // the other teams' sums first, added in order
+        static_assert(WK == 2 && MT * NT * kTeam * kWave * 64 <= 2 * kStage, "one more team, whose sums fit");
+        f32x16* sums = reinterpret_cast<f32x16*>(lds) + wave % kTeam * (MT * NT * kWave) + lane;
+        if (team == 1) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) sums[i * kWave] = acc[i / NT][i % NT];
+        }
+        __syncthreads();
+        if (team == 0) {
+#pragma unroll
+            for (int i = 0; i < MT * NT; ++i) acc[i / NT][i % NT] += sums[i * kWave];
+        }
+        __syncthreads();
+        if (team == 1) return;
+    }
     float* mine = reinterpret_cast<float*>(lds + wave * 32 * kPitch);
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
@@ -506,13 +541,13 @@ inline bool few_rows(int64_t M, int64_t N, int64_t K) {
 }
 
 // Launches the kernel of one tile size.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT, int STAGES>
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
 int launch_matmul(MatmulArgs g, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
-    constexpr size_t scale_rows = (BM + BN + WM * WN * kWave - 1) / (WM * WN * kWave) * (WM * WN * kWave);
-    constexpr size_t lds = STAGES * ((size_t)(BM + BN) * kBlockK + scale_rows * 4);
-    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT, STAGES>;
-    static_assert(lds <= 163840 && STAGES <= 4, "LDS of a CU; the waits of the loop");
+    constexpr size_t threads = WM * WN * WK * kWave, rows = WK * (size_t)(BM + BN);
+    constexpr size_t lds = 2 * (rows * kBlockK + (rows + threads - 1) / threads * threads * 4);
+    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT, WK>;
+    static_assert(lds <= 163840, "LDS of a CU");
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -522,7 +557,7 @@ int launch_matmul(MatmulArgs g, hipStream_t st) {
     g.tiles_n = (g.N + BN - 1) / BN;
     if ((int64_t)g.tiles_m * g.tiles_n > 0x7fffffff)
         return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: %d x %d is too large", g.M, g.N);
-    kernel<<<(unsigned)(g.tiles_m * g.tiles_n), WM * WN * kWave, lds, st>>>(g);
+    kernel<<<(unsigned)(g.tiles_m * g.tiles_n), threads, lds, st>>>(g);
     return capi_check_launch("matmul_kernel");
 }
 
@@ -532,9 +567,9 @@ template <typename T, bool FAST>
 int matmul(const MatmulArgs& g, hipStream_t st) {
     const auto tiles = [&](int64_t bm, int64_t bn) { return (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn); };
     if constexpr (FAST)
-        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2, 2>(g, st);
-    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2, 2>(g, st);
-    return launch_matmul<T, FAST, 2, 2, 1, 1, 4>(g, st);
+        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2, 1>(g, st);
+    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2, 1>(g, st);
+    return launch_matmul<T, FAST, 2, 2, 1, 1, 2>(g, st);
 }
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
