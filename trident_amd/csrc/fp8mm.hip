@@ -204,43 +204,57 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
     const int m0 = tm * BM, n0 = tn * BN;
     const int team = wave / kTeam, wm = wave % kTeam / WN * MT * 32, wn = wave % WN * NT * 32;
 
-    // rows of the tile: BM of a, then BN of b; those past an operand's end read its last row
-    const auto row_of = [&](int row) { return row < BM ? min(row, g.M - 1 - m0) : min(row - BM, g.N - 1 - n0); };
-    const __amdgpu_buffer_rsrc_t buf_a = buffer_at(g.a + (int64_t)m0 * g.pitch_a);
-    const __amdgpu_buffer_rsrc_t buf_b = buffer_at(g.b + (int64_t)n0 * g.pitch_b);
-    const __amdgpu_buffer_rsrc_t buf_sa = buffer_at(g.sa + (int64_t)m0 * g.spitch);
-    const __amdgpu_buffer_rsrc_t buf_sb = buffer_at(g.sb + (int64_t)n0 * g.spitch);
-    // This lane's part of each load: row l / 8 of it, piece l % 8, exchanged by bits 1 to 3 of the row,
-    // of which the last is the load's parity.  The offsets are made anew for each
-    // block (`sub` is hidden from the compiler, which would keep them all in registers, and spill).
-    int sub = lane / 8;
+    // A stage is WK times BM rows of a and BN of b, kLoads loads of eight rows for each wave: of one
+    // operand, so the wave's loads differ in a scalar only.  Rows past the operand's end repeat the last.
+    constexpr int kWaveRows = kLoads * 8;
+    static_assert(BM % kWaveRows == 0 && kRows % kWaveRows == 0, "a wave loads from one operand");
+    const auto operand = [&](int first, auto&& of_a, auto&& of_b) { return first % kRows < BM ? of_a : of_b; };
+    const int first = wave * kWaveRows, load_part = first / kRows;
+    const int row0 = first % kRows < BM ? m0 + first % kRows : n0 + first % kRows - BM;
+    const int limit = operand(first, g.M, g.N), start = min(row0, limit - 1), rows = min(kWaveRows, limit - start);
+    const int64_t pitch = operand(first, g.pitch_a, g.pitch_b);
+    const __amdgpu_buffer_rsrc_t buf = buffer_at(operand(first, g.a, g.b) + start * pitch);
+    const uint32_t row_step = (uint32_t)pitch * 8;
+    // row l / 8 of a load, piece l % 8, exchanged by bits 1 to 3 of the row, the last being the load's parity
     const uint32_t piece = (uint32_t)((lane % 8) ^ (lane / 16)) * 16;
+    const uint32_t even = (uint32_t)(lane / 8) * (uint32_t)pitch + piece, odd = even ^ 64;
+    // the scales: 64 rows a load
+    __amdgpu_buffer_rsrc_t scale_buf[kScaleLoads];
+    uint32_t scale_row[kScaleLoads];
+    int scale_part[kScaleLoads];
+#pragma unroll
+    for (int i = 0; i < kScaleLoads; ++i) {
+        const int at = min((i * kWaves + wave) * kWave, WK * kRows - kWave), in = at % kRows;
+        const int row = in < BM ? m0 + in : n0 + in - BM, last = operand(at, g.M, g.N) - 1;
+        scale_part[i] = at / kRows;
+        scale_buf[i] = buffer_at(operand(at, g.sa, g.sb) + (int64_t)min(row, last) * g.spitch);
+        scale_row[i] = (uint32_t)(min(row + lane, last) - min(row, last)) * (uint32_t)g.spitch;
+    }
     const auto fetch = [&](int step) {
-        asm volatile("" : "+v"(sub));
         uint8_t* to = lds + step % 2 * kStage + wave * kLoads * 1024;
+        const uint32_t k = (uint32_t)min(step * WK + load_part, g.kb - 1) * kBlockK;
+        if (rows == kWaveRows) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) {
-            const int at = (wave * kLoads + i) * 8, first = at % kRows;  // the same operand for the whole wave
-            const int kb = min(step * WK + at / kRows, g.kb - 1);
-            const uint32_t pitch = (uint32_t)(first < BM ? g.pitch_a : g.pitch_b);
-            const uint32_t from = (uint32_t)row_of(first + sub) * pitch + (piece ^ (i % 2 * 64));
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(first < BM ? buf_a : buf_b, (lds_ptr)(to + i * 1024), 16, from,
-                                                     kb * kBlockK, 0, 0);
+            for (int i = 0; i < kLoads; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(to + i * 1024), 16, i % 2 ? odd : even,
+                                                         k + i * row_step, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(
+                    buf, (lds_ptr)(to + i * 1024), 16,
+                    (uint32_t)min(i * 8 + lane / 8, rows - 1) * (uint32_t)pitch + (piece ^ (i % 2 * 64)), k, 0, 0);
         }
-        uint8_t* st = lds + 2 * kStage + step % 2 * kScaleStage + wave * kWave * 4;
 #pragma unroll
-        for (int i = 0; i < kScaleLoads; ++i) {
-            const int at = min((i * kWaves + wave) * kWave, WK * kRows - kWave), first = at % kRows;
-            const int kb = min(step * WK + at / kRows, g.kb - 1);
+        for (int i = 0; i < kScaleLoads; ++i)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
-                first < BM ? buf_sa : buf_sb, (lds_ptr)(st + i * kWaves * kWave * 4), 4,
-                (uint32_t)row_of(first + sub * 8 + (lane & 7)) * (uint32_t)g.spitch, kb & ~3, 0, 0);
-        }
+                scale_buf[i],
+                (lds_ptr)(lds + 2 * kStage + step % 2 * kScaleStage + (i * kWaves + wave) * kWave * 4), 4, scale_row[i],
+                min(step * WK + scale_part[i], g.kb - 1) & ~3, 0, 0);
     };
     // where this lane reads the four pieces of its first row of either operand; the other rows are 32
     // rows on, the other stage is the next bit
     static_assert((kStage & (kStage - 1)) == 0, "a stage is a bit of the address");
-    const uint32_t origin = (uint32_t)(uintptr_t)(lds_ptr)lds;
     uint32_t at_a[4], at_b[4];
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
@@ -248,10 +262,12 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
         at_a[c] = (uint32_t)(team * kRows + wm + r) * kBlockK + p;
         at_b[c] = (uint32_t)(team * kRows + BM + wn + r) * kBlockK + p;
     }
+    typedef const __attribute__((address_space(3))) uint8_t* lds_bytes;
+    typedef const __attribute__((address_space(3))) u32x4* lds_piece;
+    const lds_bytes stage0 = (lds_bytes)(lds_ptr)lds;
     const auto read = [&](const uint32_t (&at)[4], int half, int block) {
-        typedef const __attribute__((address_space(3))) u32x4* piece_ptr;
-        const u32x4 lo = *(piece_ptr)(uintptr_t)(origin + at[2 * half] + block * 32 * kBlockK);
-        const u32x4 hi = *(piece_ptr)(uintptr_t)(origin + at[2 * half + 1] + block * 32 * kBlockK);
+        const u32x4 lo = *(lds_piece)(stage0 + at[2 * half] + block * (32 * kBlockK));
+        const u32x4 hi = *(lds_piece)(stage0 + at[2 * half + 1] + block * (32 * kBlockK));
         i32x8 f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -285,12 +301,17 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
         asm volatile("" ::: "memory");
         const int kb = step * WK + team;
         const bool live = WK == 1 || kb < g.kb;  // not in the last step of the last team of an odd number
-        uint32_t ea[MT], eb[NT];                 // the scale of this block in the lowest byte
         const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + 2 * kStage + step % 2 * kScaleStage) + team * kRows;
+        uint32_t ea[MT], eb[NT];  // the scale of this block in the lowest byte
 #pragma unroll
-        for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r] >> (kb % 4 * 8);
+        for (int i = 0; i < MT; ++i) ea[i] = st[wm + i * 32 + r];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) eb[j] = st[BM + wn + j * 32 + r] >> (kb % 4 * 8);
+        for (int j = 0; j < NT; ++j) eb[j] = st[BM + wn + j * 32 + r];
+        __builtin_amdgcn_sched_barrier(0);  // these reads first: every product needs them
+#pragma unroll
+        for (int i = 0; i < MT; ++i) ea[i] >>= kb % 4 * 8;
+#pragma unroll
+        for (int j = 0; j < NT; ++j) eb[j] >>= kb % 4 * 8;
         i32x8 fa[2][MT], fb[2][NT];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -325,9 +346,9 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
         };
         if (live) multiply(0);
         if constexpr (FAST) {
-            // the first half's reads with the scales', the second half's among the first half's products
+            // the first half's reads, the second half's among the first half's products
             constexpr int kReads = 2 * (MT + NT), kProducts = MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
-            __builtin_amdgcn_sched_group_barrier(0x100, kReads + MT + NT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
                 __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
