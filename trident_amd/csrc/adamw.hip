@@ -55,15 +55,6 @@ __device__ __forceinline__ void load4(const T* p, float (&f)[kPer]) {
     for (int i = 0; i < kPer; ++i) f[i] = (float)v[i];
 }
 
-template <typename T>
-__device__ __forceinline__ void store4(T* p, const float (&f)[kPer]) {
-    typedef T tv __attribute__((ext_vector_type(kPer)));
-    tv v;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) v[i] = (T)f[i];
-    __builtin_memcpy(p, &v, sizeof(tv));
-}
-
 // Elements at .. at + 3 of a tensor of `left` more; zeros past its end.
 __device__ __forceinline__ void load_any(const void* base, int dtype, int64_t at, int64_t left, float (&f)[kPer]) {
     const auto get = [&](auto t) {
@@ -81,12 +72,13 @@ __device__ __forceinline__ void load_any(const void* base, int dtype, int64_t at
     else get(f16_t{});
 }
 
+template <bool PAST_L2>
 __device__ __forceinline__ void store_any(void* base, int dtype, int64_t at, int64_t left, const float (&f)[kPer]) {
     const auto put = [&](auto t) {
         using T = decltype(t);
         T* p = static_cast<T*>(base) + at;
         if (left >= kPer) {
-            store4(p, f);
+            put_vec<PAST_L2>(p, f);
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i)
@@ -122,7 +114,7 @@ __device__ __forceinline__ float encode(const float (&x)[kPer], float levels, fl
 constexpr float kLevelsM = 127.0f * 127.0f, kLevelsV = 255.0f * 255.0f;
 
 // Bound by bytes: every operand is read and written once, a wave a block of 256 elements at a time.
-template <int BITS>
+template <int BITS, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
     int lo = 0, hi = a.tensors - 1;  // the last tensor whose first chunk is not past this one
     while (lo < hi) {
@@ -165,10 +157,10 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
             root[i] = sqrtf(v[i]);
             p[i] = p[i] * a.decay - a.rate * (m[i] / (root[i] * a.inv_root + a.eps));
         }
-        store_any(t.param, t.dtype, at, left, p);
+        store_any<PAST_L2>(t.param, t.dtype, at, left, p);
         if constexpr (BITS == 32) {
-            store4(static_cast<float*>(a.m) + s, m);
-            store4(static_cast<float*>(a.v) + s, v);
+            put_vec<PAST_L2>(static_cast<float*>(a.m) + s, m);
+            put_vec<PAST_L2>(static_cast<float*>(a.v) + s, v);
         } else {
             float size[kPer], cm[kPer], cv[kPer];
 #pragma unroll
@@ -197,6 +189,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
 }
 
 // The values that 8-bit states stand for.
+template <bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adam_values_kernel(const uint32_t* __restrict__ cm,
                                                              const uint32_t* __restrict__ cv,
                                                              const float* __restrict__ sm,
@@ -214,8 +207,8 @@ __global__ __launch_bounds__(kBlock) void adam_values_kernel(const uint32_t* __r
         y[i] = r * r * fv;
         y[i] = y[i] * y[i];
     }
-    store4(m + q * kPer, x);
-    store4(v + q * kPer, y);
+    put_vec<PAST_L2>(m + q * kPer, x);
+    put_vec<PAST_L2>(v + q * kPer, y);
 }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
@@ -283,8 +276,11 @@ int trident_adamw(const TridentAdamTensor* tensors, int32_t count, const Trident
             chunks += c;
         }
         if (chunks == 0) continue;
-        if (state->bits == 32) adamw_kernel<32><<<(unsigned)chunks, kBlock, 0, st>>>(a);
-        else adamw_kernel<8><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+        with_bool(chunks * kChunkElems * 4 > kL2Bytes, [&](auto past) {
+            constexpr bool P = decltype(past)::value;
+            if (state->bits == 32) adamw_kernel<32, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+            else adamw_kernel<8, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+        });
         const int rc = capi_check_launch("adamw_kernel");
         if (rc) return rc;
     }
@@ -300,9 +296,11 @@ int trident_adamw_state_values(const TridentAdamState* state, float* m, float* v
     const int64_t quads = state->len / kPer, blocks = (quads + kBlock - 1) / kBlock;
     if (blocks > 0x7fffffff) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "adamw_state_values: len=%lld", (long long)state->len);
     if (quads == 0) return TRIDENT_OK;
-    adam_values_kernel<<<(unsigned)blocks, kBlock, 0, static_cast<hipStream_t>(stream)>>>(
-        static_cast<const uint32_t*>(state->m), static_cast<const uint32_t*>(state->v), state->m_scale,
-        state->v_scale, quads, m, v);
+    with_bool(state->len * 8 > kL2Bytes, [&](auto past) {
+        adam_values_kernel<decltype(past)::value><<<(unsigned)blocks, kBlock, 0, static_cast<hipStream_t>(stream)>>>(
+            static_cast<const uint32_t*>(state->m), static_cast<const uint32_t*>(state->v), state->m_scale,
+            state->v_scale, quads, m, v);
+    });
     return capi_check_launch("adam_values_kernel");
 }
 

@@ -27,7 +27,7 @@ constexpr int kEmbedUnroll = 4;
 // Bound by bytes: the rows' vectors of all tokens, one after the other, are dealt to the lanes, so a
 // row of any length leaves no lane idle; four independent gathers per lane cover the latency of the
 // id and of the row behind it.
-template <typename T, int VEC, typename ID>
+template <typename T, int VEC, typename ID, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
     const int64_t base = (int64_t)blockIdx.x * (kBlock * kEmbedUnroll);
     const int64_t row0 = base / a.nv;
@@ -60,7 +60,7 @@ __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
     }
 #pragma unroll
     for (int u = 0; u < kEmbedUnroll; ++u)
-        if (row[u] < a.n) store_vec(out + row[u] * a.ldo + col[u], f[u]);
+        if (row[u] < a.n) put_vec<PAST_L2>(out + row[u] * a.ldo + col[u], f[u]);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -375,7 +375,7 @@ constexpr int kClear = 16;  // rows of a wave that clears
 // is summed chunk by chunk into `part`, of which a chunk needs two: for the row it begins in and the
 // row it ends in; join_long_kernel adds a row's parts in order.  So every group has between one and two
 // chunks of work, whatever the frequencies.
-template <typename T, int VEC, int NVL>
+template <typename T, int VEC, int NVL, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
     constexpr int kAhead = NVL > 2 ? 4 : 8;
     const int l = threadIdx.x % a.lanes;
@@ -398,7 +398,7 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
             if (a.row[r0 + i].count) continue;
 #pragma unroll
             for (int c = 0; c < NVL; ++c)
-                if (on[c]) store_vec(out + (r0 + i) * a.ldo + col[c], acc[c]);
+                if (on[c]) put_vec<PAST_L2>(out + (r0 + i) * a.ldo + col[c], acc[c]);
         }
         return;
     }
@@ -425,7 +425,7 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
                 } else {
 #pragma unroll
                     for (int i = 0; i < VEC; ++i) acc[c][i] *= a.scale;
-                    store_vec(out + (int64_t)row * a.ldo + col[c], acc[c]);
+                    put_vec<PAST_L2>(out + (int64_t)row * a.ldo + col[c], acc[c]);
                 }
             }
 #pragma unroll
@@ -810,8 +810,10 @@ int trident_embedding(const void* weight, int32_t dtype, int64_t V, int64_t D, i
                 return;
             }
             hipStream_t st = static_cast<hipStream_t>(stream);
-            if (vec > 1) embed_kernel<T, kVec<T>, ID><<<(unsigned)blocks, kBlock, 0, st>>>(a);
-            else embed_kernel<T, 1, ID><<<(unsigned)blocks, kBlock, 0, st>>>(a);
+            if (vec == 1) embed_kernel<T, 1, ID, false><<<(unsigned)blocks, kBlock, 0, st>>>(a);
+            else if (n * D * (int64_t)sizeof(T) <= kL2Bytes)
+                embed_kernel<T, kVec<T>, ID, false><<<(unsigned)blocks, kBlock, 0, st>>>(a);
+            else embed_kernel<T, kVec<T>, ID, true><<<(unsigned)blocks, kBlock, 0, st>>>(a);
             rc = capi_check_launch("embed_kernel");
         });
     });
@@ -871,11 +873,14 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
         a.chunk_blocks = (int)((s.chunks + groups - 1) / groups);
         const dim3 grid((unsigned)(a.chunk_blocks + (V + clear - 1) / clear),
                         (unsigned)((a.nv + nvl * a.lanes - 1) / (nvl * a.lanes)));
-        if (vec == 1) embed_grad_kernel<T, 1, 1><<<grid, kBlock, 0, st>>>(a);
-        else if (nvl == 1) embed_grad_kernel<T, kVec<T>, 1><<<grid, kBlock, 0, st>>>(a);
-        else if (nvl == 2) embed_grad_kernel<T, kVec<T>, 2><<<grid, kBlock, 0, st>>>(a);
-        else if (nvl == 3) embed_grad_kernel<T, kVec<T>, 3><<<grid, kBlock, 0, st>>>(a);
-        else embed_grad_kernel<T, kVec<T>, 4><<<grid, kBlock, 0, st>>>(a);
+        with_bool(V * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
+            constexpr bool P = decltype(past)::value;
+            if (vec == 1) embed_grad_kernel<T, 1, 1, P><<<grid, kBlock, 0, st>>>(a);
+            else if (nvl == 1) embed_grad_kernel<T, kVec<T>, 1, P><<<grid, kBlock, 0, st>>>(a);
+            else if (nvl == 2) embed_grad_kernel<T, kVec<T>, 2, P><<<grid, kBlock, 0, st>>>(a);
+            else if (nvl == 3) embed_grad_kernel<T, kVec<T>, 3, P><<<grid, kBlock, 0, st>>>(a);
+            else embed_grad_kernel<T, kVec<T>, 4, P><<<grid, kBlock, 0, st>>>(a);
+        });
         if ((rc = capi_check_launch("embed_grad_kernel")) || n <= s.chunk) return;
         join_long_kernel<T><<<dim3(1u << s.shift, (unsigned)((D + kWave - 1) / kWave)), kBlock, 0, st>>>(a);
         rc = capi_check_launch("join_long_kernel");

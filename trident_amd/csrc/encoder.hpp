@@ -29,6 +29,13 @@ constexpr int kVec = 16 / (int)sizeof(T);  // elements of one 16-byte access
 
 inline bool dtype_ok(int32_t t) { return t == TRIDENT_F32 || t == TRIDENT_F16 || t == TRIDENT_BF16; }
 
+// Calls f with std::true_type or std::false_type.
+template <typename F>
+inline void with_bool(bool b, F&& f) {
+    if (b) f(std::true_type{});
+    else f(std::false_type{});
+}
+
 // Calls f with a value of the element type that `t` names.
 template <typename F>
 inline void with_dtype(int32_t t, F&& f) {
@@ -91,12 +98,32 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[N]
     if constexpr (N == 1) {
         p[0] = (T)f[0];
     } else {
-        static_assert(N == kVec<T>, "one 16-byte access");
         typedef T tv __attribute__((ext_vector_type(N)));
         tv t;
 #pragma unroll
         for (int i = 0; i < N; ++i) t[i] = (T)f[i];
-        __builtin_memcpy(p, &t, 16);
+        __builtin_memcpy(p, &t, sizeof(t));
+    }
+}
+
+// A result larger than the card's L2 (eight times 4 MB) is stored past it: nothing of it would be left
+// for the next kernel, and the rows that this one reads again stay (131,072 embedding rows of 960
+// bfloat16 from a table of 126 MB: 78 us through L2, 47 past it).
+constexpr int64_t kL2Bytes = 32 << 20;
+
+// A template argument: of two stores under a condition the compiler makes one, an ordinary one.
+template <bool PAST_L2, typename T, int N>
+__device__ __forceinline__ void put_vec(T* __restrict__ p, const float (&f)[N]) {
+    if constexpr (N == 1 || !PAST_L2) {
+        store_vec(p, f);
+    } else {
+        typedef T tv __attribute__((ext_vector_type(N)));
+        typedef uint32_t words __attribute__((ext_vector_type(N * sizeof(T) / 4)));
+        typedef words any __attribute__((aligned(2)));
+        tv t;
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = (T)f[i];
+        __builtin_nontemporal_store(__builtin_bit_cast(words, t), reinterpret_cast<any*>(p));
     }
 }
 

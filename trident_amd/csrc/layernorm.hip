@@ -86,7 +86,7 @@ __device__ __forceinline__ float row_sum(float v, float* s_red) {
 
 // Bound by bytes.  A wave (a workgroup of W = 4 waves for rows of more than 256 vectors) takes every
 // gridDim-th row and loads the next one while it works on this one.
-template <typename T, typename TW, int VEC, int NV, int W>
+template <typename T, typename TW, int VEC, int NV, int W, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
     __shared__ float s_red[W];
     constexpr int kRows = kWavesPerBlock / W;
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
                 if (a.bias) v += b[i];
                 x[c][i] = v;
             }
-            store_vec(y + k.col[c], x[c]);
+            put_vec<PAST_L2>(y + k.col[c], x[c]);
         }
         if (a.mean && (W == 1 ? lane_id() : (int)threadIdx.x) == 0) {
             a.mean[row] = mean;
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
 // Bound by bytes.  A wave (or a workgroup, W = 4) takes every gridDim-th row, the next one's loads ahead
 // of this one's work: dx from the row's two means, and dy h and dy added to the columns' sums, which stay
 // in registers until the last row.
-template <typename T, typename TW, int VEC, int NV, int W>
+template <typename T, typename TW, int VEC, int NV, int W, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
     extern __shared__ float s_part[];  // [kWavesPerBlock][D], W = 1 only
     __shared__ float s_red[W];
@@ -232,7 +232,7 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
             if (!k.on[c]) continue;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) g[c][i] = rstd * (g[c][i] - sa - h[c][i] * sh);
-            store_vec(dx + k.col[c], g[c]);
+            put_vec<PAST_L2>(dx + k.col[c], g[c]);
         }
         now_x = next_x;
         now_dy = next_dy;
@@ -392,7 +392,9 @@ int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, in
                     a.nv = (int)((D + VEC - 1) / VEC);
                     const int64_t per = kWavesPerBlock / W;
                     const unsigned grid = (unsigned)std::min<int64_t>(kNormBlocks, (rows + per - 1) / per);
-                    norm_kernel<T, TW, VEC, NV, W><<<grid, kBlock, 0, st>>>(a);
+                    with_bool(rows * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
+                        norm_kernel<T, TW, VEC, NV, W, decltype(past)::value><<<grid, kBlock, 0, st>>>(a);
+                    });
                 });
                 if (!ok) norm_long_kernel<T, TW><<<(unsigned)rows, kBlock, 0, st>>>(a);
             }
@@ -440,7 +442,10 @@ int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_
                     constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
                     const size_t lds = W == 1 ? kWavesPerBlock * (size_t)D * sizeof(float) : 0;
-                    norm_grad_kernel<T, TW, VEC, NV, W><<<(unsigned)parts, kBlock, lds, st>>>(a);
+                    with_bool(rows * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
+                        norm_grad_kernel<T, TW, VEC, NV, W, decltype(past)::value>
+                            <<<(unsigned)parts, kBlock, lds, st>>>(a);
+                    });
                     joined = joined || (W == 1 && parts == 1);
                 });
                 if (!ok) norm_grad_long_kernel<T, TW><<<(unsigned)parts, kBlock, 0, st>>>(a);
