@@ -46,22 +46,23 @@ struct AdamArgs {
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
-template <typename T>
+template <bool PAST_L2, typename T>
 __device__ __forceinline__ void load4(const T* p, float (&f)[kPer]) {
     typedef T tv __attribute__((ext_vector_type(kPer)));
-    tv v;
-    __builtin_memcpy(&v, p, sizeof(tv));
+    typedef uint32_t words __attribute__((ext_vector_type(sizeof(tv) / 4)));
+    const tv v = __builtin_bit_cast(tv, load_words<PAST_L2, words>(p));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) f[i] = (float)v[i];
 }
 
 // Elements at .. at + 3 of a tensor of `left` more; zeros past its end.
+template <bool PAST_L2>
 __device__ __forceinline__ void load_any(const void* base, int dtype, int64_t at, int64_t left, float (&f)[kPer]) {
     const auto get = [&](auto t) {
         using T = decltype(t);
         const T* p = static_cast<const T*>(base) + at;
         if (left >= kPer) {
-            load4(p, f);
+            load4<PAST_L2>(p, f);
         } else {
 #pragma unroll
             for (int i = 0; i < kPer; ++i) f[i] = i < left ? (float)p[i] : 0.0f;
@@ -131,11 +132,11 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
         const int64_t at = first + lane * kPer, left = t.numel - at, s = t.offset + at;
         const int64_t block = (t.offset + first) / kStateBlock;
         float p[kPer], g[kPer], m[kPer], v[kPer];
-        load_any(t.param, t.dtype, at, left, p);
-        load_any(t.grad, t.grad_dtype, at, left, g);
+        load_any<PAST_L2>(t.param, t.dtype, at, left, p);
+        load_any<PAST_L2>(t.grad, t.grad_dtype, at, left, g);
         if constexpr (BITS == 32) {
-            load4(static_cast<const float*>(a.m) + s, m);
-            load4(static_cast<const float*>(a.v) + s, v);
+            load4<PAST_L2>(static_cast<const float*>(a.m) + s, m);
+            load4<PAST_L2>(static_cast<const float*>(a.v) + s, v);
         } else {
             const uint32_t cm = *reinterpret_cast<const uint32_t*>(static_cast<const int8_t*>(a.m) + s);
             const uint32_t cv = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.v) + s);

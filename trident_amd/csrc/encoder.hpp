@@ -44,6 +44,21 @@ inline void with_dtype(int32_t t, F&& f) {
     else f(bf16_t{});
 }
 
+// A result larger than the card's L2 (eight times 4 MB) is written past it: nothing of it would be left
+// for the next kernel, and the rows that this one reads again stay (131,072 embedding rows of 960
+// bfloat16 from a table of 126 MB: 78 us through L2, 47 past it).  Reading past it pays where nothing is
+// read twice (AdamW on 62M elements: 314 to 300 us) and not where the next pass reads the same again
+// (layer norm's rows, forward and backward: 193 to 196 us).
+constexpr int64_t kL2Bytes = 32 << 20;
+
+// `WORDS`, 4 to 16 bytes, from any element's address.
+template <bool PAST_L2, typename WORDS>
+__device__ __forceinline__ WORDS load_words(const void* p) {
+    typedef WORDS any __attribute__((aligned(2), may_alias));
+    if constexpr (PAST_L2) return __builtin_nontemporal_load(reinterpret_cast<const any*>(p));
+    else return *reinterpret_cast<const any*>(p);
+}
+
 // N elements from any element's address, held as they are stored: one element, or whole 16-byte
 // accesses.
 template <typename T, int N>
@@ -57,7 +72,7 @@ struct Vec {
         } else {
             static_assert(N % kVec<T> == 0, "whole 16-byte accesses");
 #pragma unroll
-            for (int k = 0; k < kWords; ++k) __builtin_memcpy(&raw[k], p + k * kVec<T>, 16);
+            for (int k = 0; k < kWords; ++k) raw[k] = load_words<false, u32x4>(p + k * kVec<T>);
         }
     }
     __device__ __forceinline__ void get(float (&f)[N]) const {
@@ -105,11 +120,6 @@ __device__ __forceinline__ void store_vec(T* __restrict__ p, const float (&f)[N]
         __builtin_memcpy(p, &t, sizeof(t));
     }
 }
-
-// A result larger than the card's L2 (eight times 4 MB) is stored past it: nothing of it would be left
-// for the next kernel, and the rows that this one reads again stay (131,072 embedding rows of 960
-// bfloat16 from a table of 126 MB: 78 us through L2, 47 past it).
-constexpr int64_t kL2Bytes = 32 << 20;
 
 // A template argument: of two stores under a condition the compiler makes one, an ordinary one.
 template <bool PAST_L2, typename T, int N>
