@@ -72,6 +72,12 @@ struct RowInfo {
     int beg, count;  // a row's places among the ordered tokens
 };
 
+// Where a table row's RowInfo lies: those of one sorting workgroup (ids equal modulo 2^shift) next to
+// one another, so that it writes whole lines.
+__device__ __forceinline__ int64_t info_at(int v, int shift, int owned) {
+    return (int64_t)(v & ((1 << shift) - 1)) * owned + (v >> shift);
+}
+
 struct Token {
     int t, row;
 };
@@ -84,7 +90,7 @@ struct SortArgs {
     const void* ids;
     int n, V, owned, shift, chunk, parts;
     uint32_t skip;     // an id without a gradient; 2^32 - 1: none
-    RowInfo* row;      // [V + 1]
+    RowInfo* row;      // [2^shift, owned], and one more: the number of all tokens
     Token* token;      // [n]
     int* long_count;   // [2^shift]
     int* long_rows;    // [2^shift, owned]
@@ -267,8 +273,8 @@ struct SortShape {
     }
 };
 
-// Orders the tokens by id: row[v] says where in `token` the tokens of id v lie, in their own order;
-// row[V] holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power of two): the
+// Orders the tokens by id: row[info_at(v)] says where in `token` the tokens of id v lie, in their own
+// order; the last entry holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power of two): the
 // most frequent ids of a vocabulary are neighbours, so a range of them would be one workgroup's work.
 // Each wave goes through its share of the tokens, keeps those its workgroup owns in a list in LDS, and
 // counts them by id; the counts, and the number of tokens of lower workgroups, give every (id, wave)
@@ -320,7 +326,7 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
         int at = place + block_sum<WAVES>(count, s_sum, &total) - count;
         place += total;
         if (live) {
-            a.row[v] = RowInfo{at, count};
+            a.row[(int64_t)b * w + j] = RowInfo{at, count};
             if (count > a.chunk) a.long_rows[(int64_t)b * w + atomicAdd(&s_long, 1)] = (int)v;  // in any order
             for (int i = 0; i < WAVES; ++i) {
                 const int c = hist[i * w + j];
@@ -329,7 +335,7 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
             }
         }
     }
-    if (b == gridDim.x - 1 && threadIdx.x == 0) a.row[a.V] = RowInfo{place, 0};
+    if (b == gridDim.x - 1 && threadIdx.x == 0) a.row[(int64_t)gridDim.x * w] = RowInfo{place, 0};
     __syncthreads();
     if (threadIdx.x == 0) a.long_count[b] = s_long;
     int bits = 0;
@@ -353,14 +359,14 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
 
 struct EmbedGradArgs {
     const void* grad;       // [n, ld]
-    const RowInfo* row;     // [V + 1]
+    const RowInfo* row;     // at info_at
     const Token* token;     // tokens by id
     float* part;            // [2 chunks, D]: sums of the parts of long rows
     const int* long_count;  // [owners]: long rows of each sorting workgroup
     const int* long_rows;   // [owners, owned]
     void* out;              // [V, ldo]
     int64_t ld, ldo;
-    int V, D, nv, owned;
+    int V, D, nv, owned, shift;
     int lanes;              // lanes of a row: a power of two, 64 where a row has more vectors
     int chunk;              // tokens of a group of lanes
     int chunk_blocks;       // workgroups that take tokens; the others clear the rows without any
@@ -394,21 +400,23 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
     if ((int)blockIdx.x >= a.chunk_blocks) {
         const int per = kClear * (kWave / a.lanes);  // of this wave's rows, its groups take turns
         const int64_t r0 = ((int64_t)(blockIdx.x - a.chunk_blocks) * kWavesPerBlock + threadIdx.x / kWave) * per;
-        for (int i = lane_id() / a.lanes; i < per && r0 + i < a.V; i += kWave / a.lanes) {
-            if (a.row[r0 + i].count) continue;
+        const int64_t rows = (int64_t)a.owned << a.shift;
+        for (int i = lane_id() / a.lanes; i < per && r0 + i < rows; i += kWave / a.lanes) {
+            const int64_t v = ((r0 + i) % a.owned << a.shift) + (r0 + i) / a.owned;
+            if (v >= a.V || a.row[r0 + i].count) continue;
 #pragma unroll
             for (int c = 0; c < NVL; ++c)
-                if (on[c]) put_vec<PAST_L2>(out + (r0 + i) * a.ldo + col[c], acc[c]);
+                if (on[c]) put_vec<PAST_L2>(out + v * a.ldo + col[c], acc[c]);
         }
         return;
     }
     const int chunk = blockIdx.x * (kBlock / a.lanes) + threadIdx.x / a.lanes;
-    const int live = a.row[a.V].beg;
+    const int live = a.row[(int64_t)a.owned << a.shift].beg;
     const int64_t first = (int64_t)chunk * a.chunk;
     if (first >= live) return;
     int beg = (int)first, end = min(live, beg + a.chunk);
     const int row0 = a.token[beg].row, row1 = a.token[end - 1].row;
-    const RowInfo i0 = a.row[row0], i1 = a.row[row1];
+    const RowInfo i0 = a.row[info_at(row0, a.shift, a.owned)], i1 = a.row[info_at(row1, a.shift, a.owned)];
     const bool long0 = i0.count > a.chunk, long1 = i1.count > a.chunk;
     if (!long0 && i0.beg < beg) beg = i0.beg + i0.count;  // the chunk before has it
     if (!long1) end = i1.beg + i1.count;
@@ -476,22 +484,27 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
     __shared__ float s_sum[kWavesPerBlock][kWave];
     const int lane = lane_id(), wave = threadIdx.x / kWave, d = blockIdx.y * kWave + lane;
     const int count = a.long_count[blockIdx.x];
-    for (int i = 0; i < count; ++i) {
-        const int v = a.long_rows[(int64_t)blockIdx.x * a.owned + i];
-        const RowInfo r = a.row[v];
-        const int first = r.beg / a.chunk, parts = (r.beg + r.count - 1) / a.chunk - first + 1;
-        const int per = (parts + kWavesPerBlock - 1) / kWavesPerBlock;
-        const float* part = a.part + min(d, a.D - 1);
-        float s = 0.0f;
+    const float* part = a.part + min(d, a.D - 1);
+    for (int i0 = 0; i0 < count; i0 += kWave) {
+        // 64 rows' places at once, a row a lane
+        const int v_of = a.long_rows[(int64_t)blockIdx.x * a.owned + min(i0 + lane, count - 1)];
+        const RowInfo info = a.row[info_at(v_of, a.shift, a.owned)];
+        for (int i = 0; i < min(kWave, count - i0); ++i) {
+            const int v = __builtin_amdgcn_readlane(v_of, i), beg = __builtin_amdgcn_readlane(info.beg, i);
+            const int first = beg / a.chunk;
+            const int parts = (beg + __builtin_amdgcn_readlane(info.count, i) - 1) / a.chunk - first + 1;
+            const int per = (parts + kWavesPerBlock - 1) / kWavesPerBlock;
+            float s = 0.0f;
 #pragma unroll 16
-        for (int c = wave * per; c < min(parts, (wave + 1) * per); ++c)  // in its first chunk a row is the last one,
-            s += part[(int64_t)(2 * (first + c) + (c == 0 && r.beg % a.chunk)) * a.D];  // unless it begins the chunk
-        __syncthreads();
-        s_sum[wave][lane] = s;
-        __syncthreads();
-        if (wave == 0 && d < a.D) {
-            for (int k = 1; k < kWavesPerBlock; ++k) s += s_sum[k][lane];
-            static_cast<T*>(a.out)[(int64_t)v * a.ldo + d] = (T)(s * a.scale);
+            for (int c = wave * per; c < min(parts, (wave + 1) * per); ++c)  // in its first chunk a row is the last
+                s += part[(int64_t)(2 * (first + c) + (c == 0 && beg % a.chunk)) * a.D];  // one, unless it begins it
+            __syncthreads();
+            s_sum[wave][lane] = s;
+            __syncthreads();
+            if (wave == 0 && d < a.D) {
+                for (int k = 1; k < kWavesPerBlock; ++k) s += s_sum[k][lane];
+                static_cast<T*>(a.out)[(int64_t)v * a.ldo + d] = (T)(s * a.scale);
+            }
         }
     }
 }
@@ -708,7 +721,7 @@ GradSpace grad_space(void* base, int64_t n, int64_t V, int64_t D) {
         off += up256(bytes);
         return at;
     };
-    s.row = reinterpret_cast<RowInfo*>(take((size_t)(V + 1) * sizeof(RowInfo)));
+    s.row = reinterpret_cast<RowInfo*>(take((((size_t)s.owned << s.shift) + 1) * sizeof(RowInfo)));
     s.token = reinterpret_cast<Token*>(take((size_t)n * sizeof(Token)));
     s.part = reinterpret_cast<float*>(take(2 * (size_t)s.chunks * (size_t)D * sizeof(float)));
     s.long_count = reinterpret_cast<int*>(take(sizeof(int) << s.shift));
@@ -861,8 +874,8 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
     if (rc) return rc;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        EmbedGradArgs a{grad,   s.row,  s.token, s.part, s.long_count, s.long_rows, out, ld_grad,
-                        ld_out, (int)V, (int)D,  0,      s.owned,      0,           (int)s.chunk, 0, (float)scale};
+        EmbedGradArgs a{grad,   s.row,  s.token, s.part, s.long_count, s.long_rows, out, ld_grad,       ld_out,
+                        (int)V, (int)D, 0,       s.owned, s.shift,     0,           (int)s.chunk, 0, (float)scale};
         const int vec = D >= kVec<T> ? kVec<T> : 1;
         a.nv = (int)((D + vec - 1) / vec);
         a.lanes = 1;
@@ -871,7 +884,7 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
         const int groups = kBlock / a.lanes;
         const int64_t clear = kClear * (int64_t)groups;
         a.chunk_blocks = (int)((s.chunks + groups - 1) / groups);
-        const dim3 grid((unsigned)(a.chunk_blocks + (V + clear - 1) / clear),
+        const dim3 grid((unsigned)(a.chunk_blocks + (((int64_t)s.owned << s.shift) + clear - 1) / clear),
                         (unsigned)((a.nv + nvl * a.lanes - 1) / (nvl * a.lanes)));
         with_bool(V * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
             constexpr bool P = decltype(past)::value;
