@@ -6,6 +6,8 @@ Public surface, mirroring the reference's Python API (benchmarks/phase4a_suite.p
   train_clustering (load_or_train_clustering), metrics.eval_accuracy_v4, metrics.measure_latency_qps,
   metrics.measure_runs
   router.CostRouter / router.calibrate_w0                  (cost router)
+  encoder                  the operators that make and train the vectors: embedding, layer norm, AdamW,
+                           8-bit floating-point products (no reference counterpart)
 The compute path is libtrident_hip.so (hand-written HIP for gfx950) behind the C ABI in
 include/trident_hip.h; importing the package does not load it, calling a search does.
 """
