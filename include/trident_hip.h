@@ -350,7 +350,7 @@ int trident_adamw_state_values(const TridentAdamState* state, float* m, float* v
 
 /* 8-bit floating point (e4m3) with a scale 2^(e - 127) for each row and 128 columns.  Codes:
  * [rows, 128 ceil(K / 128)], 16-byte aligned, zeros past K.  Scales e: [rows, 4 ceil(K / 512)] bytes,
- * 127 past the last block.  A value that is not finite becomes NaN and leaves its block's scale alone. */
+ * 4-byte aligned, 127 past the last block.  A value that is not finite becomes NaN and leaves its block's scale alone. */
 int trident_fp8_quantize(const void* x, int32_t dtype, int64_t rows, int64_t K, int64_t ld_x, uint8_t* codes,
                          uint8_t* scales, void* stream);
 

@@ -101,6 +101,10 @@ def test_fp8_arguments():
     refused(L.trident_fp8_matmul(P, P, 4, P, P, 4, 100, P, 1, P, 2, 4, 0, None), 1, "bias_dtype=1")
     refused(L.trident_fp8_matmul(P, P, 4, P, P, 4, 100, None, 0, P, 2, 3, 0, None), 1, "bad sizes")
     refused(L.trident_fp8_matmul(P, None, 4, P, P, 4, 100, None, 0, P, 2, 4, 0, None), 1, "NULL")
+    refused(L.trident_fp8_matmul(P, P, 4, P + 8, P, 4, 100, None, 0, P, 2, 4, 0, None), 1, "16-byte")
+    refused(L.trident_fp8_matmul(P, P, 4, P, P + 2, 4, 100, None, 0, P, 2, 4, 0, None), 1, "4-byte")
+    refused(L.trident_fp8_matmul(P, P + 1, 4, P, P, 4, 100, None, 0, P, 2, 4, 0, None), 1, "4-byte")
+    refused(L.trident_fp8_matmul(P, P, 4, P, P, 4, 1 << 23, None, 0, P, 2, 4, 0, None), 2, "too large")
     assert L.trident_fp8_matmul(P, P, 0, P, P, 4, 100, None, 0, P, 2, 4, 0, None) == 0
     need = L.trident_fp8_linear_workspace_bytes(100, 4, 1000)
     assert need >= 100 * 1024 + 100 * 8

@@ -148,6 +148,14 @@ def test_embedding_grad_many_tokens(dev, n, V, D, wide):
     check_embedding_grad(randn(g, n, D, dtype=torch.bfloat16), token_ids(g, n, V, wide), V, skip=0 if V > 2 else None)
 
 
+def test_embedding_grad_one_id_of_a_large_table(dev):
+    """More tokens of one id than a wave keeps, where every workgroup reads all ids."""
+    g = gen(21)
+    ids = torch.full((40_000,), 599_990, device=dev)
+    ids[::1000] = torch.randint(0, 600_000, (40,), generator=g, device=dev)
+    check_embedding_grad(randn(g, 40_000, 9), ids, 600_000)
+
+
 def test_embedding_grad_without_tokens(dev):
     out = encoder.embedding_grad(torch.empty((0, 20), device=dev), torch.empty(0, dtype=torch.int64, device=dev), 300)
     assert out.shape == (300, 20) and (out == 0).all()
@@ -746,6 +754,24 @@ def test_in_a_graph(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, sequence())), i
 
 
+def test_adamw_refuses_parameters_that_changed(dev):
+    p = torch.zeros((4, 8), device=dev)
+    opt, grad = encoder.AdamW([p]), torch.ones((4, 8), device=dev)
+    opt.step([grad])
+    kept = p.data
+    for other, text in ((kept.cpu(), "on cuda"), (torch.zeros((8, 8), device=dev), "no longer"),
+                        (torch.zeros((8, 4), device=dev).t(), "no longer"),
+                        (torch.zeros((4, 8), device=dev, dtype=torch.float64), "float64")):
+        p.data = other
+        with pytest.raises(_lib.TridentError, match=text):
+            opt.step([grad])
+    p.data = kept
+    opt.step([grad])
+    assert opt.step_count == 2
+    with pytest.raises(AttributeError):
+        opt.exp_avg = torch.zeros_like(opt.exp_avg)
+
+
 def test_refusals(dev):
     f, i64 = torch.zeros((4, 8), device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
     q = encoder.quantize_fp8(f)
@@ -758,11 +784,13 @@ def test_refusals(dev):
         (lambda: encoder.embedding_grad(f, i64, 0), "num_rows"),
         (lambda: encoder.embedding_grad(f, i64, 10, padding_idx=10), "padding_idx"),
         (lambda: encoder.embedding_grad(f, i64, 10, out=f), "out must be"),
-        (lambda: encoder.layer_norm(f, torch.ones(7, device=dev)), "weight must be"),
+        (lambda: encoder.layer_norm(f, torch.ones(7, device=dev)), "weight and bias must be"),
+        (lambda: encoder.layer_norm(f, torch.ones(8)), "weight and bias must be"),
+        (lambda: encoder.layer_norm(f, f[0].half(), f[0]), "one type"),
         (lambda: encoder.layer_norm(f, torch.ones(8, device=dev).half()), "or float32"),
         (lambda: encoder.layer_norm(f, eps=-1.0), "eps"),
         (lambda: encoder.layer_norm_grad(f, f[:2], None, i64.float(), i64.float()), "grad must be"),
-        (lambda: encoder.layer_norm_grad(f, f, None, i64[:3].float(), i64.float()), "mean must be"),
+        (lambda: encoder.layer_norm_grad(f, f, None, i64[:3].float(), i64.float()), "mean and rstd must be"),
         (lambda: encoder.AdamW([]), "at least one"),
         (lambda: encoder.AdamW([f, f]), "twice"),
         (lambda: encoder.AdamW([f.t()]), "contiguous"),

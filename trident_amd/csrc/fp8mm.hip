@@ -595,6 +595,7 @@ int matmul(const MatmulArgs& g, hipStream_t st) {
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
 
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
@@ -631,8 +632,9 @@ int check_product(int64_t M, int64_t N, int64_t K, const void* a, const void* b_
     if (!counts_ok(M, K) || !counts_ok(N, K) || ld_out < N)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: bad sizes M=%lld N=%lld K=%lld ld=%lld",
                          (long long)M, (long long)N, (long long)K, (long long)ld_out);
-    if (M > 0 && N > 0 && (!a || !b_codes || !b_scales || !out || !aligned16(b_codes)))
-        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
+    if (M > 0 && N > 0 && (!a || !b_codes || !b_scales || !out || !aligned16(b_codes) || !aligned4(b_scales)))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "fp8_matmul: NULL pointer, or codes not 16-byte, scales not 4-byte aligned");
     return TRIDENT_OK;
 }
 
@@ -691,8 +693,9 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
                        int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream) {
     const int rc = check_product(M, N, K, a_codes, b_codes, b_scales, bias, bias_dtype, out, dtype, ld_out);
     if (rc || M == 0 || N == 0) return rc;
-    if (!a_scales || !aligned16(a_codes))
-        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_matmul: NULL pointer, or codes not 16-byte aligned");
+    if (!a_scales || !aligned16(a_codes) || !aligned4(a_scales))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "fp8_matmul: NULL pointer, or codes not 16-byte, scales not 4-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
     if (M <= kFewRows)
         return product_few<false>(nullptr, 0, a_codes, a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out,

@@ -32,6 +32,7 @@ STATE_BLOCK = 256  # elements of an 8-bit state that share a scale
 # conditions are plain expressions, and messages are only made for a call that is refused.
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
+_get_device, _data_ptr, _is_contiguous = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 _fns = {}
 
 
@@ -194,20 +195,16 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
 
 def _affine(index, x, D, weight, bias) -> int:
     """The type code of weight and bias, which is x's or float32."""
-    dtype = None
-    for name, t in (("weight", weight), ("bias", bias)):
+    dtype = x.dtype if weight is None and bias is None else (bias if weight is None else weight).dtype
+    for t in (weight, bias):
         if t is None:
             continue
-        _same(index, name, t)
-        if t.dim() != 1 or t.shape[0] != D or not t.is_contiguous():
-            _refuse(f"{name} must be a contiguous [{D}]")
-        if dtype is None:
-            dtype = t.dtype
-            if dtype != x.dtype and dtype != torch.float32:
-                _refuse(f"{name} must be {x.dtype} or float32, got {dtype}")
-        elif t.dtype != dtype:
-            _refuse("weight and bias must have one type")
-    return _DTYPES[x.dtype if dtype is None else dtype]
+        if t.shape != (D,) or not t.is_contiguous() or t.dtype is not dtype or t.get_device() != index:
+            _refuse(f"weight and bias must be contiguous [{D}] of one type on cuda:{index}, got "
+                    f"{[(tuple(t.shape), t.dtype, t.device) for t in (weight, bias) if t is not None]}")
+    if dtype is not x.dtype and dtype is not torch.float32:
+        _refuse(f"weight and bias must be {x.dtype} or float32, got {dtype}")
+    return _DTYPES[dtype]
 
 
 def _norm(x, weight, bias, eps, keep):
@@ -272,11 +269,10 @@ def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
     if grad.shape != x.shape or grad.dtype != x.dtype:
         _refuse(f"grad must be {tuple(x.shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
     _same(index, "grad", grad)
-    for name, t in (("mean", mean), ("rstd", rstd)):
-        _same(index, name, t)
-        if t.dtype != torch.float32 or t.shape != x.shape[:-1] or not t.is_contiguous():
-            _refuse(f"{name} must be a contiguous float32 {tuple(x.shape[:-1])}")
-    D = x.shape[-1]
+    D, lead = x.shape[-1], x.shape[:-1]
+    for t in (mean, rstd):
+        if t.dtype is not torch.float32 or t.shape != lead or not t.is_contiguous() or t.get_device() != index:
+            _refuse(f"mean and rstd must be contiguous float32 {tuple(lead)} on cuda:{index}")
     _affine(index, x, D, weight, None)
     rows = x.numel() // D
     wdtype = x.dtype if wdtype is None else wdtype
@@ -337,15 +333,10 @@ class AdamW:
         self._table["numel"] = [p.numel() for p in self.params]
         self._table["offset"] = self.offsets
         kind = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
-        self.exp_avg = torch.zeros(total, dtype=kind[0], device=self.device)
-        self.exp_avg_sq = torch.zeros(total, dtype=kind[1], device=self.device)
-        self.exp_avg_scale = self.exp_avg_sq_scale = None
-        if state_bits == 8:
-            self.exp_avg_scale = torch.zeros(total // STATE_BLOCK, device=self.device)
-            self.exp_avg_sq_scale = torch.zeros(total // STATE_BLOCK, device=self.device)
-        self._state = _lib.TridentAdamState(self.exp_avg.data_ptr(), self.exp_avg_sq.data_ptr(),
-                                            ext._ptr(self.exp_avg_scale), ext._ptr(self.exp_avg_sq_scale), total,
-                                            state_bits)
+        moments = [torch.zeros(total, dtype=k, device=self.device) for k in kind]
+        scales = [torch.zeros(total // STATE_BLOCK, device=self.device) if state_bits == 8 else None for _ in kind]
+        self._buffers = (*moments, *scales)
+        self._state = _lib.TridentAdamState(*map(ext._ptr, self._buffers), total, state_bits)
 
     def zero_grad(self) -> None:
         for p in self.params:
@@ -357,29 +348,40 @@ class AdamW:
         if len(grads) != len(self.params):
             _refuse(f"{len(self.params)} gradients are needed, got {len(grads)}")
         params, shapes, table = self.params, self._shapes, self._table
-        if any(g is None for g in grads):
+        try:
+            devices = set(map(_get_device, grads))
+        except TypeError:  # one is None
             at = [i for i, g in enumerate(grads) if g is not None]
             params, shapes, grads = [params[i] for i in at], [shapes[i] for i in at], [grads[i] for i in at]
             table = table[at]
-        if [g.shape for g in grads] != shapes or any(g.get_device() != self._index or g.is_sparse for g in grads):
+            devices = set(map(_get_device, grads))
+        devices.update(map(_get_device, params))
+        if [g.shape for g in grads] != shapes or not devices <= {self._index} or \
+                not {g.layout for g in grads} <= {torch.strided}:
             _refuse(f"gradients must be dense, on {self.device} and of their parameters' shapes "
-                    f"{[tuple(s) for s in shapes]}, got {[tuple(g.shape) for g in grads]}")
-        if [p.shape for p in params] != shapes or not all([p.is_contiguous() for p in params]):
+                    f"{[tuple(s) for s in shapes]}, got {[(tuple(g.shape), g.device, g.layout) for g in grads]}")
+        if [p.shape for p in params] != shapes or not all(map(_is_contiguous, params)):
             _refuse("a parameter is no longer the contiguous tensor it was")
-        if not all([g.is_contiguous() for g in grads]):
+        if not all(map(_is_contiguous, grads)):
             grads = [g.contiguous() for g in grads]
         try:
             table["dtype"] = [_DTYPES[p.dtype] for p in params]
             table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
         except KeyError as e:
             _refuse(f"parameters and gradients must be float32, float16 or bfloat16, got {e}")
-        table["param"] = [p.data_ptr() for p in params]
-        table["grad"] = [g.data_ptr() for g in grads]
+        table["param"] = [*map(_data_ptr, params)]
+        table["grad"] = [*map(_data_ptr, grads)]
         h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
                                    self.step_count + 1)
         _call(self._index, "trident_adamw", table.ctypes.data, len(params), ctypes.byref(self._state), ctypes.byref(h))
         self.step_count += 1
         torch.autograd.graph.increment_version(params)
+
+    # the states' buffers: to be read or changed in place (the library holds their addresses)
+    exp_avg = property(lambda self: self._buffers[0])
+    exp_avg_sq = property(lambda self: self._buffers[1])
+    exp_avg_scale = property(lambda self: self._buffers[2])
+    exp_avg_sq_scale = property(lambda self: self._buffers[3])
 
     def state_values(self) -> Tuple[torch.Tensor, torch.Tensor]:
         """The moments as flat float32 tensors: the buffers themselves, or what the 8-bit codes stand for."""
