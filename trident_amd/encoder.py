@@ -119,14 +119,19 @@ def _ids(index: int, ids: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 def _embed(ids, weight, scale):
-    if weight.dim() != 2 or weight.numel() == 0:
-        _refuse(f"weight must be [V, D], got {tuple(weight.shape)}")
-    code, index = _dtype("weight", weight), _gpu("weight", weight)
-    idc, wide = _ids(index, ids)
+    code, wide, index = _DTYPES.get(weight.dtype), _ID_TYPES.get(ids.dtype), weight.get_device()
+    if code is None or wide is None or index < 0 or ids.get_device() != index or weight.dim() != 2 or \
+            weight.numel() == 0:
+        if weight.dim() != 2 or weight.numel() == 0:
+            _refuse(f"weight must be [V, D], got {tuple(weight.shape)}")
+        _dtype("weight", weight)
+        _ids(_gpu("weight", weight), ids)
     V, D = weight.shape
-    w, ld = _rows(weight)
+    w, ld = (weight, D) if weight.is_contiguous() else _rows(weight)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
     out = weight.new_empty((*ids.shape, D))
-    _call(index, "trident_embedding", w.data_ptr(), code, V, D, ld, idc.data_ptr(), wide, idc.numel(), scale,
+    _call(index, "trident_embedding", w.data_ptr(), code, V, D, ld, ids.data_ptr(), wide, ids.numel(), scale,
           out.data_ptr(), D)
     return out
 
@@ -208,19 +213,23 @@ def _affine(index, x, D, weight, bias) -> int:
 
 
 def _norm(x, weight, bias, eps, keep):
-    code, index = _dtype("x", x), _gpu("x", x)
-    D = x.shape[-1] if x.dim() else 0
-    if D == 0:
-        _refuse(f"x must be [..., D], got {tuple(x.shape)}")
-    wcode = _affine(index, x, D, weight, bias)
-    xr, ld = _rows(x)
+    code, index = _DTYPES.get(x.dtype), x.get_device()
+    shape = x.shape
+    D = shape[-1] if shape else 0
+    if code is None or index < 0 or D == 0:
+        _dtype("x", x)
+        _gpu("x", x)
+        _refuse(f"x must be [..., D], got {tuple(shape)}")
+    wcode = code if weight is None and bias is None else _affine(index, x, D, weight, bias)
+    xr, ld = (x, D) if x.is_contiguous() else _rows(x)
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    mean = rstd = None
+    mean = rstd = pmean = prstd = None
     if keep:
-        mean, rstd = x.new_empty((2, *x.shape[:-1]), dtype=torch.float32)
+        mean, rstd = x.new_empty((2, *shape[:-1]), dtype=torch.float32)
+        pmean, prstd = mean.data_ptr(), rstd.data_ptr()
     _call(index, "trident_layer_norm", xr.data_ptr(), code, x.numel() // D, D, ld,
           None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), wcode, eps,
-          y.data_ptr(), D, mean.data_ptr() if keep else None, rstd.data_ptr() if keep else None)
+          y.data_ptr(), D, pmean, prstd)
     return y, mean, rstd
 
 
@@ -505,7 +514,10 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
                fast_accum: bool = False) -> torch.Tensor:
     """``x @ weight.T + bias`` for ``x`` [..., K], quantised in the call, in x's type: the projection of a
     query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``."""
-    code, index = _dtype("x", x), _gpu("x", x)
+    code, index = _DTYPES.get(x.dtype), x.get_device()
+    if code is None or index < 0:
+        _dtype("x", x)
+        _gpu("x", x)
     N = _check_blocks("weight", weight, index)
     codes, scales, K = weight
     shape = x.shape
