@@ -759,7 +759,7 @@ def test_adamw_refuses_parameters_that_changed(dev):
     opt, grad = encoder.AdamW([p]), torch.ones((4, 8), device=dev)
     opt.step([grad])
     kept = p.data
-    for other, text in ((kept.cpu(), "on cuda"), (torch.zeros((8, 8), device=dev), "no longer"),
+    for other, text in ((kept.cpu(), "must be on cuda"), (torch.zeros((8, 8), device=dev), "no longer"),
                         (torch.zeros((8, 4), device=dev).t(), "no longer"),
                         (torch.zeros((4, 8), device=dev, dtype=torch.float64), "float64")):
         p.data = other
@@ -799,7 +799,7 @@ def test_refusals(dev):
         (lambda: encoder.AdamW([f]).step([f, f]), "gradients are needed"),
         (lambda: encoder.AdamW([f]).step([f[:2]]), "shapes"),
         (lambda: encoder.AdamW([f]).step([f.double()]), "got torch.float64"),
-        (lambda: encoder.AdamW([f]).step([f.cpu()]), "must be dense, on"),
+        (lambda: encoder.AdamW([f]).step([f.cpu()]), "must be on cuda"),
         (lambda: encoder.AdamW([f]).step([f.to_sparse()]), "must be dense"),
         (lambda: encoder.AdamW([f], state_bits=8).load_state(1, f, f), "exp_avg must be"),
         (lambda: encoder.AdamW([f]).load_state_dict(dict(state_bits=8)), "8 bits"),

@@ -351,7 +351,6 @@ class AdamW:
         for p in self.params:
             p.grad = None
 
-    @torch.no_grad()
     def step(self, grads: Optional[Sequence[Optional[torch.Tensor]]] = None, grad_scale: float = 1.0) -> None:
         grads = [p.grad for p in self.params] if grads is None else list(grads)
         if len(grads) != len(self.params):
@@ -365,21 +364,23 @@ class AdamW:
             table = table[at]
             devices = set(map(_get_device, grads))
         devices.update(map(_get_device, params))
-        if [g.shape for g in grads] != shapes or not devices <= {self._index} or \
-                not {g.layout for g in grads} <= {torch.strided}:
-            _refuse(f"gradients must be dense, on {self.device} and of their parameters' shapes "
-                    f"{[tuple(s) for s in shapes]}, got {[(tuple(g.shape), g.device, g.layout) for g in grads]}")
+        if [g.shape for g in grads] != shapes or not devices <= {self._index}:
+            _refuse(f"gradients must be on {self.device} and of their parameters' shapes "
+                    f"{[tuple(s) for s in shapes]}, got {[(tuple(g.shape), g.device) for g in grads]}")
         if [p.shape for p in params] != shapes or not all(map(_is_contiguous, params)):
             _refuse("a parameter is no longer the contiguous tensor it was")
-        if not all(map(_is_contiguous, grads)):
-            grads = [g.contiguous() for g in grads]
+        try:
+            if not all(map(_is_contiguous, grads)):
+                grads = [g.detach().contiguous() for g in grads]
+            table["grad"] = [*map(_data_ptr, grads)]
+        except RuntimeError as e:  # sparse
+            _refuse(f"gradients must be dense: {e}")
         try:
             table["dtype"] = [_DTYPES[p.dtype] for p in params]
             table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
         except KeyError as e:
             _refuse(f"parameters and gradients must be float32, float16 or bfloat16, got {e}")
         table["param"] = [*map(_data_ptr, params)]
-        table["grad"] = [*map(_data_ptr, grads)]
         h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
                                    self.step_count + 1)
         _call(self._index, "trident_adamw", table.ctypes.data, len(params), ctypes.byref(self._state), ctypes.byref(h))
