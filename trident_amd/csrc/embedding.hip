@@ -303,9 +303,15 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
     int found = 0;
     const int lower = Source::read(a, [&](int t, int rel) {
         const uint64_t m = __ballot(rel >= 0);
+        if (!m) return;
+        // the first token's id is counted at once: a frequent one would else be most lanes' atomic, one
+        // after the other on one word, and all waves share the LDS unit (16.4 us where this takes 11)
+        const int first = __ffsll((unsigned long long)m) - 1, id = __builtin_amdgcn_readlane(rel, first);
+        const uint64_t same = __ballot(rel == id);
+        if (lane == first) atomicAdd(&mine[id], __popcll((unsigned long long)same));
         if (rel >= 0) {
             const int at = found + mask_rank(m);
-            atomicAdd(&mine[rel], 1);
+            if (rel != id) atomicAdd(&mine[rel], 1);
             if (at < kList) {
                 kept[at] = t;
                 kept_id[at] = (uint16_t)rel;
@@ -477,14 +483,13 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
     flush(row);
 }
 
-// Adds the parts of the long rows, those of one sorting workgroup's ids here: 64 columns a workgroup,
+// Adds the parts of the long rows, those of one sorting workgroup's ids here: 64 VEC columns a workgroup,
 // each of its waves a quarter of a row's parts, then the waves' sums in order.
-template <typename T>
+template <typename T, int VEC>
 __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
-    __shared__ float s_sum[kWavesPerBlock][kWave];
-    const int lane = lane_id(), wave = threadIdx.x / kWave, d = blockIdx.y * kWave + lane;
-    const int count = a.long_count[blockIdx.x];
-    const float* part = a.part + min(d, a.D - 1);
+    __shared__ float s_sum[kWavesPerBlock][VEC][kWave];
+    const int lane = lane_id(), wave = threadIdx.x / kWave, d = (blockIdx.y * kWave + lane) * VEC;
+    const int count = a.long_count[blockIdx.x], col = min(d, a.D - VEC);
     for (int i0 = 0; i0 < count; i0 += kWave) {
         // 64 rows' places at once, a row a lane
         const int v_of = a.long_rows[(int64_t)blockIdx.x * a.owned + min(i0 + lane, count - 1)];
@@ -494,16 +499,27 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
             const int first = beg / a.chunk;
             const int parts = (beg + __builtin_amdgcn_readlane(info.count, i) - 1) / a.chunk - first + 1;
             const int per = (parts + kWavesPerBlock - 1) / kWavesPerBlock;
-            float s = 0.0f;
-#pragma unroll 16
-            for (int c = wave * per; c < min(parts, (wave + 1) * per); ++c)  // in its first chunk a row is the last
-                s += part[(int64_t)(2 * (first + c) + (c == 0 && beg % a.chunk)) * a.D];  // one, unless it begins it
+            float s[VEC] = {};
+#pragma unroll 8
+            for (int c = wave * per; c < min(parts, (wave + 1) * per); ++c) {
+                // in its first chunk a row is the last one, unless it begins it
+                const int64_t at = 2 * (first + c) + (c == 0 && beg % a.chunk);
+                float x[VEC];
+                load_vec(a.part + at * a.D + col, x);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) s[e] += x[e];
+            }
             __syncthreads();
-            s_sum[wave][lane] = s;
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) s_sum[wave][e][lane] = s[e];
             __syncthreads();
             if (wave == 0 && d < a.D) {
-                for (int k = 1; k < kWavesPerBlock; ++k) s += s_sum[k][lane];
-                static_cast<T*>(a.out)[(int64_t)v * a.ldo + d] = (T)(s * a.scale);
+                T* out = static_cast<T*>(a.out) + (int64_t)v * a.ldo + col;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) {
+                    for (int k = 1; k < kWavesPerBlock; ++k) s[e] += s_sum[k][e][lane];
+                    out[e] = (T)(s[e] * a.scale);
+                }
             }
         }
     }
@@ -895,7 +911,9 @@ int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, con
             else embed_grad_kernel<T, kVec<T>, 4, P><<<grid, kBlock, 0, st>>>(a);
         });
         if ((rc = capi_check_launch("embed_grad_kernel")) || n <= s.chunk) return;
-        join_long_kernel<T><<<dim3(1u << s.shift, (unsigned)((D + kWave - 1) / kWave)), kBlock, 0, st>>>(a);
+        const auto tiles = [&](int v) { return dim3(1u << s.shift, (unsigned)((D + kWave * v - 1) / (kWave * v))); };
+        if (D >= 4) join_long_kernel<T, 4><<<tiles(4), kBlock, 0, st>>>(a);
+        else join_long_kernel<T, 1><<<tiles(1), kBlock, 0, st>>>(a);
         rc = capi_check_launch("join_long_kernel");
     });
     return rc;
