@@ -361,8 +361,8 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
                        const uint8_t* b_scales, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
                        int32_t dtype, int64_t ld_out, int32_t fast_accum, void* stream);
 
-/* The same with A quantised in the call from x [M, K]; out has x's type.  Few rows need no workspace
- * (0 bytes). */
+/* The same with A quantised in the call from x [M, K]; out has x's type.  A few short rows need no
+ * workspace (0 bytes: one launch does all). */
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K);
 int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* w_codes,
                        const uint8_t* w_scales, int64_t N, const void* bias, int32_t bias_dtype, void* out,

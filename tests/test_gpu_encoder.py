@@ -658,6 +658,18 @@ def test_fp8_matmul_and_linear(dev, dtype, M, N, K):
         check_product(encoder.fp8_linear(x, w, bs, fast_accum=True), a, w, bs, "linear", True)
 
 
+# several blocks of columns a workgroup, rows quantised beforehand for few rows, and each size of tile
+WIDE = [(1, 8195, 200), (5, 16390, 136), (16, 8192, 640), (16, 16400, 130), (9, 8200, 4200), (3, 16500, 8200),
+        (20, 4096, 6200), (20, 4100, 300), (32, 1000, 4100), (1, 300, 8300), (16, 40, 6144), (1300, 1300, 130),
+        (2000, 1700, 130), (3900, 3300, 130)]
+
+
+@pytest.mark.parametrize("dtype", TYPES[:2])
+@pytest.mark.parametrize("M,N,K", WIDE)
+def test_fp8_products_of_wide_and_long_weights(dev, dtype, M, N, K):
+    test_fp8_matmul_and_linear(dev, dtype, M, N, K)
+
+
 def test_fp8_linear_shapes_strides_and_empty(dev):
     g = gen(11)
     w, bias = encoder.quantize_fp8(randn(g, 70, 100)), randn(g, 70)

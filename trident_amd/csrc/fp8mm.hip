@@ -427,7 +427,7 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
 
 constexpr int kFewWaves = 8;
 constexpr int kFewRows = 16;    // rows that one instruction takes
-constexpr int kFewBlocks = 24;  // blocks of 16 rows by 128 columns that a CU quantises, past 16 rows
+constexpr int kFewCost = 512;   // of quantising the rows in every workgroup: what a second launch costs
 
 struct FewArgs {
     const void* x;           // [M, ldx], or null: the codes of a
@@ -435,37 +435,51 @@ struct FewArgs {
     const uint8_t *b, *sb;
     const void* bias;
     void* out;
-    int64_t ldx, pitch_b, ldo;
+    int64_t ldx, pitch_a, pitch_b, ldo;
     int M, N, K, kb, spitch, bias_f32;
 };
 
 // Up to 64 rows, bound by the weight's bytes or, for one query, by the latency of a launch.  A workgroup
-// takes 16 columns; its eight waves take the blocks of 128 of K in turn, the weight straight from memory
-// to registers, and their sums are added in order at the end.  The rows are quantised on the way (QUANT):
-// a lane holds the 32 columns of its row that the instruction wants from it, and a block's largest value
-// is that of four lanes, so one launch does all and nothing is stored between.
-template <typename T, bool FAST, bool QUANT, int MT>
+// takes 16 NT columns; its eight waves take the blocks of 128 of K in turn, the weight straight from memory
+// to registers, and their sums are added in order at the end.  The rows may be quantised on the way
+// (QUANT): a lane holds the 32 columns of its row that the instruction wants from it, and a block's largest
+// value is that of four lanes, so one launch does all and nothing is stored between.
+//
+// Each workgroup begins at another block: the rows of a weight are a power of two apart in most models, so
+// all workgroups would else read the same few channels of memory at a time (one row by 8192 x 8192: 19.8
+// us, 14.9 so: 4.5 TB/s).  One row of 960 columns by 1024 x 960: 4.9 us.
+template <typename T, bool FAST, bool QUANT, int MT, int NT>
 __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g) {
-    constexpr int U = MT > 1 ? 1 : sizeof(T) == 4 ? 2 : 4;  // blocks of a wave in flight
-    __shared__ f32x4 s_acc[kFewWaves][MT][kWave];
+    constexpr int U = MT > 1 || NT > 2 ? 1 : NT > 1 || sizeof(T) == 4 ? 2 : 4;  // blocks of a wave in flight
+    __shared__ f32x4 s_acc[kFewWaves][MT * NT][kWave];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * 16;
-    const int64_t n = min(n0 + r, g.N - 1);
-    const uint8_t* b = g.b + n * g.pitch_b + q * 32;
-    const uint8_t* sb = g.sb + n * g.spitch;
-    float bias[4];
-    load_bias<T, 4>(g.bias, g.bias_f32, n0 + q * 4, g.N, bias);
-    f32x4 acc[MT] = {};
+    const int r = lane & 15, q = lane >> 4, n0 = blockIdx.x * (16 * NT);
+    const uint8_t *b[NT], *sb[NT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int64_t n = min(n0 + j * 16 + r, g.N - 1);
+        b[j] = g.b + n * g.pitch_b + q * 32;
+        sb[j] = g.sb + n * g.spitch;
+    }
+    float bias[4];  // of the columns that this lane writes: wave w joins 16 rows and 16 columns
+    const int m = wave % MT * 16 + r, c0 = n0 + wave / MT * 16 + q * 4;
+    load_bias<T, 4>(g.bias, g.bias_f32, c0, g.N, bias);
+    const int turn = (int)(blockIdx.x % (unsigned)g.kb);
+    f32x4 acc[MT][NT] = {};
     for (int k0 = wave; k0 < g.kb; k0 += kFewWaves * U) {
-        u32x4 wb[U][2], wa[U][MT][2];
+        u32x4 wb[U][NT][2], wa[U][MT][2];
         Vec<T, 8> x[U][MT][4];
-        int eb[U], ea[U][MT];
+        int eb[U][NT], ea[U][MT];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int kb = k0 + u * kFewWaves;
+            int kb = k0 + u * kFewWaves;
             if (kb >= g.kb) break;
-            __builtin_memcpy(wb[u], b + (int64_t)kb * kBlockK, 32);
-            eb[u] = sb[kb];
+            if ((kb += turn) >= g.kb) kb -= g.kb;
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                __builtin_memcpy(wb[u][j], b[j] + (int64_t)kb * kBlockK, 32);
+                eb[u][j] = sb[j][kb];
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 const int64_t m = min(i * kFewRows + r, g.M - 1);
@@ -486,8 +500,7 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
                         }
                     }
                 } else {
-                    __builtin_memcpy(wa[u][i], g.a + m * ((int64_t)g.kb * kBlockK) + (int64_t)kb * kBlockK + q * 32,
-                                     32);
+                    __builtin_memcpy(wa[u][i], g.a + m * g.pitch_a + (int64_t)kb * kBlockK + q * 32, 32);
                     ea[u][i] = g.sa[m * g.spitch + kb];
                 }
             }
@@ -495,11 +508,14 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             if (k0 + u * kFewWaves >= g.kb) break;
-            i32x8 fb;
+            i32x8 fb[NT];
+            bf16x8 hb[NT][4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) fb[e] = (int)wb[u][e / 4][e % 4];
-            bf16x8 hb[4];
-            if constexpr (!FAST) to_bf16(fb, scale_value((uint32_t)eb[u]), hb);
+            for (int j = 0; j < NT; ++j) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) fb[j][e] = (int)wb[u][j][e / 4][e % 4];
+                if constexpr (!FAST) to_bf16(fb[j], scale_value((uint32_t)eb[u][j]), hb[j]);
+            }
 #pragma unroll
             for (int i = 0; i < MT; ++i) {
                 i32x8 fa;
@@ -524,42 +540,57 @@ __global__ __launch_bounds__(kFewWaves* kWave) void matmul_few_kernel(FewArgs g)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) fa[e] = (int)wa[u][i][e / 4][e % 4];
                 }
-                if constexpr (FAST) {
-                    acc[i] =
-                        __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc[i], 0, 0, 0, eb[u], 0, ea[u][i]);
-                } else {
-                    bf16x8 ha[4];
-                    to_bf16(fa, scale_value((uint32_t)ea[u][i]), ha);
+                bf16x8 ha[4];
+                if constexpr (!FAST) to_bf16(fa, scale_value((uint32_t)ea[u][i]), ha);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[k], ha[k], acc[i], 0, 0, 0);
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (FAST) {
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[j], fa, acc[i][j], 0, 0, 0,
+                                                                                     eb[u][j], 0, ea[u][i]);
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(hb[j][k], ha[k], acc[i][j], 0, 0, 0);
+                    }
                 }
             }
         }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) s_acc[wave][i][lane] = acc[i];
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) s_acc[wave][j * MT + i][lane] = acc[i][j];
     __syncthreads();
-    const int m = wave * kFewRows + r;  // a wave for 16 rows
-    if (wave >= MT || m >= g.M) return;
+    if (wave >= MT * NT || m >= g.M) return;
     f32x4 sum = s_acc[0][wave][lane];
     for (int w = 1; w < kFewWaves; ++w) sum += s_acc[w][wave][lane];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-        const int c = n0 + q * 4 + e;
-        if (c >= g.N) break;
-        static_cast<T*>(g.out)[(int64_t)m * g.ldo + c] = (T)(sum[e] + bias[e]);
+        if (c0 + e >= g.N) break;
+        static_cast<T*>(g.out)[(int64_t)m * g.ldo + c0 + e] = (T)(sum[e] + bias[e]);
     }
 }
 
-// Whether the kernel for few rows takes a projection: 16 rows always; up to 64 where what a CU's
-// workgroups quantise again (all of them quantise all rows) costs less than a launch.  Measured with
-// float32 rows, against 11 to 13 us for two launches: 24 blocks 8.9 us, 32 11.6 (N = 1024); 16 blocks of
-// N = 8192, two workgroups a CU, 15.4.
-inline bool few_rows(int64_t M, int64_t N, int64_t K) {
-    return M <= kFewRows || (M <= 4 * kFewRows && (M + kFewRows - 1) / kFewRows * blocks_of(K) *
-                                                          ((N + 4095) / 4096) <= kFewBlocks);
+// Blocks of 16 columns that a workgroup takes: more than one, which reads the rows less often, where that
+// still leaves every CU a workgroup (16 float32 rows by 16384 x 2048: one block 22.6 us, four 11.8).
+inline int few_columns(int64_t M, int64_t N) { return M > kFewRows || N < 8192 ? 1 : N < 16384 ? 2 : 4; }
+
+// Whether a projection is one launch, in which every workgroup quantises all rows: where that costs a CU
+// less than a second launch.  It grows with the blocks, and for each with the bytes of the rows beside a
+// fixed part.  Measured, one launch against two: float32, 1 row, K = 4096 9.3 and 12.6 us, K = 8192 13.5
+// and 11.5; 8 rows, K = 4096 10.6 and 11.6; 16 rows, K = 2048 9.0 and 12.2, K = 4096 14.4 and 11.3; 64
+// rows, K = 768 10.2 and 11.5, K = 2048 21 and 12.  bfloat16, 16 rows, K = 4096 10.9 and 11.2, K = 8192
+// 17.1 and 16.0; 32 rows, K = 2048 8.5 and 11.9 (N = 4096, 64 rows 1024).
+inline bool one_launch(int64_t M, int64_t N, int64_t K, int64_t bytes) {
+    if (M > 4 * kFewRows) return false;
+    const int64_t groups = (N + 16 * few_columns(M, N) - 1) / (16 * few_columns(M, N));
+    return blocks_of(K) * (8 + M * bytes / 4) * ((groups + 255) / 256) <= kFewCost;
 }
+
+// Whether the kernel for few rows takes codes.  Against the tiles, which wait for the length of K where
+// there are few of them: 16 rows by 4096 x 4096 8.7 and 15.6 us, 32 rows 10.6 and 15.7, but 64 rows 16.6
+// and 15.9, 32 rows by 16384 x 2048 16.3 and 9.8.
+inline bool few_codes(int64_t M, int64_t N) { return M <= kFewRows || (M <= 2 * kFewRows && N <= 4096); }
 
 // Launches the kernel of one tile size.
 template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
@@ -582,15 +613,23 @@ int launch_matmul(MatmulArgs g, hipStream_t st) {
     return capi_check_launch("matmul_kernel");
 }
 
-// The largest tile that still gives every CU one: a larger tile reads its operands less often (256 x
-// 256: 64 bytes of LDS for 8,192 products), but 256 CUs want 256 tiles.
+// The tile.  A larger one reads its operands less often (256 x 256: 64 bytes of LDS for 8,192 products),
+// but takes a CU alone, so its tiles are worked off in rounds of 256: it wins where the rounds are three
+// quarters full (K = 4096, against 128 x 128: 4096 x 3328, 208 tiles, 67 and 76 us; 6144 x 4352, 408, 116
+// and 128; 4352 x 4352, 289, 114 and 93; two rounds 70% full of 5000 x 4608 x 1024 43 and 40).  The
+// smallest, whose two teams take K in half the steps, wins while a CU has two at most (1024 x 2048 x 4096,
+// 512 tiles, 20.7 us and 24.2 with 128 x 128; 2048 x 1152, 576, 29.5 and 24.7; 4096 x 768 x 768, 768, 10.5
+// and 9.4).  The exact products turn at the same sizes (25.7 and 35.9, 35.8 and 36.6, 12.2 and 11.5); their
+// 256 x 256 tile does not fit the registers.
 template <typename T, bool FAST>
 int matmul(const MatmulArgs& g, hipStream_t st) {
     const auto tiles = [&](int64_t bm, int64_t bn) { return (g.M + bm - 1) / bm * ((g.N + bn - 1) / bn); };
-    if constexpr (FAST)
-        if (tiles(256, 256) >= 256) return launch_matmul<T, FAST, 2, 4, 4, 2, 1>(g, st);
-    if (tiles(128, 128) >= 256) return launch_matmul<T, FAST, 2, 2, 2, 2, 1>(g, st);
-    return launch_matmul<T, FAST, 2, 2, 1, 1, 2>(g, st);
+    if constexpr (FAST) {
+        const int64_t large = tiles(256, 256);
+        if (large * 4 >= (large + 255) / 256 * 256 * 3) return launch_matmul<T, FAST, 2, 4, 4, 2, 1>(g, st);
+    }
+    if (tiles(64, 64) <= 512) return launch_matmul<T, FAST, 2, 2, 1, 1, 2>(g, st);
+    return launch_matmul<T, FAST, 2, 2, 2, 2, 1>(g, st);
 }
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
@@ -638,10 +677,44 @@ int check_product(int64_t M, int64_t N, int64_t K, const void* a, const void* b_
     return TRIDENT_OK;
 }
 
-// Codes and scales of A from `a`, or (few rows) A itself from x, of out's type.
+// Few rows: of codes and scales, or (QUANT) rows of out's type themselves.
+template <bool QUANT>
+int product_few(const void* x, int64_t ld_x, const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M,
+                const uint8_t* b, const uint8_t* sb, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
+                int32_t dtype, int64_t ld_out, int32_t fast_accum, hipStream_t st) {
+    const FewArgs g{x, a, sa, b, sb, bias, out, ld_x, pitch_a, pitch_of(K), ld_out, (int)M, (int)N, (int)K,
+                    (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32};
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        const auto go = [&](auto fast, auto mt, auto nt) {
+            constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
+            matmul_few_kernel<T, decltype(fast)::value, QUANT, MT, NT>
+                <<<(unsigned)((N + 16 * NT - 1) / (16 * NT)), kFewWaves * kWave, 0, st>>>(g);
+        };
+        using std::integral_constant;
+        const auto rows = [&](auto fast) {
+            const integral_constant<int, 1> one;
+            const integral_constant<int, 2> two;
+            const integral_constant<int, 4> four;
+            const int nt = few_columns(M, N);
+            if (nt == 4) go(fast, one, four);
+            else if (nt == 2) go(fast, one, two);
+            else if (M <= kFewRows) go(fast, one, one);
+            else if (!QUANT || M <= 2 * kFewRows) go(fast, two, one);
+            else if constexpr (QUANT) go(fast, four, one);
+        };
+        if (fast_accum) rows(std::true_type{});
+        else rows(std::false_type{});
+    });
+    return capi_check_launch("matmul_few_kernel");
+}
+
 int product(const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M, const uint8_t* b, const uint8_t* sb,
             int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out, int32_t dtype, int64_t ld_out,
             int32_t fast_accum, hipStream_t st) {
+    if (few_codes(M, N))
+        return product_few<false>(nullptr, 0, a, pitch_a, sa, M, b, sb, N, K, bias, bias_dtype, out, dtype, ld_out,
+                                  fast_accum, st);
     const MatmulArgs g{a, b, sa, sb, bias, out, pitch_a, pitch_of(K), ld_out, (int)M, (int)N,
                        (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
     int rc = TRIDENT_OK;
@@ -650,30 +723,6 @@ int product(const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M, con
         rc = fast_accum ? matmul<T, true>(g, st) : matmul<T, false>(g, st);
     });
     return rc;
-}
-
-template <bool QUANT>
-int product_few(const void* x, int64_t ld_x, const uint8_t* a, const uint8_t* sa, int64_t M, const uint8_t* b,
-                const uint8_t* sb, int64_t N, int64_t K, const void* bias, int32_t bias_dtype, void* out,
-                int32_t dtype, int64_t ld_out, int32_t fast_accum, hipStream_t st) {
-    const FewArgs g{x, a, sa, b, sb, bias, out, ld_x, pitch_of(K), ld_out, (int)M, (int)N, (int)K,
-                    (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32};
-    const unsigned grid = (unsigned)((N + 15) / 16);
-    with_dtype(dtype, [&](auto t) {
-        using T = decltype(t);
-        const auto go = [&](auto fast, auto mt) {
-            matmul_few_kernel<T, decltype(fast)::value, QUANT, decltype(mt)::value>
-                <<<grid, kFewWaves * kWave, 0, st>>>(g);
-        };
-        const auto rows = [&](auto fast) {
-            if (M <= kFewRows) go(fast, std::integral_constant<int, 1>{});
-            else if (M <= 2 * kFewRows) go(fast, std::integral_constant<int, 2>{});
-            else go(fast, std::integral_constant<int, 4>{});
-        };
-        if (fast_accum) rows(std::true_type{});
-        else rows(std::false_type{});
-    });
-    return capi_check_launch("matmul_few_kernel");
 }
 
 }  // namespace
@@ -697,15 +746,12 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
                          "fp8_matmul: NULL pointer, or codes not 16-byte, scales not 4-byte aligned");
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (M <= kFewRows)
-        return product_few<false>(nullptr, 0, a_codes, a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out,
-                                  dtype, ld_out, fast_accum, st);
     return product(a_codes, pitch_of(K), a_scales, M, b_codes, b_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
                    fast_accum, st);
 }
 
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (!counts_ok(M, K) || !counts_ok(N, K) || few_rows(M, N, K)) return 0;
+    if (!counts_ok(M, K) || !counts_ok(N, K) || one_launch(M, N, K, 4)) return 0;
     return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
 }
 
@@ -718,8 +764,8 @@ int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "fp8_linear: ld=%lld < K=%lld", (long long)ld_x, (long long)K);
     if (M == 0 || N == 0) return TRIDENT_OK;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (few_rows(M, N, K))
-        return product_few<true>(x, ld_x, nullptr, nullptr, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype,
+    if (one_launch(M, N, K, dtype == TRIDENT_F32 ? 4 : 2))
+        return product_few<true>(x, ld_x, nullptr, 0, nullptr, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype,
                                  ld_out, fast_accum, st);
     const size_t need = trident_fp8_linear_workspace_bytes(M, N, K);
     if (!workspace || workspace_bytes < need || !aligned16(workspace))
