@@ -156,6 +156,18 @@ def test_embedding_grad_one_id_of_a_large_table(dev):
     check_embedding_grad(randn(g, 40_000, 9), ids, 600_000)
 
 
+@pytest.mark.parametrize("V", [1 << 19, (1 << 19) + 1, (1 << 21) - 3, 1 << 21, (1 << 21) + 1, 2_300_000])
+def test_embedding_grad_of_large_tables(dev, V):
+    """Sizes at and around which the ordering's workgroups take more ids each, or read all tokens; one id
+    with more tokens than a wave keeps, few and many tokens."""
+    g = gen(V)
+    check_embedding_grad(randn(g, 8200, 8), token_ids(g, 8200, V), V)
+    check_embedding_grad(randn(g, 700, 3), token_ids(g, 700, V, False), V)
+    ids = torch.full((30_000,), V - 1, device=dev)
+    ids[::500] = torch.randint(0, V, (60,), generator=g, device=dev)
+    check_embedding_grad(randn(g, 30_000, 5), ids, V)
+
+
 def test_embedding_grad_without_tokens(dev):
     out = encoder.embedding_grad(torch.empty((0, 20), device=dev), torch.empty(0, dtype=torch.int64, device=dev), 300)
     assert out.shape == (300, 20) and (out == 0).all()

@@ -26,7 +26,8 @@ constexpr int kEmbedUnroll = 4;
 
 // Bound by bytes: the rows' vectors of all tokens, one after the other, are dealt to the lanes, so a
 // row of any length leaves no lane idle; four independent gathers per lane cover the latency of the
-// id and of the row behind it.
+// id and of the row behind it.  131,072 tokens x 768 bfloat16 of 30,522 rows: 45 us, 4.5 TB/s written
+// and as much read, mostly from the caches.
 template <typename T, int VEC, typename ID, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
     const int64_t base = (int64_t)blockIdx.x * (kBlock * kEmbedUnroll);
@@ -66,7 +67,8 @@ __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
 // ---------------------------------------------------------------------------------------------
 // gradient
 
-constexpr int kMaxOwned = 512;  // ids of one sorting workgroup at most
+constexpr int kOwned = 512;      // ids of one sorting workgroup, of a table of up to kMaxBuckets of them;
+constexpr int kMaxOwned = 2048;  // of a larger table
 
 struct RowInfo {
     int beg, count;  // a row's places among the ordered tokens
@@ -82,7 +84,10 @@ struct Token {
     int t, row;
 };
 
-constexpr int kSmallTokens = 4 * 2048;  // ordered in one launch: four waves can keep all of them
+// Tokens ordered in one launch, and not in two: four waves can keep all of them.  The whole gradient,
+// 768 columns, one and two: 4,096 tokens 22.0 and 26.4 us, 8,192 25.8 and 26.5, 12,288 33.3 and 32.3,
+// 16,384 38.5 and 34.7.
+constexpr int kSmallTokens = 4 * 2048;
 constexpr int kPartTokens = 1024;       // tokens that bucket_ids_kernel orders at a time
 constexpr int kMaxBuckets = 1024;
 
@@ -274,15 +279,16 @@ struct SortShape {
 };
 
 // Orders the tokens by id: row[info_at(v)] says where in `token` the tokens of id v lie, in their own
-// order; the last entry holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power of two): the
-// most frequent ids of a vocabulary are neighbours, so a range of them would be one workgroup's work.
-// Each wave goes through its share of the tokens, keeps those its workgroup owns in a list in LDS, and
+// order; the last entry holds the number of all.  Workgroup b owns the ids = b modulo gridDim.x (a power
+// of two): the most frequent ids of a vocabulary are neighbours, so a range of them would be one
+// workgroup's work.  Each wave goes through its share of the tokens, keeps those its workgroup owns in a list in LDS, and
 // counts them by id; the counts, and the number of tokens of lower workgroups, give every (id, wave)
 // its first place, and the lists are placed in order.  A wave whose list overflows (an id with a large
 // share of many tokens) goes through its share again instead.  No workgroup waits for another.
 //
 // Few tokens are read by every workgroup.  For many that is most of the time (131,072: 35 us), so they
-// are bucketed first, which leaves each workgroup its own (4 + 8 us).
+// are bucketed first, which leaves each workgroup its own (5.4 + 13.4 us, most of it in the workgroups of
+// the most frequent ids).
 template <typename ID, int WAVES, bool SKIP, bool FROM_PARTS>
 __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
     using Source = SortSource<ID, WAVES, SKIP, FROM_PARTS>;
@@ -305,7 +311,7 @@ __global__ __launch_bounds__(WAVES* kWave) void sort_ids_kernel(SortArgs a) {
         const uint64_t m = __ballot(rel >= 0);
         if (!m) return;
         // the first token's id is counted at once: a frequent one would else be most lanes' atomic, one
-        // after the other on one word, and all waves share the LDS unit (16.4 us where this takes 11)
+        // after the other on one word, and all waves share the LDS unit (16.4 us where this takes 13.4)
         const int first = __ffsll((unsigned long long)m) - 1, id = __builtin_amdgcn_readlane(rel, first);
         const uint64_t same = __ballot(rel == id);
         if (lane == first) atomicAdd(&mine[id], __popcll((unsigned long long)same));
@@ -386,7 +392,7 @@ constexpr int kClear = 16;  // rows of a wave that clears
 // the chunk that it begins in, which sums it to its end and writes it.  A longer row (a frequent token)
 // is summed chunk by chunk into `part`, of which a chunk needs two: for the row it begins in and the
 // row it ends in; join_long_kernel adds a row's parts in order.  So every group has between one and two
-// chunks of work, whatever the frequencies.
+// chunks of work, whatever the frequencies.  131,072 x 768 bfloat16 into 30,522 rows: 40 us, 6 TB/s.
 template <typename T, int VEC, int NVL, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
     constexpr int kAhead = NVL > 2 ? 4 : 8;
@@ -484,7 +490,8 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
 }
 
 // Adds the parts of the long rows, those of one sorting workgroup's ids here: 64 VEC columns a workgroup,
-// each of its waves a quarter of a row's parts, then the waves' sums in order.
+// each of its waves a quarter of a row's parts, then the waves' sums in order.  Bound by the longest row:
+// 9.4 us where one id has a fifteenth of 131,072 tokens; eight or sixteen waves take as long.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
     __shared__ float s_sum[kWavesPerBlock][VEC][kWave];
@@ -528,10 +535,11 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
 // Few tokens, in one launch: the time is that of launches, not of bytes.  Workgroup b owns the ids = b
 // modulo gridDim.x as in sort_ids_kernel, orders its tokens in LDS, and sums and writes its own rows, so
 // nothing passes between workgroups: groups of lanes clear the rows without tokens, take those with up to
-// kShared of them in turn, and sum the others together.
+// kShared of them in turn, and sum the others together.  16 tokens x 768 into 30,522 rows: 7.1 us, 6.6 TB/s
+// of zeros.
 constexpr int kFewThreads = 512;
 constexpr int kFewTokens = 8192;           // 16 a thread, held in registers
-constexpr int kFewElements = 512 * 1024;   // tokens * columns: past it one workgroup may have too much to sum
+constexpr int kFewElements = 1024 * 1024;  // tokens * columns: past it one workgroup may have too much to sum
 constexpr int kShared = 8;
 
 struct FewArgs {
@@ -722,12 +730,14 @@ size_t up256(size_t x) { return (x + 255) & ~(size_t)255; }
 
 GradSpace grad_space(void* base, int64_t n, int64_t V, int64_t D) {
     GradSpace s;
-    // Chunks as long as leave about 2,000 waves (8 on each CU): the parts of long rows cost a write and
-    // a read of four bytes a column each.
-    s.chunk = n * D <= (16 << 20) ? 8 : n * D <= (32 << 20) ? 16 : 32;
+    // Short chunks leave waves for every CU, long ones fewer parts, each a write and a read of four bytes
+    // a column.  Chunks of 8, 16 and 32 tokens, ids by a 1 / rank law, us: 16,384 x 768 34.3, 38.2, 37.3;
+    // 16,384 x 2,048 61.9, 53.8, 62.2; 32,768 x 768 45.9, 41.4, 43.6; 49,152 x 768 58.1, 48.9, 49.8;
+    // 65,536 x 768 69, 58, 52; 131,072 x 64 59.3, 46.8, 47.9; 131,072 x 768 114, 92, 79.
+    s.chunk = n > 49152 ? 32 : n > 24576 || n * D > (16 << 20) ? 16 : 8;
     s.chunks = (n + s.chunk - 1) / s.chunk;
     s.shift = 8;  // one sorting workgroup per CU, more where they would own too many ids
-    while (((int64_t)kMaxOwned << s.shift) < V) ++s.shift;
+    while (((int64_t)((1 << s.shift) < kMaxBuckets ? kOwned : kMaxOwned) << s.shift) < V) ++s.shift;
     s.parts = n > kSmallTokens && (1 << s.shift) <= kMaxBuckets ? (int)((n + kPartTokens - 1) / kPartTokens) : 0;
     s.owned = (int)((V + ((int64_t)1 << s.shift) - 1) >> s.shift);
     char* p = static_cast<char*>(base);
@@ -765,16 +775,21 @@ int sort_ids(const SortArgs& a, hipStream_t st) {
 template <typename ID, bool SKIP>
 int order_tokens(const SortArgs& a, hipStream_t st) {
     if (a.n <= kSmallTokens) return sort_ids<ID, 4, SKIP, false>(a, st);
-    if (a.parts == 0) return sort_ids<ID, 16, SKIP, false>(a, st);  // a table of more than 2^19 rows
+    if (a.parts == 0) return sort_ids<ID, 8, SKIP, false>(a, st);  // a table of more than 2^21 rows
     bucket_ids_kernel<ID, SKIP><<<(unsigned)a.parts, kBlock, 0, st>>>(a);
     const int rc = capi_check_launch("bucket_ids_kernel");
-    return rc ? rc : sort_ids<ID, 16, SKIP, true>(a, st);
+    if (rc) return rc;
+    // the waves' counters of more ids leave room for fewer waves
+    return a.owned <= kOwned ? sort_ids<ID, 16, SKIP, true>(a, st) : sort_ids<ID, 8, SKIP, true>(a, st);
 }
 
-// Which calls take one launch (of about 5 us) instead of three: at most kFewTokens and kFewElements, rows
-// within one group's registers, and ids within the 256 workgroups' counters.
+// Which calls take one launch instead of three: at most kFewTokens and kFewElements, rows within one
+// group's registers, and ids within the 256 workgroups' counters.  One and three, ids uniform and by a
+// 1 / rank law: 64 x 768 11.8 and 15.8 us; 1,024 x 768 12.6 and 16.9, 18.6 and 19.0; 8,192 x 128 10.7 and
+// 17.8, 19.9 and 23.5; 4,096 x 768 15.1 and 19.5, 26.3 and 22.0.  With one id for all tokens, the worst
+// that one workgroup can be given, 1,024 x 768 takes 45 and 22.
 bool few_ok(int64_t n, int64_t V, int64_t D) {
-    return n > 0 && n <= kFewTokens && n * D <= kFewElements && D <= 1024 && V <= (int64_t)kMaxOwned << 8;
+    return n > 0 && n <= kFewTokens && n * D <= kFewElements && D <= 1024 && V <= (int64_t)kOwned << 8;
 }
 
 template <typename T, typename ID>
