@@ -309,6 +309,32 @@ def test_layer_norm_grad(dev, dtype, rows, D):
         within(db, d.sum(0), (rows + 4) * u * d.abs().sum(0) + U[dtype] * d.sum(0).abs() + TINY[dtype], "db")
 
 
+# rows of which a wave takes several: each number of lanes, full, one over and one under
+NARROW = [(1000, 1), (777, 3), (3001, 4), (500, 7), (4100, 9), (63, 16), (64, 17), (65, 31), (9000, 32), (300, 33),
+          (129, 63), (2500, 65), (17, 127), (20_000, 128), (1, 129), (33, 200), (515, 255), (1030, 256), (66, 257)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,D", NARROW)
+def test_layer_norm_narrow_rows(dev, dtype, rows, D):
+    test_layer_norm(dev, dtype, rows, D)
+    test_layer_norm_grad(dev, dtype, rows, D)
+
+
+def test_layer_norm_narrow_rows_keep_nan_to_themselves(dev):
+    for D in (5, 24, 100, 200):
+        x = randn(gen(D), 1000, D)
+        x[3, D // 2], x[700, 0] = float("nan"), float("inf")
+        y, mean, rstd = encoder.layer_norm_forward(x)
+        bad = torch.tensor([3, 700], device=dev)
+        assert y[bad].isnan().any(1).all()
+        dx, _, _ = encoder.layer_norm_grad(torch.ones_like(x), x, None, mean, rstd)
+        assert dx[bad].isnan().any(1).all()
+        keep = torch.ones(1000, dtype=torch.bool, device=dev)
+        keep[bad] = False
+        assert y[keep].isfinite().all() and dx[keep].isfinite().all()
+
+
 def test_layer_norm_strides_and_shapes(dev):
     g = gen(3)
     big = randn(g, 12, 150, dtype=torch.float16)

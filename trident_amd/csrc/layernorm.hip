@@ -29,17 +29,17 @@ struct NormArgs {
     float eps, inv_D;
 };
 
-// The vectors of a row that this lane holds: W waves share a row, lane l of them holds the vectors
-// l + 64 W c.  The last vector of a row ends with the row; its first `dup` elements are also the
+// The vectors of a row that this lane holds: G lanes share a row (a part of a wave, or whole waves), and
+// lane l of them holds the vectors l + G c.  The last vector of a row ends with the row; its first `dup` elements are also the
 // vector before's and count there.
-template <int VEC, int NV, int W>
+template <int VEC, int NV, int G>
 struct Columns {
     int col[NV], dup[NV];
     bool on[NV];
     __device__ __forceinline__ void init(const NormArgs& a, int l) {
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
-            const int v = l + kWave * W * c;
+            const int v = l + G * c;
             on[c] = v < a.nv;
             col[c] = min(v * VEC, a.D - VEC);
             dup[c] = v * VEC - col[c];
@@ -50,15 +50,15 @@ struct Columns {
 template <typename T, int VEC, int NV>
 struct Row {
     Vec<T, VEC> v[NV];
-    template <int W>
-    __device__ __forceinline__ void load(const T* __restrict__ p, const Columns<VEC, NV, W>& k) {
+    template <int G>
+    __device__ __forceinline__ void load(const T* __restrict__ p, const Columns<VEC, NV, G>& k) {
 #pragma unroll
         for (int c = 0; c < NV; ++c)
             if (k.on[c]) v[c].load(p + k.col[c]);
     }
     // the values, zeros in a lane's vectors past the row
-    template <int W>
-    __device__ __forceinline__ void get(const Columns<VEC, NV, W>& k, float (&f)[NV][VEC]) const {
+    template <int G>
+    __device__ __forceinline__ void get(const Columns<VEC, NV, G>& k, float (&f)[NV][VEC]) const {
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             if (k.on[c]) v[c].get(f[c]);
@@ -69,33 +69,49 @@ struct Row {
     }
 };
 
-// Sum over the W waves that share a row; with W > 1 every thread of the workgroup calls it.
-template <int W>
+// Sum over the G lanes that share a row, the same in each; with more than a wave (G > 64) every thread of
+// the workgroup calls it.
+template <int G>
 __device__ __forceinline__ float row_sum(float v, float* s_red) {
+    if constexpr (G < kWave) {
+        v = add_from<0xb1>(v);                        // the neighbour's
+        v = add_from<0x4e>(v);                        // the other two's of four
+        if constexpr (G >= 8) v = add_from<0x141>(v);  // eight lanes mirrored: the other four's
+        if constexpr (G >= 16) v = add_from<0x140>(v);
+        if constexpr (G >= 32) v += __shfl_xor(v, 16, kWave);
+        return v;
+    }
     v = wave_sum(v);
-    if constexpr (W > 1) {
+    if constexpr (G > kWave) {
         __syncthreads();
         if (lane_id() == 0) s_red[threadIdx.x / kWave] = v;
         __syncthreads();
         v = s_red[0];
 #pragma unroll
-        for (int i = 1; i < W; ++i) v += s_red[i];
+        for (int i = 1; i < G / kWave; ++i) v += s_red[i];
     }
     return v;
 }
 
-// Bound by bytes.  A wave (a workgroup of W = 4 waves for rows of more than 256 vectors) takes every
-// gridDim-th row and loads the next one while it works on this one.
-template <typename T, typename TW, int VEC, int NV, int W, bool PAST_L2>
+// The row that this lane's group takes first, and the lane's number in it.
+template <int G>
+__device__ __forceinline__ int64_t first_row(int* lane) {
+    *lane = threadIdx.x % G;
+    if constexpr (G < kWave) return (int64_t)blockIdx.x * (kBlock / G) + threadIdx.x / G;
+    return (int64_t)blockIdx.x * (kBlock / G) + __builtin_amdgcn_readfirstlane(threadIdx.x / G);
+}
+
+// Bound by bytes.  G lanes (a wave; a part of one for rows of up to 32 vectors; a workgroup of four for
+// more than 256) take every so many rows and load the next one while they work on this one.
+template <typename T, typename TW, int VEC, int NV, int G, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
-    __shared__ float s_red[W];
-    constexpr int kRows = kWavesPerBlock / W;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t step = (int64_t)gridDim.x * kRows;
-    int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0);
+    __shared__ float s_red[kWavesPerBlock];
+    const int64_t step = (int64_t)gridDim.x * (kBlock / G);
+    int lane;
+    int64_t row = first_row<G>(&lane);
     if (row >= a.rows) return;
-    Columns<VEC, NV, W> k;
-    k.init(a, W == 1 ? lane_id() : threadIdx.x);
+    Columns<VEC, NV, G> k;
+    k.init(a, lane);
     const T* X = static_cast<const T*>(a.x);
     Row<T, VEC, NV> now, next;
     Row<TW, VEC, NV> weight, bias;
@@ -113,7 +129,7 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
                 if (i >= k.dup[c]) s += x[c][i];
-        const float mean = row_sum<W>(s, s_red) * a.inv_D;
+        const float mean = row_sum<G>(s, s_red) * a.inv_D;
         s = 0.0f;
 #pragma unroll
         for (int c = 0; c < NV; ++c)
@@ -122,7 +138,7 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
                 x[c][i] -= mean;
                 if (k.on[c] && i >= k.dup[c]) s += x[c][i] * x[c][i];
             }
-        const float rstd = 1.0f / sqrtf(row_sum<W>(s, s_red) * a.inv_D + a.eps);
+        const float rstd = 1.0f / sqrtf(row_sum<G>(s, s_red) * a.inv_D + a.eps);
         T* y = static_cast<T*>(a.y) + row * a.ldy;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
@@ -139,7 +155,7 @@ __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
             }
             put_vec<PAST_L2>(y + k.col[c], x[c]);
         }
-        if (a.mean && (W == 1 ? lane_id() : (int)threadIdx.x) == 0) {
+        if (a.mean && lane == 0) {
             a.mean[row] = mean;
             a.rstd[row] = rstd;
         }
@@ -158,10 +174,10 @@ __global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
     T* y = static_cast<T*>(a.y) + row * a.ldy;
     float s = 0.0f;
     for (int d = threadIdx.x; d < a.D; d += kBlock) s += (float)x[d];
-    const float mean = row_sum<kWavesPerBlock>(s, s_red) * a.inv_D;
+    const float mean = row_sum<kBlock>(s, s_red) * a.inv_D;
     s = 0.0f;
     for (int d = threadIdx.x; d < a.D; d += kBlock) s += ((float)x[d] - mean) * ((float)x[d] - mean);
-    const float rstd = 1.0f / sqrtf(row_sum<kWavesPerBlock>(s, s_red) * a.inv_D + a.eps);
+    const float rstd = 1.0f / sqrtf(row_sum<kBlock>(s, s_red) * a.inv_D + a.eps);
     for (int d = threadIdx.x; d < a.D; d += kBlock) {
         float v = ((float)x[d] - mean) * rstd;
         if (a.weight) v *= (float)static_cast<const TW*>(a.weight)[d];
@@ -174,24 +190,23 @@ __global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
     }
 }
 
-// Bound by bytes.  A wave (or a workgroup, W = 4) takes every gridDim-th row, the next one's loads ahead
-// of this one's work: dx from the row's two means, and dy h and dy added to the columns' sums, which stay
+// Bound by bytes.  G lanes as above take every so many rows, the next one's loads ahead of this one's work: dx from the row's two means, and dy h and dy added to the columns' sums, which stay
 // in registers until the last row.
-template <typename T, typename TW, int VEC, int NV, int W, bool PAST_L2>
+template <typename T, typename TW, int VEC, int NV, int G, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
-    extern __shared__ float s_part[];  // [kWavesPerBlock][D], W = 1 only
-    __shared__ float s_red[W];
-    constexpr int kRows = kWavesPerBlock / W;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    Columns<VEC, NV, W> k;
-    k.init(a, W == 1 ? lane_id() : threadIdx.x);
+    extern __shared__ float s_part[];  // [kGroups][D], more groups than one only
+    __shared__ float s_red[kWavesPerBlock];
+    constexpr int kGroups = kBlock / G;
+    const int64_t step = (int64_t)gridDim.x * kGroups;
+    int lane;
+    int64_t row = first_row<G>(&lane);
+    Columns<VEC, NV, G> k;
+    k.init(a, lane);
     float dw[NV][VEC] = {}, db[NV][VEC] = {};
     Row<TW, VEC, NV> weight;
     if (a.weight) weight.load(static_cast<const TW*>(a.weight), k);
     const T* X = static_cast<const T*>(a.x);
     const T* DY = static_cast<const T*>(a.dy);
-    const int64_t step = (int64_t)gridDim.x * kRows;
-    int64_t row = (int64_t)blockIdx.x * kRows + (W == 1 ? wave : 0);
     Row<T, VEC, NV> now_x, now_dy, next_x, next_dy;
     if (row < a.rows) {
         now_x.load(X + row * a.ldx, k);
@@ -224,8 +239,8 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
                 }
             }
         }
-        sa = row_sum<W>(sa, s_red) * a.inv_D;
-        sh = row_sum<W>(sh, s_red) * a.inv_D;
+        sa = row_sum<G>(sa, s_red) * a.inv_D;
+        sh = row_sum<G>(sh, s_red) * a.inv_D;
         T* dx = static_cast<T*>(a.dx) + row * a.lddx;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
@@ -238,7 +253,7 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
         now_dy = next_dy;
     }
     float* part = a.part + (int64_t)blockIdx.x * 2 * a.D;
-    if constexpr (W == 1) {
+    if constexpr (kGroups > 1) {
         const bool only = gridDim.x == 1;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -249,12 +264,12 @@ __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
                 if (k.on[c])
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
-                        s_part[wave * a.D + k.col[c] + i] = which ? db[c][i] : dw[c][i];
+                        s_part[threadIdx.x / G * a.D + k.col[c] + i] = which ? db[c][i] : dw[c][i];
             __syncthreads();
             for (int d = threadIdx.x; d < a.D; d += kBlock) {
                 float s = s_part[d];
 #pragma unroll
-                for (int i = 1; i < kWavesPerBlock; ++i) s += s_part[i * a.D + d];
+                for (int i = 1; i < kGroups; ++i) s += s_part[i * a.D + d];
                 if (!only) part[which * a.D + d] = s;
                 else if (out) out[d] = (TW)s;
             }
@@ -293,8 +308,8 @@ __global__ __launch_bounds__(kBlock) void norm_grad_long_kernel(NormArgs a) {
             part[d] = (first ? 0.0f : part[d]) + g * h;
             part[a.D + d] = (first ? 0.0f : part[a.D + d]) + g;
         }
-        sa = row_sum<kWavesPerBlock>(sa, s_red) * a.inv_D;
-        sh = row_sum<kWavesPerBlock>(sh, s_red) * a.inv_D;
+        sa = row_sum<kBlock>(sa, s_red) * a.inv_D;
+        sh = row_sum<kBlock>(sh, s_red) * a.inv_D;
         for (int d = threadIdx.x; d < a.D; d += kBlock) {
             const float h = ((float)x[d] - mean) * rstd, g = (float)dy[d];
             const float v = a.weight ? g * (float)static_cast<const TW*>(a.weight)[d] : g;
@@ -330,34 +345,42 @@ __global__ __launch_bounds__(kJoinBlock) void norm_join_kernel(const float* __re
     }
 }
 
-// Calls f<VEC, NV, W> for rows of D elements of type T; false if they are too long for registers.
+// Calls f<VEC, NV, G> for rows of D elements of type T; false if they are too long for registers.
 template <typename T, typename F>
 bool with_shape(int64_t D, F&& f) {
     constexpr int V = kVec<T>;
-    using std::integral_constant;
     const int64_t nv = D < V ? D : (D + V - 1) / V;
-    const auto go = [&](auto vec, auto n, auto w) { f(vec, n, w); return true; };
-    integral_constant<int, 1> i1;
-    integral_constant<int, 2> i2;
-    integral_constant<int, 3> i3;
-    integral_constant<int, 4> i4;
-    integral_constant<int, V> v;
-    if (D < V) return go(i1, i1, i1);
-    if (nv <= 64) return go(v, i1, i1);
-    if (nv <= 128) return go(v, i2, i1);
-    if (nv <= 192) return go(v, i3, i1);
-    if (nv <= 256) return go(v, i4, i1);
-    if (nv <= 512) return go(v, i2, i4);
-    if (nv <= 1024) return go(v, i4, i4);
+    const auto go = [&](auto vec, auto n, auto g) { f(vec, n, g); return true; };
+    const std::integral_constant<int, 1> i1;
+    const std::integral_constant<int, 2> i2;
+    const std::integral_constant<int, 3> i3;
+    const std::integral_constant<int, 4> i4;
+    const std::integral_constant<int, 8> i8;
+    const std::integral_constant<int, 16> i16;
+    const std::integral_constant<int, 32> i32;
+    const std::integral_constant<int, kWave> wave;
+    const std::integral_constant<int, kBlock> block;
+    const std::integral_constant<int, V> v;
+    if (D < V) return go(i1, i1, i8);
+    if (nv <= 4) return go(v, i1, i4);
+    if (nv <= 16) return go(v, i1, i16);
+    if (nv <= 32) return go(v, i1, i32);
+    if (nv <= 64) return go(v, i1, wave);
+    if (nv <= 128) return go(v, i2, wave);
+    if (nv <= 192) return go(v, i3, wave);
+    if (nv <= 256) return go(v, i4, wave);
+    if (nv <= 512) return go(v, i2, block);
+    if (nv <= 1024) return go(v, i4, block);
     return false;
 }
 
 constexpr int kNormBlocks = 2048;  // workgroups of a forward pass: all that 256 CUs hold
 constexpr int kGradBlocks = 512;   // of a backward pass, each of which leaves a share of the weight's gradient
-constexpr int kFewRows = 32;       // one workgroup takes these, and its share is the gradient
+constexpr int kFewRows = 32;       // one workgroup takes these of kFewElements, and its share is the gradient
+constexpr int kFewElements = 32 * 1024;
 
-int64_t grad_parts(int64_t rows) {
-    return rows <= kFewRows ? 1 : std::min<int64_t>(kGradBlocks, (rows + kWavesPerBlock - 1) / kWavesPerBlock);
+int64_t grad_parts(int64_t rows, int64_t D, int64_t per) {
+    return rows <= kFewRows && rows * D <= kFewElements ? 1 : std::min<int64_t>(kGradBlocks, (rows + per - 1) / per);
 }
 
 bool sizes_ok(int64_t rows, int64_t D) { return rows >= 0 && rows <= 0x7fffffff && D >= 1 && D <= (1 << 29); }
@@ -387,13 +410,13 @@ int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, in
             if constexpr (std::is_same<T, TW>::value || std::is_same<TW, float>::value) {
                 NormArgs a{x, nullptr, weight, bias, y, nullptr, mean, rstd, nullptr, nullptr, nullptr, rows, ld_x, 0, ld_y,
                            0, (int)D, 0, (float)eps, (float)(1.0 / (double)D)};
-                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
-                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
+                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto g) {
+                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, G = decltype(g)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
-                    const int64_t per = kWavesPerBlock / W;
+                    const int64_t per = kBlock / G;
                     const unsigned grid = (unsigned)std::min<int64_t>(kNormBlocks, (rows + per - 1) / per);
                     with_bool(rows * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
-                        norm_kernel<T, TW, VEC, NV, W, decltype(past)::value><<<grid, kBlock, 0, st>>>(a);
+                        norm_kernel<T, TW, VEC, NV, G, decltype(past)::value><<<grid, kBlock, 0, st>>>(a);
                     });
                 });
                 if (!ok) norm_long_kernel<T, TW><<<(unsigned)rows, kBlock, 0, st>>>(a);
@@ -405,7 +428,7 @@ int trident_layer_norm(const void* x, int32_t dtype, int64_t rows, int64_t D, in
 
 size_t trident_layer_norm_grad_workspace_bytes(int64_t rows, int64_t D) {
     if (!sizes_ok(rows, D)) return 0;
-    return (size_t)grad_parts(rows) * 2 * (size_t)D * sizeof(float);
+    return (size_t)grad_parts(rows, D, kWavesPerBlock) * 2 * (size_t)D * sizeof(float);
 }
 
 int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_t ld_x, int32_t dtype, int64_t rows,
@@ -421,7 +444,6 @@ int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_
                          (long long)D, (long long)ld_dy, (long long)ld_x, (long long)ld_dx);
     if (rows > 0 && (!dy || !x || !mean || !rstd || !dx))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "layer_norm_grad: NULL pointer");
-    const int64_t parts = grad_parts(rows);
     const size_t need = trident_layer_norm_grad_workspace_bytes(rows, D);
     if (!workspace || workspace_bytes < need)
         return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "layer_norm_grad: workspace %zu < %zu bytes",
@@ -438,15 +460,18 @@ int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_
                            0.0f, (float)(1.0 / (double)D)};
                 // with no rows every share is zero: the kernels' loops are empty
                 bool joined = !dweight && !dbias;
-                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto w) {
-                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, W = decltype(w)::value;
+                int64_t parts = grad_parts(rows, D, kWavesPerBlock);
+                const bool ok = with_shape<T>(D, [&](auto vec, auto nv, auto g) {
+                    constexpr int VEC = decltype(vec)::value, NV = decltype(nv)::value, G = decltype(g)::value;
                     a.nv = (int)((D + VEC - 1) / VEC);
-                    const size_t lds = W == 1 ? kWavesPerBlock * (size_t)D * sizeof(float) : 0;
+                    constexpr int groups = kBlock / G;
+                    const size_t lds = groups > 1 ? groups * (size_t)D * sizeof(float) : 0;
+                    parts = grad_parts(rows, D, std::max(groups, kWavesPerBlock));
                     with_bool(rows * D * (int64_t)sizeof(T) > kL2Bytes, [&](auto past) {
-                        norm_grad_kernel<T, TW, VEC, NV, W, decltype(past)::value>
+                        norm_grad_kernel<T, TW, VEC, NV, G, decltype(past)::value>
                             <<<(unsigned)parts, kBlock, lds, st>>>(a);
                     });
-                    joined = joined || (W == 1 && parts == 1);
+                    joined = joined || (groups > 1 && parts == 1);
                 });
                 if (!ok) norm_grad_long_kernel<T, TW><<<(unsigned)parts, kBlock, 0, st>>>(a);
                 if ((rc = capi_check_launch("norm_grad_kernel")) || joined) return;
