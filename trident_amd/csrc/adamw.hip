@@ -114,7 +114,10 @@ __device__ __forceinline__ float encode(const float (&x)[kPer], float levels, fl
 
 constexpr float kLevelsM = 127.0f * 127.0f, kLevelsV = 255.0f * 255.0f;
 
-// Bound by bytes: every operand is read and written once, a wave a block of 256 elements at a time.
+// Bound by bytes: every operand is read and written once, a wave a block of 256 elements at a time, so that
+// an 8-bit block's largest value is one wave's.  All tensors are one launch (26 small ones 6.8 us).  62
+// million float32 elements: states in 32 bits and bfloat16 gradients 300 us, 5.4 TB/s; states in 8 bits and
+// float32 gradients 187 us, 5.3 TB/s.
 template <int BITS, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
     int lo = 0, hi = a.tensors - 1;  // the last tensor whose first chunk is not past this one
@@ -189,7 +192,7 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
     }
 }
 
-// The values that 8-bit states stand for.
+// The values that 8-bit states stand for.  Bound by bytes: 62 million 88 us, 7 TB/s, most of it written.
 template <bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adam_values_kernel(const uint32_t* __restrict__ cm,
                                                              const uint32_t* __restrict__ cv,

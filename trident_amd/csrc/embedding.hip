@@ -26,7 +26,7 @@ constexpr int kEmbedUnroll = 4;
 
 // Bound by bytes: the rows' vectors of all tokens, one after the other, are dealt to the lanes, so a
 // row of any length leaves no lane idle; four independent gathers per lane cover the latency of the
-// id and of the row behind it.  131,072 tokens x 768 bfloat16 of 30,522 rows: 45 us, 4.5 TB/s written
+// id and of the row behind it.  131,072 tokens x 960 bfloat16 of 65,536 rows: 46 us, 5.5 TB/s written
 // and as much read, mostly from the caches.
 template <typename T, int VEC, typename ID, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_kernel(EmbedArgs a) {
@@ -392,7 +392,8 @@ constexpr int kClear = 16;  // rows of a wave that clears
 // the chunk that it begins in, which sums it to its end and writes it.  A longer row (a frequent token)
 // is summed chunk by chunk into `part`, of which a chunk needs two: for the row it begins in and the
 // row it ends in; join_long_kernel adds a row's parts in order.  So every group has between one and two
-// chunks of work, whatever the frequencies.  131,072 x 768 bfloat16 into 30,522 rows: 40 us, 6 TB/s.
+// chunks of work, whatever the frequencies.  131,072 x 768 bfloat16 into 65,536 rows: 41 us,
+// about 6 TB/s.
 template <typename T, int VEC, int NVL, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
     constexpr int kAhead = NVL > 2 ? 4 : 8;
@@ -491,7 +492,7 @@ __global__ __launch_bounds__(kBlock) void embed_grad_kernel(EmbedGradArgs a) {
 
 // Adds the parts of the long rows, those of one sorting workgroup's ids here: 64 VEC columns a workgroup,
 // each of its waves a quarter of a row's parts, then the waves' sums in order.  Bound by the longest row:
-// 9.4 us where one id has a fifteenth of 131,072 tokens; eight or sixteen waves take as long.
+// 9.6 us for the same; eight or sixteen waves take as long.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
     __shared__ float s_sum[kWavesPerBlock][VEC][kWave];
@@ -535,8 +536,8 @@ __global__ __launch_bounds__(kBlock) void join_long_kernel(EmbedGradArgs a) {
 // Few tokens, in one launch: the time is that of launches, not of bytes.  Workgroup b owns the ids = b
 // modulo gridDim.x as in sort_ids_kernel, orders its tokens in LDS, and sums and writes its own rows, so
 // nothing passes between workgroups: groups of lanes clear the rows without tokens, take those with up to
-// kShared of them in turn, and sum the others together.  16 tokens x 768 into 30,522 rows: 7.1 us, 6.6 TB/s
-// of zeros.
+// kShared of them in turn, and sum the others together.  2,368 tokens x 128 float32 into
+// 32,768 rows: 11.3 us, of which uniform ids leave 9; the zeros take 3.
 constexpr int kFewThreads = 512;
 constexpr int kFewTokens = 8192;           // 16 a thread, held in registers
 constexpr int kFewElements = 1024 * 1024;  // tokens * columns: past it one workgroup may have too much to sum
@@ -641,12 +642,13 @@ __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) 
 #pragma unroll
             for (int i = 0; i < VEC; ++i) acc[c][i] = 0.0f;
     };
-    // adds the tokens order[beg], order[beg + step] .. below end, four in flight
+    // adds the tokens order[beg], order[beg + step] .. below end, kAhead in flight
+    constexpr int kAhead = NVL > 1 ? 4 : 8;
     const auto add = [&](int beg, int end, int step) {
-        for (int k = beg; k < end; k += 4 * step) {
-            Vec<T, VEC> f[4][NVL];
+        for (int k = beg; k < end; k += kAhead * step) {
+            Vec<T, VEC> f[kAhead][NVL];
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < kAhead; ++u)
                 if (k + u * step < end) {
                     const T* row = g + (int64_t)order[k + u * step] * a.ld;
 #pragma unroll
@@ -654,7 +656,7 @@ __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) 
                         if (on[c]) f[u][c].load(row + col[c]);
                 }
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < kAhead; ++u)
                 if (k + u * step < end)
 #pragma unroll
                     for (int c = 0; c < NVL; ++c) {
@@ -697,11 +699,12 @@ __global__ __launch_bounds__(kFewThreads) void embed_grad_few_kernel(FewArgs a) 
         __syncthreads();
         if (group == 0) {
             const int used = min(groups, end - beg);
+#pragma unroll 4
+            for (int k = 1; k < used; ++k)
 #pragma unroll
-            for (int c = 0; c < NVL; ++c)
+                for (int c = 0; c < NVL; ++c)
 #pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    for (int k = 1; k < used; ++k) acc[c][i] += sums[(c * VEC + i) * kFewThreads + k * a.lanes + l];
+                    for (int i = 0; i < VEC; ++i) acc[c][i] += sums[(c * VEC + i) * kFewThreads + k * a.lanes + l];
             write(j);
         }
     }
@@ -785,9 +788,9 @@ int order_tokens(const SortArgs& a, hipStream_t st) {
 
 // Which calls take one launch instead of three: at most kFewTokens and kFewElements, rows within one
 // group's registers, and ids within the 256 workgroups' counters.  One and three, ids uniform and by a
-// 1 / rank law: 64 x 768 11.8 and 15.8 us; 1,024 x 768 12.6 and 16.9, 18.6 and 19.0; 8,192 x 128 10.7 and
-// 17.8, 19.9 and 23.5; 4,096 x 768 15.1 and 19.5, 26.3 and 22.0.  With one id for all tokens, the worst
-// that one workgroup can be given, 1,024 x 768 takes 45 and 22.
+// 1 / rank law: 64 x 768 11.8 and 15.8 us; 1,024 x 768 12.6 and 16.9, 15.6 and 19.0; 8,192 x 128 10.9 and
+// 17.8, 16.7 and 23.5; but 4,096 x 768 by the law 26.3 and 22.0.  With one id for all tokens, the worst that
+// one workgroup can be given, 1,024 x 768 takes 43 and 22.
 bool few_ok(int64_t n, int64_t V, int64_t D) {
     return n > 0 && n <= kFewTokens && n * D <= kFewElements && D <= 1024 && V <= (int64_t)kOwned << 8;
 }

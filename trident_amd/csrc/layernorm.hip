@@ -192,8 +192,9 @@ __global__ __launch_bounds__(kBlock) void norm_long_kernel(NormArgs a) {
     }
 }
 
-// Bound by bytes.  G lanes as above take every so many rows, the next one's loads ahead of this one's work: dx from the row's two means, and dy h and dy added to the columns' sums, which stay
-// in registers until the last row.  131,072 x 768 bfloat16: 111 us, 5.4 TB/s.
+// Bound by bytes.  G lanes as above take every so many rows, the next one's loads ahead of this one's work:
+// dx from the row's two means, and dy h and dy added to the columns' sums, which stay in registers until the
+// last row.  131,072 x 768 bfloat16: 111 us, 5.4 TB/s.
 template <typename T, typename TW, int VEC, int NV, int G, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_grad_kernel(NormArgs a) {
     extern __shared__ float s_part[];  // [kGroups][D], more groups than one only
