@@ -3,7 +3,7 @@ from test_build_guards import code_objects, kernel_resources, pytestmark  # noqa
 
 KERNELS = ("embed_kernel", "bucket_ids_kernel", "sort_ids_kernel", "embed_grad_kernel", "join_long_kernel",
            "embed_grad_few_kernel", "norm_kernel", "norm_grad_kernel", "norm_join_kernel", "adamw_kernel",
-           "adam_values_kernel", "quantize_kernel", "matmul_kernel", "matmul_few_kernel")
+           "adam_values_kernel", "quantize_kernel", "matmul_kernel", "join_products_kernel", "matmul_few_kernel")
 
 
 def test_no_scratch_in_the_encoders_kernels(code_objects):  # noqa: F811

@@ -29,9 +29,9 @@ def randn(g, *shape, dtype=torch.float32):
 
 
 def within(got, ref, bound, what=""):
-    """|got - ref| <= bound; where ref rounds to an infinity of got's type, that infinity."""
-    past = ref.to(got.dtype).isinf() & ref.isfinite()
-    off = torch.where(past & (got.to(F64) == ref.to(got.dtype).to(F64)), 0.0, (got.to(F64) - ref).abs())
+    """|got - ref| <= bound; an infinity of got's type where a value within the bound rounds to it."""
+    past = (ref.abs() + bound).to(got.dtype).isinf() & ref.isfinite()
+    off = torch.where(past & got.isinf() & ((got > 0) == (ref > 0)), 0.0, (got.to(F64) - ref).abs())
     bad = ~(off <= bound)
     assert not bad.any(), (f"{what}: {int(bad.sum())} of {bad.numel()} values past their bound, worst by "
                            f"{float((off / bound.clamp(min=1e-300))[bad].max()):.3g}x")
@@ -706,6 +706,32 @@ WIDE = [(1, 8195, 200), (5, 16390, 136), (16, 8192, 640), (16, 16400, 130), (9, 
 @pytest.mark.parametrize("M,N,K", WIDE)
 def test_fp8_products_of_wide_and_long_weights(dev, dtype, M, N, K):
     test_fp8_matmul_and_linear(dev, dtype, M, N, K)
+
+
+# few tiles of a long K, shared by several workgroups: shares of even and odd numbers of blocks, odd columns
+SPLIT = [(33, 1, 4096), (64, 130, 4100), (100, 101, 8192), (65, 1023, 5000), (300, 500, 4097), (129, 258, 12_800),
+         (500, 1000, 4224), (40, 4099, 4300)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,N,K", SPLIT)
+def test_fp8_linear_split_over_columns(dev, dtype, M, N, K):
+    test_fp8_matmul_and_linear(dev, dtype, M, N, K)
+
+
+def test_fp8_linear_split_keeps_to_its_output(dev):
+    """A padded result's other columns are left alone, and each call gives the same bits."""
+    g = gen(77)
+    x, w, bias = randn(g, 100, 5000), encoder.quantize_fp8(randn(g, 37, 5000)), randn(g, 37)
+    y = encoder.fp8_linear(x, w, bias)
+    assert all(torch.equal(encoder.fp8_linear(x, w, bias), y) for _ in range(5))
+    big = torch.full((100, 64), 7.0, device=dev)
+    L, need = _lib.lib(), _lib.lib().trident_fp8_linear_workspace_bytes(100, 37, 5000)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    rc = L.trident_fp8_linear(x.data_ptr(), 0, 100, 5000, 5000, w.codes.data_ptr(), w.scales.data_ptr(), 37,
+                              bias.data_ptr(), 0, big.data_ptr(), 64, 0, ws.data_ptr(), need,
+                              torch.cuda.current_stream().cuda_stream)
+    assert rc == 0 and torch.equal(big[:, :37], y) and (big[:, 37:] == 7.0).all()
 
 
 def test_fp8_linear_shapes_strides_and_empty(dev):

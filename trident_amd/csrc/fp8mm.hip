@@ -120,6 +120,7 @@ struct MatmulArgs {
     void* out;               // [M, ldo]
     int64_t pitch_a, pitch_b, ldo;
     int M, N, kb, spitch, bias_f32, tiles_m, tiles_n;
+    int share;               // blocks of K of one workgroup, SPLIT only
 };
 
 __device__ __forceinline__ float scale_value(uint32_t e) {
@@ -192,7 +193,10 @@ __device__ __forceinline__ void load_bias(const void* bias, int f32, int first, 
 // 2.0 PFLOP/s, x 8192 252 us, 2.2; as bfloat16, 128 x 128: 8192 x 4096 x 8192 470 us, 1.17 PFLOP/s, where
 // the conversion shares the time.  A small product is bound by its few tiles' latency: 1237 x 777 x 1000
 // in float32 10 us.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
+//
+// With SPLIT a tile's K is shared by the workgroups of a column of the grid, each of which writes its sums to
+// an array of its own.
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK, bool SPLIT>
 __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g) {
     constexpr int kTeam = WM * WN, kWaves = kTeam * WK, BM = WM * MT * 32, BN = WN * NT * 32, kRows = BM + BN;
     constexpr int kStage = WK * kRows * kBlockK;
@@ -209,6 +213,8 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
     tile_of(blockIdx.x, g.tiles_m, g.tiles_n, 8, &tm, &tn);
     const int m0 = tm * BM, n0 = tn * BN;
     const int team = wave / kTeam, wm = wave % kTeam / WN * MT * 32, wn = wave % WN * NT * 32;
+
+    const int kb0 = SPLIT ? (int)blockIdx.y * g.share : 0, kb1 = SPLIT ? min(g.kb, kb0 + g.share) : g.kb;
 
     // A stage is WK times BM rows of a and BN of b, kLoads loads of eight rows for each wave: of one
     // operand, so the wave's loads differ in a scalar only.  Rows past the operand's end repeat the last.
@@ -238,7 +244,7 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
     }
     const auto fetch = [&](int step) {
         uint8_t* to = lds + step % 2 * kStage + wave * kLoads * 1024;
-        const uint32_t k = (uint32_t)min(step * WK + load_part, g.kb - 1) * kBlockK;
+        const uint32_t k = (uint32_t)min(kb0 + step * WK + load_part, kb1 - 1) * kBlockK;
         if (rows == kWaveRows) {
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
@@ -256,7 +262,7 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
             __builtin_amdgcn_raw_ptr_buffer_load_lds(
                 scale_buf[i],
                 (lds_ptr)(lds + 2 * kStage + step % 2 * kScaleStage + (i * kWaves + wave) * kWave * 4), 4, scale_row[i],
-                min(step * WK + scale_part[i], g.kb - 1) & ~3, 0, 0);
+                min(kb0 + step * WK + scale_part[i], kb1 - 1) & ~3, 0, 0);
     };
     // where this lane reads the four pieces of its first row of either operand; the other rows are 32
     // rows on, the other stage is the next bit
@@ -296,7 +302,7 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
     f32x16 acc[MT][NT] = {};
     // Two stages.  A stage's next loads are issued as soon as every wave holds its part of it in
     // registers, halfway through its products, so they have a step and a half to arrive.
-    const int steps = (g.kb + WK - 1) / WK;
+    const int steps = (kb1 - kb0 + WK - 1) / WK;
     fetch(0);
     if (steps > 1) fetch(1);
     for (int step = 0; step < steps; ++step) {
@@ -305,8 +311,8 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
         else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        const int kb = step * WK + team;
-        const bool live = WK == 1 || kb < g.kb;  // not in the last step of the last team of an odd number
+        const int kb = kb0 + step * WK + team;
+        const bool live = WK == 1 || kb < kb1;  // not in the last step of the last team of an odd number
         const uint32_t* st = reinterpret_cast<const uint32_t*>(lds + 2 * kStage + step % 2 * kScaleStage) + team * kRows;
         uint32_t ea[MT], eb[NT];  // the scale of this block in the lowest byte
 #pragma unroll
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
 #pragma unroll
             for (int e = 0; e < kPer; ++e) v[e] = (T)(from[e / 4][e % 4] + bias[e]);
             if (m >= g.M) continue;
-            T* out = static_cast<T*>(g.out) + (int64_t)m * g.ldo + piece_col;
+            T* out = static_cast<T*>(g.out) + ((SPLIT ? (int64_t)blockIdx.y * g.M : 0) + m) * g.ldo + piece_col;
             if (left >= kPer) {
                 __builtin_memcpy(out, v, 16);
             } else {
@@ -429,6 +435,25 @@ __global__ __launch_bounds__(WM* WN* WK* kWave) void matmul_kernel(MatmulArgs g)
         }
         wave_sync();
     }
+}
+
+// The sums of SPLIT workgroups, in order, with the bias: four columns a thread.  A launch's time, 3.3 us
+// beside the others.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void join_products_kernel(const float* __restrict__ part, int shares, int64_t M,
+                                                               int N, int quads, const void* bias, int bias_f32,
+                                                               T* __restrict__ out, int64_t ldo) {
+    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (at >= M * quads) return;
+    const int64_t m = at / quads;
+    const int col = (int)(at - m * quads) * 4;
+    f32x4 sum = {};
+    for (int s = 0; s < shares; ++s) sum += *reinterpret_cast<const f32x4*>(part + (s * M * quads + at) * 4);
+    float b[4];
+    load_bias<T, 4>(bias, bias_f32, col, N, b);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (col + e < N) out[m * ldo + col + e] = (T)(sum[e] + b[e]);
 }
 
 constexpr int kFewWaves = 8;
@@ -599,12 +624,12 @@ inline bool one_launch(int64_t M, int64_t N, int64_t K, int64_t bytes) {
 inline bool few_codes(int64_t M, int64_t N) { return M <= kFewRows || (M <= 2 * kFewRows && N <= 4096); }
 
 // Launches the kernel of one tile size.
-template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK>
+template <typename T, bool FAST, int WM, int WN, int MT, int NT, int WK, bool SPLIT = false>
 int launch_matmul(MatmulArgs g, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32;
     constexpr size_t threads = WM * WN * WK * kWave, rows = WK * (size_t)(BM + BN);
     constexpr size_t lds = 2 * (rows * kBlockK + (rows + threads - 1) / threads * threads * 4);
-    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT, WK>;
+    const auto kernel = matmul_kernel<T, FAST, WM, WN, MT, NT, WK, SPLIT>;
     static_assert(lds <= 163840, "LDS of a CU");
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -615,7 +640,8 @@ int launch_matmul(MatmulArgs g, hipStream_t st) {
     g.tiles_n = (g.N + BN - 1) / BN;
     if ((int64_t)g.tiles_m * g.tiles_n > 0x7fffffff)
         return capi_fail(TRIDENT_ERR_UNSUPPORTED, "fp8_matmul: %d x %d is too large", g.M, g.N);
-    kernel<<<(unsigned)(g.tiles_m * g.tiles_n), threads, lds, st>>>(g);
+    const unsigned shares = SPLIT ? (unsigned)((g.kb + g.share - 1) / g.share) : 1;
+    kernel<<<dim3((unsigned)(g.tiles_m * g.tiles_n), shares), threads, lds, st>>>(g);
     return capi_check_launch("matmul_kernel");
 }
 
@@ -637,6 +663,19 @@ int matmul(const MatmulArgs& g, hipStream_t st) {
     if (tiles(64, 64) <= 512) return launch_matmul<T, FAST, 2, 2, 1, 1, 2>(g, st);
     return launch_matmul<T, FAST, 2, 2, 2, 2, 1>(g, st);
 }
+
+// Blocks of K of one workgroup where a product has so few tiles and so long a K that its tiles are split,
+// else 0.  A tile takes 0.4 us a block of K, joining the shares another launch.  The whole projection, tiles
+// whole and split: float32, exact sums, 64 x 1024 x 2048 12.2 and 16.0 us, x 4096 18.4 and 16.2, x 8192 30.7
+// and 16.2; 512 x 1024 (128 tiles) x 4096 20.9 and 20.0, x 8192 34.5 and 26.5; bfloat16, fast sums, 64 x 1024
+// x 4096 15.7 and 15.6, x 8192 25.3 and 15.6.
+inline int split_share(int64_t M, int64_t N, int64_t K) {
+    const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64), kb = blocks_of(K);
+    if (few_codes(M, N) || tiles > 128 || kb < 32) return 0;
+    const int64_t shares = std::min(256 / tiles, kb / 8);
+    return (int)((kb + shares - 1) / shares + 1) / 2 * 2;
+}
+inline int64_t shares_of(int64_t K, int share) { return (blocks_of(K) + share - 1) / share; }
 
 bool counts_ok(int64_t M, int64_t K) { return M >= 0 && M <= (1 << 30) && K >= 1 && K <= (1 << 30); }
 
@@ -722,13 +761,32 @@ int product(const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M, con
         return product_few<false>(nullptr, 0, a, pitch_a, sa, M, b, sb, N, K, bias, bias_dtype, out, dtype, ld_out,
                                   fast_accum, st);
     const MatmulArgs g{a, b, sa, sb, bias, out, pitch_a, pitch_of(K), ld_out, (int)M, (int)N,
-                       (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0};
+                       (int)blocks_of(K), (int)scale_pitch_of(K), bias_dtype == TRIDENT_F32, 0, 0, 0};
     int rc = TRIDENT_OK;
     with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
         rc = fast_accum ? matmul<T, true>(g, st) : matmul<T, false>(g, st);
     });
     return rc;
+}
+
+// A product whose tiles' K is split: `part` holds the shares' sums, rows of N rounded up to four columns.
+int product_split(const uint8_t* a, int64_t pitch_a, const uint8_t* sa, int64_t M, const uint8_t* b,
+                  const uint8_t* sb, int64_t N, int64_t K, int share, float* part, const void* bias,
+                  int32_t bias_dtype, void* out, int32_t dtype, int64_t ld_out, int32_t fast_accum, hipStream_t st) {
+    const int quads = (int)((N + 3) / 4);
+    const MatmulArgs g{a, b, sa, sb, nullptr, part, pitch_a, pitch_of(K), 4 * (int64_t)quads, (int)M, (int)N,
+                       (int)blocks_of(K), (int)scale_pitch_of(K), 0, 0, 0, share};
+    const int rc = fast_accum ? launch_matmul<float, true, 2, 2, 1, 1, 2, true>(g, st)
+                              : launch_matmul<float, false, 2, 2, 1, 1, 2, true>(g, st);
+    if (rc) return rc;
+    with_dtype(dtype, [&](auto t) {
+        using T = decltype(t);
+        join_products_kernel<T><<<(unsigned)((M * quads + kBlock - 1) / kBlock), kBlock, 0, st>>>(
+            part, (int)shares_of(K, share), M, (int)N, quads, bias, bias_dtype == TRIDENT_F32, static_cast<T*>(out),
+            ld_out);
+    });
+    return capi_check_launch("join_products_kernel");
 }
 
 }  // namespace
@@ -758,7 +816,9 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
 
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (!counts_ok(M, K) || !counts_ok(N, K) || one_launch(M, N, K, 4)) return 0;
-    return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K)));
+    const int share = split_share(M, N, K);
+    return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K))) +
+           (share ? (size_t)(shares_of(K, share) * M * ((N + 3) / 4)) * 16 : 0);
 }
 
 int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* w_codes,
@@ -780,6 +840,11 @@ int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64
     uint8_t* codes = static_cast<uint8_t*>(workspace);
     uint8_t* scales = codes + up256((size_t)(M * own_pitch_of(K)));
     if ((rc = quantize(x, dtype, M, K, ld_x, codes, own_pitch_of(K), scales, stream))) return rc;
+    if (const int share = split_share(M, N, K)) {
+        float* part = reinterpret_cast<float*>(scales + up256((size_t)(M * scale_pitch_of(K))));
+        return product_split(codes, own_pitch_of(K), scales, M, w_codes, w_scales, N, K, share, part, bias, bias_dtype,
+                             out, dtype, ld_out, fast_accum, st);
+    }
     return product(codes, own_pitch_of(K), scales, M, w_codes, w_scales, N, K, bias, bias_dtype, out, dtype, ld_out,
                    fast_accum, st);
 }
