@@ -225,7 +225,8 @@ def _norm(x, weight, bias, eps, keep):
     y = torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = pmean = prstd = None
     if keep:
-        mean, rstd = x.new_empty((2, *shape[:-1]), dtype=torch.float32)
+        mean = x.new_empty(shape[:-1], dtype=torch.float32)
+        rstd = torch.empty_like(mean)
         pmean, prstd = mean.data_ptr(), rstd.data_ptr()
     _call(index, "trident_layer_norm", xr.data_ptr(), code, x.numel() // D, D, ld,
           None if weight is None else weight.data_ptr(), None if bias is None else bias.data_ptr(), wcode, eps,
@@ -274,26 +275,36 @@ def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.
 
 
 def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
-    code, index = _dtype("x", x), _gpu("x", x)
-    if grad.shape != x.shape or grad.dtype != x.dtype:
-        _refuse(f"grad must be {tuple(x.shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
-    _same(index, "grad", grad)
-    D, lead = x.shape[-1], x.shape[:-1]
-    for t in (mean, rstd):
-        if t.dtype is not torch.float32 or t.shape != lead or not t.is_contiguous() or t.get_device() != index:
-            _refuse(f"mean and rstd must be contiguous float32 {tuple(lead)} on cuda:{index}")
-    _affine(index, x, D, weight, None)
+    code, index = _DTYPES.get(x.dtype), x.get_device()
+    shape, lead = x.shape, x.shape[:-1]
+    if code is None or index < 0 or grad.shape != shape or grad.dtype is not x.dtype or grad.get_device() != index:
+        _dtype("x", x)
+        _gpu("x", x)
+        if grad.shape != shape or grad.dtype is not x.dtype:
+            _refuse(f"grad must be {tuple(shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
+        _same(index, "grad", grad)
+    if mean.dtype is not torch.float32 or rstd.dtype is not torch.float32 or mean.shape != lead or \
+            rstd.shape != lead or not mean.is_contiguous() or not rstd.is_contiguous() or \
+            mean.get_device() != index or rstd.get_device() != index:
+        _refuse(f"mean and rstd must be contiguous float32 {tuple(lead)} on cuda:{index}")
+    D = shape[-1]
+    wcode = code if wdtype is None else _DTYPES[wdtype]
+    if weight is not None:
+        _affine(index, x, D, weight, None)
     rows = x.numel() // D
-    wdtype = x.dtype if wdtype is None else wdtype
-    xr, ldx = _rows(x)
-    gr, ldg = _rows(grad)
+    xr, ldx = (x, D) if x.is_contiguous() else _rows(x)
+    gr, ldg = (grad, D) if grad.is_contiguous() else _rows(grad)
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dw = x.new_empty(D, dtype=wdtype) if need_w else None
-    db = x.new_empty(D, dtype=wdtype) if need_b else None
-    nbytes = _fn("trident_layer_norm_grad_workspace_bytes")(rows, D)
-    _call_ws(x.device, index, "trident_layer_norm_grad", nbytes, gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D,
-             ext._ptr(weight), _DTYPES[wdtype], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, ext._ptr(dw),
-             ext._ptr(db))
+    dw = db = pdw = pdb = None
+    if need_w:
+        dw = x.new_empty(D, dtype=wdtype)
+        pdw = dw.data_ptr()
+    if need_b:
+        db = x.new_empty(D, dtype=wdtype)
+        pdb = db.data_ptr()
+    _call_ws(x.device, index, "trident_layer_norm_grad", _fn("trident_layer_norm_grad_workspace_bytes")(rows, D),
+             gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D, None if weight is None else weight.data_ptr(),
+             wcode, mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), D, pdw, pdb)
     return dx, dw, db
 
 
