@@ -890,3 +890,24 @@ def test_refusals(dev):
     for call, text in bad:
         with pytest.raises(_lib.TridentError, match=text):
             call()
+
+
+def test_refusals_before_a_launch(dev):
+    f, i64 = torch.zeros((4, 8), device=dev), torch.zeros(4, dtype=torch.int64, device=dev)
+    stat, none = torch.zeros(4, device=dev), torch.zeros((4, 0), device=dev)
+    table = torch.zeros((4, 8), device=dev, requires_grad=True)
+    bad = [
+        (lambda: encoder.layer_norm_grad(none, none, None, stat, stat), r"\[..., D\]"),
+        (lambda: encoder.layer_norm_grad(stat[0], stat[0], None, stat[0], stat[0]), r"\[..., D\]"),
+        (lambda: encoder.layer_norm_grad(f, f, torch.ones(8, device=dev).double(), stat, stat), "or float32"),
+        (lambda: encoder.layer_norm_grad(f, f.cpu(), None, stat, stat), "device tensor"),
+        (lambda: encoder.layer_norm_grad(f.cpu(), f, None, stat, stat), "must be on"),
+        (lambda: encoder.embedding(i64, table, padding_idx=4), "padding_idx"),
+        (lambda: encoder.embedding(i64, table, padding_idx=-1), "padding_idx"),
+        (lambda: encoder.AdamW([f, f.view(-1)]), "share memory"),
+        (lambda: encoder.AdamW([f.view(-1)[:20], f.view(-1)[19:]]), "share memory"),
+    ]
+    for call, text in bad:
+        with pytest.raises(_lib.TridentError, match=text):
+            call()
+    assert encoder.AdamW([f[:2], f[2:], f.new_empty(0), f.new_empty(0)]).offsets == [0, 256, 512, 512]

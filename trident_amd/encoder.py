@@ -158,6 +158,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     (the ids stay on the device, so no call can refuse them).  Neither has a gradient, nor has
     ``padding_idx``, whose row is looked up like any other.
     """
+    if padding_idx is not None and not 0 <= padding_idx < len(weight):
+        _refuse(f"padding_idx={padding_idx} outside [0, {len(weight)})")
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, weight, scale, padding_idx)
     return _embed(ids, weight, scale)
@@ -277,9 +279,13 @@ def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.
 def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
     code, index = _DTYPES.get(x.dtype), x.get_device()
     shape, lead = x.shape, x.shape[:-1]
-    if code is None or index < 0 or grad.shape != shape or grad.dtype is not x.dtype or grad.get_device() != index:
+    D = shape[-1] if shape else 0
+    if code is None or index < 0 or D == 0 or grad.shape != shape or grad.dtype is not x.dtype or \
+            grad.get_device() != index:
         _dtype("x", x)
         _gpu("x", x)
+        if D == 0:
+            _refuse(f"x must be [..., D], got {tuple(shape)}")
         if grad.shape != shape or grad.dtype is not x.dtype:
             _refuse(f"grad must be {tuple(shape)} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
         _same(index, "grad", grad)
@@ -287,10 +293,9 @@ def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
             rstd.shape != lead or not mean.is_contiguous() or not rstd.is_contiguous() or \
             mean.get_device() != index or rstd.get_device() != index:
         _refuse(f"mean and rstd must be contiguous float32 {tuple(lead)} on cuda:{index}")
-    D = shape[-1]
-    wcode = code if wdtype is None else _DTYPES[wdtype]
     if weight is not None:
         _affine(index, x, D, weight, None)
+    wcode = code if wdtype is None else _DTYPES[wdtype]
     rows = x.numel() // D
     xr, ldx = (x, D) if x.is_contiguous() else _rows(x)
     gr, ldg = (grad, D) if grad.is_contiguous() else _rows(grad)
@@ -348,6 +353,9 @@ class AdamW:
             _need(p.is_contiguous(), f"parameter {i} must be contiguous")
             self.offsets.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
+        # a step reads and writes each element once, by workgroups that know nothing of each other
+        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
+        _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "parameters share memory")
         self._shapes = [p.shape for p in self.params]
         self._table = np.zeros(len(self.params), _TABLE)
         self._table["numel"] = [p.numel() for p in self.params]
