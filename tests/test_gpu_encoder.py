@@ -911,3 +911,25 @@ def test_refusals_before_a_launch(dev):
         with pytest.raises(_lib.TridentError, match=text):
             call()
     assert encoder.AdamW([f[:2], f[2:], f.new_empty(0), f.new_empty(0)]).offsets == [0, 256, 512, 512]
+
+
+def test_adamw_gradients_change_type_between_steps(dev):
+    """Each step takes its gradients' types anew: also after one with gradients missing or refused."""
+    g = torch.Generator(device=dev).manual_seed(3)
+    shapes = [(5,), (300,), (7, 9)]
+    start = [torch.randn(s, generator=g, device=dev) for s in shapes]
+    grads = [torch.randint(-8, 9, s, generator=g, device=dev) / 8 for s in shapes]  # exact in every type
+    ours, want = ([p.clone() for p in start] for _ in range(2))
+    opt, plain = encoder.AdamW(ours), encoder.AdamW(want)
+    f32, f16, bf16 = torch.float32, torch.float16, torch.bfloat16
+    for kinds in ((f32, f32, f32), (f16, f32, bf16), (f16, None, f32), (f16, f32, bf16), (bf16, bf16, f16), "refused",
+                  (bf16, bf16, f16), (f32, f32, f32)):
+        if kinds == "refused":
+            with pytest.raises(_lib.TridentError, match="float64"):
+                opt.step([grads[0].half(), grads[1].double(), grads[2]])
+            continue
+        opt.step([None if k is None else t.to(k) for t, k in zip(grads, kinds)])
+        plain.step([None if k is None else t for t, k in zip(grads, kinds)])
+        for a, b in zip(ours, want):
+            assert torch.equal(a, b), kinds
+    assert torch.equal(opt.exp_avg_sq, plain.exp_avg_sq)

@@ -33,6 +33,7 @@ STATE_BLOCK = 256  # elements of an 8-bit state that share a scale
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _get_device, _data_ptr, _is_contiguous = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
+_increment_version = torch.autograd.graph.increment_version
 _fns = {}
 
 
@@ -223,8 +224,10 @@ def _norm(x, weight, bias, eps, keep):
         _gpu("x", x)
         _refuse(f"x must be [..., D], got {tuple(shape)}")
     wcode = code if weight is None and bias is None else _affine(index, x, D, weight, bias)
-    xr, ld = (x, D) if x.is_contiguous() else _rows(x)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if x.is_contiguous():
+        xr, ld, y = x, D, torch.empty_like(x)
+    else:
+        (xr, ld), y = _rows(x), torch.empty_like(x, memory_format=torch.contiguous_format)
     mean = rstd = pmean = prstd = None
     if keep:
         mean = x.new_empty(shape[:-1], dtype=torch.float32)
@@ -302,10 +305,10 @@ def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
     dx = torch.empty_like(x, memory_format=torch.contiguous_format)
     dw = db = pdw = pdb = None
     if need_w:
-        dw = x.new_empty(D, dtype=wdtype)
+        dw = torch.empty_like(weight)
         pdw = dw.data_ptr()
     if need_b:
-        db = x.new_empty(D, dtype=wdtype)
+        db = x.new_empty(D, dtype=wdtype) if weight is None else torch.empty_like(weight)
         pdb = db.data_ptr()
     _call_ws(x.device, index, "trident_layer_norm_grad", _fn("trident_layer_norm_grad_workspace_bytes")(rows, D),
              gr.data_ptr(), ldg, xr.data_ptr(), ldx, code, rows, D, None if weight is None else weight.data_ptr(),
@@ -360,6 +363,8 @@ class AdamW:
         self._table = np.zeros(len(self.params), _TABLE)
         self._table["numel"] = [p.numel() for p in self.params]
         self._table["offset"] = self.offsets
+        self._table_at = self._table.ctypes.data
+        self._kinds = None  # the types of parameters and gradients that the table names
         kind = (torch.float32, torch.float32) if state_bits == 32 else (torch.int8, torch.uint8)
         moments = [torch.zeros(total, dtype=k, device=self.device) for k in kind]
         scales = [torch.zeros(total // STATE_BLOCK, device=self.device) if state_bits == 8 else None for _ in kind]
@@ -394,17 +399,23 @@ class AdamW:
             table["grad"] = [*map(_data_ptr, grads)]
         except RuntimeError as e:  # sparse
             _refuse(f"gradients must be dense: {e}")
-        try:
-            table["dtype"] = [_DTYPES[p.dtype] for p in params]
-            table["grad_dtype"] = [_DTYPES[g.dtype] for g in grads]
-        except KeyError as e:
-            _refuse(f"parameters and gradients must be float32, float16 or bfloat16, got {e}")
+        kinds = [p.dtype for p in params], [g.dtype for g in grads]
+        whole = table is self._table
+        if not whole or kinds != self._kinds:  # else the table has them
+            try:
+                codes = [[_DTYPES[t] for t in of] for of in kinds]
+            except KeyError as e:
+                _refuse(f"parameters and gradients must be float32, float16 or bfloat16, got {e}")
+            table["dtype"], table["grad_dtype"] = codes
+            if whole:
+                self._kinds = kinds
         table["param"] = [*map(_data_ptr, params)]
         h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
                                    self.step_count + 1)
-        _call(self._index, "trident_adamw", table.ctypes.data, len(params), ctypes.byref(self._state), ctypes.byref(h))
+        _call(self._index, "trident_adamw", self._table_at if whole else table.ctypes.data, len(params),
+              ctypes.byref(self._state), ctypes.byref(h))
         self.step_count += 1
-        torch.autograd.graph.increment_version(params)
+        _increment_version(params)
 
     # the states' buffers: to be read or changed in place (the library holds their addresses)
     exp_avg = property(lambda self: self._buffers[0])
