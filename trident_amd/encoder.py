@@ -336,6 +336,8 @@ class AdamW:
     lie in flat buffers ``exp_avg`` and ``exp_avg_sq`` (with ``exp_avg_scale`` and ``exp_avg_sq_scale``),
     tensor i's from ``offsets[i]``, a multiple of 256, zeros up to the next tensor's.  A gradient that is
     not finite shows in its parameter and state; in 8 bits in the state of its block of 256.
+
+    A step captured in a graph takes the learning rate and the step count of its capture at every replay.
     """
 
     def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
