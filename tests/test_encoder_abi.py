@@ -118,3 +118,11 @@ def test_python_boundary_refuses_host_tensors():
                  lambda: encoder.fp8_linear(f, encoder.Fp8Blocks(f, f, 8))):
         with pytest.raises(_lib.TridentError, match="device tensor"):
             call()
+
+
+@pytest.mark.parametrize("M,N,K", [(100, 0, 4096), (0, 100, 4096), (1 << 20, 0, 1 << 20), (0, 0, 1)])
+def test_a_projection_without_rows_or_columns(M, N, K):
+    """No workspace and nothing to do, whatever the length of K."""
+    L = _lib.lib()
+    assert L.trident_fp8_linear_workspace_bytes(M, N, K) == 0
+    assert L.trident_fp8_linear(P, 0, M, K, K, P, P, N, None, 0, P, max(N, 1), 0, None, 0, None) == 0

@@ -933,3 +933,9 @@ def test_adamw_gradients_change_type_between_steps(dev):
         for a, b in zip(ours, want):
             assert torch.equal(a, b), kinds
     assert torch.equal(opt.exp_avg_sq, plain.exp_avg_sq)
+
+
+def test_fp8_linear_by_a_weight_without_rows(dev):
+    for M, K in ((1, 8), (100, 4096), (700, 5000)):
+        w = encoder.quantize_fp8(torch.empty((0, K), device=dev))
+        assert encoder.fp8_linear(torch.ones((M, K), device=dev), w).shape == (M, 0)

@@ -671,7 +671,7 @@ int matmul(const MatmulArgs& g, hipStream_t st) {
 // x 4096 15.7 and 15.6, x 8192 25.3 and 15.6.
 inline int split_share(int64_t M, int64_t N, int64_t K) {
     const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64), kb = blocks_of(K);
-    if (few_codes(M, N) || tiles > 128 || kb < 32) return 0;
+    if (tiles < 1 || few_codes(M, N) || tiles > 128 || kb < 32) return 0;
     const int64_t shares = std::min(256 / tiles, kb / 8);
     return (int)((kb + shares - 1) / shares + 1) / 2 * 2;
 }
@@ -815,7 +815,7 @@ int trident_fp8_matmul(const uint8_t* a_codes, const uint8_t* a_scales, int64_t 
 }
 
 size_t trident_fp8_linear_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-    if (!counts_ok(M, K) || !counts_ok(N, K) || one_launch(M, N, K, 4)) return 0;
+    if (!counts_ok(M, K) || !counts_ok(N, K) || M == 0 || N == 0 || one_launch(M, N, K, 4)) return 0;
     const int share = split_share(M, N, K);
     return up256((size_t)(M * own_pitch_of(K))) + up256((size_t)(M * scale_pitch_of(K))) +
            (share ? (size_t)(shares_of(K, share) * M * ((N + 3) / 4)) * 16 : 0);
