@@ -8,8 +8,9 @@
 ``embedding`` and ``layer_norm`` take part in autograd; the ``*_forward`` / ``*_grad`` functions are the
 bare passes.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics and states are
 float32 and every result is rounded once.  Each call runs on the current stream of its tensors' device,
-with the library's workspace of that stream (``trident_amd.ext.workspace``); results are the same bits
-every time.  Wrong arguments raise ``TridentError``.
+with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a graph is
+captured there, with scratch of the graph's own; results are the same bits every time.  Wrong arguments
+raise ``TridentError``.
 
 The reference has no counterpart: its vectors come from data sets.  The kernels are in libtrident_hip.so
 (include/trident_hip.h); there is no fallback.
@@ -30,8 +31,7 @@ STATE_BLOCK = 256  # elements of an 8-bit state that share a scale
 
 # A call on one query takes a few microseconds on the GPU, so the path to the library is kept short: the
 # conditions are plain expressions, and messages are only made for a call that is refused.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_current_device = torch._C._cuda_getDevice
+_raw_stream, _current_device = ext._raw_stream, ext._current_device
 _get_device, _data_ptr, _is_contiguous = torch.Tensor.get_device, torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 _increment_version = torch.autograd.graph.increment_version
 _fns = {}
@@ -93,8 +93,8 @@ def _call(index: int, name: str, *args) -> None:
 
 
 def _call_ws(device: torch.device, index: int, name: str, nbytes: int, *args) -> None:
-    """_call with this stream's workspace of at least ``nbytes`` as the last two arguments, or, for none,
-    without one."""
+    """_call with scratch of at least ``nbytes`` as the last two arguments, or, for none, without: this
+    stream's workspace, or, under capture, memory of the graph's own (see ext._scratch)."""
     if nbytes == 0:
         return _call(index, name, *args, None, 0)
     slot = ext._ws_cache.get((device, _raw_stream(index)))
@@ -102,8 +102,8 @@ def _call_ws(device: torch.device, index: int, name: str, nbytes: int, *args) ->
         slot = ext._workspace_slot(device, torch.cuda.current_stream(device))
     with slot.lock:
         ws = slot.buf
-        if ws is None or ws.numel() < nbytes:
-            ws = ext._grow(slot, device, nbytes, torch.cuda.current_stream(device))
+        if ws is None or ws.numel() < nbytes or index != _current_device() or ext._current_capturing():
+            ws = ext._scratch(slot, device, nbytes, torch.cuda.current_stream(device))
         _call(index, name, *args, ws.data_ptr(), ws.numel())
 
 

@@ -140,6 +140,32 @@ def _grow(slot: _Workspace, device, nbytes: int, st) -> torch.Tensor:
     return slot.buf
 
 
+# the current stream's, by device; the handle's type is int
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", None)
+
+
+def _capturing(st) -> bool:
+    """Whether work on ``st`` is being captured into a graph."""
+    if st.device_index == _current_device() and st.cuda_stream == _raw_stream(st.device_index):
+        return _current_capturing()
+    with torch.cuda.stream(st):
+        return _current_capturing()
+
+
+def _scratch(slot: _Workspace, device, nbytes: int, st) -> torch.Tensor:
+    """Scratch of at least ``nbytes`` for one call on ``st``, kept until the call is enqueued.
+
+    The slot's buffer, except under capture: a graph replays with the addresses it was captured with, when
+    and where its owner likes, and the slot's buffer may by then have been replaced or be in use by another
+    call.  A tensor made during the capture lies in the graph's own memory, which lives as long as it."""
+    if _capturing(st):
+        with torch.cuda.stream(st):
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return _grow(slot, device, nbytes, st)
+
+
 def release_workspace(device: torch.device, stream) -> None:
     """Drop the workspace of one (device, stream); the next search on it allocates again."""
     key = _ws_key(device, stream)
@@ -336,7 +362,7 @@ def search_view(view: TridentIndexView, xq: torch.Tensor, nprobe: int, topk_d: t
         ev0, ev1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         ev0.record(st)
     with slot.lock:
-        ws = _grow(slot, xq.device, nbytes, st)
+        ws = _scratch(slot, xq.device, nbytes, st)
         rc = L.trident_search(ctypes.byref(view), ctypes.byref(sp), ctypes.c_void_p(xq.data_ptr()),
                               ctypes.c_void_p(ws.data_ptr()), ctypes.c_size_t(ws.numel()),
                               ctypes.byref(out), ctypes.c_void_p(st.cuda_stream))
