@@ -10,11 +10,22 @@
 // 8 bits, a block of 256 shares one float32 scale per moment:
 //   m       = c |c| sm   c in [-127, 127]   sm = max |m| / 127^2
 //   sqrt(v) = c^2 sv     c in [0, 255]      sv = max sqrt(v) / 255^2
-// with c the nearest integer of the root of the value over the scale.  The square spaces the codes
-// finely near zero: the smallest code is 6e-5 (m) and 1.5e-5 (sqrt v) of the block's largest value.  A
-// second moment that is not zero keeps a code of at least 1, which errs towards the shorter step: a
+// with c one of the two integers around the root of the value over the scale.  The square spaces the
+// codes finely near zero: the smallest code is 6e-5 (m) and 1.5e-5 (sqrt v) of the block's largest value.
+// A second moment that is not zero keeps a code of at least 1, which errs towards the shorter step: a
 // zero there would divide by eps alone.  A block with a value that is not finite gets the scale NaN, so
 // that every later step shows it; blocks whose largest value is below 2^-100 are stored as zeros.
+//
+// Which of the two: the upper one with the probability that makes the stored m, or v, its value in the
+// mean, decided by a hash of the element's place and the step, so that equal calls give equal bits (a
+// graph replays its capture's step, so there the codes fall one way each time).  The nearest would not do: a step moves v by a thousandth, which is never half a code, and m below code
+// 10 by less than half of one, so beside a larger value of its block a moment would stand still for good.
+// (256 elements, half with a gradient in every step and half with one at step 10: 5,000 steps move the
+// second half 5.2 lr with states in 32 bits, 5.2 so, and 1,700, without end, by the nearest code.)
+// The first 2 / (1 - b1) steps do take the nearest code: they are too few for that, and the rounding's
+// noise counts most in them (10,240 parameters with noisy gradients of all magnitudes, distance to the
+// 32-bit run after 100 steps: 0.073, 0.079 and 0.078 so for three seeds, 0.079, 0.081 and 0.084 without;
+// after 300 they agree to 2%; the gradient at step 10 above then moves 8 lr).
 #include <algorithm>
 #include <cmath>
 
@@ -43,6 +54,7 @@ struct AdamArgs {
     float *m_scale, *v_scale;
     int32_t tensors;
     float b1, b1c, b2, b2c, eps, decay, rate, inv_root, grad_scale;
+    uint32_t step_hash;
 };
 static_assert(sizeof(AdamArgs) <= 4096, "kernel arguments");
 
@@ -101,14 +113,43 @@ __device__ __forceinline__ float block_top(const float (&x)[kPer]) {
     return __uint_as_float(top);
 }
 
-// Codes of the block's values x >= 0 with `levels` = (largest code)^2; returns the scale.
+// A round of a hash: a multiplication by an odd constant takes a key's low bits up, shifts take its high
+// bits down.  Four elements of a lane share the first round and have a constant each in the second.
+__device__ __forceinline__ uint32_t scatter(uint32_t key, uint32_t by) {
+    key = (key ^ (key >> 16)) * by;
+    return key ^ (key >> 15);
+}
+// the fractions of (1 + root 5) / 2 and of the roots of 2, 3, 7 and 11 in 32 bits, made odd
+constexpr uint32_t kPhi = 0x9e3779b1u, kRoot2 = 0x6a09e667u, kRoot3 = 0xbb67ae85u, kRoot7 = 0xa54ff53bu,
+                   kRoot11 = 0x510e527fu;
+
+// Codes of the block's values x >= 0 with `levels` = (largest code)^2; returns the scale.  POWER: what is
+// stored in the mean is x (1) or x^2 (2).  dither: a random number in (0, 1) a value, or null: the nearest
+// code.  The root finds the two codes only, so there the instruction's own will do: where it is an ulp off
+// over an integer, that integer is the upper code with probability one, or the lower.
+template <int POWER>
 __device__ __forceinline__ float encode(const float (&x)[kPer], float levels, float inv_levels, float most,
-                                        float (&c)[kPer]) {
+                                        const float* dither, float (&c)[kPer]) {
     const float top = block_top(x);
     const bool fine = top >= kTiny && __float_as_uint(top) < 0x7f800000u;
     const float factor = fine ? (1.0f / top) * levels : 0.0f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) c[i] = fine ? fminf(rintf(sqrtf(x[i] * factor)), most) : 0.0f;
+    for (int i = 0; i < kPer; ++i) {
+        const float y = x[i] * factor;
+        float code;
+        if (dither) {
+            const float lo = floorf(__builtin_amdgcn_sqrtf(y)), a = lo * lo, gap = lo + lo + 1.0f;
+            float step = dither[i] * gap, past = y - a;  // over the scale; past the lower code's value
+            if constexpr (POWER == 2) {
+                step *= a + (a + gap);
+                past *= y + a;
+            }
+            code = step < past || x[i] == top ? lo + 1.0f : lo;  // the largest value's is exact
+        } else {
+            code = rintf(sqrtf(y));
+        }
+        c[i] = fine ? fminf(code, most) : 0.0f;
+    }
     return __float_as_uint(top) >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : fine ? top * inv_levels : 0.0f;
 }
 
@@ -117,8 +158,8 @@ constexpr float kLevelsM = 127.0f * 127.0f, kLevelsV = 255.0f * 255.0f;
 // Bound by bytes: every operand is read and written once, a wave a block of 256 elements at a time, so that
 // an 8-bit block's largest value is one wave's.  All tensors are one launch (26 small ones 6.8 us).  62
 // million float32 elements: states in 32 bits and bfloat16 gradients 300 us, 5.4 TB/s; states in 8 bits and
-// float32 gradients 187 us, 5.3 TB/s.
-template <int BITS, bool PAST_L2>
+// float32 gradients 197 us, 5.1 TB/s, and 192 in the first steps, whose codes are the nearest.
+template <int BITS, bool DITHER, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
     int lo = 0, hi = a.tensors - 1;  // the last tensor whose first chunk is not past this one
     while (lo < hi) {
@@ -172,8 +213,20 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
                 size[i] = i < left ? fabsf(m[i]) : 0.0f;
                 root[i] = i < left ? root[i] : 0.0f;
             }
-            const float sm = encode(size, kLevelsM, (float)(1.0 / 16129.0), 127.0f, cm);
-            const float sv = encode(root, kLevelsV, (float)(1.0 / 65025.0), 255.0f, cv);
+            float um[kPer], uv[kPer];  // 16 random bits each, centred
+            if constexpr (DITHER) {
+                constexpr uint32_t kBy[kPer] = {kPhi, kRoot2, kRoot7, kRoot11};
+                const uint64_t quad = (uint64_t)s / kPer;
+                const uint32_t key = scatter((uint32_t)quad * kPhi + (uint32_t)(quad >> 32) * kRoot11 + a.step_hash, kRoot3);
+#pragma unroll
+                for (int i = 0; i < kPer; ++i) {
+                    const uint32_t bits = scatter(key, kBy[i]);
+                    um[i] = (float)(bits & 0xffffu) * 0x1p-16f + 0x1p-17f;
+                    uv[i] = (float)(bits >> 16) * 0x1p-16f + 0x1p-17f;
+                }
+            }
+            const float sm = encode<1>(size, kLevelsM, (float)(1.0 / 16129.0), 127.0f, DITHER ? um : nullptr, cm);
+            const float sv = encode<2>(root, kLevelsV, (float)(1.0 / 65025.0), 255.0f, DITHER ? uv : nullptr, cv);
             uint32_t wm = 0, wv = 0;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
@@ -266,6 +319,8 @@ int trident_adamw(const TridentAdamTensor* tensors, int32_t count, const Trident
     a.rate = (float)(h.lr / (1.0 - std::pow(h.beta1, (double)h.step)));
     a.inv_root = (float)(1.0 / std::sqrt(1.0 - std::pow(h.beta2, (double)h.step)));
     a.grad_scale = (float)h.grad_scale;
+    a.step_hash = (uint32_t)h.step * kRoot2 + (uint32_t)((uint64_t)h.step >> 32) * kRoot7;
+    const bool dither = (double)h.step * (1.0 - h.beta1) > 2.0;
     hipStream_t st = static_cast<hipStream_t>(stream);
     for (int i = 0; i < count;) {
         int64_t chunks = 0;
@@ -282,8 +337,9 @@ int trident_adamw(const TridentAdamTensor* tensors, int32_t count, const Trident
         if (chunks == 0) continue;
         with_bool(chunks * kChunkElems * 4 > kL2Bytes, [&](auto past) {
             constexpr bool P = decltype(past)::value;
-            if (state->bits == 32) adamw_kernel<32, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
-            else adamw_kernel<8, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+            if (state->bits == 32) adamw_kernel<32, false, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+            else if (dither) adamw_kernel<8, true, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
+            else adamw_kernel<8, false, P><<<(unsigned)chunks, kBlock, 0, st>>>(a);
         });
         const int rc = capi_check_launch("adamw_kernel");
         if (rc) return rc;

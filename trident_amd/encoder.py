@@ -337,7 +337,12 @@ class AdamW:
     tensor i's from ``offsets[i]``, a multiple of 256, zeros up to the next tensor's.  A gradient that is
     not finite shows in its parameter and state; in 8 bits in the state of its block of 256.
 
-    A step captured in a graph takes the learning rate and the step count of its capture at every replay.
+    8-bit codes are the nearest ones in the first 2 / (1 - betas[0]) steps.  After them each is one of the two
+    around its value, chosen by a hash of place and step so that the moment is right in the mean: one that
+    changes by less than a code a step still falls or grows as it should.
+
+    A step captured in a graph takes the learning rate and the step count of its capture at every replay; with
+    8-bit states the codes then fall the same way each time, and small moments may stand still.
     """
 
     def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
