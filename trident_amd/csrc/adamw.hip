@@ -18,10 +18,11 @@
 //
 // Which of the two: the upper one with the probability that makes the stored m, or v, its value in the
 // mean, decided by a hash of the element's place and the step, so that equal calls give equal bits (a
-// graph replays its capture's step, so there the codes fall one way each time).  The nearest would not do: a step moves v by a thousandth, which is never half a code, and m below code
-// 10 by less than half of one, so beside a larger value of its block a moment would stand still for good.
-// (256 elements, half with a gradient in every step and half with one at step 10: 5,000 steps move the
-// second half 5.2 lr with states in 32 bits, 5.2 so, and 1,700, without end, by the nearest code.)
+// graph replays its capture's step, so there the codes fall one way each time).  The nearest would not do:
+// a step moves v by a thousandth, which is never half a code, and m below code 10 by less than half of one,
+// so beside a larger value of its block a moment would stand still for good.  (256 elements, half with a
+// gradient in every step and half with one at step 10: 5,000 steps move the second half 5.2 lr with states
+// in 32 bits, 5.2 so, and 1,700, without end, by the nearest code.)
 // The first 2 / (1 - b1) steps do take the nearest code: they are too few for that, and the rounding's
 // noise counts most in them (10,240 parameters with noisy gradients of all magnitudes, distance to the
 // 32-bit run after 100 steps: 0.073, 0.079 and 0.078 so for three seeds, 0.079, 0.081 and 0.084 without;
