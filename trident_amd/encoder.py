@@ -6,11 +6,11 @@
   quantize_fp8, fp8_matmul, fp8_linear products in 8-bit floating point, one scale per row and 128 columns
 
 ``embedding`` and ``layer_norm`` take part in autograd; the ``*_forward`` / ``*_grad`` functions are the
-bare passes.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics and states are
-float32 and every result is rounded once.  Each call runs on the current stream of its tensors' device,
-with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a graph is
-captured there, with scratch of the graph's own; results are the same bits every time.  Wrong arguments
-raise ``TridentError``.
+bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors are
+float32, float16 or bfloat16 on one GPU; sums, statistics and states are float32 and every result is
+rounded once.  Each call runs on the current stream of its tensors' device, with the library's workspace
+of that stream (``trident_amd.ext.workspace``), or, while a graph is captured there, with scratch of the
+graph's own; results are the same bits every time.  Wrong arguments raise ``TridentError``.
 
 The reference has no counterpart: its vectors come from data sets.  The kernels are in libtrident_hip.so
 (include/trident_hip.h); there is no fallback.
@@ -73,6 +73,13 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
         elif t.shape[0] > 1:
             return t, t.stride(0)
     return t, max(D, 1)
+
+
+def _constant(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses operands whose gradient the caller could be waiting for: the products have none."""
+    for t in tensors:
+        if t is not None and t.requires_grad and torch.is_grad_enabled():
+            _refuse(f"{name} has no gradient: pass detached tensors, or call it under torch.no_grad()")
 
 
 def _fn(name: str):
@@ -502,8 +509,10 @@ def _check_blocks(name: str, b: Fp8Blocks, index: int) -> int:
 
 def quantize_fp8(x: torch.Tensor) -> Fp8Blocks:
     """``x`` [rows, K] in 8-bit floating point: each row's 128 columns share the least power of two under
-    which their largest value is at most 448.  A value that is not finite becomes NaN."""
+    which their largest value is at most 448.  A value that is not finite becomes NaN.  No gradient: ``x``
+    that requires one is refused under grad mode."""
     code, index = _dtype("x", x), _gpu("x", x)
+    _constant("quantize_fp8", x)
     if x.dim() != 2 or x.shape[1] == 0:
         _refuse(f"x must be [rows, K], got {tuple(x.shape)}")
     rows, K = x.shape
@@ -531,7 +540,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
 
     ``fast_accum`` takes the 8-bit matrix instruction, which is twice as fast and keeps 13 bits below the
     largest of each 8 products: the sums are off by up to about 5e-5 of their size, which a bfloat16
-    result does not show."""
+    result does not show.  No gradient: a bias that requires one is refused under grad mode."""
     if not isinstance(a, Fp8Blocks):
         _refuse("a must be Fp8Blocks (quantize_fp8)")
     index = _gpu("a", a.codes)
@@ -541,6 +550,7 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
     if out_dtype not in _DTYPES:
         _refuse(f"out_dtype must be float32, float16 or bfloat16, got {out_dtype}")
     bcode = _bias(bias, N, out_dtype, index)
+    _constant("fp8_matmul", bias)
     out = a.codes.new_empty((M, N), dtype=out_dtype)
     _call(index, "trident_fp8_matmul", a.codes.data_ptr(), a.scales.data_ptr(), M, b.codes.data_ptr(),
           b.scales.data_ptr(), N, a.K, None if bias is None else bias.data_ptr(), bcode, out.data_ptr(),
@@ -551,7 +561,8 @@ def fp8_matmul(a: Fp8Blocks, b: Fp8Blocks, bias: Optional[torch.Tensor] = None,
 def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] = None,
                fast_accum: bool = False) -> torch.Tensor:
     """``x @ weight.T + bias`` for ``x`` [..., K], quantised in the call, in x's type: the projection of a
-    query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``."""
+    query or a corpus by a weight kept in 8 bits.  ``fast_accum``: see ``fp8_matmul``.  No gradient: ``x`` or
+    a bias that requires one is refused under grad mode."""
     code, index = _DTYPES.get(x.dtype), x.get_device()
     if code is None or index < 0:
         _dtype("x", x)
@@ -565,6 +576,7 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     bcode, bptr = code, None
     if bias is not None:
         bcode, bptr = _bias(bias, N, x.dtype, index), bias.data_ptr()
+    _constant("fp8_linear", x, bias)
     xr, ld = (x, K) if x.is_contiguous() else _rows(x)
     out = x.new_empty((M, N) if len(shape) == 2 else (*shape[:-1], N))
     _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, N, K), xr.data_ptr(),
