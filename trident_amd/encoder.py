@@ -6,11 +6,12 @@
   quantize_fp8, fp8_matmul, fp8_linear products in 8-bit floating point, one scale per row and 128 columns
 
 ``embedding`` and ``layer_norm`` take part in autograd; the ``*_forward`` / ``*_grad`` functions are the
-bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors are
-float32, float16 or bfloat16 on one GPU; sums, statistics and states are float32 and every result is
-rounded once.  Each call runs on the current stream of its tensors' device, with the library's workspace
-of that stream (``trident_amd.ext.workspace``), or, while a graph is captured there, with scratch of the
-graph's own; results are the same bits every time.  Wrong arguments raise ``TridentError``.
+bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors with a
+forward-mode tangent are refused.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics
+and states are float32 and every result is rounded once.  Each call runs on the current stream of its
+tensors' device, with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a
+graph is captured there, with scratch of the graph's own; results are the same bits every time.  Wrong
+arguments raise ``TridentError``.
 
 The reference has no counterpart: its vectors come from data sets.  The kernels are in libtrident_hip.so
 (include/trident_hip.h); there is no fallback.
@@ -21,6 +22,7 @@ import ctypes
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib, ext
 from .ext import _need
@@ -75,11 +77,21 @@ def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return t, max(D, 1)
 
 
+def _no_tangents(name: str, *tensors: Optional[torch.Tensor]) -> None:
+    """Refuses dual tensors: the library computes values, and their tangents would be lost.  Called where
+    a level of forward differentiation is open, ``_forward_ad._current_level >= 0``."""
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            _refuse(f"{name} has no forward-mode derivative: an operand has a tangent")
+
+
 def _constant(name: str, *tensors: Optional[torch.Tensor]) -> None:
     """Refuses operands whose gradient the caller could be waiting for: the products have none."""
     for t in tensors:
         if t is not None and t.requires_grad and torch.is_grad_enabled():
             _refuse(f"{name} has no gradient: pass detached tensors, or call it under torch.no_grad()")
+    if _forward_ad._current_level >= 0:
+        _no_tangents(name, *tensors)
 
 
 def _fn(name: str):
@@ -168,6 +180,8 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
     """
     if padding_idx is not None and not 0 <= padding_idx < len(weight):
         _refuse(f"padding_idx={padding_idx} outside [0, {len(weight)})")
+    if _forward_ad._current_level >= 0:
+        _no_tangents("embedding", weight)
     if weight.requires_grad and torch.is_grad_enabled():
         return _Embedding.apply(ids, weight, scale, padding_idx)
     return _embed(ids, weight, scale)
@@ -179,6 +193,8 @@ def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: 
     ``scale`` times the sum of the gradients of the tokens with id v, in their order.  ``out`` (rows of
     any pitch) is written whole."""
     code, index = _dtype("grad", grad), _gpu("grad", grad)
+    if _forward_ad._current_level >= 0:
+        _no_tangents("embedding_grad", grad)
     if grad.dim() < 1 or grad.shape[:-1] != ids.shape or grad.shape[-1] == 0:
         _refuse(f"grad must be [*ids.shape, D], got {tuple(grad.shape)} for ids {tuple(ids.shape)}")
     if num_rows < 1:
@@ -267,6 +283,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last dimension of ``x``; ``weight`` and ``bias`` ([D], of x's type or
     float32) may be left out."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or
                                     (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
@@ -276,6 +294,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                        eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd): layer norm and the rows' float32 statistics, which the backward pass takes."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("layer_norm_forward", x, weight, bias)
     return _norm(x, weight, bias, eps, True)
 
 
@@ -287,6 +307,8 @@ def layer_norm_grad(grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.
 
 
 def _norm_grad(grad, x, weight, mean, rstd, need_w, need_b, wdtype):
+    if _forward_ad._current_level >= 0:
+        _no_tangents("layer_norm_grad", grad, x, weight, mean, rstd)
     code, index = _DTYPES.get(x.dtype), x.get_device()
     shape, lead = x.shape, x.shape[:-1]
     D = shape[-1] if shape else 0
