@@ -392,9 +392,8 @@ class AdamW:
             _need(p.is_contiguous(), f"parameter {i} must be contiguous")
             self.offsets.append(total)
             total += -(-p.numel() // STATE_BLOCK) * STATE_BLOCK
-        # a step reads and writes each element once, by workgroups that know nothing of each other
-        spans = sorted((p.data_ptr(), p.data_ptr() + p.numel() * p.element_size()) for p in self.params if p.numel())
-        _need(all(a[1] <= b[0] for a, b in zip(spans, spans[1:])), "parameters share memory")
+        self._apart = None  # the last step's parameters, by address and type, which share no memory
+        self._need_apart(self.params, list(map(_data_ptr, self.params)))
         self._shapes = [p.shape for p in self.params]
         self._table = np.zeros(len(self.params), _TABLE)
         self._table["numel"] = [p.numel() for p in self.params]
@@ -406,6 +405,13 @@ class AdamW:
         scales = [torch.zeros(total // STATE_BLOCK, device=self.device) if state_bits == 8 else None for _ in kind]
         self._buffers = (*moments, *scales)
         self._state = _lib.TridentAdamState(*map(ext._ptr, self._buffers), total, state_bits)
+
+    @staticmethod
+    def _need_apart(params, addresses) -> None:
+        """A step reads and writes each element once, by workgroups that know nothing of each other."""
+        spans = sorted((a, a + p.numel() * p.element_size()) for p, a in zip(params, addresses) if p.numel())
+        if not all(a[1] <= b[0] for a, b in zip(spans, spans[1:])):
+            _refuse("parameters share memory")
 
     def zero_grad(self) -> None:
         for p in self.params:
@@ -445,7 +451,11 @@ class AdamW:
             table["dtype"], table["grad_dtype"] = codes
             if whole:
                 self._kinds = kinds
-        table["param"] = [*map(_data_ptr, params)]
+        addresses = [*map(_data_ptr, params)]
+        if (addresses, kinds[0]) != self._apart:
+            self._need_apart(params, addresses)
+            self._apart = addresses, kinds[0]
+        table["param"] = addresses
         h = _lib.TridentAdamParams(self.lr, self.betas[0], self.betas[1], self.eps, self.weight_decay, grad_scale,
                                    self.step_count + 1)
         _call(self._index, "trident_adamw", self._table_at if whole else table.ctypes.data, len(params),
