@@ -45,3 +45,24 @@ def test_parameters_that_grow_into_one_another(dev):
         with pytest.raises(_lib.TridentError, match="share memory"):
             opt.step(grads)
     assert opt.step_count == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_state_of_other_tensors(dev, bits):
+    """The same length in all, in other pieces: 257 and 256 elements are three blocks of 256, as 256 and 257
+    are, and as 700 are."""
+    make = lambda *sizes: encoder.AdamW([torch.ones(n, device=dev) for n in sizes], state_bits=bits)  # noqa: E731
+    opt = make(257, 256)
+    opt.step([torch.ones(257, device=dev), torch.ones(256, device=dev)])
+    state = opt.state_dict()
+    for other in (make(256, 257), make(700), make(258, 256), make(257, 256, 0)):
+        with pytest.raises(_lib.TridentError, match="the state is of tensors"):
+            other.load_state_dict(state)
+        assert other.step_count == 0 and (other.exp_avg == 0).all()
+    same = make(257, 256)
+    same.load_state_dict(state)
+    assert same.step_count == 1 and torch.equal(same.exp_avg, opt.exp_avg)
+    del state["numels"]  # as an earlier version saved it
+    old = make(257, 256)
+    old.load_state_dict(state)
+    assert old.step_count == 1 and torch.equal(old.exp_avg, opt.exp_avg)

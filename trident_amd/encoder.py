@@ -496,12 +496,17 @@ class AdamW:
 
     def state_dict(self) -> dict:
         names = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")
-        return dict(step_count=self.step_count, state_bits=self.state_bits,
+        return dict(step_count=self.step_count, state_bits=self.state_bits, numels=self._table["numel"].tolist(),
                     **{n: getattr(self, n).clone() for n in names if getattr(self, n) is not None})
 
     def load_state_dict(self, state: dict) -> None:
+        """Takes what ``state_dict`` gave, for tensors of the same sizes in the same order (``numels``; a state
+        saved without them has to have the same length in all)."""
         _need(state.get("state_bits") == self.state_bits,
               f"the state has {state.get('state_bits')} bits, this optimizer {self.state_bits}")
+        numels = self._table["numel"].tolist()
+        _need(list(state.get("numels", numels)) == numels,
+              f"the state is of tensors of {state.get('numels')} elements, the parameters have {numels}")
         self.load_state(state["step_count"], state["exp_avg"], state["exp_avg_sq"], state.get("exp_avg_scale"),
                         state.get("exp_avg_sq_scale"))
 
