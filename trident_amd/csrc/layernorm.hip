@@ -104,7 +104,7 @@ __device__ __forceinline__ int64_t first_row(int* lane) {
 // Bound by bytes.  G lanes (a wave; a part of one for rows of up to 32 vectors; a workgroup of four for
 // more than 256) take every so many rows and load the next one while they work on this one.  Narrow rows
 // share a wave because its lanes are what it is fed by: 131,072 x 128 bfloat16 a wave a row 36.6 us, four
-// rows a wave 13.8.  131,072 x 768 bfloat16 with the statistics: 67 us, 6.0 TB/s.
+// rows a wave 13.8.  131,072 x 768 bfloat16 with the statistics: 75 us, 5.4 TB/s.
 template <typename T, typename TW, int VEC, int NV, int G, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void norm_kernel(NormArgs a) {
     __shared__ float s_red[kWavesPerBlock];
@@ -378,9 +378,11 @@ bool with_shape(int64_t D, F&& f) {
 }
 
 // Workgroups of a forward pass, of which 256 CUs hold 2,048 at a time: more of them, with fewer rows each,
-// end more evenly, until the next row's loads ahead are lost.  131,072 x 768, 2,048, 4,096, 8,192, 16,384
-// and 32,768 workgroups: float32 147, 145, 139, 136, 134 us; bfloat16, whose rows are half as long, 69, 69,
-// 67, 70, 77; 65,536 x 512 bfloat16 24.4, 23.0, 22.5, 24.5, 25.2.
+// end more evenly, until the next row's loads ahead are lost.  float32 rows are twice as long: 131,072 x 768,
+// 2,048, 4,096, 8,192, 16,384 and 32,768 workgroups 147, 145, 139, 136, 134 us.  For 16 bits no number is the
+// best: 2,048, 4,096 and 8,192, bfloat16, 131,072 x 768 77, 75.5, 74.5 us; x 960 81.6, 78, 73.5; x 256 23.9,
+// 23.1, 21.5; x 128 13.1, 13.0, 13.9; 65,536 x 512 23.9, 23.0, 23.1; 32,768 x 1,024 23.2, 21.9, 23.2; float16
+// 131,072 x 768 68.6, 69.0, 72.4; 32,768 x 1,024 23.1, 23.1, 25.5: 4,096 loses 7% at most, 8,192 11.
 template <typename T>
 constexpr int kNormBlocks = sizeof(T) == 4 ? 16384 : 4096;
 
