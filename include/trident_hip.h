@@ -293,8 +293,9 @@ enum TridentDtype { TRIDENT_F32 = 0, TRIDENT_F16 = 1, TRIDENT_BF16 = 2 };
 int trident_embedding(const void* weight, int32_t dtype, int64_t V, int64_t D, int64_t ld_weight, const void* ids,
                       int32_t ids64, int64_t n, double scale, void* out, int64_t ld_out, void* stream);
 
-/* out[v, :] = scale * sum of grad[t, :] over the tokens with ids[t] == v, in token order; all V rows
- * are written.  Ids outside [0, V) and padding_idx (-1: none) add nothing.  Few tokens need no workspace
+/* out[v, :] = scale * sum of grad[t, :] over the tokens with ids[t] == v; all V rows are written.  The
+ * order of a sum is fixed by the sizes and all of the ids: equal calls give equal bits, but a row's last bits may
+ * change with the other tokens of the batch.  Ids outside [0, V) and padding_idx (-1: none) add nothing.  Few tokens need no workspace
  * (0 bytes). */
 size_t trident_embedding_grad_workspace_bytes(int64_t n, int64_t V, int64_t D);
 int trident_embedding_grad(const void* grad, int32_t dtype, int64_t ld_grad, const void* ids, int32_t ids64,

@@ -3,9 +3,10 @@
 //   y[t, :] = s W[id_t, :]        id_t < 0: an empty slot of a padded batch, zeros; id_t >= V: NaN
 //   dW[v, :] = s sum_{t : id_t = v} dY[t, :]
 //
-// The gradient is summed without float atomics, each row in the order of its tokens, so a call gives
-// the same bits every time: the tokens are ordered by id (a stable counting sort), then every table
-// row is summed over its tokens by one group of lanes and written once, rows without tokens as zeros.
+// The gradient is summed without float atomics, so a call gives the same bits every time: the tokens are
+// ordered by id (a stable counting sort), and every table row is summed over its tokens and written once,
+// rows without tokens as zeros.  A row of few tokens is summed in their order by one group of lanes, a longer
+// one in parts, which are then added in order; where the parts begin goes by the sizes and the other ids.
 #include <algorithm>
 
 #include "encoder.hpp"

@@ -190,8 +190,9 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
 def embedding_grad(grad: torch.Tensor, ids: torch.Tensor, num_rows: int, scale: float = 1.0,
                    padding_idx: Optional[int] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The table's gradient ``[num_rows, D]`` in the type of ``grad`` (``[*ids.shape, D]``): row v is
-    ``scale`` times the sum of the gradients of the tokens with id v, in their order.  ``out`` (rows of
-    any pitch) is written whole."""
+    ``scale`` times the sum of the gradients of the tokens with id v.  Equal calls give equal bits; the order
+    of a sum, and so its last bits, may change with the other tokens.  ``out`` (rows of any pitch) is written
+    whole."""
     code, index = _dtype("grad", grad), _gpu("grad", grad)
     if _forward_ad._current_level >= 0:
         _no_tangents("embedding_grad", grad)
@@ -355,8 +356,12 @@ _TABLE = np.dtype([("param", "u8"), ("grad", "u8"), ("numel", "i8"), ("offset", 
 class AdamW:
     """AdamW (decoupled weight decay) over a list of tensors of float32, float16 or bfloat16.
 
+    A class of its own, not a ``torch.optim.Optimizer``: schedulers and gradient scalers that ask for one do
+    not take it; set ``lr`` and pass ``grad_scale`` instead.
+
     ``step()`` updates the parameters in place from their ``.grad`` (or from a list of gradients, each of
-    any of the three types); a parameter without one is left alone.  ``grad_scale`` multiplies the
+    any of the three types); a parameter without one is left alone, though the step count, which is the
+    optimizer's, goes on for all.  ``grad_scale`` multiplies the
     gradients (one over a loss scale).  ``lr``, ``weight_decay`` and ``step_count`` may be set between
     steps; groups with other settings are other optimizers.
 
