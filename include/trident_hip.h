@@ -320,7 +320,7 @@ int trident_layer_norm_grad(const void* dy, int64_t ld_dy, const void* x, int64_
  * elements, and the rest of its last block of 256 is its own.  bits 32: m, v float32.  bits 8: m int8,
  * v uint8 codes and m_scale, v_scale [len / 256] float32, with m = c |c| m_scale and
  * v = (c^2 v_scale)^2; the nearest codes while step * (1 - beta1) <= 2, then one of the two around the value,
- * by a hash of element and step, so that m and v are stored right in the mean.  step: the step being taken,
+ * by a hash of place, step and the block's largest values, so that m and v are stored right in the mean.  step: the step being taken,
  * from 1.  Gradients are multiplied by grad_scale. */
 typedef struct TridentAdamTensor {
     void* param;

@@ -17,8 +17,9 @@
 // that every later step shows it; blocks whose largest value is below 2^-100 are stored as zeros.
 //
 // Which of the two: the upper one with the probability that makes the stored m, or v, its value in the
-// mean, decided by a hash of the element's place and the step, so that equal calls give equal bits (a
-// graph replays its capture's step, so there the codes fall one way each time).  The nearest would not do:
+// mean, decided by a hash of the element's place, the step and the block's two largest values, so that equal
+// calls give equal bits (and a graph, which replays its capture's step number, still goes on to other
+// ones).  The nearest would not do:
 // a step moves v by a thousandth, which is never half a code, and m below code 10 by less than half of one,
 // so beside a larger value of its block a moment would stand still for good.  (256 elements, half with a
 // gradient in every step and half with one at step 10: 5,000 steps move the second half 5.2 lr with states
@@ -124,14 +125,13 @@ __device__ __forceinline__ uint32_t scatter(uint32_t key, uint32_t by) {
 constexpr uint32_t kPhi = 0x9e3779b1u, kRoot2 = 0x6a09e667u, kRoot3 = 0xbb67ae85u, kRoot7 = 0xa54ff53bu,
                    kRoot11 = 0x510e527fu;
 
-// Codes of the block's values x >= 0 with `levels` = (largest code)^2; returns the scale.  POWER: what is
-// stored in the mean is x (1) or x^2 (2).  dither: a random number in (0, 1) a value, or null: the nearest
+// Codes of the block's values x >= 0, the largest of them `top`, with `levels` = (largest code)^2; returns the
+// scale.  POWER: what is stored in the mean is x (1) or x^2 (2).  dither: a random number in (0, 1) a value, or null: the nearest
 // code.  The root finds the two codes only, so there the instruction's own will do: where it is an ulp off
 // over an integer, that integer is the upper code with probability one, or the lower.
 template <int POWER>
-__device__ __forceinline__ float encode(const float (&x)[kPer], float levels, float inv_levels, float most,
-                                        const float* dither, float (&c)[kPer]) {
-    const float top = block_top(x);
+__device__ __forceinline__ float encode(const float (&x)[kPer], float top, float levels, float inv_levels,
+                                        float most, const float* dither, float (&c)[kPer]) {
     const bool fine = top >= kTiny && __float_as_uint(top) < 0x7f800000u;
     const float factor = fine ? (1.0f / top) * levels : 0.0f;
 #pragma unroll
@@ -214,11 +214,14 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
                 size[i] = i < left ? fabsf(m[i]) : 0.0f;
                 root[i] = i < left ? root[i] : 0.0f;
             }
+            const float top_m = block_top(size), top_v = block_top(root);
             float um[kPer], uv[kPer];  // 16 random bits each, centred
             if constexpr (DITHER) {
                 constexpr uint32_t kBy[kPer] = {kPhi, kRoot2, kRoot7, kRoot11};
                 const uint64_t quad = (uint64_t)s / kPer;
-                const uint32_t key = scatter((uint32_t)quad * kPhi + (uint32_t)(quad >> 32) * kRoot11 + a.step_hash, kRoot3);
+                const uint32_t tops = __float_as_uint(top_m) * kRoot7 + __float_as_uint(top_v) * kRoot2;
+                const uint32_t key = scatter((uint32_t)quad * kPhi + (uint32_t)(quad >> 32) * kRoot11 + a.step_hash + tops,
+                                             kRoot3);
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const uint32_t bits = scatter(key, kBy[i]);
@@ -226,8 +229,10 @@ __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
                     uv[i] = (float)(bits >> 16) * 0x1p-16f + 0x1p-17f;
                 }
             }
-            const float sm = encode<1>(size, kLevelsM, (float)(1.0 / 16129.0), 127.0f, DITHER ? um : nullptr, cm);
-            const float sv = encode<2>(root, kLevelsV, (float)(1.0 / 65025.0), 255.0f, DITHER ? uv : nullptr, cv);
+            const float sm =
+                encode<1>(size, top_m, kLevelsM, (float)(1.0 / 16129.0), 127.0f, DITHER ? um : nullptr, cm);
+            const float sv =
+                encode<2>(root, top_v, kLevelsV, (float)(1.0 / 65025.0), 255.0f, DITHER ? uv : nullptr, cv);
             uint32_t wm = 0, wv = 0;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {

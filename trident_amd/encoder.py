@@ -361,9 +361,9 @@ class AdamW:
 
     ``step()`` updates the parameters in place from their ``.grad`` (or from a list of gradients, each of
     any of the three types); a parameter without one is left alone, though the step count, which is the
-    optimizer's, goes on for all.  ``grad_scale`` multiplies the
-    gradients (one over a loss scale).  ``lr``, ``weight_decay`` and ``step_count`` may be set between
-    steps; groups with other settings are other optimizers.
+    optimizer's, goes on for all.  ``grad_scale`` multiplies the gradients (one over a loss scale).  ``lr``,
+    ``weight_decay`` and ``step_count`` may be set between steps; groups with other settings are other
+    optimizers.
 
     The moments are float32 (``state_bits=32``) or 8-bit codes with a float32 scale for every 256
     (``state_bits=8``: 2.03 bytes a parameter instead of 8); the arithmetic is float32 either way.  They
@@ -372,11 +372,10 @@ class AdamW:
     not finite shows in its parameter and state; in 8 bits in the state of its block of 256.
 
     8-bit codes are the nearest ones in the first 2 / (1 - betas[0]) steps.  After them each is one of the two
-    around its value, chosen by a hash of place and step so that the moment is right in the mean: one that
-    changes by less than a code a step still falls or grows as it should.
+    around its value, chosen by a hash (of place, step and the block's largest moments) so that the moment is
+    right in the mean: one that changes by less than a code a step still falls or grows as it should.
 
-    A step captured in a graph takes the learning rate and the step count of its capture at every replay; with
-    8-bit states the codes then fall the same way each time, and small moments may stand still.
+    A step captured in a graph takes the learning rate and the step count of its capture at every replay.
     """
 
     def __init__(self, params: Iterable[torch.Tensor], lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
