@@ -617,7 +617,8 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     bcode, bptr = code, None
     if bias is not None:
         bcode, bptr = _bias(bias, N, x.dtype, index), bias.data_ptr()
-    _constant("fp8_linear", x, bias)
+    if x.requires_grad or (bias is not None and bias.requires_grad) or _forward_ad._current_level >= 0:
+        _constant("fp8_linear", x, bias)
     xr, ld = (x, K) if x.is_contiguous() else _rows(x)
     out = x.new_empty((M, N) if len(shape) == 2 else (*shape[:-1], N))
     _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, N, K), xr.data_ptr(),
