@@ -159,7 +159,7 @@ constexpr float kLevelsM = 127.0f * 127.0f, kLevelsV = 255.0f * 255.0f;
 // Bound by bytes: every operand is read and written once, a wave a block of 256 elements at a time, so that
 // an 8-bit block's largest value is one wave's.  All tensors are one launch (26 small ones 6.8 us).  62
 // million float32 elements: states in 32 bits and bfloat16 gradients 300 us, 5.4 TB/s; states in 8 bits and
-// float32 gradients 197 us, 5.1 TB/s, and 192 in the first steps, whose codes are the nearest.
+// float32 gradients 192 us, 5.2 TB/s, and 182 in the first steps, whose codes are the nearest.
 template <int BITS, bool DITHER, bool PAST_L2>
 __global__ __launch_bounds__(kBlock) void adamw_kernel(AdamArgs a) {
     int lo = 0, hi = a.tensors - 1;  // the last tensor whose first chunk is not past this one
