@@ -21,13 +21,13 @@
 // calls give equal bits (and a graph, which replays its capture's step number, still goes on to other
 // ones).  The nearest would not do:
 // a step moves v by a thousandth, which is never half a code, and m below code 10 by less than half of one,
-// so beside a larger value of its block a moment would stand still for good.  (256 elements, half with a
-// gradient in every step and half with one at step 10: 5,000 steps move the second half 5.2 lr with states
-// in 32 bits, 5.2 so, and 1,700, without end, by the nearest code.)
+// so beside a larger value of its block a moment would stand still for good.  (These formulas evaluated on
+// 256-element blocks, half with a gradient in every step and half with one at step 10: 5,000 steps move the
+// second half 5.2 lr with states in 32 bits, 5.2 so, and 1,700, without end, by the nearest code.)
 // The first 2 / (1 - b1) steps do take the nearest code: they are too few for that, and the rounding's
 // noise counts most in them (10,240 parameters with noisy gradients of all magnitudes, distance to the
-// 32-bit run after 100 steps: 0.073, 0.079 and 0.078 so for three seeds, 0.079, 0.081 and 0.084 without;
-// after 300 they agree to 2%; the gradient at step 10 above then moves 8 lr).
+// 32-bit run after 100 steps, three seeds: 0.079, 0.077 and 0.078 so, 0.083, 0.084 and 0.085 without them,
+// 0.15 by nearest codes throughout; the gradient at step 10 above then moves 8 lr).
 #include <algorithm>
 #include <cmath>
 
