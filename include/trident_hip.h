@@ -371,6 +371,47 @@ int trident_fp8_linear(const void* x, int32_t dtype, int64_t M, int64_t K, int64
                        const uint8_t* w_scales, int64_t N, const void* bias, int32_t bias_dtype, void* out,
                        int64_t ld_out, int32_t fast_accum, void* workspace, size_t workspace_bytes, void* stream);
 
+/* out[t, h, :] = x[t, h, :] with its first 2 * pairs columns turned, pair i by positions[t % period] *
+ * frequencies[i] radians (in float64) and times amplitude; the other columns are copied.  Pair i is columns 2 i and 2 i + 1
+ * where interleaved is not 0, else i and i + pairs.  positions: int32, or int64 where ids64 is not 0, or NULL
+ * (t % period itself).  inverse: turned back (the gradient).  Strides in elements; out may be x with x's
+ * strides, otherwise they must not overlap. */
+int trident_rotary(const void* x, int32_t dtype, int64_t tokens, int64_t heads, int64_t head_dim, int64_t x_row,
+                   int64_t x_head, const double* frequencies, int64_t pairs, const void* positions, int32_t ids64,
+                   int64_t period, int32_t interleaved, double amplitude, int32_t inverse, void* out, int64_t out_row,
+                   int64_t out_head, void* stream);
+
+/* Attention of every token over its own sequence: out = softmax(scale q k^T) v, in causal attention over the
+ * keys up to the token.  `rows` token rows in all, of which
+ *   packed (slots 0): sequence i has rows offsets[i] .. offsets[i + 1] - 1, offsets ascending, [sequences + 1];
+ *   padded (slots > 0, rows = sequences * slots): sequence i has the first lengths[i] rows of its slots, or all
+ *     of them without lengths.
+ * Rows without a token get zeros, in out and in the gradients.  offsets and lengths are device arrays, int32, or int64 where
+ * ids64 is not 0; values outside the rows are brought inside.  q [rows, q_heads, head_dim], k and v [rows,
+ * kv_heads, head_dim]: strides in elements, of 16-byte pieces, a row's at least head_dim; query head h takes key and value head
+ * h / (q_heads / kv_heads).  out, grad, dq, dk and dv are contiguous.  Every tensor 16-byte aligned.  head_dim: a multiple of
+ * 8 up to 128.  lse [q_heads, rows]: the base-2 logarithm of the rows' sums of exp, for the
+ * backward pass, or NULL. */
+typedef struct TridentAttention {
+    const void *q, *k, *v;
+    void* out;
+    float* lse;
+    const void* grad;          /* the backward pass's, as are the three below */
+    void *dq, *dk, *dv;
+    const void *offsets, *lengths;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+    int64_t rows, sequences, slots;
+    int64_t q_heads, kv_heads, head_dim;
+    double scale;
+    int32_t dtype, ids64, causal;
+} TridentAttention;
+
+int trident_attention(const TridentAttention* a, void* stream);
+
+/* dq, dk, dv from grad (of out), what the forward pass took, its out and its lse. */
+size_t trident_attention_grad_workspace_bytes(const TridentAttention* a);
+int trident_attention_grad(const TridentAttention* a, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* trident_last_error(void);
 int trident_abi_version(void);
 

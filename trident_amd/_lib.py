@@ -76,6 +76,13 @@ class TridentAdamParams(ctypes.Structure):
                 ("grad_scale", _f64), ("step", _i64)]
 
 
+class TridentAttention(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("q", "k", "v", "out", "lse", "grad", "dq", "dk", "dv", "offsets", "lengths")] + \
+               [(n, _i64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "rows", "sequences", "slots",
+                                    "q_heads", "kv_heads", "head_dim")] + \
+               [("scale", _f64)] + [(n, _i32) for n in ("dtype", "ids64", "causal")]
+
+
 # Stage boundaries recorded into TridentSearchOutputs.events (enum TridentStageEvent).
 EV_START, EV_PROBED, EV_GROUPED, EV_P1_SCAN, EV_P1_MERGE, EV_P2_SCAN, EV_END, EV_COUNT = range(8)
 
@@ -119,6 +126,11 @@ EXPORTS = {
     "trident_fp8_linear_workspace_bytes": (_size, [_i64, _i64, _i64]),
     "trident_fp8_linear": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _P, _P, _i64, _P, _i32, _P, _i64, _i32, _P,
                                           _size, _P]),
+    "trident_rotary": (ctypes.c_int, [_P, _i32, _i64, _i64, _i64, _i64, _i64, _P, _i64, _P, _i32, _i64, _i32, _f64, _i32,
+                                      _P, _i64, _i64, _P]),
+    "trident_attention": (ctypes.c_int, [ctypes.POINTER(TridentAttention), _P]),
+    "trident_attention_grad_workspace_bytes": (_size, [ctypes.POINTER(TridentAttention)]),
+    "trident_attention_grad": (ctypes.c_int, [ctypes.POINTER(TridentAttention), _P, _size, _P]),
     "trident_last_error": (ctypes.c_char_p, []),
     "trident_abi_version": (ctypes.c_int, []),
 }

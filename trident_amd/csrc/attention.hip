@@ -1,0 +1,268 @@
+// Attention of every token over its own sequence,
+//
+//   S = scale q k^T,   P = softmax over the row's keys (causal: those up to the row),   out = P v,
+//
+// with sequences packed one after another or padded to one length, and query heads in groups that share a
+// key and value head.  A workgroup takes a tile of queries of one head and passes over the keys once: tiles of keys and
+// values go straight from memory to LDS, the next one while this one is multiplied, and each row keeps a running
+// reference value and sum.
+#include "attention.hpp"
+
+namespace trident {
+namespace {
+
+// The scores are computed transposed, keys by queries, so a lane holds one query: its maximum and sum are of
+// its own registers and one other lane's, and exp(S) is the second operand of the product with the values as it is
+// (mfma.hpp).  P is rounded to the elements' type for that product, relative to a reference that the row's largest score exceeds by
+// at most 2^kSlack: the accumulators are only scaled when it would be more.  float16's small exponents are used
+// by holding P times 2^kShift, so that probabilities of 2^-21 are still held in full.
+template <typename T>
+constexpr float kShift = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
+constexpr float kSlack = 8.0f;
+
+template <typename T, int DP, int WAVES, int QB>
+__global__ __launch_bounds__(WAVES* kWave) void attention_kernel(AttentionArgs a) {
+    constexpr int BM = WAVES * QB * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
+    constexpr int KB = BN / 32;
+    using L = Tile<T, kPitch>;
+    extern __shared__ __align__(16) uint8_t lds[];  // [2][keys, values]
+    const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles, hk = h / (a.Hq / a.Hkv);
+    SequenceTile t;
+    if (!find_tile(a, a.causal ? a.tiles - 1 - tile : tile, BM, &t)) return;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
+    const int64_t out_row = (int64_t)a.Hq * a.D;
+    T* out = static_cast<T*>(a.out) + t.start * out_row + (int64_t)h * a.D;
+    const int live = min(t.first + BM, t.length);  // rows past it are slots without a token
+    if (live < t.first + BM) zero_rows(out, out_row, max(live, t.first), min(t.first + BM, t.extent), a.D, WAVES * kWave);
+    if (live <= t.first) return;
+
+    const uint8_t* k = static_cast<const uint8_t*>(a.k) + t.start * a.k_row + hk * a.k_head;
+    const uint8_t* v = static_cast<const uint8_t*>(a.v) + t.start * a.v_row + hk * a.v_head;
+    const int bytes = a.D * (int)sizeof(T);
+    const auto fetch = [&](int n) {
+        uint8_t* to = lds + n % 2 * 2 * kTile;
+        fetch_tile<T, kPitch, BN, WAVES>(to, k + (int64_t)n * BN * a.k_row, a.k_row, t.length - n * BN, bytes, wave);
+        fetch_tile<T, kPitch, BN, WAVES>(to + kTile, v + (int64_t)n * BN * a.v_row, a.v_row, t.length - n * BN, bytes,
+                                         wave);
+    };
+    fetch(0);
+
+    int row[QB];
+    frag<T> q[QB][DP / 16];
+    f32x16 acc[QB][DP / 32] = {};
+    float top[QB], sum[QB];  // the reference, times scale2, and this half's part of the sum
+    const int first = t.first + wave * QB * 32;
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        row[b] = first + b * 32 + (lane & 31);
+        load_row<T, DP>(static_cast<const uint8_t*>(a.q) + (t.start + min(row[b], t.length - 1)) * a.q_row + h * a.q_head,
+                        a.D, q[b]);
+        top[b] = -INFINITY;
+        sum[b] = 0.0f;
+    }
+    const int last = first + QB * 32 - 1;
+    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    for (int n = 0; n < tiles; ++n) {
+        wait_and_meet<0>();  // this tile is there, and every wave is done with the other one
+        if (n + 1 < tiles) fetch(n + 1);
+        if (first >= live || (a.causal && n * BN > last)) continue;
+        const lds_bytes keys = base + n % 2 * 2 * kTile, values = keys + kTile;
+        f32x16 s[KB][QB] = {};
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                const frag<T> f = L::row_frag(keys, kb * 32 + (lane & 31), i);
+#pragma unroll
+                for (int b = 0; b < QB; ++b) s[kb][b] = mma<T>(f, q[b][i], s[kb][b]);
+            }
+        if ((n + 1) * BN > t.length || (a.causal && (n + 1) * BN - 1 > first)) {
+#pragma unroll
+            for (int b = 0; b < QB; ++b) {
+                const int end = a.causal ? min(row[b] + 1, t.length) : t.length;
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (n * BN + kb * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[kb][b][i] = -INFINITY;
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < QB; ++b) {
+            float m = s[0][b][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kb][b][i]);
+            m = fmaxf(m, other_half(m)) * a.scale2;
+            if (__any(m > top[b] + kSlack)) {
+                const float by = m > top[b] ? __builtin_amdgcn_exp2f(top[b] - m) : 1.0f;
+                top[b] = fmaxf(m, top[b]);
+                sum[b] *= by;
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[b][j][i] *= by;
+            }
+            const float from = top[b] == -INFINITY ? 0.0f : kShift<T> - top[b];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][b][i], a.scale2, from));
+                    sum[b] += e;
+                    s[kb][b][i] = e;
+                }
+        }
+        // causal: blocks past the last row are left out, those on the diagonal looked at first
+        const bool edge = a.causal && (n + 1) * BN - 1 > first;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const int key = n * BN + kb * 32;
+            if (edge && key > last) continue;
+            const bool apart = edge && key >= first && any_not_finite<T, kPitch>(values + kb * 32 * kPitch);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                frag<T> p[QB];
+#pragma unroll
+                for (int b = 0; b < QB; ++b)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) p[b][e] = (T)s[kb][b][8 * i + e];
+                if (apart) {
+#pragma unroll
+                    for (int b = 0; b < QB; ++b)
+                        add_seen_rows<T, kPitch, DP>(values, kb * 32 + i * 16, p[b], acc[b],
+                                                     [&](int r) { return key + i * 16 + r <= row[b]; });
+                    continue;
+                }
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    const frag<T> f = L::col_frag(values, kb * 32 + i * 16, j * 32);
+#pragma unroll
+                    for (int b = 0; b < QB; ++b) acc[b][j] = mma<T>(f, p[b], acc[b][j]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int b = 0; b < QB; ++b) {
+        const float all = sum[b] + other_half(sum[b]);
+        if (row[b] >= live) continue;
+        store_column<T, DP>(out + (int64_t)row[b] * out_row, a.D, acc[b], 1.0f / all);
+        if (a.lse && half == 0)
+            a.lse[h * a.rows + t.start + row[b]] = top[b] - kShift<T> + __builtin_amdgcn_logf(all);
+    }
+}
+
+template <typename T, int DP, int WAVES, int QB>
+int launch(AttentionArgs a, hipStream_t st) {
+    constexpr int BM = WAVES * QB * 32;
+    constexpr size_t lds = 4 * (size_t)kTileRows<T> * kTilePitch<T, DP>;
+    const auto kernel = attention_kernel<T, DP, WAVES, QB>;
+    static_assert(lds <= 163840, "LDS of a CU");
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(attention): %s", hipGetErrorString(e));
+    }
+    const int64_t tiles = a.slots ? a.count * ((a.slots + BM - 1) / BM) : a.rows / BM + a.count + 2;
+    if (tiles * a.Hq > 0x7fffffff) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention: too many tiles");
+    a.tiles = (int)tiles;
+    kernel<<<(unsigned)(tiles * a.Hq), WAVES * kWave, lds, st>>>(a);
+    return capi_check_launch("attention_kernel");
+}
+
+template <typename T, int DP>
+int by_length(const AttentionArgs& a, hipStream_t st) {
+    const int64_t mean = a.slots ? a.slots : a.rows / std::max<int64_t>(a.count, 1);
+    if (mean <= 32) return launch<T, DP, 1, 1>(a, st);
+    return launch<T, DP, 4, 1>(a, st);
+}
+
+}  // namespace
+
+// Strides are those of 16-byte pieces, so that rows go to LDS whole.
+int attention_check(const TridentAttention* t, bool backward, AttentionArgs* a) {
+    const char* name = backward ? "attention_grad" : "attention";
+    if (!t) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: NULL arguments", name);
+    if (!dtype_ok(t->dtype)) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: dtype=%d", name, t->dtype);
+    if (t->rows < 0 || t->rows > (1 << 30) || t->sequences < 0 || t->sequences > (1 << 30) || t->slots < 0 ||
+        t->slots > (1 << 30) || t->q_heads < 1 || t->kv_heads < 1 || t->q_heads > (1 << 15) ||
+        t->q_heads % t->kv_heads || t->head_dim < 1)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "%s: bad sizes rows=%lld sequences=%lld slots=%lld q_heads=%lld kv_heads=%lld head_dim=%lld", name,
+                         (long long)t->rows, (long long)t->sequences, (long long)t->slots, (long long)t->q_heads,
+                         (long long)t->kv_heads, (long long)t->head_dim);
+    if (t->head_dim > kMaxHeadDim || t->head_dim % 8)
+        return capi_fail(TRIDENT_ERR_UNSUPPORTED, "%s: head_dim=%lld is not a multiple of 8 up to %d", name,
+                         (long long)t->head_dim, kMaxHeadDim);
+    if (t->slots ? t->sequences * t->slots != t->rows || t->offsets : t->lengths != nullptr)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "%s: %lld rows are not %lld sequences of %lld slots, or offsets and lengths do not go with them",
+                         name, (long long)t->rows, (long long)t->sequences, (long long)t->slots);
+    if (!(t->scale > 0.0) || !(t->scale < 1e30))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: scale=%g", name, t->scale);
+    const int64_t es = t->dtype == TRIDENT_F32 ? 4 : 2;
+    const int64_t strides[6] = {t->q_row, t->q_head, t->k_row, t->k_head, t->v_row, t->v_head};
+    for (int i = 0; i < 6; ++i)
+        if (strides[i] < (i % 2 ? 0 : t->head_dim) || strides[i] * es % 16 || strides[i] > (i % 2 ? (int64_t)1 << 40 : (1 << 24) / es))
+            return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: stride %lld", name, (long long)strides[i]);
+    *a = {};
+    if (t->rows == 0) return TRIDENT_OK;
+    if (!t->q || !t->k || !t->v || !t->out || (!t->slots && !t->offsets) ||
+        (backward && (!t->lse || !t->grad || !t->dq || !t->dk || !t->dv)))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: NULL pointer", name);
+    const void* all[] = {t->q, t->k, t->v, t->out, t->grad, t->dq, t->dk, t->dv};
+    for (const void* p : all)
+        if (reinterpret_cast<uintptr_t>(p) & 15)
+            return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: tensors must be 16-byte aligned", name);
+    a->q = t->q;
+    a->k = t->k;
+    a->v = t->v;
+    a->grad = t->grad;
+    a->out = t->out;
+    a->dq = t->dq;
+    a->dk = t->dk;
+    a->dv = t->dv;
+    a->lse = t->lse;
+    a->offsets = t->offsets;
+    a->lengths = t->lengths;
+    a->q_row = t->q_row * es;
+    a->q_head = t->q_head * es;
+    a->k_row = t->k_row * es;
+    a->k_head = t->k_head * es;
+    a->v_row = t->v_row * es;
+    a->v_head = t->v_head * es;
+    a->rows = t->rows;
+    a->count = t->sequences;
+    a->slots = (int)t->slots;
+    a->wide = t->ids64;
+    a->Hq = (int)t->q_heads;
+    a->Hkv = (int)t->kv_heads;
+    a->D = (int)t->head_dim;
+    a->causal = t->causal != 0;
+    a->scale = (float)t->scale;
+    a->scale2 = (float)(t->scale * 1.4426950408889634);
+    return TRIDENT_OK;
+}
+
+}  // namespace trident
+
+using namespace trident;
+
+extern "C" int trident_attention(const TridentAttention* t, void* stream) {
+    AttentionArgs a;
+    const int rc = attention_check(t, false, &a);
+    if (rc != TRIDENT_OK || t->rows == 0) return rc;
+    int out = TRIDENT_OK;
+    with_dtype(t->dtype, [&](auto e) {
+        using T = decltype(e);
+        const hipStream_t st = (hipStream_t)stream;
+        if (a.D <= 32) out = by_length<T, 32>(a, st);
+        else if (a.D <= 64) out = by_length<T, 64>(a, st);
+        else if (a.D <= 96) out = by_length<T, 96>(a, st);
+        else out = by_length<T, 128>(a, st);
+    });
+    return out;
+}

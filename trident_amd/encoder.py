@@ -4,9 +4,13 @@
   layer_norm, layer_norm_forward / _grad
   AdamW                                one launch per step for up to 88 tensors, states in 32 or 8 bits
   quantize_fp8, fp8_matmul, fp8_linear products in 8-bit floating point, one scale per row and 128 columns
+  rotary, rotary_frequencies           queries and keys turned by their positions
+  attention, attention_forward / _grad over packed or padded sequences, full or causal, grouped heads
+  gated_linear, gated_linear_forward / _grad
+                                       the gated half of a feed-forward block: act(x Wg^T) * (x Wu^T)
 
-``embedding`` and ``layer_norm`` take part in autograd; the ``*_forward`` / ``*_grad`` functions are the
-bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors with a
+``embedding``, ``layer_norm``, ``rotary``, ``attention`` and ``gated_linear`` take part in autograd; the
+``*_forward`` / ``*_grad`` functions are the bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors with a
 forward-mode tangent are refused.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics
 and states are float32 and every result is rounded once.  Each call runs on the current stream of its
 tensors' device, with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a
@@ -19,6 +23,7 @@ The reference has no counterpart: its vectors come from data sets.  The kernels 
 from typing import Iterable, List, NamedTuple, Optional, Sequence, Tuple
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -624,3 +629,305 @@ def fp8_linear(x: torch.Tensor, weight: Fp8Blocks, bias: Optional[torch.Tensor] 
     _call_ws(x.device, index, "trident_fp8_linear", _fn("trident_fp8_linear_workspace_bytes")(M, N, K), xr.data_ptr(),
              code, M, K, ld, codes.data_ptr(), scales.data_ptr(), N, bptr, bcode, out.data_ptr(), N or 1, fast_accum)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# rotary positions
+
+
+def rotary_frequencies(dim: int, base: float = 10000.0, scaling: str = "none", factor: float = 1.0,
+                       trained: int = 0, low: float = 1.0, high: float = 32.0, device=None) -> torch.Tensor:
+    """Radians a position for each of ``dim / 2`` pairs of columns, float64: ``base ** (-2 i / dim)``, scaled
+    for contexts ``factor`` times as long as those the model was trained on:
+
+      "linear"  all divided by the factor
+      "base"    the base grows by ``factor ** (dim / (dim - 2))``: the last pair's is divided by the factor, the
+                first one's stays
+      "turns"   a pair that turns less than ``low`` times over the ``trained`` positions is divided by the factor, one
+                that turns more than ``high`` times stays, those between by the share of the way
+    """
+    if dim < 2 or dim % 2:
+        _refuse(f"dim must be even and positive, got {dim}")
+    if not base > 0.0 or not factor > 0.0:
+        _refuse(f"base and factor must be positive, got {base} and {factor}")
+    if scaling not in ("none", "linear", "base", "turns"):
+        _refuse(f"scaling must be none, linear, base or turns, got {scaling!r}")
+    if scaling == "turns" and not (trained > 0 and low < high):
+        _refuse(f"turns scaling needs trained positions and low < high, got {trained}, {low} and {high}")
+    if scaling == "base":
+        if dim == 2:
+            _refuse("base scaling needs more than one pair")
+        base = base * factor ** (dim / (dim - 2))
+    f = [base ** (-2.0 * i / dim) for i in range(dim // 2)]
+    if scaling == "linear":
+        f = [w / factor for w in f]
+    elif scaling == "turns":
+        keep = [min(1.0, max(0.0, (trained * w / (2 * math.pi) - low) / (high - low))) for w in f]
+        f = [w * k + w / factor * (1.0 - k) for w, k in zip(f, keep)]
+    return torch.tensor(f, dtype=torch.float64, device=device)
+
+
+def _heads(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """(t [..., H, D] or a copy, in which a token's elements are next to each other in every head and all tokens
+    are one stride apart; that stride; the heads')."""
+    shape, stride = t.shape, t.stride()
+    if t.is_contiguous():
+        return t, shape[-2] * shape[-1], shape[-1]
+    ok, row, tokens = stride[-1] == 1 or shape[-1] == 1, None, 1
+    for n, st in zip(reversed(shape[:-2]), reversed(stride[:-2])):
+        if n == 1:
+            continue
+        if row is None:
+            row = st
+        ok &= st == row * tokens
+        tokens *= n
+    if not ok:
+        t = t.contiguous()
+        return t, shape[-2] * shape[-1], shape[-1]
+    return t, shape[-2] * shape[-1] if row is None else row, stride[-2] if shape[-2] > 1 else shape[-1]
+
+
+def _apart(row: int, head: int, heads: int, D: int) -> bool:
+    """Whether no two elements of a tensor of such strides share their place."""
+    return (head >= D and row >= (heads - 1) * head + D) or (row >= D and head >= row) or heads == 1 and row >= D
+
+
+def _rotary(x, frequencies, positions, interleaved, amplitude, inverse, out):
+    code, index, shape = _DTYPES.get(x.dtype), x.get_device(), x.shape
+    if code is None or index < 0 or len(shape) < 2 or shape[-1] == 0:
+        _dtype("x", x)
+        _gpu("x", x)
+        _refuse(f"x must be [..., heads, head_dim], got {tuple(shape)}")
+    H, D = shape[-2], shape[-1]
+    tokens = shape[:-2].numel()
+    if frequencies.dtype is not torch.float64 or frequencies.dim() != 1 or 2 * frequencies.numel() > D or \
+            not frequencies.is_contiguous() or frequencies.get_device() != index:
+        _refuse(f"frequencies must be contiguous float64 of at most {D // 2} pairs on cuda:{index}, got "
+                f"{frequencies.dtype} {tuple(frequencies.shape)} on {frequencies.device}")
+    wide, pos, period = 0, None, shape[-3] if len(shape) > 2 else 1
+    if positions is not None:
+        wide, period = _ID_TYPES.get(positions.dtype), positions.numel()
+        if wide is None or positions.shape not in (shape[:-2], shape[-3:-2]):
+            _refuse(f"positions must be int64 or int32 {tuple(shape[:-2])} or {tuple(shape[-3:-2])}, got "
+                    f"{positions.dtype} {tuple(positions.shape)}")
+        _same(index, "positions", positions)
+        if not positions.is_contiguous():
+            positions = positions.contiguous()
+        pos = positions.data_ptr()
+    xr, row, head = _heads(x)
+    if out is None:
+        y, out_row, out_head = x.new_empty(shape), H * D, D
+    else:
+        if out.dtype is not x.dtype or out.shape != shape or out.get_device() != index:
+            _refuse(f"out must be {tuple(shape)} {x.dtype} on cuda:{index}")
+        y, out_row, out_head = _heads(out)
+        if y is not out or (tokens > 1 and not _apart(out_row, out_head, H, D)) or (H > 1 and out_head < D):
+            _refuse("out must have its tokens one stride apart, and no two elements in one place")
+        if out.data_ptr() == x.data_ptr() and (xr is not x or (out_row, out_head) != (row, head)):
+            _refuse("out begins where x does: then it must be x, with the same strides")
+        if (x.requires_grad or out.requires_grad) and torch.is_grad_enabled():
+            _refuse("out= has no gradient: call it under torch.no_grad()")
+    _call(index, "trident_rotary", xr.data_ptr(), code, tokens, H, D, row, head, frequencies.data_ptr(),
+          frequencies.numel(), pos, wide, max(period, 1), interleaved, amplitude, inverse, y.data_ptr(), out_row,
+          out_head)
+    if out is not None:
+        _increment_version([out])
+        return out
+    return y
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, frequencies, positions, interleaved, amplitude, inverse):
+        ctx.save_for_backward(frequencies, positions)
+        ctx.how = interleaved, amplitude, inverse
+        return _rotary(x, frequencies, positions, interleaved, amplitude, inverse, None)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        frequencies, positions = ctx.saved_tensors
+        interleaved, amplitude, inverse = ctx.how
+        return (_rotary(grad, frequencies, positions, interleaved, amplitude, not inverse, None),) + (None,) * 5
+
+
+def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch.Tensor] = None,
+           interleaved: bool = False, amplitude: float = 1.0, inverse: bool = False,
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``x`` [..., heads, head_dim] with the first ``2 * len(frequencies)`` columns of each head turned by
+    ``position * frequency``, pair by pair, and multiplied by ``amplitude``; the other columns as they are.
+
+    Pair i is columns i and i + pairs, or 2 i and 2 i + 1 (``interleaved``).  ``positions`` (int32 or int64,
+    any value) are the tokens', [...], or those of the last token dimension, shared by the others; without
+    them a token's position is its index there.  Angles are made in float64.  Queries and keys that lie in one
+    tensor are one call: ``rotary(qkv[:, :q_heads + k_heads], ...)``.  ``inverse`` turns back, by the same
+    amplitude: it is the gradient.  ``out`` may be ``x`` (in place) or not overlap it, and has no gradient."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("rotary", x)
+    if out is None and x.requires_grad and torch.is_grad_enabled():
+        return _Rotary.apply(x, frequencies, positions, bool(interleaved), float(amplitude), bool(inverse))
+    return _rotary(x, frequencies, positions, bool(interleaved), float(amplitude), bool(inverse), out)
+
+
+# ---------------------------------------------------------------------------------------------
+# attention
+
+
+def _strided_heads(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
+    """_heads, in pieces of 16 bytes."""
+    t, row, head = _heads(t)
+    per = 16 // t.element_size()
+    if row % per or head % per or t.data_ptr() % 16 or row < t.shape[-1] or row > (1 << 24) // t.element_size() or \
+            head < 0:
+        t = t.clone(memory_format=torch.contiguous_format)
+        row, head = t.shape[-2] * t.shape[-1], t.shape[-1]
+    return t, row, head
+
+
+def _attention_args(q, k, v, offsets, lengths, causal, scale):
+    """(TridentAttention without results, what it points to, the device's index)"""
+    code, index, shape = _DTYPES.get(q.dtype), q.get_device(), q.shape
+    if code is None or index < 0:
+        _dtype("q", q)
+        _gpu("q", q)
+    padded = len(shape) == 4
+    if len(shape) not in (3, 4) or k.shape != v.shape or k.dim() != len(shape) or k.shape[:-2] != shape[:-2] or \
+            k.shape[-1] != shape[-1]:
+        _refuse("q, k and v must be [rows, heads, head_dim] or [sequences, slots, heads, head_dim], k and v alike, got "
+                f"{tuple(shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    Hq, Hkv, D = shape[-2], k.shape[-2], shape[-1]
+    if Hkv == 0 or Hq == 0 or Hq % Hkv or Hq > 32768:
+        _refuse(f"{Hq} query heads do not go by {Hkv} key and value heads")
+    if D == 0 or D % 8 or D > 128:
+        _refuse(f"head_dim must be a multiple of 8 up to 128, got {D}")
+    for name, t in (("k", k), ("v", v)):
+        if t.dtype is not q.dtype:
+            _refuse(f"{name} must be {q.dtype} as q, got {t.dtype}")
+        _same(index, name, t)
+    rows = shape[:-2].numel()
+    wide, where, sequences, slots = 0, None, 1, 0
+    if padded:
+        sequences, slots = shape[0], shape[1]
+        if offsets is not None:
+            _refuse("padded sequences have lengths, not offsets")
+        if lengths is not None:
+            wide, where = _sequence_ids("lengths", lengths, index)
+            if where.shape != (sequences,):
+                _refuse(f"lengths must be [{sequences}], got {tuple(where.shape)}")
+    else:
+        if lengths is not None:
+            _refuse("packed sequences have offsets, not lengths")
+        if offsets is not None:
+            wide, where = _sequence_ids("offsets", offsets, index)
+            if where.dim() != 1 or where.numel() < 1:
+                _refuse(f"offsets must be [sequences + 1], got {tuple(where.shape)}")
+            sequences = where.numel() - 1
+        else:  # one sequence
+            slots = rows
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        _refuse(f"scale must be positive, got {scale}")
+    (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = map(_strided_heads, (q, k, v))
+    ids = None if where is None else where.data_ptr()
+    a = _lib.TridentAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, None, None, None, None,
+                              ids if slots == 0 else None, ids if slots else None, q_row, q_head, k_row, k_head, v_row,
+                              v_head, rows, sequences, slots, Hq, Hkv, D, scale, code, wide, causal)
+    return a, (q, k, v, where), index
+
+
+def _sequence_ids(name: str, t: torch.Tensor, index: int) -> Tuple[int, torch.Tensor]:
+    wide = _ID_TYPES.get(t.dtype)
+    if wide is None:
+        _refuse(f"{name} must be int64 or int32, got {t.dtype}")
+    _same(index, name, t)
+    return wide, t if t.is_contiguous() else t.contiguous()
+
+
+def _attend(q, k, v, offsets, lengths, causal, scale, keep):
+    a, kept, index = _attention_args(q, k, v, offsets, lengths, causal, scale)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((q.shape[-2], a.rows), dtype=torch.float32) if keep else None
+    a.out = out.data_ptr()
+    if keep:
+        a.lse = lse.data_ptr()
+    if a.rows:
+        _call(index, "trident_attention", ctypes.byref(a))
+    return out, lse
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, offsets, lengths, causal, scale):
+        out, lse = _attend(q, k, v, offsets, lengths, causal, scale, True)
+        ctx.save_for_backward(q, k, v, out, lse, offsets, lengths)
+        ctx.how = causal, scale
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        q, k, v, out, lse, offsets, lengths = ctx.saved_tensors
+        return *attention_grad(grad, q, k, v, out, lse, offsets, lengths, *ctx.how), None, None, None, None
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+              lengths: Optional[torch.Tensor] = None, causal: bool = False, scale: Optional[float] = None) -> torch.Tensor:
+    """``softmax(scale * q k^T) v`` of every token over the tokens of its own sequence, or, ``causal``, over
+    those up to itself.
+
+    Packed: q [rows, q_heads, head_dim], k and v [rows, kv_heads, head_dim], sequence i being rows ``offsets[i]``
+    to ``offsets[i + 1] - 1`` (ascending, [sequences + 1]; without offsets all rows are one).  Padded: q, k and v
+    [sequences, slots, heads, head_dim], sequence i being the first ``lengths[i]`` of its slots (without lengths all).
+    Offsets and lengths are int32 or int64 on the device, so no call can check them; values outside the rows are
+    brought inside.  Rows without a token, and sequences of no tokens, are allowed: what they hold is never used, and they
+    get zeros.  Within a sequence a value that is not finite shows wherever the formula has it, in causal attention not before its own token.
+
+    head_dim is a multiple of 8 up to 128; q_heads a multiple of kv_heads (query head h takes key head h //
+    (q_heads // kv_heads)).  ``scale`` is 1 / sqrt(head_dim) if not given.  Strided views, such as parts of one projection's
+    result, are taken as they are where their strides are whole pieces of 16 bytes.  Scores, softmax and sums are
+    float32; probabilities are rounded to the tensors' type for the product with v."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("attention", q, k, v)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _Attention.apply(q, k, v, offsets, lengths, bool(causal), scale)
+    return _attend(q, k, v, offsets, lengths, bool(causal), scale, False)[0]
+
+
+def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Optional[torch.Tensor] = None,
+                      lengths: Optional[torch.Tensor] = None, causal: bool = False,
+                      scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse): attention and, for the backward pass, the base-2 logarithm of each row's sum of
+    ``exp(scale * q k^T)``, float32 [q_heads, rows] (undefined for rows without a token)."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("attention_forward", q, k, v)
+    return _attend(q, k, v, offsets, lengths, bool(causal), scale, True)
+
+
+def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                   lse: torch.Tensor, offsets: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+                   causal: bool = False, scale: Optional[float] = None):
+    """(dq, dk, dv) from the gradient of ``out``, what ``attention_forward`` took and what it gave.  Those of k
+    and v are sums over the query heads of their group."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("attention_grad", grad, q, k, v, out, lse)
+    a, kept, index = _attention_args(q, k, v, offsets, lengths, bool(causal), scale)
+    for name, t in (("grad", grad), ("out", out)):
+        if t.shape != q.shape or t.dtype is not q.dtype:
+            _refuse(f"{name} must be {tuple(q.shape)} {q.dtype}, got {tuple(t.shape)} {t.dtype}")
+        _same(index, name, t)
+    if lse.shape != (q.shape[-2], a.rows) or lse.dtype is not torch.float32 or not lse.is_contiguous():
+        _refuse(f"lse must be contiguous float32 {(q.shape[-2], a.rows)}, got {lse.dtype} {tuple(lse.shape)}")
+    _same(index, "lse", lse)
+    grad, out = _whole(grad), _whole(out)
+    dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    a.grad, a.out, a.lse = grad.data_ptr(), out.data_ptr(), lse.data_ptr()
+    a.dq, a.dk, a.dv = dq.data_ptr(), dk.data_ptr(), dv.data_ptr()
+    if a.rows:
+        at = ctypes.byref(a)
+        _call_ws(q.device, index, "trident_attention_grad", _fn("trident_attention_grad_workspace_bytes")(at), at)
+    return dq, dk, dv
+
+
+def _whole(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy, contiguous from a 16-byte address on."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
