@@ -412,6 +412,30 @@ int trident_attention(const TridentAttention* a, void* stream);
 size_t trident_attention_grad_workspace_bytes(const TridentAttention* a);
 int trident_attention_grad(const TridentAttention* a, void* workspace, size_t workspace_bytes, void* stream);
 
+/* The gated half of a feed-forward block: h [M, N] = act(x gate_weight^T) * (x up_weight^T), x [M, K], both weights
+ * [N, K], rows of the given pitches in elements.  gate and up [M, N]: the two products, kept for the backward
+ * pass, or both NULL.  h, gate, up and the results of the backward pass are contiguous.  Rows that begin at 16-byte addresses
+ * and hold whole 16 bytes are taken as they are; the workspace is for others, and none for up to 16 rows. */
+enum TridentActivation { TRIDENT_SILU = 0, TRIDENT_GELU = 1, TRIDENT_GELU_TANH = 2 };
+
+typedef struct TridentGated {
+    const void *x, *gate_weight, *up_weight;
+    void *h, *gate, *up;
+    const void* grad;          /* of h: the backward pass's, as are the three below */
+    void *dx, *dgate_weight, *dup_weight;
+    int64_t M, N, K;
+    int64_t ld_x, ld_gate, ld_up, ld_grad;
+    int32_t dtype, activation;
+} TridentGated;
+
+size_t trident_gated_linear_workspace_bytes(const TridentGated* a);
+int trident_gated_linear(const TridentGated* a, void* workspace, size_t workspace_bytes, void* stream);
+
+/* dx, and dgate_weight with dup_weight, from grad, what the forward pass took and the gate and up that it kept.
+ * dx, or both of the others, may be NULL. */
+size_t trident_gated_linear_grad_workspace_bytes(const TridentGated* a);
+int trident_gated_linear_grad(const TridentGated* a, void* workspace, size_t workspace_bytes, void* stream);
+
 const char* trident_last_error(void);
 int trident_abi_version(void);
 

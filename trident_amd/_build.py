@@ -30,8 +30,8 @@ OUT_DIR = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libtrident_hip.so")
 SOURCES = ["frontend.hip", "scan.hip", "batch.hip", "cm.hip", "capi.hip",
            "embedding.hip", "layernorm.hip", "adamw.hip", "fp8mm.hip",
-           "rotary.hip", "attention.hip", "attention_grad.hip"]
-# Per-source flags.  batch.hip, cm.hip, frontend.hip, fp8mm.hip, attention*.hip: matrix-core results in VGPRs (no
+           "rotary.hip", "attention.hip", "attention_grad.hip", "gated.hip"]
+# Per-source flags.  batch.hip, cm.hip, frontend.hip, fp8mm.hip, attention*.hip, gated.hip: matrix-core results in VGPRs (no
 # accumulator-register reads in the per-tile epilogues; the coarse pass gains 13 us at configs[4]);
 # batch.hip: no atomic optimizer (it turns the one-lane work-counter atomic into a wave-wide one
 # whose result is waited for at once, which would undo taking the next unit early).
@@ -40,7 +40,7 @@ EXTRA = {"batch.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1",
          "cm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
          "frontend.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
          **{s: ["-mllvm", "-amdgpu-mfma-vgpr-form=1"] for s in
-            ("fp8mm.hip", "attention.hip", "attention_grad.hip")}}
+            ("fp8mm.hip", "attention.hip", "attention_grad.hip", "gated.hip")}}
 HEADERS = ["common.hpp", "kernels.hpp", "encoder.hpp", "mfma.hpp", "attention.hpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

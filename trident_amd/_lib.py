@@ -83,6 +83,16 @@ class TridentAttention(ctypes.Structure):
                [("scale", _f64)] + [(n, _i32) for n in ("dtype", "ids64", "causal")]
 
 
+class TridentGated(ctypes.Structure):
+    _fields_ = [(n, _P) for n in ("x", "gate_weight", "up_weight", "h", "gate", "up", "grad", "dx", "dgate_weight",
+                                  "dup_weight")] + \
+               [(n, _i64) for n in ("M", "N", "K", "ld_x", "ld_gate", "ld_up", "ld_grad")] + \
+               [("dtype", _i32), ("activation", _i32)]
+
+
+SILU, GELU, GELU_TANH = range(3)  # enum TridentActivation
+
+
 # Stage boundaries recorded into TridentSearchOutputs.events (enum TridentStageEvent).
 EV_START, EV_PROBED, EV_GROUPED, EV_P1_SCAN, EV_P1_MERGE, EV_P2_SCAN, EV_END, EV_COUNT = range(8)
 
@@ -131,6 +141,10 @@ EXPORTS = {
     "trident_attention": (ctypes.c_int, [ctypes.POINTER(TridentAttention), _P]),
     "trident_attention_grad_workspace_bytes": (_size, [ctypes.POINTER(TridentAttention)]),
     "trident_attention_grad": (ctypes.c_int, [ctypes.POINTER(TridentAttention), _P, _size, _P]),
+    "trident_gated_linear_workspace_bytes": (_size, [ctypes.POINTER(TridentGated)]),
+    "trident_gated_linear": (ctypes.c_int, [ctypes.POINTER(TridentGated), _P, _size, _P]),
+    "trident_gated_linear_grad_workspace_bytes": (_size, [ctypes.POINTER(TridentGated)]),
+    "trident_gated_linear_grad": (ctypes.c_int, [ctypes.POINTER(TridentGated), _P, _size, _P]),
     "trident_last_error": (ctypes.c_char_p, []),
     "trident_abi_version": (ctypes.c_int, []),
 }

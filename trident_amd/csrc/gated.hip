@@ -1,0 +1,625 @@
+// The gated half of a feed-forward block and its backward pass,
+//
+//   g = x Wg^T,   u = x Wu^T,   h = act(g) u
+//   dg = dh u act'(g),   du = dh act(g),   dx = dg Wg + du Wu,   dWg = dg^T x,   dWu = du^T x
+//
+// with x [M, K], Wg and Wu [N, K], all row-major.  One kernel of tiles computes every product: an operand's tile is read by
+// rows where the summed axis is its columns (x, Wg, Wu in the forward pass; dg, du in dx) and by columns where it is its
+// rows (Wg, Wu in dx; all of dWg, dWu).  Sums are float32; g and u are kept in the elements' type for the backward
+// pass, and dg, du are rounded to it for their products.
+#include <algorithm>
+
+#include "mfma.hpp"
+
+namespace trident {
+namespace {
+
+enum Activation { kSilu = TRIDENT_SILU, kGelu = TRIDENT_GELU, kGeluTanh = TRIDENT_GELU_TANH };
+
+// act(g), and act'(g) where SLOPE.
+template <bool SLOPE>
+__device__ __forceinline__ void activate(int kind, float g, float* value, float* slope) {
+    if (kind == kGelu) {
+        // g Phi(g); Phi by the complementary error function keeps its digits where it is small
+        const float p = 0.5f * erfcf(-0.70710678118654752f * g);
+        *value = g * p;
+        if constexpr (SLOPE)
+            *slope = __builtin_fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), p);
+        return;
+    }
+    // both others are g times a logistic: of g, or of 2 sqrt(2 / pi) (g + 0.044715 g^3)
+    const float g2 = g * g;
+    const float z = kind == kSilu ? g : 1.5957691216057308f * g * __builtin_fmaf(0.044715f, g2, 1.0f);
+    const float p = 1.0f / (1.0f + expf(-z));
+    *value = g * p;
+    if constexpr (SLOPE) {
+        const float dz = kind == kSilu ? 1.0f : 1.5957691216057308f * __builtin_fmaf(3 * 0.044715f, g2, 1.0f);
+        // 1 - p by its own quotient: no digits are lost where p is near 1
+        *slope = __builtin_fmaf(g * p * dz, 1.0f / (1.0f + expf(z)), p);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// products
+
+// An operand: rows of `pitch` bytes.  By rows, its rows are the tile's and its columns are summed over; by columns the
+// other way round.
+struct Operand {
+    const uint8_t* p;
+    int64_t pitch;
+};
+
+struct ProductArgs {
+    // out[m, n] = sum over k of second[m, k] first[n, k]; two sums one after another where there are second
+    // operands of both (dx), or first ones whose sums are kept apart (gate and up)
+    Operand first[2], second[2];
+    void* out[3];
+    int64_t ldo;       // elements
+    int M, N, K;       // rows and columns of the result, length of a sum
+    int parts;         // sums one after another
+    int tiles_m, tiles_n, activation;
+};
+
+// One of a grid's tiles in an order that keeps neighbours on one XCD: workgroups go to the eight XCDs, each
+// with its own L2, in turn, so each takes a contiguous eighth, in bands of 8 tile rows.
+__device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* tm, int* tn) {
+    constexpr int kBand = 8;
+    const int total = tiles_m * tiles_n, each = total / 8, more = total % 8;
+    const int xcd = id % 8, t = xcd * each + min(xcd, more) + id / 8;
+    const int first = t / (kBand * tiles_n) * kBand, rows = min(kBand, tiles_m - first);
+    const int in = t - first * tiles_n;
+    *tm = first + in % rows;
+    *tn = in / rows;
+}
+
+// How the first and the second operand are read.
+enum Reading { kRowsRows, kColumnsRows, kColumnsColumns };
+
+template <typename T>
+constexpr int kStep = 128 / (int)sizeof(T);  // of the summed axis in LDS at a time
+
+// A tile of `ROWS` operand rows (by columns: columns) and kStep of the summed axis, and its loads.
+template <typename T, bool COLUMNS, int ROWS, int WAVES>
+struct OperandTile {
+    static constexpr int kPitch = COLUMNS ? ROWS * (int)sizeof(T) : 128;
+    static constexpr int kBytes = ROWS * 128, kLoads = kBytes / 1024 / WAVES;
+    static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
+    using L = Tile<T, kPitch>;
+    const uint8_t* base;
+    int64_t pitch;
+    int length;          // of the summed axis
+    uint32_t at[kLoads]; // of this lane's piece in the first step
+
+    // rows `first` on of `limit`; those past it are zeros
+    __device__ __forceinline__ void start(const Operand& o, int first, int limit, int K, int wave) {
+        pitch = o.pitch;
+        length = K;
+        base = o.p + (COLUMNS ? (int64_t)first * sizeof(T) : first * o.pitch);
+        const int lane = lane_id(), in = lane / L::kPieces, slot = lane % L::kPieces;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            const int r = (i * WAVES + wave) * L::kRowsAtOnce + in, piece = slot ^ L::exchange(r);
+            const bool there = COLUMNS ? first + piece * (16 / (int)sizeof(T)) < limit : first + r < limit;
+            at[i] = there ? (uint32_t)r * (uint32_t)pitch + piece * 16 : kPastBuffer;
+        }
+    }
+    __device__ __forceinline__ void fetch(uint8_t* to, int step, int wave) const {
+        const int k = step * kStep<T>, left = length - k;
+        if constexpr (COLUMNS) {
+            const __amdgpu_buffer_rsrc_t buf =
+                buffer_of(base + k * pitch, (uint32_t)min(left, kStep<T>) * (uint32_t)pitch);
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(to + (i * WAVES + wave) * 1024), 16, at[i], 0, 0, 0);
+        } else {
+            const __amdgpu_buffer_rsrc_t buf = buffer_of(base + (int64_t)step * 128, 0x7fffffffu);
+            const int lane = lane_id(), slot = lane % L::kPieces;
+#pragma unroll
+            for (int i = 0; i < kLoads; ++i) {
+                uint32_t from = at[i];
+                if (left < kStep<T>) {  // columns past the last one are zeros
+                    const int r = (i * WAVES + wave) * L::kRowsAtOnce + lane / L::kPieces;
+                    if ((slot ^ L::exchange(r)) * (16 / (int)sizeof(T)) >= left) from = kPastBuffer;
+                }
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(to + (i * WAVES + wave) * 1024), 16, from, 0, 0, 0);
+            }
+        }
+    }
+    // eight steps 16 s + 8 half .. of this lane's row (column) `row`
+    static __device__ __forceinline__ frag<T> read(lds_bytes tile, int row, int s) {
+        if constexpr (COLUMNS) return L::col_frag_in_order(tile, 16 * s, row);
+        else return L::row_frag(tile, row + (lane_id() & 31), s);
+    }
+};
+
+// A workgroup of WM x WN waves computes WM MT x WN NT blocks of 32 x 32, a wave MT x NT.  A step's tiles of both operands go
+// straight from memory to LDS, the next step's while this one's are multiplied.  The first operand gives the result's columns,
+// so a lane holds four neighbours of a row.
+//
+// GATED: the first operand's tile is half gate, half up, and each wave's blocks too, so that a lane holds both sums
+// of the same places: out[0] = act(g) u, and g and u themselves where KEEP.
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
+__device__ __forceinline__ void product(const ProductArgs& a) {
+    constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32;
+    constexpr int BR = GATED ? BN / 2 : BN;  // the result's columns
+    using First = OperandTile<T, READ != kRowsRows, BR, kWaves>;
+    using Second = OperandTile<T, READ == kColumnsColumns, BM, kWaves>;
+    constexpr int kFirst = BN * 128, kStage = kFirst + Second::kBytes;
+    extern __shared__ __align__(16) uint8_t lds[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
+    int tm, tn;
+    tile_of(blockIdx.x, a.tiles_m, a.tiles_n, &tm, &tn);
+    const int m0 = tm * BM, n0 = tn * BR, z = blockIdx.y;  // z: one of two results of their own (dWg, dWu)
+    const int wm = wave / WN * MT * 32, wn = wave % WN * NT * 32;
+
+    First first[GATED ? 2 : 1];
+    Second second;
+    const auto begin = [&](int part) {
+        first[0].start(a.first[part], n0, a.N, a.K, wave);
+        if constexpr (GATED) first[1].start(a.first[1], n0, a.N, a.K, wave);
+        second.start(a.second[part + z], m0, a.M, a.K, wave);
+    };
+    const int each = (a.K + kStep<T> - 1) / kStep<T>, steps = each * a.parts;
+    const auto fetch = [&](int n) {
+        uint8_t* to = lds + n % 2 * kStage;
+        const int step = n < each ? n : n - each;
+        if (n == each) begin(1);
+        first[0].fetch(to, step, wave);
+        if constexpr (GATED) first[1].fetch(to + kFirst / 2, step, wave);
+        second.fetch(to + kFirst, step, wave);
+    };
+    begin(0);
+    fetch(0);
+
+    f32x16 acc[MT][NT] = {};
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    for (int n = 0; n < steps; ++n) {
+        wait_and_meet<0>();
+        if (n + 1 < steps) fetch(n + 1);
+        const lds_bytes t1 = base + n % 2 * kStage, t2 = t1 + kFirst;
+#pragma unroll
+        for (int s = 0; s < kStep<T> / 16; ++s) {
+            frag<T> f1[NT], f2[MT];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                if constexpr (GATED) {  // the wave's first half of blocks from the gate's tile
+                    f1[j] = First::read(t1 + (j < NT / 2 ? 0 : kFirst / 2), wn / 2 + j % (NT / 2) * 32, s);
+                } else {
+                    f1[j] = First::read(t1, wn + j * 32, s);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < MT; ++i) f2[i] = Second::read(t2, wm + i * 32, s);
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) acc[i][j] = mma<T>(f1[j], f2[i], acc[i][j]);
+        }
+    }
+    // Results go through LDS, 32 rows of a wave at a time, so that whole lines are written.
+    wait_and_meet<0>();
+    constexpr int kBlocks = GATED ? NT / 2 : NT, kCols = kBlocks * 32, kPitch = kCols * (int)sizeof(T) + 16;
+    constexpr int kPer = 16 / (int)sizeof(T), kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
+    static_assert(kWaves * 32 * kPitch <= 2 * kStage, "the results fit where the operands were");
+    uint8_t* mine = lds + wave * 32 * kPitch;
+    const int col = n0 + (GATED ? wn / 2 : wn) + lane % kRowPieces * kPer, left = a.N - col;
+    const auto put = [&](int i, void* out, auto&& value) {
+#pragma unroll
+        for (int j = 0; j < kBlocks; ++j)
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = value(j, 4 * p + e);
+                store_vec(reinterpret_cast<T*>(mine + (lane & 31) * kPitch) + j * 32 + p * 8 + half * 4, v);
+            }
+        wave_sync();
+#pragma unroll
+        for (int k = 0; k < 32; k += kRowsAtOnce) {
+            const int row = k + lane / kRowPieces, m = m0 + wm + i * 32 + row;
+            if (m >= a.M || left <= 0) continue;
+            const uint8_t* from = mine + row * kPitch + lane % kRowPieces * 16;
+            T* to = static_cast<T*>(out) + m * a.ldo + col;
+            if (left >= kPer) {
+                __builtin_memcpy(to, from, 16);
+            } else {
+                for (int e = 0; e < left; ++e) to[e] = reinterpret_cast<const T*>(from)[e];
+            }
+        }
+        wave_sync();
+    };
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        if constexpr (GATED) {
+            put(i, a.out[0], [&](int j, int e) {
+                float v;
+                activate<false>(a.activation, acc[i][j][e], &v, nullptr);
+                return v * acc[i][j + kBlocks][e];
+            });
+            if constexpr (KEEP) {
+                put(i, a.out[1], [&](int j, int e) { return acc[i][j][e]; });
+                put(i, a.out[2], [&](int j, int e) { return acc[i][j + kBlocks][e]; });
+            }
+        } else {
+            put(i, a.out[z], [&](int j, int e) { return acc[i][j][e]; });
+        }
+    }
+}
+
+// (A function of its own: with the body in the kernel template the compiler leaves out the host's half of some
+// instantiations.)
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
+__global__ __launch_bounds__(WM* WN* kWave) void product_kernel(ProductArgs a) {
+    product<T, READ, WM, WN, MT, NT, GATED, KEEP>(a);
+}
+
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED = false, bool KEEP = false>
+int launch_product(ProductArgs a, int results, hipStream_t st) {
+    constexpr int BM = WM * MT * 32, BN = WN * NT * 32, BR = GATED ? BN / 2 : BN;
+    constexpr size_t lds = 2 * (size_t)(BM + BN) * 128;
+    static_assert(lds <= 163840, "LDS of a CU");
+    const auto kernel = product_kernel<T, READ, WM, WN, MT, NT, GATED, KEEP>;
+    if (lds > 65536) {
+        const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+        if (e != hipSuccess) return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(product): %s", hipGetErrorString(e));
+    }
+    a.tiles_m = (a.M + BM - 1) / BM;
+    a.tiles_n = (a.N + BR - 1) / BR;
+    if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff)
+        return capi_fail(TRIDENT_ERR_UNSUPPORTED, "gated_linear: %d x %d is too large", a.M, a.N);
+    kernel<<<dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)results), WM * WN * kWave, lds, st>>>(a);
+    return capi_check_launch("product_kernel");
+}
+
+// ------------------------------------------------------------------------------------------------
+// the rest
+
+struct SlopeArgs {
+    const void *grad, *gate, *up;
+    void *dgate, *dup;
+    int64_t ld_grad, ld, pitch;  // of grad, of gate and up, of dgate and dup: elements
+    int64_t M;
+    int N, activation;
+};
+
+// dg and du: eight columns a thread, zeros from N up to the pitch.  Bound by bytes: three reads, two writes.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
+    const int pieces = (int)(a.pitch / 8);
+    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (at >= a.M * pieces) return;
+    const int64_t m = at / pieces;
+    const int col = (int)(at - m * pieces) * 8;
+    const T* dh = static_cast<const T*>(a.grad) + m * a.ld_grad + col;
+    const T* g = static_cast<const T*>(a.gate) + m * a.ld + col;
+    const T* u = static_cast<const T*>(a.up) + m * a.ld + col;
+    float fh[8], fg[8], fu[8], dg[8], du[8];
+    if (col + 8 <= a.N) {
+        load_vec<T, 8>(dh, fh);
+        load_vec<T, 8>(g, fg);
+        load_vec<T, 8>(u, fu);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool in = col + e < a.N;
+            fh[e] = in ? (float)dh[e] : 0.0f;
+            fg[e] = in ? (float)g[e] : 0.0f;
+            fu[e] = in ? (float)u[e] : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        float v, s;
+        activate<true>(a.activation, fg[e], &v, &s);
+        dg[e] = fh[e] * fu[e] * s;
+        du[e] = fh[e] * v;
+    }
+    store_vec<T, 8>(static_cast<T*>(a.dgate) + m * a.pitch + col, dg);
+    store_vec<T, 8>(static_cast<T*>(a.dup) + m * a.pitch + col, du);
+}
+
+// Rows copied to a pitch of whole pieces of 16 bytes, zeros behind: for operands whose rows do not begin at such
+// pieces, which LDS cannot take straight.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void pack_kernel(const T* from, int64_t ld, T* to, int64_t pitch, int64_t rows,
+                                                      int cols) {
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const int pieces = (int)(pitch / kPer);
+    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (at >= rows * pieces) return;
+    const int64_t r = at / pieces;
+    const int col = (int)(at - r * pieces) * kPer;
+    float f[kPer];
+    if (col + kPer <= cols) {
+        load_vec<T, kPer>(from + r * ld + col, f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) f[e] = col + e < cols ? (float)from[r * ld + col + e] : 0.0f;
+    }
+    store_vec<T, kPer>(to + r * pitch + col, f);
+}
+
+constexpr int kFewRows = 16;   // rows of x that one instruction takes
+constexpr int kFewWaves = 8;
+
+struct FewArgs {
+    const void *x, *gate, *up;
+    void* out[3];
+    int64_t ld_x, ld_gate, ld_up, ldo;
+    int M, N, K, activation;
+};
+
+typedef float f32x4v __attribute__((ext_vector_type(4)));
+
+template <typename T>
+__device__ __forceinline__ f32x4v mma16(const frag<T>& a, const frag<T>& b, f32x4v c) {
+    if constexpr (std::is_same<T, bf16_t>::value) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    else if constexpr (std::is_same<T, f16_t>::value) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+}
+
+// Eight elements from p on, those past `left` zeros; any element's address.
+template <typename T>
+__device__ __forceinline__ frag<T> load_eight(const T* p, int left) {
+    frag<T> f = {};
+    if (left >= 8) {
+        __builtin_memcpy(&f, p, sizeof(f));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) f[e] = p[e];
+    }
+    return f;
+}
+
+// Up to 16 rows, such as a query's: a workgroup takes 16 columns of gate and up, and its waves share K by blocks of 64.
+// Bound by the bytes of the weights, each of which one wave reads once, straight to registers: rows of 16 lanes' pieces.
+template <typename T, bool KEEP>
+__global__ __launch_bounds__(kFewWaves* kWave) void few_kernel(FewArgs a) {
+    __shared__ f32x4v s_acc[2][kFewWaves][kWave];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int r = lane % 16, quarter = lane / 16;
+    const int n0 = blockIdx.x * 16, n = min(n0 + r, a.N - 1), m = min(r, a.M - 1);
+    const T* x = static_cast<const T*>(a.x) + m * a.ld_x;
+    const T* wg = static_cast<const T*>(a.gate) + n * a.ld_gate;
+    const T* wu = static_cast<const T*>(a.up) + n * a.ld_up;
+    f32x4v g = {}, u = {};
+    for (int k = wave * 64; k < a.K; k += kFewWaves * 64) {
+        frag<T> fg[2], fu[2], fx[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int at = k + i * 32 + quarter * 8, left = a.K - at;
+            fg[i] = load_eight(wg + at, left);
+            fu[i] = load_eight(wu + at, left);
+            fx[i] = load_eight(x + at, left);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            g = mma16<T>(fg[i], fx[i], g);
+            u = mma16<T>(fu[i], fx[i], u);
+        }
+    }
+    s_acc[0][wave][lane] = g;
+    s_acc[1][wave][lane] = u;
+    __syncthreads();
+    if (wave != 0 || r >= a.M) return;
+    for (int w = 1; w < kFewWaves; ++w) {
+        g += s_acc[0][w][lane];
+        u += s_acc[1][w][lane];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const int col = n0 + quarter * 4 + e;
+        if (col >= a.N) break;
+        float v;
+        activate<false>(a.activation, g[e], &v, nullptr);
+        const int64_t at = r * a.ldo + col;
+        static_cast<T*>(a.out[0])[at] = (T)(v * u[e]);
+        if constexpr (KEEP) {
+            static_cast<T*>(a.out[1])[at] = (T)g[e];
+            static_cast<T*>(a.out[2])[at] = (T)u[e];
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------
+// calls
+
+inline int64_t size_of(int32_t dtype) { return dtype == TRIDENT_F32 ? 4 : 2; }
+inline int64_t round_up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+// Elements of a packed row: whole pieces, no power of two apart.
+inline int64_t pitch_of(int64_t cols, int64_t es) {
+    const int64_t p = round_up(cols, 8);
+    return p * es % 1024 == 0 ? p + 64 / es * 2 : p;
+}
+inline size_t bytes_of(int64_t rows, int64_t pitch, int64_t es) { return (size_t)round_up(rows * pitch * es, 256); }
+
+inline bool whole(const void* p, int64_t ld, int64_t es) {
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0;
+}
+
+struct Scratch {
+    uint8_t* p;
+    size_t left;
+    void* take(size_t n) {
+        void* r = p;
+        p += n;
+        left -= n;
+        return r;
+    }
+};
+
+// The operand as it is, or packed into scratch.
+template <typename T>
+int operand(Operand* o, const void* p, int64_t ld, int64_t rows, int64_t cols, Scratch* s, hipStream_t st) {
+    if (whole(p, ld, sizeof(T)) && cols % (16 / sizeof(T)) == 0) {
+        *o = {static_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T)};
+        return TRIDENT_OK;
+    }
+    const int64_t pitch = pitch_of(cols, sizeof(T)), pieces = rows * (pitch / (16 / (int64_t)sizeof(T)));
+    T* to = static_cast<T*>(s->take(bytes_of(rows, pitch, sizeof(T))));
+    pack_kernel<T><<<(unsigned)((pieces + kBlock - 1) / kBlock), kBlock, 0, st>>>(static_cast<const T*>(p), ld, to, pitch,
+                                                                                 rows, (int)cols);
+    *o = {reinterpret_cast<const uint8_t*>(to), pitch * (int64_t)sizeof(T)};
+    return capi_check_launch("pack_kernel");
+}
+
+size_t packed_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int64_t es) {
+    return whole(p, ld, es) && cols % (16 / es) == 0 ? 0 : bytes_of(rows, pitch_of(cols, es), es);
+}
+
+size_t forward_bytes(const TridentGated* t) {
+    if (t->M <= kFewRows) return 0;
+    const int64_t es = size_of(t->dtype);
+    return packed_bytes(t->x, t->ld_x, t->M, t->K, es) + packed_bytes(t->gate_weight, t->ld_gate, t->N, t->K, es) +
+           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es);
+}
+
+size_t backward_bytes(const TridentGated* t) {
+    const int64_t es = size_of(t->dtype);
+    return packed_bytes(t->x, t->ld_x, t->M, t->K, es) + packed_bytes(t->gate_weight, t->ld_gate, t->N, t->K, es) +
+           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + 2 * bytes_of(t->M, pitch_of(t->N, es), es);
+}
+
+int check(const TridentGated* t, bool backward) {
+    const char* name = backward ? "gated_linear_grad" : "gated_linear";
+    if (!t) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: NULL arguments", name);
+    if (!dtype_ok(t->dtype)) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: dtype=%d", name, t->dtype);
+    if (t->activation < TRIDENT_SILU || t->activation > TRIDENT_GELU_TANH)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: activation=%d", name, t->activation);
+    const int64_t most = 1 << 21;  // so that a tile's rows are within 32-bit offsets
+    if (t->M < 0 || t->N < 0 || t->K < 1 || t->M > (1 << 30) || t->N > most || t->K > most || t->ld_x < t->K ||
+        t->ld_gate < t->K || t->ld_up < t->K || t->ld_x > most || t->ld_gate > most || t->ld_up > most)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: bad sizes M=%lld N=%lld K=%lld pitches %lld, %lld, %lld", name,
+                         (long long)t->M, (long long)t->N, (long long)t->K, (long long)t->ld_x, (long long)t->ld_gate,
+                         (long long)t->ld_up);
+    return TRIDENT_OK;
+}
+
+template <typename T>
+int forward(const TridentGated* t, Scratch s, hipStream_t st) {
+    const bool keep = t->gate != nullptr;
+    if (t->M <= kFewRows) {
+        FewArgs a{t->x, t->gate_weight, t->up_weight, {t->h, t->gate, t->up}, t->ld_x, t->ld_gate, t->ld_up, t->N,
+                  (int)t->M, (int)t->N, (int)t->K, t->activation};
+        const unsigned grid = (unsigned)((t->N + 15) / 16);
+        if (keep) few_kernel<T, true><<<grid, kFewWaves * kWave, 0, st>>>(a);
+        else few_kernel<T, false><<<grid, kFewWaves * kWave, 0, st>>>(a);
+        return capi_check_launch("few_kernel");
+    }
+    ProductArgs a{};
+    int rc = operand<T>(&a.second[0], t->x, t->ld_x, t->M, t->K, &s, st);
+    if (rc == TRIDENT_OK) rc = operand<T>(&a.first[0], t->gate_weight, t->ld_gate, t->N, t->K, &s, st);
+    if (rc == TRIDENT_OK) rc = operand<T>(&a.first[1], t->up_weight, t->ld_up, t->N, t->K, &s, st);
+    if (rc != TRIDENT_OK) return rc;
+    a.out[0] = t->h;
+    a.out[1] = t->gate;
+    a.out[2] = t->up;
+    a.ldo = t->N;
+    a.M = (int)t->M;
+    a.N = (int)t->N;
+    a.K = (int)t->K;
+    a.parts = 1;
+    a.activation = t->activation;
+    if (keep) return launch_product<T, kRowsRows, 2, 2, 2, 2, true, true>(a, 1, st);
+    return launch_product<T, kRowsRows, 2, 2, 2, 2, true, false>(a, 1, st);
+}
+
+template <typename T>
+int backward(const TridentGated* t, Scratch s, hipStream_t st) {
+    const int64_t pitch = pitch_of(t->N, sizeof(T));
+    SlopeArgs d{t->grad, t->gate, t->up, s.take(bytes_of(t->M, pitch, sizeof(T))), s.take(bytes_of(t->M, pitch, sizeof(T))),
+                t->ld_grad, t->N, pitch, t->M, (int)t->N, t->activation};
+    slope_kernel<T><<<(unsigned)((t->M * (pitch / 8) + kBlock - 1) / kBlock), kBlock, 0, st>>>(d);
+    int rc = capi_check_launch("slope_kernel");
+    const Operand dg{static_cast<const uint8_t*>(d.dgate), pitch * (int64_t)sizeof(T)},
+        du{static_cast<const uint8_t*>(d.dup), pitch * (int64_t)sizeof(T)};
+    if (rc == TRIDENT_OK && t->dx) {
+        ProductArgs a{};
+        rc = operand<T>(&a.first[0], t->gate_weight, t->ld_gate, t->N, t->K, &s, st);
+        if (rc == TRIDENT_OK) rc = operand<T>(&a.first[1], t->up_weight, t->ld_up, t->N, t->K, &s, st);
+        if (rc != TRIDENT_OK) return rc;
+        a.second[0] = dg;
+        a.second[1] = du;
+        a.out[0] = t->dx;
+        a.ldo = t->K;
+        a.M = (int)t->M;
+        a.N = (int)t->K;
+        a.K = (int)t->N;
+        a.parts = 2;
+        rc = launch_product<T, kColumnsRows, 2, 2, 2, 2>(a, 1, st);
+    }
+    if (rc == TRIDENT_OK && t->dgate_weight) {
+        ProductArgs a{};
+        rc = operand<T>(&a.first[0], t->x, t->ld_x, t->M, t->K, &s, st);
+        if (rc != TRIDENT_OK) return rc;
+        a.second[0] = dg;
+        a.second[1] = du;
+        a.out[0] = t->dgate_weight;
+        a.out[1] = t->dup_weight;
+        a.ldo = t->K;
+        a.M = (int)t->N;
+        a.N = (int)t->K;
+        a.K = (int)t->M;
+        a.parts = 1;
+        rc = launch_product<T, kColumnsColumns, 2, 2, 2, 2>(a, 2, st);
+    }
+    return rc;
+}
+
+}  // namespace
+}  // namespace trident
+
+using namespace trident;
+
+extern "C" {
+
+size_t trident_gated_linear_workspace_bytes(const TridentGated* t) {
+    return check(t, false) == TRIDENT_OK && t->M > 0 && t->N > 0 ? forward_bytes(t) : 0;
+}
+
+size_t trident_gated_linear_grad_workspace_bytes(const TridentGated* t) {
+    return check(t, true) == TRIDENT_OK && t->M > 0 && t->N > 0 ? backward_bytes(t) : 0;
+}
+
+int trident_gated_linear(const TridentGated* t, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check(t, false);
+    if (rc != TRIDENT_OK || t->M == 0 || t->N == 0) return rc;
+    if (!t->x || !t->gate_weight || !t->up_weight || !t->h || (t->gate == nullptr) != (t->up == nullptr))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "gated_linear: NULL pointer, or one of gate and up without the other");
+    const size_t need = forward_bytes(t);
+    if (need && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15)))
+        return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "gated_linear needs %zu bytes, 16-byte aligned, got %zu", need,
+                         workspace ? workspace_bytes : 0);
+    with_dtype(t->dtype, [&](auto e) {
+        rc = forward<decltype(e)>(t, {static_cast<uint8_t*>(workspace), workspace_bytes}, (hipStream_t)stream);
+    });
+    return rc;
+}
+
+int trident_gated_linear_grad(const TridentGated* t, void* workspace, size_t workspace_bytes, void* stream) {
+    int rc = check(t, true);
+    if (rc != TRIDENT_OK) return rc;
+    if (t->ld_grad < t->N) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "gated_linear_grad: ld_grad=%lld", (long long)t->ld_grad);
+    if (t->M == 0 || t->N == 0)
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "gated_linear_grad: no rows or columns: the gradients are zeros");
+    if (!t->x || !t->gate_weight || !t->up_weight || !t->grad || !t->gate || !t->up ||
+        (t->dgate_weight == nullptr) != (t->dup_weight == nullptr))
+        return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
+                         "gated_linear_grad: NULL pointer, or one of dgate_weight and dup_weight without the other");
+    const size_t need = backward_bytes(t);
+    if (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return capi_fail(TRIDENT_ERR_WORKSPACE_TOO_SMALL, "gated_linear_grad needs %zu bytes, 16-byte aligned, got %zu", need,
+                         workspace ? workspace_bytes : 0);
+    with_dtype(t->dtype, [&](auto e) {
+        rc = backward<decltype(e)>(t, {static_cast<uint8_t*>(workspace), workspace_bytes}, (hipStream_t)stream);
+    });
+    return rc;
+}
+
+}  // extern "C"

@@ -64,20 +64,22 @@ struct Tile {
         }
     }
 
-    // Eight rows of this lane's column col + lane % 32: rows row + 4 half + {0..3, 8..11}; row and col are
-    // multiples of 16 and 32.  16-bit types by the transposing read: of 16 lanes that read 4 x 16 elements, each
-    // gets a column of four.
-    static __device__ __forceinline__ frag<T> col_frag(lds_bytes tile, int row, int col) {
-        const int lane = lane_id(), half = lane >> 5;
+    // Eight rows of this lane's column col + lane % 32: rows row + 4 half + {0..3, 8..11} (a result's), or
+    // row + 8 half + {0..7} (a row_frag's); row and col are multiples of 16 and 32.  16-bit types by the
+    // transposing read: of 16 lanes that read 4 x 16 elements, each gets a column of four.
+    template <bool ROW_ORDER>
+    static __device__ __forceinline__ frag<T> read_columns(lds_bytes tile, int row, int col) {
+        const int lane = lane_id(), first = (ROW_ORDER ? 8 : 4) * (lane >> 5);
+        constexpr int kNext = ROW_ORDER ? 4 : 8;
         if constexpr (sizeof(T) == 2) {
             typedef short s16x4 __attribute__((ext_vector_type(4)));
             typedef __attribute__((address_space(3))) s16x4* quads;
-            const int in = 4 * half + (lane >> 2 & 3);  // of 16 rows
+            const int in = first + (lane >> 2 & 3);  // of 16 rows
             const int piece = (lane >> 4 & 1) * 2 + (lane >> 1 & 1) + col / 8;
             const lds_bytes at = tile + (row + in) * PITCH + (lane & 1) * 8;
             const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((quads)(at + ((piece ^ exchange(in)) << 4)));
-            const s16x4 hi =
-                __builtin_amdgcn_ds_read_tr16_b64_v4i16((quads)(at + 8 * PITCH + ((piece ^ exchange(in + 8)) << 4)));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (quads)(at + kNext * PITCH + ((piece ^ exchange(in + kNext)) << 4)));
             return __builtin_bit_cast(frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             typedef const __attribute__((address_space(3))) float* one;
@@ -85,11 +87,17 @@ struct Tile {
             frag<T> f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int in = 4 * half + i % 4 + i / 4 * 8;
+                const int in = first + i % 4 + i / 4 * kNext;
                 f[i] = *(one)(tile + (row + in) * PITCH + ((piece ^ exchange(in)) << 4) + (lane & 3) * 4);
             }
             return f;
         }
+    }
+    static __device__ __forceinline__ frag<T> col_frag(lds_bytes tile, int row, int col) {
+        return read_columns<false>(tile, row, col);
+    }
+    static __device__ __forceinline__ frag<T> col_frag_in_order(lds_bytes tile, int row, int col) {
+        return read_columns<true>(tile, row, col);
     }
 };
 

@@ -10,8 +10,8 @@
                                        the gated half of a feed-forward block: act(x Wg^T) * (x Wu^T)
 
 ``embedding``, ``layer_norm``, ``rotary``, ``attention`` and ``gated_linear`` take part in autograd; the
-``*_forward`` / ``*_grad`` functions are the bare passes; the 8-bit products have no gradient and refuse operands that require one.  Tensors with a
-forward-mode tangent are refused.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics
+``*_forward`` / ``*_grad`` functions are the bare passes; the 8-bit products have no gradient and refuse
+operands that require one.  Tensors with a forward-mode tangent are refused.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics
 and states are float32 and every result is rounded once.  Each call runs on the current stream of its
 tensors' device, with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a
 graph is captured there, with scratch of the graph's own; results are the same bits every time.  Wrong
@@ -931,3 +931,117 @@ def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
 def _whole(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy, contiguous from a 16-byte address on."""
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+# ---------------------------------------------------------------------------------------------
+# gated feed-forward
+
+_ACTIVATIONS = {"silu": _lib.SILU, "gelu": _lib.GELU, "gelu_tanh": _lib.GELU_TANH}
+
+
+def _gated_args(x, w_gate, w_up, activation):
+    """(TridentGated without results, the tensors it points to, the device's index)"""
+    code, index, act = _DTYPES.get(x.dtype), x.get_device(), _ACTIVATIONS.get(activation)
+    if code is None or index < 0:
+        _dtype("x", x)
+        _gpu("x", x)
+    if act is None:
+        _refuse(f"activation must be one of {', '.join(_ACTIVATIONS)}, got {activation!r}")
+    shape = x.shape
+    K = shape[-1] if shape else 0
+    if w_gate.dim() != 2 or w_gate.shape != w_up.shape or w_gate.shape[1] != K or K == 0:
+        _refuse(f"x must be [..., K] and the weights [N, K], got {tuple(shape)}, {tuple(w_gate.shape)} and "
+                f"{tuple(w_up.shape)}")
+    for name, t in (("w_gate", w_gate), ("w_up", w_up)):
+        if t.dtype is not x.dtype:
+            _refuse(f"{name} must be {x.dtype} as x, got {t.dtype}")
+        _same(index, name, t)
+    xr, ld_x = (x, K) if x.is_contiguous() else _rows(x)
+    g, ld_g = (w_gate, K) if w_gate.is_contiguous() else _rows(w_gate)
+    u, ld_u = (w_up, K) if w_up.is_contiguous() else _rows(w_up)
+    a = _lib.TridentGated(xr.data_ptr(), g.data_ptr(), u.data_ptr(), None, None, None, None, None, None, None,
+                          x.numel() // K, w_gate.shape[0], K, ld_x, ld_g, ld_u, 0, code, act)
+    return a, (xr, g, u), index
+
+
+def _gated(x, w_gate, w_up, activation, keep):
+    a, kept, index = _gated_args(x, w_gate, w_up, activation)
+    shape = (*x.shape[:-1], a.N)
+    h = x.new_empty(shape)
+    gate = up = None
+    a.h = h.data_ptr()
+    if keep:
+        gate, up = x.new_empty(shape), x.new_empty(shape)
+        a.gate, a.up = gate.data_ptr(), up.data_ptr()
+    if h.numel():
+        at = ctypes.byref(a)
+        _call_ws(x.device, index, "trident_gated_linear", _fn("trident_gated_linear_workspace_bytes")(at), at)
+    return h, gate, up
+
+
+class _GatedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_gate, w_up, activation):
+        h, gate, up = _gated(x, w_gate, w_up, activation, True)
+        ctx.save_for_backward(x, w_gate, w_up, gate, up)
+        ctx.activation = activation
+        return h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        need = ctx.needs_input_grad
+        dx, dg, du = _gated_grad(grad, *ctx.saved_tensors, ctx.activation, need[0], need[1] or need[2])
+        return dx, dg if need[1] else None, du if need[2] else None, None
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
+    """``act(x @ w_gate.T) * (x @ w_up.T)`` in one kernel: [..., N] in x's type from x [..., K] and weights [N, K] of
+    its type (rows of any pitch, such as the halves of one matrix).  ``activation``: "silu", "gelu", or "gelu_tanh"
+    (gelu by its tanh formula).  The sums, the activation and the product are float32."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("gated_linear", x, w_gate, w_up)
+    if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
+        return _GatedLinear.apply(x, w_gate, w_up, activation)
+    return _gated(x, w_gate, w_up, activation, False)[0]
+
+
+def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                         activation: str = "silu") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(h, gate, up): ``gated_linear`` and its two products [..., N] in x's type, for the backward pass."""
+    if _forward_ad._current_level >= 0:
+        _no_tangents("gated_linear_forward", x, w_gate, w_up)
+    return _gated(x, w_gate, w_up, activation, True)
+
+
+def gated_linear_grad(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
+                      gate: torch.Tensor, up: torch.Tensor, activation: str = "silu"):
+    """(dx, dw_gate, dw_up) from the gradient of h and what ``gated_linear_forward`` took and gave.  The
+    gradients of the two products are rounded to x's type before they are multiplied."""
+    return _gated_grad(grad, x, w_gate, w_up, gate, up, activation, True, True)
+
+
+def _gated_grad(grad, x, w_gate, w_up, gate, up, activation, need_x, need_w):
+    if _forward_ad._current_level >= 0:
+        _no_tangents("gated_linear_grad", grad, x, w_gate, w_up, gate, up)
+    a, kept, index = _gated_args(x, w_gate, w_up, activation)
+    shape = (*x.shape[:-1], a.N)
+    for name, t in (("grad", grad), ("gate", gate), ("up", up)):
+        if t.shape != shape or t.dtype is not x.dtype or (name != "grad" and not t.is_contiguous()):
+            _refuse(f"{name} must be {shape} {x.dtype}{'' if name == 'grad' else ', contiguous'}, got {tuple(t.shape)} "
+                    f"{t.dtype}")
+        _same(index, name, t)
+    dx = x.new_empty(x.shape) if need_x else None
+    dg, du = (x.new_empty(w_gate.shape), x.new_empty(w_up.shape)) if need_w else (None, None)
+    if a.M == 0 or a.N == 0:  # sums of nothing
+        for t in (dx, dg, du):
+            if t is not None:
+                t.zero_()
+        return dx, dg, du
+    gr, a.ld_grad = (grad, a.N) if grad.is_contiguous() else _rows(grad)
+    a.grad, a.gate, a.up = gr.data_ptr(), gate.data_ptr(), up.data_ptr()
+    a.dx = ext._ptr(dx)
+    a.dgate_weight, a.dup_weight = ext._ptr(dg), ext._ptr(du)
+    at = ctypes.byref(a)
+    _call_ws(x.device, index, "trident_gated_linear_grad", _fn("trident_gated_linear_grad_workspace_bytes")(at), at)
+    return dx, dg, du
