@@ -16,26 +16,34 @@ namespace {
 
 enum Activation { kSilu = TRIDENT_SILU, kGelu = TRIDENT_GELU, kGeluTanh = TRIDENT_GELU_TANH };
 
-// act(g), and act'(g) where SLOPE.
+// act(g), and act'(g) where SLOPE.  By the vector unit's own exp2 and reciprocal, off by 1 ulp each: a tile of a
+// short sum is not much longer than its activations (expf, erfcf and divisions are several times as many instructions).
 template <bool SLOPE>
 __device__ __forceinline__ void activate(int kind, float g, float* value, float* slope) {
+    constexpr float kLog2e = 1.4426950408889634f;
+    const float g2 = g * g;
     if (kind == kGelu) {
-        // g Phi(g); Phi by the complementary error function keeps its digits where it is small
-        const float p = 0.5f * erfcf(-0.70710678118654752f * g);
+        // g Phi(g), Phi(-x) = erfc(x / sqrt 2) / 2.  For x >= 0, erfc(x) = t q(t) exp(-x^2) with t = 1 / (1 + x / 2) and q a
+        // polynomial fitted to exp(x^2) erfc(x) / t, off by 5e-8 relative up to x = 14, so small values keep their digits.
+        const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, x, 1.0f));
+        constexpr float q[] = {0.282084331f, 0.282412099f, 0.242835108f, 0.203752563f, -0.0291486356f, 0.281733461f, -0.490406549f, 0.286124062f, -0.0593864829f};
+        float v = q[8];
+#pragma unroll
+        for (int i = 7; i >= 0; --i) v = __builtin_fmaf(v, t, q[i]);
+        const float e = __builtin_amdgcn_exp2f(g2 * (-0.5f * kLog2e));
+        const float tail = 0.5f * (v * t) * e, p = g < 0.0f ? tail : 1.0f - tail;
         *value = g * p;
-        if constexpr (SLOPE)
-            *slope = __builtin_fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), p);
+        if constexpr (SLOPE) *slope = __builtin_fmaf(g * 0.39894228040143268f, e, p);
         return;
     }
     // both others are g times a logistic: of g, or of 2 sqrt(2 / pi) (g + 0.044715 g^3)
-    const float g2 = g * g;
     const float z = kind == kSilu ? g : 1.5957691216057308f * g * __builtin_fmaf(0.044715f, g2, 1.0f);
-    const float p = 1.0f / (1.0f + expf(-z));
+    const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
     *value = g * p;
     if constexpr (SLOPE) {
         const float dz = kind == kSilu ? 1.0f : 1.5957691216057308f * __builtin_fmaf(3 * 0.044715f, g2, 1.0f);
         // 1 - p by its own quotient: no digits are lost where p is near 1
-        *slope = __builtin_fmaf(g * p * dz, 1.0f / (1.0f + expf(z)), p);
+        *slope = __builtin_fmaf(g * p * dz, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kLog2e * z)), p);
     }
 }
 
@@ -171,30 +179,64 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
     begin(0);
     fetch(0);
 
+    if (steps > 1) fetch(1);
+
     f32x16 acc[MT][NT] = {};
     const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    // A step's next loads are issued as soon as every wave holds its part of it in registers, halfway through its products,
+    // so that they have a step and a half to arrive.
+    constexpr int kFlight = (GATED ? 2 : 1) * First::kLoads + Second::kLoads, kHalf = kStep<T> / 32;
     for (int n = 0; n < steps; ++n) {
-        wait_and_meet<0>();
-        if (n + 1 < steps) fetch(n + 1);
+        if (n + 1 < steps) wait_and_meet<kFlight>();
+        else wait_and_meet<0>();
         const lds_bytes t1 = base + n % 2 * kStage, t2 = t1 + kFirst;
+        frag<T> f1[2][kHalf][NT], f2[2][kHalf][MT];
 #pragma unroll
-        for (int s = 0; s < kStep<T> / 16; ++s) {
-            frag<T> f1[NT], f2[MT];
+        for (int hf = 0; hf < 2; ++hf)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                if constexpr (GATED) {  // the wave's first half of blocks from the gate's tile
-                    f1[j] = First::read(t1 + (j < NT / 2 ? 0 : kFirst / 2), wn / 2 + j % (NT / 2) * 32, s);
-                } else {
-                    f1[j] = First::read(t1, wn + j * 32, s);
+            for (int s = 0; s < kHalf; ++s) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    if constexpr (GATED) {  // the wave's first half of blocks from the gate's tile
+                        f1[hf][s][j] = First::read(t1 + (j < NT / 2 ? 0 : kFirst / 2), wn / 2 + j % (NT / 2) * 32,
+                                                   hf * kHalf + s);
+                    } else {
+                        f1[hf][s][j] = First::read(t1, wn + j * 32, hf * kHalf + s);
+                    }
                 }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) f2[hf][s][i] = Second::read(t2, wm + i * 32, hf * kHalf + s);
             }
+        const auto multiply = [&](int hf) {
 #pragma unroll
-            for (int i = 0; i < MT; ++i) f2[i] = Second::read(t2, wm + i * 32, s);
+            for (int s = 0; s < kHalf; ++s)
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) acc[i][j] = mma<T>(f1[j], f2[i], acc[i][j]);
+                    for (int j = 0; j < NT; ++j) acc[i][j] = mma<T>(f1[hf][s][j], f2[hf][s][i], acc[i][j]);
+        };
+        multiply(0);
+        if constexpr (sizeof(T) == 2) {
+            // the first half's reads, the second half's among the first half's products
+            constexpr int kReads = kHalf * (NT * (READ != kRowsRows ? 2 : 1) + MT * (READ == kColumnsColumns ? 2 : 1));
+            constexpr int kProducts = kHalf * MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+#pragma unroll
+            for (int i = 0; i < kProducts; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+            }
         }
+        // the first half's products stay before the wait (the compiler would sink them past it)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();  // every wave has read the step
+        asm volatile("" ::: "memory");
+        if (n + 2 < steps) fetch(n + 2);
+        multiply(1);
     }
     // Results go through LDS, 32 rows of a wave at a time, so that whole lines are written.
     wait_and_meet<0>();
@@ -253,7 +295,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void product_kernel(ProductArgs a) {
     product<T, READ, WM, WN, MT, NT, GATED, KEEP>(a);
 }
 
-template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED = false, bool KEEP = false>
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
 int launch_product(ProductArgs a, int results, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32, BR = GATED ? BN / 2 : BN;
     constexpr size_t lds = 2 * (size_t)(BM + BN) * 128;
@@ -270,6 +312,24 @@ int launch_product(ProductArgs a, int results, hipStream_t st) {
         return capi_fail(TRIDENT_ERR_UNSUPPORTED, "gated_linear: %d x %d is too large", a.M, a.N);
     kernel<<<dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)results), WM * WN * kWave, lds, st>>>(a);
     return capi_check_launch("product_kernel");
+}
+
+// The tile.  A larger one reads its operands less often (256 x 256: 64 bytes of LDS for 8,192 products), but takes a CU
+// alone, so its tiles go in rounds of 256: it wins where the rounds are three quarters full (bfloat16, against 128 x
+// 128: the forward pass of 16,384 x 1,024 by 2 x 4,096, 2,048 tiles, 336 and 378 us; dx, 256 tiles, 265 and 330; but dWg and dWu,
+// 128 tiles, 445 and 315).  Where 128 x 128 leaves CUs idle, 64 x 64 (float32, 1,237 x 333 by 2 x 777: forward 39 to 32
+// us, dx 112 to 42, both weights 96 to 34).
+template <typename T, int READ, bool GATED = false, bool KEEP = false>
+int product_of(const ProductArgs& a, int results, hipStream_t st) {
+    const auto tiles = [&](int64_t bm, int64_t bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) * results; };
+    constexpr int kShare = GATED ? 2 : 1;  // of a tile's columns are one of two sums
+    if constexpr (sizeof(T) == 2) {
+        const int64_t large = tiles(256, 256 / kShare);
+        if (large * 4 >= (large + 255) / 256 * 256 * 3)
+            return launch_product<T, READ, 2, 4, 4, 2, GATED, KEEP>(a, results, st);
+    }
+    if (tiles(128, 128 / kShare) >= 256) return launch_product<T, READ, 2, 2, 2, 2, GATED, KEEP>(a, results, st);
+    return launch_product<T, READ, 2, 2, 1, kShare, GATED, KEEP>(a, results, st);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -526,8 +586,8 @@ int forward(const TridentGated* t, Scratch s, hipStream_t st) {
     a.K = (int)t->K;
     a.parts = 1;
     a.activation = t->activation;
-    if (keep) return launch_product<T, kRowsRows, 2, 2, 2, 2, true, true>(a, 1, st);
-    return launch_product<T, kRowsRows, 2, 2, 2, 2, true, false>(a, 1, st);
+    if (keep) return product_of<T, kRowsRows, true, true>(a, 1, st);
+    return product_of<T, kRowsRows, true, false>(a, 1, st);
 }
 
 template <typename T>
@@ -552,7 +612,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->N;
         a.parts = 2;
-        rc = launch_product<T, kColumnsRows, 2, 2, 2, 2>(a, 1, st);
+        rc = product_of<T, kColumnsRows>(a, 1, st);
     }
     if (rc == TRIDENT_OK && t->dgate_weight) {
         ProductArgs a{};
@@ -567,7 +627,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->M;
         a.parts = 1;
-        rc = launch_product<T, kColumnsColumns, 2, 2, 2, 2>(a, 2, st);
+        rc = product_of<T, kColumnsColumns>(a, 2, st);
     }
     return rc;
 }
