@@ -20,15 +20,15 @@ template <typename T>
 constexpr float kShift = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
 constexpr float kSlack = 8.0f;
 
-template <typename T, int DP, int WAVES, int QB>
-__global__ __launch_bounds__(WAVES* kWave) void attention_kernel(AttentionArgs a) {
-    constexpr int BM = WAVES * QB * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
+template <typename T, int DP, int WAVES>
+__global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <= 64) ? 2 : 1) void attention_kernel(AttentionArgs a) {
+    constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
-    using L = Tile<T, kPitch>;
     extern __shared__ __align__(16) uint8_t lds[];  // [2][keys, values]
-    const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles, hk = h / (a.Hq / a.Hkv);
+    int tile, h, hk;
+    tile_and_head(a, &tile, &h, &hk);
     SequenceTile t;
-    if (!find_tile(a, a.causal ? a.tiles - 1 - tile : tile, BM, &t)) return;
+    if (!find_tile(a, tile, BM, &t)) return;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
     const int64_t out_row = (int64_t)a.Hq * a.D;
     T* out = static_cast<T*>(a.out) + t.start * out_row + (int64_t)h * a.D;
@@ -39,127 +39,129 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_kernel(AttentionArgs a
     const uint8_t* k = static_cast<const uint8_t*>(a.k) + t.start * a.k_row + hk * a.k_head;
     const uint8_t* v = static_cast<const uint8_t*>(a.v) + t.start * a.v_row + hk * a.v_head;
     const int bytes = a.D * (int)sizeof(T);
-    const auto fetch = [&](int n) {
-        uint8_t* to = lds + n % 2 * 2 * kTile;
+    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    const auto fetch = [&](int n, lds_bytes to) {
+        if (n >= tiles) return;
         fetch_tile<T, kPitch, BN, WAVES>(to, k + (int64_t)n * BN * a.k_row, a.k_row, t.length - n * BN, bytes, wave);
         fetch_tile<T, kPitch, BN, WAVES>(to + kTile, v + (int64_t)n * BN * a.v_row, a.v_row, t.length - n * BN, bytes,
                                          wave);
     };
-    fetch(0);
+    fetch(0, base);
 
-    int row[QB];
-    frag<T> q[QB][DP / 16];
-    f32x16 acc[QB][DP / 32] = {};
-    float top[QB], sum[QB];  // the reference, times scale2, and this half's part of the sum
-    const int first = t.first + wave * QB * 32;
+    const int first = t.first + wave * 32, last = first + 31, row = first + (lane & 31);
+    frag<T> q[DP / 16];
+    load_row<T, DP>(static_cast<const uint8_t*>(a.q) + (t.start + min(row, t.length - 1)) * a.q_row + h * a.q_head, a.D, q);
+    arrived(q);
+    f32x16 acc[DP / 32] = {};
+    float top = -INFINITY, sum = 0.0f;  // the reference, times scale2, and this half's part of the sum
+    const int end = a.causal ? min(row + 1, t.length) : t.length;  // the keys that this row sees
+
+    const TileReader<T, kPitch, DP> reader;
+    f32x16 s[KB];
+    frag<T> p[KB][2];
+    const auto scores = [&](lds_bytes keys) {
 #pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        row[b] = first + b * 32 + (lane & 31);
-        load_row<T, DP>(static_cast<const uint8_t*>(a.q) + (t.start + min(row[b], t.length - 1)) * a.q_row + h * a.q_head,
-                        a.D, q[b]);
-        top[b] = -INFINITY;
-        sum[b] = 0.0f;
-    }
-    const int last = first + QB * 32 - 1;
-    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
-    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
-    for (int n = 0; n < tiles; ++n) {
-        wait_and_meet<0>();  // this tile is there, and every wave is done with the other one
-        if (n + 1 < tiles) fetch(n + 1);
-        if (first >= live || (a.causal && n * BN > last)) continue;
-        const lds_bytes keys = base + n % 2 * 2 * kTile, values = keys + kTile;
-        f32x16 s[KB][QB] = {};
+        for (int kb = 0; kb < KB; ++kb) s[kb] = f32x16{};
+#pragma unroll
+        for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] = mma<T>(reader.rows(keys, kb, i), q[i], s[kb]);
+    };
+    // EDGE: with keys that some row of the wave does not see.
+    const auto exponentials = [&](int n, auto edge) {
+        if constexpr (decltype(edge)::value) {
+            const int seen_here = end - n * BN - 4 * half;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    if (kb * 32 + 8 * (i / 4) + i % 4 >= seen_here) s[kb][i] = -INFINITY;
+        }
+        float m = s[0][0];
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                const frag<T> f = L::row_frag(keys, kb * 32 + (lane & 31), i);
+            for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kb][i]);
+        m = fmaxf(m, other_half(m)) * a.scale2;
+        if (__any(m > top + kSlack)) {
+            const float by = m > top ? __builtin_amdgcn_exp2f(top - m) : 1.0f;
+            top = fmaxf(m, top);
+            sum *= by;
 #pragma unroll
-                for (int b = 0; b < QB; ++b) s[kb][b] = mma<T>(f, q[b][i], s[kb][b]);
-            }
-        if ((n + 1) * BN > t.length || (a.causal && (n + 1) * BN - 1 > first)) {
+            for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
-            for (int b = 0; b < QB; ++b) {
-                const int end = a.causal ? min(row[b] + 1, t.length) : t.length;
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (n * BN + kb * 32 + 8 * (i / 4) + 4 * half + i % 4 >= end) s[kb][b][i] = -INFINITY;
-            }
+                for (int i = 0; i < 16; ++i) acc[j][i] *= by;
         }
+        const float from = top == -INFINITY ? 0.0f : kShift<T> - top;
 #pragma unroll
-        for (int b = 0; b < QB; ++b) {
-            float m = s[0][b][0];
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) m = fmaxf(m, s[kb][b][i]);
-            m = fmaxf(m, other_half(m)) * a.scale2;
-            if (__any(m > top[b] + kSlack)) {
-                const float by = m > top[b] ? __builtin_amdgcn_exp2f(top[b] - m) : 1.0f;
-                top[b] = fmaxf(m, top[b]);
-                sum[b] *= by;
-#pragma unroll
-                for (int j = 0; j < DP / 32; ++j)
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[b][j][i] *= by;
+            for (int i = 0; i < 16; ++i) {
+                const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][i], a.scale2, from));
+                p[kb][i / 8][i % 8] = (T)e;
+                sum += e;
             }
-            const float from = top[b] == -INFINITY ? 0.0f : kShift<T> - top[b];
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][b][i], a.scale2, from));
-                    sum[b] += e;
-                    s[kb][b][i] = e;
-                }
-        }
-        // causal: blocks past the last row are left out, those on the diagonal looked at first
-        const bool edge = a.causal && (n + 1) * BN - 1 > first;
+    };
+    const auto add_values = [&](int n, lds_bytes values, auto edge) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
+            // causal: blocks past the last row are left out, those on the diagonal looked at first
             const int key = n * BN + kb * 32;
-            if (edge && key > last) continue;
-            const bool apart = edge && key >= first && any_not_finite<T, kPitch>(values + kb * 32 * kPitch);
+            bool apart = false;
+            if constexpr (decltype(edge)::value) {
+                if (a.causal && key > last) continue;
+                apart = a.causal && key >= first && any_not_finite<T, kPitch>(values + kb * 32 * kPitch);
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                frag<T> p[QB];
-#pragma unroll
-                for (int b = 0; b < QB; ++b)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) p[b][e] = (T)s[kb][b][8 * i + e];
-                if (apart) {
-#pragma unroll
-                    for (int b = 0; b < QB; ++b)
-                        add_seen_rows<T, kPitch, DP>(values, kb * 32 + i * 16, p[b], acc[b],
-                                                     [&](int r) { return key + i * 16 + r <= row[b]; });
+                if (decltype(edge)::value && apart) {
+                    add_seen_rows<T, kPitch, DP>(values, kb * 32 + i * 16, p[kb][i], acc,
+                                                 [&](int r) { return key + i * 16 + r <= row; });
                     continue;
                 }
 #pragma unroll
-                for (int j = 0; j < DP / 32; ++j) {
-                    const frag<T> f = L::col_frag(values, kb * 32 + i * 16, j * 32);
-#pragma unroll
-                    for (int b = 0; b < QB; ++b) acc[b][j] = mma<T>(f, p[b], acc[b][j]);
-                }
+                for (int j = 0; j < DP / 32; ++j)
+                    acc[j] = mma<T>(reader.columns(values, kb * 32 + i * 16, j), p[kb][i], acc[j]);
             }
         }
+    };
+    // Tiles that every row of the wave sees whole, those that some see in part, and (in step with the other waves) the
+    // rest, for which this wave only loads.
+    const int whole = first >= live ? 0 : (a.causal ? min(first + 1, t.length) : t.length) / BN;
+    const int seen = first >= live ? 0 : a.causal ? min(last / BN + 1, tiles) : tiles;
+    constexpr std::false_type kWhole{};
+    constexpr std::true_type kEdge{};
+    // Past a barrier tile n is there, and every wave is done with the one before, in whose place the next one goes.  That lies
+    // elsewhere than what is read, which __restrict says: else the compiler waits for every load before a transposing read.
+    const auto pass = [&](int n, lds_bytes __restrict from, lds_bytes __restrict to, bool work, auto edge) {
+        fetch(n + 1, to);
+        if (!work) return;
+        scores(from);
+        exponentials(n, edge);
+        add_values(n, from + kTile, edge);
+    };
+    const auto place = [&](int n) { return base + n % 2 * 2 * kTile; };
+    int n = 0;
+    for (; n < whole; ++n) {
+        wait_and_meet<0>();
+        pass(n, place(n), place(n + 1), true, kWhole);
     }
-#pragma unroll
-    for (int b = 0; b < QB; ++b) {
-        const float all = sum[b] + other_half(sum[b]);
-        if (row[b] >= live) continue;
-        store_column<T, DP>(out + (int64_t)row[b] * out_row, a.D, acc[b], 1.0f / all);
-        if (a.lse && half == 0)
-            a.lse[h * a.rows + t.start + row[b]] = top[b] - kShift<T> + __builtin_amdgcn_logf(all);
+    for (; n < tiles; ++n) {
+        wait_and_meet<0>();
+        pass(n, place(n), place(n + 1), n < seen, kEdge);
     }
+    const float all = sum + other_half(sum);
+    if (row >= live) return;
+    store_column<T, DP>(out + (int64_t)row * out_row, a.D, acc, 1.0f / all);
+    if (a.lse && half == 0) a.lse[h * a.rows + t.start + row] = top - kShift<T> + __builtin_amdgcn_logf(all);
 }
 
-template <typename T, int DP, int WAVES, int QB>
+template <typename T, int DP, int WAVES>
 int launch(AttentionArgs a, hipStream_t st) {
-    constexpr int BM = WAVES * QB * 32;
+    constexpr int BM = WAVES * 32;
     constexpr size_t lds = 4 * (size_t)kTileRows<T> * kTilePitch<T, DP>;
-    const auto kernel = attention_kernel<T, DP, WAVES, QB>;
+    const auto kernel = attention_kernel<T, DP, WAVES>;
     static_assert(lds <= 163840, "LDS of a CU");
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -176,8 +178,8 @@ int launch(AttentionArgs a, hipStream_t st) {
 template <typename T, int DP>
 int by_length(const AttentionArgs& a, hipStream_t st) {
     const int64_t mean = a.slots ? a.slots : a.rows / std::max<int64_t>(a.count, 1);
-    if (mean <= 32) return launch<T, DP, 1, 1>(a, st);
-    return launch<T, DP, 4, 1>(a, st);
+    if (mean <= 32) return launch<T, DP, 1>(a, st);
+    return launch<T, DP, 4>(a, st);
 }
 
 }  // namespace

@@ -74,6 +74,16 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs& a, int tile, int 
     return t->first >= 0 && t->first < t->extent;
 }
 
+// A workgroup's tile of queries and head.  Tiles in the order of their work where they differ (causal: a sequence's last ones
+// first), so that the longest do not begin last; for each the heads, the key heads changing fastest: workgroups go to
+// the eight XCDs in turn, so with eight key heads each XCD's L2 sees one.
+__device__ __forceinline__ void tile_and_head(const AttentionArgs& a, int* tile, int* h, int* hk) {
+    const int at = blockIdx.x / a.Hq, j = blockIdx.x % a.Hq;
+    *tile = a.causal ? a.tiles - 1 - at : at;
+    *hk = j % a.Hkv;
+    *h = *hk * (a.Hq / a.Hkv) + j / a.Hkv;
+}
+
 template <typename T, int DP>
 constexpr int kTilePitch = sizeof(T) == 2 ? (DP <= 32 ? 64 : DP <= 64 ? 128 : 256) : (DP <= 32 ? 128 : DP <= 64 ? 256 : 512);
 // tokens of a tile in LDS
@@ -83,7 +93,7 @@ constexpr int kTileRows = sizeof(T) == 2 ? 64 : 32;
 // One wave's share of loading rows 0 .. ROWS - 1 at `p` (pitch `row` bytes, `live` of them there) to LDS.
 // Rows past the live ones and columns past D bytes become zeros: what lies there is never multiplied.
 template <typename T, int PITCH, int ROWS, int WAVES>
-__device__ __forceinline__ void fetch_tile(uint8_t* to, const void* p, int64_t row, int live, int bytes, int wave) {
+__device__ __forceinline__ void fetch_tile(lds_bytes to, const void* p, int64_t row, int live, int bytes, int wave) {
     using L = Tile<T, PITCH>;
     constexpr int kLoads = ROWS / L::kRowsAtOnce;
     const __amdgpu_buffer_rsrc_t buf = buffer_of(p, (uint32_t)(max(min(live, ROWS), 0) * (int)row));
@@ -108,6 +118,13 @@ __device__ __forceinline__ void load_row(const void* p, int D, frag<T> (&f)[DP /
         f[s] = frag<T>{};
         if (col < D) f[s] = *reinterpret_cast<const frag<T>*>(static_cast<const T*>(p) + col);
     }
+}
+
+// Waits for a row's fragments: else every pass of a loop that uses them would wait for all of its loads.
+template <typename F, int N>
+__device__ __forceinline__ void arrived(F (&f)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 
 // Whether 32 rows of a tile hold a value that is not finite.

@@ -43,11 +43,11 @@ template <typename T, int DP, int WAVES>
 __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArgs a) {
     constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
-    using L = Tile<T, kPitch>;
     extern __shared__ __align__(16) uint8_t lds[];  // [2][keys, values]
-    const int tile = blockIdx.x % a.tiles, h = blockIdx.x / a.tiles, hk = h / (a.Hq / a.Hkv);
+    int tile, h, hk;
+    tile_and_head(a, &tile, &h, &hk);
     SequenceTile t;
-    if (!find_tile(a, a.causal ? a.tiles - 1 - tile : tile, BM, &t)) return;
+    if (!find_tile(a, tile, BM, &t)) return;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
     const int64_t out_row = (int64_t)a.Hq * a.D;
     T* dq = static_cast<T*>(a.dq) + t.start * out_row + (int64_t)h * a.D;
@@ -58,13 +58,15 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
     const uint8_t* k = static_cast<const uint8_t*>(a.k) + t.start * a.k_row + hk * a.k_head;
     const uint8_t* v = static_cast<const uint8_t*>(a.v) + t.start * a.v_row + hk * a.v_head;
     const int bytes = a.D * (int)sizeof(T);
-    const auto fetch = [&](int n) {
-        uint8_t* to = lds + n % 2 * 2 * kTile;
+    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    const auto fetch = [&](int n, lds_bytes to) {
+        if (n >= tiles) return;
         fetch_tile<T, kPitch, BN, WAVES>(to, k + (int64_t)n * BN * a.k_row, a.k_row, t.length - n * BN, bytes, wave);
         fetch_tile<T, kPitch, BN, WAVES>(to + kTile, v + (int64_t)n * BN * a.v_row, a.v_row, t.length - n * BN, bytes,
                                          wave);
     };
-    fetch(0);
+    fetch(0, base);
 
     const int first = t.first + wave * 32, row = first + (lane & 31);
     const int64_t at = t.start + min(row, t.length - 1);
@@ -83,34 +85,37 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
     }
     const float lse = a.lse[h * a.rows + at];
     if (row < live && half == 0) a.delta[h * a.rows + at] = delta;
+    arrived(q);
+    arrived(go);
     f32x16 acc[DP / 32] = {};
     Power<DP / 32> power;
-    const int last = first + 31;
-    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
-    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
-    for (int n = 0; n < tiles; ++n) {
-        wait_and_meet<0>();
-        if (n + 1 < tiles) fetch(n + 1);
-        if (first >= live || (a.causal && n * BN > last)) continue;
-        const lds_bytes keys = base + n % 2 * 2 * kTile, values = keys + kTile;
-        const bool edge = (n + 1) * BN > t.length || (a.causal && (n + 1) * BN - 1 > first);
-        const int end = a.causal ? min(row + 1, t.length) : t.length;
+    const int last = first + 31, end = a.causal ? min(row + 1, t.length) : t.length;
+    const TileReader<T, kPitch, DP> reader;
+    // One tile of keys; EDGE: with keys that some row of the wave does not see.  What is loaded meanwhile lies elsewhere
+    // than what is read, which __restrict says: else the compiler waits for every load before a transposing read.
+    const auto pass = [&](int n, lds_bytes __restrict from, lds_bytes __restrict to, bool work, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        fetch(n + 1, to);
+        if (!work) return;
+        const lds_bytes keys = from, values = from + kTile;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             const int key = n * BN + kb * 32;
-            if (a.causal && key > last) continue;
+            if (EDGE && a.causal && key > last) continue;
             f32x16 s = {}, dp = {};
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) s = mma<T>(L::row_frag(keys, kb * 32 + (lane & 31), i), q[i], s);
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) dp = mma<T>(L::row_frag(values, kb * 32 + (lane & 31), i), go[i], dp);
+            for (int i = 0; i < DP / 16; ++i) {
+                s = mma<T>(reader.rows(keys, kb, i), q[i], s);
+                dp = mma<T>(reader.rows(values, kb, i), go[i], dp);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * (dp[i] - delta);
-            if (edge) {
+            if constexpr (EDGE) {
+                const int seen_here = end - key - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (key + 8 * (i / 4) + 4 * half + i % 4 >= end) s[i] = 0.0f;
+                    if (8 * (i / 4) + i % 4 >= seen_here) s[i] = 0.0f;
             }
             if constexpr (kFollow<T>) {
                 float top = 0.0f;
@@ -123,19 +128,30 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dq_kernel(AttentionArg
             frag<T> ds[2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = (T)s[i];
-            const bool apart = a.causal && key >= first && any_not_finite<T, kPitch>(keys + kb * 32 * kPitch);
+            const bool apart = EDGE && a.causal && key >= first && any_not_finite<T, kPitch>(keys + kb * 32 * kPitch);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (apart) {
+                if (EDGE && apart) {
                     add_seen_rows<T, kPitch, DP>(keys, kb * 32 + i * 16, ds[i], acc,
                                                  [&](int r) { return key + i * 16 + r <= row; });
                     continue;
                 }
 #pragma unroll
-                for (int j = 0; j < DP / 32; ++j)
-                    acc[j] = mma<T>(L::col_frag(keys, kb * 32 + i * 16, j * 32), ds[i], acc[j]);
+                for (int j = 0; j < DP / 32; ++j) acc[j] = mma<T>(reader.columns(keys, kb * 32 + i * 16, j), ds[i], acc[j]);
             }
         }
+    };
+    const int whole = first >= live ? 0 : (a.causal ? min(first + 1, t.length) : t.length) / BN;
+    const int seen = first >= live ? 0 : a.causal ? min(last / BN + 1, tiles) : tiles;
+    const auto place = [&](int n) { return base + n % 2 * 2 * kTile; };
+    int n = 0;
+    for (; n < whole; ++n) {
+        wait_and_meet<0>();
+        pass(n, place(n), place(n + 1), true, std::false_type{});
+    }
+    for (; n < tiles; ++n) {
+        wait_and_meet<0>();
+        pass(n, place(n), place(n + 1), n < seen, std::true_type{});
     }
     if (row < live) store_column<T, DP>(dq + (int64_t)row * out_row, a.D, acc, kFollow<T> ? a.scale / power.by : a.scale);
 }
@@ -148,9 +164,8 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
     constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
     constexpr int kStage = 2 * kTile + 2 * kWave * 4;  // queries, gradients, 64 words of lse and of delta
-    using L = Tile<T, kPitch>;
     extern __shared__ __align__(16) uint8_t lds[];
-    const int tile = blockIdx.x % a.tiles, hk = blockIdx.x / a.tiles, group = a.Hq / a.Hkv;
+    const int tile = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, group = a.Hq / a.Hkv;
     SequenceTile t;
     if (!find_tile(a, tile, BM, &t)) return;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
@@ -167,8 +182,9 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
 
     const int bytes = a.D * (int)sizeof(T);
     const int n0 = a.causal ? t.first / BN : 0, each = (t.length + BN - 1) / BN - n0, tiles = each * group;
-    const auto fetch = [&](int n) {
-        uint8_t* to = lds + n % 2 * kStage;
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    const auto fetch = [&](int n, lds_bytes to) {
+        if (n >= tiles) return;
         const int g = n / each, r = (n0 + n - g * each) * BN, h = hk * group + g;
         const int64_t at = t.start + r;
         fetch_tile<T, kPitch, BN, WAVES>(to, static_cast<const uint8_t*>(a.q) + at * a.q_row + h * a.q_head, a.q_row,
@@ -184,7 +200,7 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
             __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_of(a.delta + h * a.rows + at, words),
                                                      (lds_ptr)(to + 2 * kTile + kWave * 4), 4, mine, 0, 0, 0);
     };
-    fetch(0);
+    fetch(0, base);
 
     const int first = t.first + wave * 32, row = first + (lane & 31);
     const int64_t at = t.start + min(row, t.length - 1);
@@ -197,39 +213,42 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
     if constexpr (kHold) {
         load_row<T, DP>(k_at, a.D, k);
         load_row<T, DP>(v_at, a.D, v);
+        arrived(k);
+        arrived(v);
     }
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     Power<DP / 32> power;
-    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
-    for (int n = 0; n < tiles; ++n) {
-        wait_and_meet<0>();
-        if (n + 1 < tiles) fetch(n + 1);
-        const int r = (n0 + n % each) * BN;
-        if (first >= live || (a.causal && r + BN <= first)) continue;
-        const lds_bytes queries = base + n % 2 * kStage, grads = queries + kTile;
+    const TileReader<T, kPitch, DP> reader;
+    // One tile of queries from row r on; EDGE: causal, with queries before some key of the wave.  For __restrict see above.
+    const auto pass = [&](int n, int r, lds_bytes __restrict from, lds_bytes __restrict to, bool work, auto edge) {
+        constexpr bool EDGE = decltype(edge)::value;
+        fetch(n + 1, to);
+        if (!work) return;
+        const lds_bytes queries = from, grads = from + kTile;
         typedef const __attribute__((address_space(3))) f32x4* quads;
         const quads lse = (quads)(grads + kTile), delta = (quads)(grads + kTile + kWave * 4);
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
             const int query = r + kb * 32;
-            if (a.causal && query < first) continue;
-            const bool edge = a.causal && query < first + 32;
+            if (EDGE && query < first) continue;
             f32x16 s = {}, dp = {};
             if constexpr (!kHold) {
                 asm volatile("" : "+v"(k_at), "+v"(v_at));  // not before the loop
                 load_row<T, DP>(k_at, a.D, k);
+                load_row<T, DP>(v_at, a.D, v);
             }
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) s = mma<T>(L::row_frag(queries, kb * 32 + (lane & 31), i), k[i], s);
-            if constexpr (!kHold) load_row<T, DP>(v_at, a.D, v);
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) dp = mma<T>(L::row_frag(grads, kb * 32 + (lane & 31), i), v[i], dp);
+            for (int i = 0; i < DP / 16; ++i) {
+                s = mma<T>(reader.rows(queries, kb, i), k[i], s);
+                dp = mma<T>(reader.rows(grads, kb, i), v[i], dp);
+            }
+            const int hidden = EDGE ? row - query - 4 * half : 0;  // of this half's rows are before the key
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const f32x4 le = lse[kb * 8 + 2 * i + half], de = delta[kb * 8 + 2 * i + half];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const bool masked = edge && query + 8 * i + 4 * half + e < row;
+                    const bool masked = EDGE && 8 * i + e < hidden;
                     const float x =
                         masked ? 0.0f
                                : __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * i + e], a.scale2, kShift<T> - le[e]));
@@ -251,11 +270,11 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
                 p[i / 8][i % 8] = (T)s[i];
                 ds[i / 8][i % 8] = (T)dp[i];
             }
-            const bool apart = edge && (any_not_finite<T, kPitch>(queries + kb * 32 * kPitch) ||
-                                        any_not_finite<T, kPitch>(grads + kb * 32 * kPitch));
+            const bool apart = EDGE && query < first + 32 && (any_not_finite<T, kPitch>(queries + kb * 32 * kPitch) ||
+                                                              any_not_finite<T, kPitch>(grads + kb * 32 * kPitch));
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                if (apart) {
+                if (EDGE && apart) {
                     const auto sees = [&](int r) { return query + i * 16 + r >= row; };
                     add_seen_rows<T, kPitch, DP>(grads, kb * 32 + i * 16, p[i], av, sees);
                     add_seen_rows<T, kPitch, DP>(queries, kb * 32 + i * 16, ds[i], ak, sees);
@@ -263,10 +282,25 @@ __global__ __launch_bounds__(WAVES* kWave) void attention_dkv_kernel(AttentionAr
                 }
 #pragma unroll
                 for (int j = 0; j < DP / 32; ++j) {
-                    av[j] = mma<T>(L::col_frag(grads, kb * 32 + i * 16, j * 32), p[i], av[j]);
-                    ak[j] = mma<T>(L::col_frag(queries, kb * 32 + i * 16, j * 32), ds[i], ak[j]);
+                    av[j] = mma<T>(reader.columns(grads, kb * 32 + i * 16, j), p[i], av[j]);
+                    ak[j] = mma<T>(reader.columns(queries, kb * 32 + i * 16, j), ds[i], ak[j]);
                 }
             }
+        }
+    };
+    const auto place = [&](int n) { return base + n % 2 * kStage; };
+    // of each head's tiles, those before this wave's last key come first
+    const int edges = a.causal ? min((first + 32 + BN - 1) / BN - n0, each) : 0;
+    for (int n = 0, g = 0; g < group; ++g) {
+        int m = 0;
+        for (; m < edges; ++m, ++n) {
+            const int r = (n0 + m) * BN;
+            wait_and_meet<0>();
+            pass(n, r, place(n), place(n + 1), first < live && r + BN > first, std::true_type{});
+        }
+        for (; m < each; ++m, ++n) {
+            wait_and_meet<0>();
+            pass(n, (n0 + m) * BN, place(n), place(n + 1), first < live, std::false_type{});
         }
     }
     if (row >= live) return;

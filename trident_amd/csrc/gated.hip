@@ -83,14 +83,16 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* t
 // How the first and the second operand are read.
 enum Reading { kRowsRows, kColumnsRows, kColumnsColumns };
 
-template <typename T>
-constexpr int kStep = 128 / (int)sizeof(T);  // of the summed axis in LDS at a time
+// Of the summed axis, bytes of a stage in LDS; and the stages there at a time.  Operands that are both read by rows come in
+// whole lines of 128 bytes, two stages; else four of 64 (forward pass of 16,384 x 1,024 by 2 x 4,096 bfloat16 307 us, 315 by four of 64; its dx 252 by four, 268 by two).
+constexpr int stage_row(int read) { return read == kRowsRows ? 128 : 64; }
+constexpr int stages(int read) { return read == kRowsRows ? 2 : 4; }
 
-// A tile of `ROWS` operand rows (by columns: columns) and kStep of the summed axis, and its loads.
-template <typename T, bool COLUMNS, int ROWS, int WAVES>
+// A stage of `ROWS` operand rows (by columns: columns) and ROW bytes of the summed axis, and its loads.
+template <typename T, bool COLUMNS, int ROWS, int ROW, int WAVES>
 struct OperandTile {
-    static constexpr int kPitch = COLUMNS ? ROWS * (int)sizeof(T) : 128;
-    static constexpr int kBytes = ROWS * 128, kLoads = kBytes / 1024 / WAVES;
+    static constexpr int kStep = ROW / (int)sizeof(T), kPitch = COLUMNS ? ROWS * (int)sizeof(T) : ROW;
+    static constexpr int kBytes = ROWS * ROW, kLoads = kBytes / 1024 / WAVES;
     static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
     using L = Tile<T, kPitch>;
     const uint8_t* base;
@@ -111,21 +113,21 @@ struct OperandTile {
             at[i] = there ? (uint32_t)r * (uint32_t)pitch + piece * 16 : kPastBuffer;
         }
     }
-    __device__ __forceinline__ void fetch(uint8_t* to, int step, int wave) const {
-        const int k = step * kStep<T>, left = length - k;
+    __device__ __forceinline__ void fetch(lds_bytes to, int step, int wave) const {
+        const int k = step * kStep, left = length - k;
         if constexpr (COLUMNS) {
             const __amdgpu_buffer_rsrc_t buf =
-                buffer_of(base + k * pitch, (uint32_t)min(left, kStep<T>) * (uint32_t)pitch);
+                buffer_of(base + k * pitch, (uint32_t)min(left, kStep) * (uint32_t)pitch);
 #pragma unroll
             for (int i = 0; i < kLoads; ++i)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(buf, (lds_ptr)(to + (i * WAVES + wave) * 1024), 16, at[i], 0, 0, 0);
         } else {
-            const __amdgpu_buffer_rsrc_t buf = buffer_of(base + (int64_t)step * 128, 0x7fffffffu);
+            const __amdgpu_buffer_rsrc_t buf = buffer_of(base + (int64_t)step * ROW, 0x7fffffffu);
             const int lane = lane_id(), slot = lane % L::kPieces;
 #pragma unroll
             for (int i = 0; i < kLoads; ++i) {
                 uint32_t from = at[i];
-                if (left < kStep<T>) {  // columns past the last one are zeros
+                if (left < kStep) {  // columns past the last one are zeros
                     const int r = (i * WAVES + wave) * L::kRowsAtOnce + lane / L::kPieces;
                     if ((slot ^ L::exchange(r)) * (16 / (int)sizeof(T)) >= left) from = kPastBuffer;
                 }
@@ -140,9 +142,9 @@ struct OperandTile {
     }
 };
 
-// A workgroup of WM x WN waves computes WM MT x WN NT blocks of 32 x 32, a wave MT x NT.  A step's tiles of both operands go
-// straight from memory to LDS, the next step's while this one's are multiplied.  The first operand gives the result's columns,
-// so a lane holds four neighbours of a row.
+// A workgroup of WM x WN waves computes WM MT x WN NT blocks of 32 x 32, a wave MT x NT.  Stages of both operands go
+// straight from memory to LDS, ahead of the one that is multiplied.  The first operand gives the result's columns, so a
+// lane holds four neighbours of a row.
 //
 // GATED: the first operand's tile is half gate, half up, and each wave's blocks too, so that a lane holds both sums
 // of the same places: out[0] = act(g) u, and g and u themselves where KEEP.
@@ -150,9 +152,10 @@ template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool
 __device__ __forceinline__ void product(const ProductArgs& a) {
     constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32;
     constexpr int BR = GATED ? BN / 2 : BN;  // the result's columns
-    using First = OperandTile<T, READ != kRowsRows, BR, kWaves>;
-    using Second = OperandTile<T, READ == kColumnsColumns, BM, kWaves>;
-    constexpr int kFirst = BN * 128, kStage = kFirst + Second::kBytes;
+    constexpr int kRow = stage_row(READ), kStep = kRow / (int)sizeof(T), kStages = stages(READ);
+    using First = OperandTile<T, READ != kRowsRows, BR, kRow, kWaves>;
+    using Second = OperandTile<T, READ == kColumnsColumns, BM, kRow, kWaves>;
+    constexpr int kFirst = BN * kRow, kStage = kFirst + Second::kBytes, G = kStep / 16;
     extern __shared__ __align__(16) uint8_t lds[];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), half = lane >> 5;
     int tm, tn;
@@ -167,9 +170,10 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
         if constexpr (GATED) first[1].start(a.first[1], n0, a.N, a.K, wave);
         second.start(a.second[part + z], m0, a.M, a.K, wave);
     };
-    const int each = (a.K + kStep<T> - 1) / kStep<T>, steps = each * a.parts;
-    const auto fetch = [&](int n) {
-        uint8_t* to = lds + n % 2 * kStage;
+    const int each = (a.K + kStep - 1) / kStep, steps = each * a.parts;
+    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
+    const auto fetch = [&](int n, lds_bytes to) {
+        if (n >= steps) return;
         const int step = n < each ? n : n - each;
         if (n == each) begin(1);
         first[0].fetch(to, step, wave);
@@ -177,72 +181,114 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
         second.fetch(to + kFirst, step, wave);
     };
     begin(0);
-    fetch(0);
+    constexpr int kAhead = READ == kRowsRows ? 2 : kStages - 1;  // stages loaded before the first is read
+#pragma unroll
+    for (int n = 0; n < kAhead; ++n) fetch(n, base + n * kStage);
 
-    if (steps > 1) fetch(1);
-
+    constexpr int kSets = READ == kRowsRows ? G : 2;  // groups held
     f32x16 acc[MT][NT] = {};
-    const lds_bytes base = (lds_bytes)(lds_ptr)lds;
-    // A step's next loads are issued as soon as every wave holds its part of it in registers, halfway through its products,
-    // so that they have a step and a half to arrive.
-    constexpr int kFlight = (GATED ? 2 : 1) * First::kLoads + Second::kLoads, kHalf = kStep<T> / 32;
-    for (int n = 0; n < steps; ++n) {
-        if (n + 1 < steps) wait_and_meet<kFlight>();
-        else wait_and_meet<0>();
-        const lds_bytes t1 = base + n % 2 * kStage, t2 = t1 + kFirst;
-        frag<T> f1[2][kHalf][NT], f2[2][kHalf][MT];
+    frag<T> f1[kSets][NT], f2[kSets][MT];
+    const auto read = [&](lds_bytes from, int g, int set) {
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf)
-#pragma unroll
-            for (int s = 0; s < kHalf; ++s) {
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if constexpr (GATED) {  // the wave's first half of blocks from the gate's tile
-                        f1[hf][s][j] = First::read(t1 + (j < NT / 2 ? 0 : kFirst / 2), wn / 2 + j % (NT / 2) * 32,
-                                                   hf * kHalf + s);
-                    } else {
-                        f1[hf][s][j] = First::read(t1, wn + j * 32, hf * kHalf + s);
-                    }
-                }
-#pragma unroll
-                for (int i = 0; i < MT; ++i) f2[hf][s][i] = Second::read(t2, wm + i * 32, hf * kHalf + s);
-            }
-        const auto multiply = [&](int hf) {
-#pragma unroll
-            for (int s = 0; s < kHalf; ++s)
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) acc[i][j] = mma<T>(f1[hf][s][j], f2[hf][s][i], acc[i][j]);
-        };
-        multiply(0);
-        if constexpr (sizeof(T) == 2) {
-            // the first half's reads, the second half's among the first half's products
-            constexpr int kReads = kHalf * (NT * (READ != kRowsRows ? 2 : 1) + MT * (READ == kColumnsColumns ? 2 : 1));
-            constexpr int kProducts = kHalf * MT * NT, kEach = (kReads + kProducts - 1) / kProducts;
-            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
-#pragma unroll
-            for (int i = 0; i < kProducts; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+        for (int j = 0; j < NT; ++j) {
+            if constexpr (GATED) {  // the wave's first half of blocks from the gate's tile
+                f1[set][j] = First::read(from + (j < NT / 2 ? 0 : kFirst / 2), wn / 2 + j % (NT / 2) * 32, g);
+            } else {
+                f1[set][j] = First::read(from, wn + j * 32, g);
             }
         }
-        // the first half's products stay before the wait (the compiler would sink them past it)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) f2[set][i] = Second::read(from + kFirst, wm + i * 32, g);
+    };
+    const auto multiply = [&](int set) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
-            for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        __builtin_amdgcn_s_barrier();  // every wave has read the step
-        asm volatile("" ::: "memory");
-        if (n + 2 < steps) fetch(n + 2);
-        multiply(1);
+            for (int j = 0; j < NT; ++j) acc[i][j] = mma<T>(f1[set][j], f2[set][i], acc[i][j]);
+    };
+    constexpr int kFlight = (GATED ? 2 : 1) * First::kLoads + Second::kLoads;  // a wave's loads of one stage
+    if constexpr (READ == kRowsRows) {
+        // A stage's next loads are issued as soon as every wave holds its part of it in registers, halfway through its
+        // products, so that they have a stage and a half to arrive.
+        for (int n = 0; n < steps; ++n) {
+            if (n + 1 < steps) wait_and_meet<kFlight>();
+            else wait_and_meet<0>();
+            const lds_bytes from = base + n % 2 * kStage;
+#pragma unroll
+            for (int g = 0; g < G; ++g) read(from, g, g);
+#pragma unroll
+            for (int g = 0; g < G / 2; ++g) multiply(g);
+            if constexpr (sizeof(T) == 2) {
+                // the first half's reads, the second half's among the first half's products
+                constexpr int kReads = G / 2 * (NT + MT), kProducts = G / 2 * MT * NT;
+                constexpr int kEach = (kReads + kProducts - 1) / kProducts;
+                __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+#pragma unroll
+                for (int i = 0; i < kProducts; ++i) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);
+                }
+            }
+            // the first half's products stay before the wait (the compiler would sink them past it)
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) asm volatile("" : "+v"(acc[i][j]));
+            meet();  // every wave has read the stage
+            fetch(n + 2, from);
+#pragma unroll
+            for (int g = G / 2; g < G; ++g) multiply(g);
+        }
+    } else {
+        // One barrier a stage, past which it has arrived and the one before is no longer read; a group's blocks are read
+        // while the group before is multiplied.  What is loaded and what is read between two barriers lie in different
+        // stages, which __restrict says: else the compiler waits for every load before a transposing read.
+        const auto body = [&](int n, lds_bytes __restrict from, lds_bytes __restrict to, int of, bool before) {
+            fetch(n + kStages - 1, to);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const int set = (of + g) % 2;
+                read(from, g, set);
+                if (g > 0 || before) multiply(1 - set);
+            }
+        };
+        const auto arrive = [&](int n) {
+            if (n + 2 < steps) wait_and_meet<2 * kFlight>();
+            else if (n + 1 < steps) wait_and_meet<kFlight>();
+            else wait_and_meet<0>();
+        };
+        const auto stage = [&](int n) { return base + n % kStages * kStage; };
+        arrive(0);
+        body(0, stage(0), stage(kStages - 1), 0, false);
+        int n = 1;
+        if constexpr (G == 2) {
+            for (; n < steps; ++n) {
+                arrive(n);
+                body(n, stage(n), stage(n + kStages - 1), 0, true);
+            }
+            multiply(1);
+        } else {
+            static_assert(G == 1, "groups of a stage");
+            for (; n + 1 < steps; n += 2) {
+                arrive(n);
+                body(n, stage(n), stage(n + kStages - 1), 1, true);
+                arrive(n + 1);
+                body(n + 1, stage(n + 1), stage(n + kStages), 0, true);
+            }
+            if (n < steps) {
+                arrive(n);
+                body(n, stage(n), stage(n + kStages - 1), 1, true);
+                multiply(1);
+            } else {
+                multiply(0);
+            }
+        }
     }
     // Results go through LDS, 32 rows of a wave at a time, so that whole lines are written.
     wait_and_meet<0>();
     constexpr int kBlocks = GATED ? NT / 2 : NT, kCols = kBlocks * 32, kPitch = kCols * (int)sizeof(T) + 16;
     constexpr int kPer = 16 / (int)sizeof(T), kRowPieces = kCols / kPer, kRowsAtOnce = kWave / kRowPieces;
-    static_assert(kWaves * 32 * kPitch <= 2 * kStage, "the results fit where the operands were");
+    static_assert(kWaves * 32 * kPitch <= kStages * kStage, "the results fit where the operands were");
     uint8_t* mine = lds + wave * 32 * kPitch;
     const int col = n0 + (GATED ? wn / 2 : wn) + lane % kRowPieces * kPer, left = a.N - col;
     const auto put = [&](int i, void* out, auto&& value) {
@@ -298,7 +344,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void product_kernel(ProductArgs a) {
 template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
 int launch_product(ProductArgs a, int results, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32, BR = GATED ? BN / 2 : BN;
-    constexpr size_t lds = 2 * (size_t)(BM + BN) * 128;
+    constexpr size_t lds = stages(READ) * (size_t)(BM + BN) * stage_row(READ);
     static_assert(lds <= 163840, "LDS of a CU");
     const auto kernel = product_kernel<T, READ, WM, WN, MT, NT, GATED, KEEP>;
     if (lds > 65536) {

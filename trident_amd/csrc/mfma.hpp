@@ -16,7 +16,7 @@ namespace trident {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* lds_ptr;
-typedef const __attribute__((address_space(3))) uint8_t* lds_bytes;
+typedef __attribute__((address_space(3))) uint8_t* lds_bytes;
 
 template <typename T>
 struct FragOf {
@@ -98,6 +98,63 @@ struct Tile {
     }
     static __device__ __forceinline__ frag<T> col_frag_in_order(lds_bytes tile, int row, int col) {
         return read_columns<true>(tile, row, col);
+    }
+};
+
+// A barrier for waves that hold what they read from LDS.
+__device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// A lane's places in such tiles, made once: of its first row's DP / 16 steps, and of its first column of DP / 32 blocks, in a
+// result's order.  A read is then one addition and a constant.
+template <typename T, int PITCH, int DP>
+struct TileReader {
+    using L = Tile<T, PITCH>;
+    static constexpr bool kPlaces = sizeof(T) == 2;
+    uint32_t row_at[DP / 16], col_at[2][DP / 32];
+
+    __device__ __forceinline__ TileReader() {
+        if constexpr (kPlaces) {
+            const int lane = lane_id(), row = lane & 31, half = lane >> 5;
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                row_at[i] = row * PITCH + (((2 * i + half) ^ L::exchange(row)) << 4);
+                asm volatile("" : "+v"(row_at[i]));  // not made again for every read
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    const int in = 4 * half + (lane >> 2 & 3) + 8 * h;
+                    const int piece = (lane >> 4 & 1) * 2 + (lane >> 1 & 1) + 4 * j;
+                    col_at[h][j] = in * PITCH + (lane & 1) * 8 + ((piece ^ L::exchange(in)) << 4);
+                    asm volatile("" : "+v"(col_at[h][j]));
+                }
+        }
+    }
+    // row_frag of row block * 32 + lane % 32
+    __device__ __forceinline__ frag<T> rows(lds_bytes tile, int block, int step) const {
+        if constexpr (kPlaces) {
+            typedef const __attribute__((address_space(3))) u32x4* words;
+            return __builtin_bit_cast(frag<T>, *(words)(tile + row_at[step] + block * 32 * PITCH));
+        } else {
+            return L::row_frag(tile, block * 32 + (lane_id() & 31), step);
+        }
+    }
+    // col_frag of columns j * 32 ..
+    __device__ __forceinline__ frag<T> columns(lds_bytes tile, int row, int j) const {
+        if constexpr (kPlaces) {
+            typedef short s16x4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s16x4* quads;
+            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((quads)(tile + col_at[0][j] + row * PITCH));
+            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((quads)(tile + col_at[1][j] + row * PITCH));
+            return __builtin_bit_cast(frag<T>, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            return L::col_frag(tile, row, j * 32);
+        }
     }
 };
 
