@@ -408,7 +408,8 @@ typedef struct TridentAttention {
 
 int trident_attention(const TridentAttention* a, void* stream);
 
-/* dq, dk, dv from grad (of out), what the forward pass took, its out and its lse. */
+/* dq, dk, dv from grad (of out), what the forward pass took, its out and its lse.  The workspace's size is asked for with
+ * all arguments in place. */
 size_t trident_attention_grad_workspace_bytes(const TridentAttention* a);
 int trident_attention_grad(const TridentAttention* a, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -20,9 +20,13 @@ template <typename T>
 constexpr float kShift = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
 constexpr float kSlack = 8.0f;
 
-template <typename T, int DP, int WAVES>
-__global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <= 64) ? 2 : 1) void attention_kernel(AttentionArgs a) {
-    constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
+// Waves of a workgroup, 32 queries each.  Short sequences leave some without a row, and still four load their keys sooner: 12 heads of
+// 64, bfloat16, one sequence of 16 tokens 3.8 us (one wave 4.5), 1,000 of them 44 (50).
+constexpr int kWaves = 4;
+
+template <typename T, int DP, bool CAUSAL>
+__global__ __launch_bounds__(kWaves* kWave, sizeof(T) == 2 || DP <= 64 ? 2 : 1) void attention_kernel(AttentionArgs a) {
+    constexpr int BM = kWaves * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
     extern __shared__ __align__(16) uint8_t lds[];  // [2][keys, values]
     int tile, h, hk;
@@ -33,18 +37,18 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <=
     const int64_t out_row = (int64_t)a.Hq * a.D;
     T* out = static_cast<T*>(a.out) + t.start * out_row + (int64_t)h * a.D;
     const int live = min(t.first + BM, t.length);  // rows past it are slots without a token
-    if (live < t.first + BM) zero_rows(out, out_row, max(live, t.first), min(t.first + BM, t.extent), a.D, WAVES * kWave);
+    if (live < t.first + BM) zero_rows(out, out_row, max(live, t.first), min(t.first + BM, t.extent), a.D, kWaves * kWave);
     if (live <= t.first) return;
 
     const uint8_t* k = static_cast<const uint8_t*>(a.k) + t.start * a.k_row + hk * a.k_head;
     const uint8_t* v = static_cast<const uint8_t*>(a.v) + t.start * a.v_row + hk * a.v_head;
     const int bytes = a.D * (int)sizeof(T);
-    const int tiles = ((a.causal ? live : t.length) + BN - 1) / BN;
+    const int tiles = ((CAUSAL ? live : t.length) + BN - 1) / BN;
     const lds_bytes base = (lds_bytes)(lds_ptr)lds;
     const auto fetch = [&](int n, lds_bytes to) {
         if (n >= tiles) return;
-        fetch_tile<T, kPitch, BN, WAVES>(to, k + (int64_t)n * BN * a.k_row, a.k_row, t.length - n * BN, bytes, wave);
-        fetch_tile<T, kPitch, BN, WAVES>(to + kTile, v + (int64_t)n * BN * a.v_row, a.v_row, t.length - n * BN, bytes,
+        fetch_tile<T, kPitch, BN, kWaves>(to, k + (int64_t)n * BN * a.k_row, a.k_row, t.length - n * BN, bytes, wave);
+        fetch_tile<T, kPitch, BN, kWaves>(to + kTile, v + (int64_t)n * BN * a.v_row, a.v_row, t.length - n * BN, bytes,
                                          wave);
     };
     fetch(0, base);
@@ -55,7 +59,7 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <=
     arrived(q);
     f32x16 acc[DP / 32] = {};
     float top = -INFINITY, sum = 0.0f;  // the reference, times scale2, and this half's part of the sum
-    const int end = a.causal ? min(row + 1, t.length) : t.length;  // the keys that this row sees
+    const int end = CAUSAL ? min(row + 1, t.length) : t.length;  // the keys that this row sees
 
     const TileReader<T, kPitch, DP> reader;
     f32x16 s[KB];
@@ -103,33 +107,33 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <=
                 sum += e;
             }
     };
+    bool not_finite = false;
     const auto add_values = [&](int n, lds_bytes values, auto edge) {
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb) {
-            // causal: blocks past the last row are left out, those on the diagonal looked at first
             const int key = n * BN + kb * 32;
-            bool apart = false;
-            if constexpr (decltype(edge)::value) {
-                if (a.causal && key > last) continue;
-                apart = a.causal && key >= first && any_not_finite<T, kPitch>(values + kb * 32 * kPitch);
+            bool apart = false;  // on the diagonal and not finite
+            if constexpr (CAUSAL && decltype(edge)::value) {
+                if (key > last) continue;
+                apart = key >= first && any_not_finite<T, kPitch>(values + kb * 32 * kPitch);
+                not_finite |= apart;
             }
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (decltype(edge)::value && apart) {
-                    add_seen_rows<T, kPitch, DP>(values, kb * 32 + i * 16, p[kb][i], acc,
-                                                 [&](int r) { return key + i * 16 + r <= row; });
-                    continue;
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < DP / 32; ++j) {
+                    frag<T> f = reader.columns(values, kb * 32 + i * 16, j);
+                    if constexpr (CAUSAL && decltype(edge)::value) {
+                        if (apart) f = finite_only<T>(f);
+                    }
+                    acc[j] = mma<T>(f, p[kb][i], acc[j]);
                 }
-#pragma unroll
-                for (int j = 0; j < DP / 32; ++j)
-                    acc[j] = mma<T>(reader.columns(values, kb * 32 + i * 16, j), p[kb][i], acc[j]);
-            }
         }
     };
     // Tiles that every row of the wave sees whole, those that some see in part, and (in step with the other waves) the
     // rest, for which this wave only loads.
-    const int whole = first >= live ? 0 : (a.causal ? min(first + 1, t.length) : t.length) / BN;
-    const int seen = first >= live ? 0 : a.causal ? min(last / BN + 1, tiles) : tiles;
+    const int whole = first >= live ? 0 : (CAUSAL ? min(first + 1, t.length) : t.length) / BN;
+    const int seen = first >= live ? 0 : CAUSAL ? min(last / BN + 1, tiles) : tiles;
     constexpr std::false_type kWhole{};
     constexpr std::true_type kEdge{};
     // Past a barrier tile n is there, and every wave is done with the one before, in whose place the next one goes.  That lies
@@ -151,17 +155,22 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 1 && (sizeof(T) == 2 || DP <=
         wait_and_meet<0>();
         pass(n, place(n), place(n + 1), n < seen, kEdge);
     }
+    if constexpr (CAUSAL) {
+        if (not_finite)
+            add_not_finite<T, DP, false>(v + first * a.v_row, a.v_row, min(32, t.length - first), a.D, acc,
+                                         [&](int r) { return first + r <= row; });
+    }
     const float all = sum + other_half(sum);
     if (row >= live) return;
     store_column<T, DP>(out + (int64_t)row * out_row, a.D, acc, 1.0f / all);
     if (a.lse && half == 0) a.lse[h * a.rows + t.start + row] = top - kShift<T> + __builtin_amdgcn_logf(all);
 }
 
-template <typename T, int DP, int WAVES>
+template <typename T, int DP, bool CAUSAL>
 int launch(AttentionArgs a, hipStream_t st) {
-    constexpr int BM = WAVES * 32;
+    constexpr int BM = kWaves * 32;
     constexpr size_t lds = 4 * (size_t)kTileRows<T> * kTilePitch<T, DP>;
-    const auto kernel = attention_kernel<T, DP, WAVES>;
+    const auto kernel = attention_kernel<T, DP, CAUSAL>;
     static_assert(lds <= 163840, "LDS of a CU");
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
@@ -171,15 +180,8 @@ int launch(AttentionArgs a, hipStream_t st) {
     const int64_t tiles = a.slots ? a.count * ((a.slots + BM - 1) / BM) : a.rows / BM + a.count + 2;
     if (tiles * a.Hq > 0x7fffffff) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention: too many tiles");
     a.tiles = (int)tiles;
-    kernel<<<(unsigned)(tiles * a.Hq), WAVES * kWave, lds, st>>>(a);
+    kernel<<<(unsigned)(tiles * a.Hq), kWaves * kWave, lds, st>>>(a);
     return capi_check_launch("attention_kernel");
-}
-
-template <typename T, int DP>
-int by_length(const AttentionArgs& a, hipStream_t st) {
-    const int64_t mean = a.slots ? a.slots : a.rows / std::max<int64_t>(a.count, 1);
-    if (mean <= 32) return launch<T, DP, 1>(a, st);
-    return launch<T, DP, 4>(a, st);
 }
 
 }  // namespace
@@ -261,10 +263,13 @@ extern "C" int trident_attention(const TridentAttention* t, void* stream) {
     with_dtype(t->dtype, [&](auto e) {
         using T = decltype(e);
         const hipStream_t st = (hipStream_t)stream;
-        if (a.D <= 32) out = by_length<T, 32>(a, st);
-        else if (a.D <= 64) out = by_length<T, 64>(a, st);
-        else if (a.D <= 96) out = by_length<T, 96>(a, st);
-        else out = by_length<T, 128>(a, st);
+        with_bool(a.causal, [&](auto causal) {
+            constexpr bool CAUSAL = decltype(causal)::value;
+            if (a.D <= 32) out = launch<T, 32, CAUSAL>(a, st);
+            else if (a.D <= 64) out = launch<T, 64, CAUSAL>(a, st);
+            else if (a.D <= 96) out = launch<T, 96, CAUSAL>(a, st);
+            else out = launch<T, 128, CAUSAL>(a, st);
+        });
     });
     return out;
 }

@@ -12,12 +12,14 @@ struct AttentionArgs {
     void *out, *dq, *dk, *dv;
     float* lse;    // [Hq, rows], base 2
     float* delta;  // [Hq, rows]
+    float* part;   // of several shares: [2][shares][rows, Hkv, D]
     const void *offsets, *lengths;
     int64_t q_row, q_head, k_row, k_head, v_row, v_head;  // bytes
     int64_t rows, count;
     int slots;     // rows of a padded sequence, 0 if packed
     int wide;      // offsets and lengths are int64
     int Hq, Hkv, D, causal;
+    int shares;
     int tiles;     // of all sequences, at most
     float scale, scale2;  // scale2 = scale log2(e)
 };
@@ -146,25 +148,45 @@ __device__ __forceinline__ bool any_not_finite(lds_bytes rows) {
     return __any((seen & ~kMask) != 0);
 }
 
-// acc += rows^T p over 16 rows of a tile, p the second operand, for the rows that `sees(row)` leaves this lane's
-// column: the block on the diagonal of causal attention where a row is not finite.  A whole product would add zero
-// times infinity to the columns that do not see it, so the rows are multiplied one by one.  Slow, and rarely taken.
-template <typename T, int PITCH, int DP, typename F>
-__device__ __forceinline__ void add_seen_rows(lds_bytes tile, int row, const frag<T>& p, f32x16 (&acc)[DP / 32], F&& sees) {
+// The block on the diagonal of causal attention is seen in part by each column, and its product would add zero times
+// infinity where a row that is not finite is not seen.  So there such values are multiplied as zeros (finite_only), and
+// after the loop added to the columns that do see them (add_not_finite), from memory: slow, and rarely taken.
+template <typename T>
+__device__ __forceinline__ frag<T> finite_only(const frag<T>& f) {
+    if constexpr (sizeof(T) == 2) {
+        constexpr uint32_t kCarry = std::is_same<T, bf16_t>::value ? 0x00800080u : 0x04000400u;
+        u32x4 w = __builtin_bit_cast(u32x4, f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t past = ((w[e] & 0x7fff7fffu) + kCarry) & 0x80008000u;  // the sign's place: not finite
+            w[e] &= ~((past >> 15) * 0xffffu);
+        }
+        return __builtin_bit_cast(frag<T>, w);
+    } else {
+        frag<T> g;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) g[e] = fabsf(f[e]) < INFINITY ? f[e] : 0.0f;
+        return g;
+    }
+}
+
+// The values that are not finite in `rows` rows at p (NANS: a NaN for each) to the columns that `sees(row)` names.
+template <typename T, int DP, bool NANS, typename F>
+__device__ __forceinline__ void add_not_finite(const void* p, int64_t pitch, int rows, int D, f32x16 (&acc)[DP / 32],
+                                               F&& sees) {
     const int half = lane_id() >> 5;
 #pragma unroll 1
-    for (int r = 0; r < 16; ++r) {
-        const int mine = half == r / 4 % 2 ? r / 8 * 4 + r % 4 : -1;  // the lane's element of this row
+    for (int r = 0; r < rows; ++r) {
+        const T* x = reinterpret_cast<const T*>(static_cast<const uint8_t*>(p) + r * pitch);
         const bool seen = sees(r);
 #pragma unroll
-        for (int j = 0; j < DP / 32; ++j) {
-            frag<T> f = Tile<T, PITCH>::col_frag(tile, row, j * 32);
+        for (int j = 0; j < DP / 32; ++j)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = e == mine ? f[e] : (T)0.0f;
-            const f32x16 one = mma<T>(f, p, f32x16{});
-#pragma unroll
-            for (int i = 0; i < 16; ++i) acc[j][i] = seen ? acc[j][i] + one[i] : acc[j][i];
-        }
+            for (int i = 0; i < 16; ++i) {
+                const int col = 32 * j + 8 * (i / 4) + 4 * half + i % 4;
+                const float v = col < D ? (float)x[col] : 0.0f;
+                if (seen && !(fabsf(v) < INFINITY)) acc[j][i] += NANS ? NAN : v;
+            }
     }
 }
 
