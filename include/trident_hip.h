@@ -414,14 +414,15 @@ size_t trident_attention_grad_workspace_bytes(const TridentAttention* a);
 int trident_attention_grad(const TridentAttention* a, void* workspace, size_t workspace_bytes, void* stream);
 
 /* The gated half of a feed-forward block: h [M, N] = act(x gate_weight^T) * (x up_weight^T), x [M, K], both weights
- * [N, K], rows of the given pitches in elements.  gate and up [M, N]: the two products, kept for the backward
- * pass, or both NULL.  h, gate, up and the results of the backward pass are contiguous.  Rows that begin at 16-byte addresses
+ * [N, K], rows of the given pitches in elements.  gate and up [M, N] float32: the two products, kept for the
+ * backward pass, or both NULL.  h, gate, up and the results of the backward pass are contiguous.  Rows that begin at 16-byte addresses
  * and hold whole 16 bytes are taken as they are; the workspace is for others, and none for up to 16 rows. */
 enum TridentActivation { TRIDENT_SILU = 0, TRIDENT_GELU = 1, TRIDENT_GELU_TANH = 2 };
 
 typedef struct TridentGated {
     const void *x, *gate_weight, *up_weight;
-    void *h, *gate, *up;
+    void* h;
+    float *gate, *up;
     const void* grad;          /* of h: the backward pass's, as are the three below */
     void *dx, *dgate_weight, *dup_weight;
     int64_t M, N, K;

@@ -2,7 +2,7 @@
 
 Bounds: a sum of n float32 products is off by (n + 2) u times the sum of their magnitudes.  The activations' slopes are at
 most 1.13 in size and change by at most 0.8 a unit; their float32 evaluation is off by at most 16 u (1 + |g|).  g and u are
-kept, and dg, du multiplied, in the elements' type: U[dtype] relative each.
+kept in float32; dg, du are multiplied in the elements' type: U[dtype] relative.
 """
 import pytest
 import torch
@@ -38,7 +38,7 @@ def reference(x, wg, wu, act, grad=None):
         return res
     dh = grad.to(F64).reshape(g.shape)
     M, N = dh.shape
-    rg, ru = eg + Un * g.abs() + tiny, eu + Un * up.abs() + tiny  # of what is kept
+    rg, ru = eg + u * g.abs(), eu + u * up.abs()  # of what is kept
     ea, es = 1.13 * rg + 16 * u * (1 + g.abs()), 0.8 * rg + 16 * u * (1 + g.abs())
     dg, du = dh * up * slope, dh * a
     edg = dh.abs() * (ru * (slope.abs() + es) + up.abs() * es) + (Un + 3 * u) * dg.abs() + tiny

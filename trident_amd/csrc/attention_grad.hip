@@ -40,7 +40,7 @@ struct Power {
 
 // dq: as the forward pass, with the values' rows for dP and the keys' columns for dq.
 template <typename T, int DP, int WAVES, bool CAUSAL>
-__global__ __launch_bounds__(WAVES* kWave, sizeof(T) == 2 && DP <= 96 ? 2 : 1) void attention_dq_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 96 ? 2 : 1) void attention_dq_kernel(AttentionArgs a) {
     constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
     extern __shared__ __align__(16) uint8_t lds[];  // [2][keys, values]
@@ -167,7 +167,7 @@ __global__ __launch_bounds__(WAVES* kWave, sizeof(T) == 2 && DP <= 96 ? 2 : 1) v
 // LDS with the rows' lse and delta.  S is queries by keys, so a lane holds one key.  Rows past the
 // sequence's end are zeros in LDS, lse and delta among them, and add nothing.
 template <typename T, int DP, int WAVES, bool CAUSAL>
-__global__ __launch_bounds__(WAVES* kWave, sizeof(T) == 2 && DP <= 96 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 96 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
     constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
     constexpr int kStage = 2 * kTile + 2 * kWave * 4;  // queries, gradients, 64 words of lse and of delta

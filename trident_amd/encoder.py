@@ -971,7 +971,7 @@ def _gated(x, w_gate, w_up, activation, keep):
     gate = up = None
     a.h = h.data_ptr()
     if keep:
-        gate, up = x.new_empty(shape), x.new_empty(shape)
+        gate, up = (x.new_empty(shape, dtype=torch.float32) for _ in range(2))
         a.gate, a.up = gate.data_ptr(), up.data_ptr()
     if h.numel():
         at = ctypes.byref(a)
@@ -1008,7 +1008,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
 
 def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                          activation: str = "silu") -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(h, gate, up): ``gated_linear`` and its two products [..., N] in x's type, for the backward pass."""
+    """(h, gate, up): ``gated_linear`` and, for the backward pass, its two products [..., N] in float32."""
     if _forward_ad._current_level >= 0:
         _no_tangents("gated_linear_forward", x, w_gate, w_up)
     return _gated(x, w_gate, w_up, activation, True)
@@ -1026,10 +1026,12 @@ def _gated_grad(grad, x, w_gate, w_up, gate, up, activation, need_x, need_w):
         _no_tangents("gated_linear_grad", grad, x, w_gate, w_up, gate, up)
     a, kept, index = _gated_args(x, w_gate, w_up, activation)
     shape = (*x.shape[:-1], a.N)
-    for name, t in (("grad", grad), ("gate", gate), ("up", up)):
-        if t.shape != shape or t.dtype is not x.dtype or (name != "grad" and not t.is_contiguous()):
-            _refuse(f"{name} must be {shape} {x.dtype}{'' if name == 'grad' else ', contiguous'}, got {tuple(t.shape)} "
-                    f"{t.dtype}")
+    if grad.shape != shape or grad.dtype is not x.dtype:
+        _refuse(f"grad must be {shape} {x.dtype}, got {tuple(grad.shape)} {grad.dtype}")
+    _same(index, "grad", grad)
+    for name, t in (("gate", gate), ("up", up)):
+        if t.shape != shape or t.dtype is not torch.float32 or not t.is_contiguous():
+            _refuse(f"{name} must be contiguous float32 {shape}, got {t.dtype} {tuple(t.shape)}")
         _same(index, name, t)
     dx = x.new_empty(x.shape) if need_x else None
     dg, du = (x.new_empty(w_gate.shape), x.new_empty(w_up.shape)) if need_w else (None, None)
