@@ -74,7 +74,8 @@ def check(x, wg, wu, act, grad):
 
 
 SIZES = [(1, 1, 1), (1, 16, 64), (2, 17, 7), (16, 100, 960), (17, 33, 8), (16, 64, 1000), (33, 65, 72), (64, 64, 64),
-         (100, 130, 200), (129, 257, 136), (200, 96, 333), (300, 40, 1024), (777, 333, 100), (1030, 70, 48), (3, 2000, 515)]
+         (100, 130, 200), (129, 257, 136), (200, 96, 333), (300, 40, 1024), (777, 333, 100), (1030, 70, 48), (3, 2000, 515),
+         (100, 333, 2500), (33, 65, 2101), (64, 64, 4500), (5000, 40, 56), (2100, 70, 33), (1, 1, 3000), (17, 2600, 24)]
 
 
 @pytest.mark.parametrize("M,N,K", SIZES)

@@ -67,6 +67,8 @@ struct ProductArgs {
     int M, N, K;       // rows and columns of the result, length of a sum
     int parts;         // sums one after another
     int tiles_m, tiles_n, activation;
+    int shares;        // SPLIT: workgroups that share a tile's sum
+    float* part;       // [shares][sums of a place: gate and up, or the results][M, N]
 };
 
 // One of a grid's tiles in an order that keeps neighbours on one XCD: workgroups go to the eight XCDs, each
@@ -149,7 +151,9 @@ struct OperandTile {
 //
 // GATED: the first operand's tile is half gate, half up, and each wave's blocks too, so that a lane holds both sums
 // of the same places: out[0] = act(g) u, and g and u themselves where KEEP.
-template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
+//
+// SPLIT: a workgroup takes a share of the stages and writes its sums as they are, for the join.
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP, bool SPLIT>
 __device__ __forceinline__ void product(const ProductArgs& a) {
     constexpr int kWaves = WM * WN, BM = WM * MT * 32, BN = WN * NT * 32;
     constexpr int BR = GATED ? BN / 2 : BN;  // the result's columns
@@ -171,17 +175,19 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
         if constexpr (GATED) first[1].start(a.first[1], n0, a.N, a.K, wave);
         second.start(a.second[part + z], m0, a.M, a.K, wave);
     };
-    const int each = (a.K + kStep - 1) / kStep, steps = each * a.parts;
+    const int each = (a.K + kStep - 1) / kStep, total = each * a.parts;
+    const int from0 = SPLIT ? total * (int)blockIdx.z / a.shares : 0;
+    const int steps = SPLIT ? total * ((int)blockIdx.z + 1) / a.shares - from0 : total;
     const lds_bytes base = (lds_bytes)(lds_ptr)lds;
     const auto fetch = [&](int n, lds_bytes to) {
         if (n >= steps) return;
-        const int step = n < each ? n : n - each;
-        if (n == each) begin(1);
+        const int at = n + from0, step = at < each ? at : at - each;
+        if (at == each && n > 0) begin(1);
         first[0].fetch(to, step, wave);
         if constexpr (GATED) first[1].fetch(to + kFirst / 2, step, wave);
         second.fetch(to + kFirst, step, wave);
     };
-    begin(0);
+    begin(from0 >= each ? 1 : 0);
     constexpr int kAhead = READ == kRowsRows ? 2 : kStages - 1;  // stages loaded before the first is read
 #pragma unroll
     for (int n = 0; n < kAhead; ++n) fetch(n, base + n * kStage);
@@ -288,7 +294,7 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
     // Results go through LDS, 32 rows of a wave at a time, so that whole lines are written.
     wait_and_meet<0>();
     constexpr int kBlocks = GATED ? NT / 2 : NT, kCols = kBlocks * 32;
-    constexpr int kRegion = 32 * (kCols * (KEEP ? 4 : (int)sizeof(T)) + 16);  // a wave's, for the widest results
+    constexpr int kRegion = 32 * (kCols * (KEEP || SPLIT ? 4 : (int)sizeof(T)) + 16);  // a wave's, for the widest results
     static_assert(kWaves * kRegion <= kStages * kStage, "the results fit where the operands were");
     uint8_t* mine = lds + wave * kRegion;
     const auto put = [&](int i, auto* out, auto&& value) {
@@ -322,7 +328,12 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
     };
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
-        if constexpr (GATED) {
+        if constexpr (SPLIT) {
+            const int64_t plane = (int64_t)a.M * a.ldo;
+            float* to = a.part + (blockIdx.z * (GATED ? 2 : gridDim.y) + z) * plane;
+            put(i, to, [&](int j, int e) { return acc[i][j][e]; });
+            if constexpr (GATED) put(i, to + plane, [&](int j, int e) { return acc[i][j + kBlocks][e]; });
+        } else if constexpr (GATED) {
             put(i, static_cast<T*>(a.out[0]), [&](int j, int e) {
                 float v;
                 activate<false>(a.activation, acc[i][j][e], &v, nullptr);
@@ -340,17 +351,49 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
 
 // (A function of its own: with the body in the kernel template the compiler leaves out the host's half of some
 // instantiations.)
-template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP, bool SPLIT>
 __global__ __launch_bounds__(WM* WN* kWave) void product_kernel(ProductArgs a) {
-    product<T, READ, WM, WN, MT, NT, GATED, KEEP>(a);
+    product<T, READ, WM, WN, MT, NT, GATED, KEEP, SPLIT>(a);
 }
 
-template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP>
+// The sums of SPLIT workgroups, in order: four places a thread, or one where rows do not hold whole fours.
+template <typename T, int V, bool GATED, bool KEEP>
+__global__ __launch_bounds__(kBlock) void join_product_kernel(ProductArgs a, int results) {
+    const int64_t n = (int64_t)a.M * a.N, at = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * V;
+    if (at >= n) return;
+    constexpr int kSums = GATED ? 2 : 1;
+    float sum[kSums][V] = {};
+    for (int s = 0; s < a.shares; ++s)
+#pragma unroll
+        for (int k = 0; k < kSums; ++k) {
+            float f[V];
+            load_vec<float, V>(a.part + (s * (GATED ? 2 : results) + (GATED ? k : (int)blockIdx.y)) * n + at, f);
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[k][e] += f[e];
+        }
+    if constexpr (GATED) {
+        float h[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            activate<false>(a.activation, sum[0][e], &h[e], nullptr);
+            h[e] *= sum[1][e];
+        }
+        store_vec<T, V>(static_cast<T*>(a.out[0]) + at, h);
+        if constexpr (KEEP) {
+            store_vec<float, V>(static_cast<float*>(a.out[1]) + at, sum[0]);
+            store_vec<float, V>(static_cast<float*>(a.out[2]) + at, sum[1]);
+        }
+    } else {
+        store_vec<T, V>(static_cast<T*>(a.out[blockIdx.y]) + at, sum[0]);
+    }
+}
+
+template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP, bool SPLIT = false>
 int launch_product(ProductArgs a, int results, hipStream_t st) {
     constexpr int BM = WM * MT * 32, BN = WN * NT * 32, BR = GATED ? BN / 2 : BN;
     constexpr size_t lds = stages(READ) * (size_t)(BM + BN) * stage_row(READ);
     static_assert(lds <= 163840, "LDS of a CU");
-    const auto kernel = product_kernel<T, READ, WM, WN, MT, NT, GATED, KEEP>;
+    const auto kernel = product_kernel<T, READ, WM, WN, MT, NT, GATED, KEEP, SPLIT>;
     if (lds > 65536) {
         const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
@@ -360,8 +403,33 @@ int launch_product(ProductArgs a, int results, hipStream_t st) {
     a.tiles_n = (a.N + BR - 1) / BR;
     if ((int64_t)a.tiles_m * a.tiles_n > 0x7fffffff)
         return capi_fail(TRIDENT_ERR_UNSUPPORTED, "gated_linear: %d x %d is too large", a.M, a.N);
-    kernel<<<dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)results), WM * WN * kWave, lds, st>>>(a);
-    return capi_check_launch("product_kernel");
+    kernel<<<dim3((unsigned)(a.tiles_m * a.tiles_n), (unsigned)results, (unsigned)(SPLIT ? a.shares : 1)), WM * WN * kWave, lds,
+             st>>>(a);
+    const int rc = capi_check_launch("product_kernel");
+    if (!SPLIT || rc != TRIDENT_OK) return rc;
+    const int64_t n = (int64_t)a.M * a.N;
+    with_bool(a.N % 4 == 0, [&](auto fours) {
+        constexpr int V = decltype(fours)::value ? 4 : 1;
+        const dim3 grid((unsigned)((n / V + kBlock - 1) / kBlock), (unsigned)(GATED ? 1 : results));
+        join_product_kernel<T, V, GATED, KEEP><<<grid, kBlock, 0, st>>>(a, results);
+    });
+    return capi_check_launch("join_product_kernel");
+}
+
+// Workgroups that share the sum of a tile of 64 x 64, where the tiles leave CUs idle and the sum is long: a stage takes 0.3 us
+// (float32 1.2, or 0.6 of half the length) however few the tiles, the join another launch.  bfloat16, whole and shared: the
+// forward pass of 100 x 5,000 by 2 x 333 31 and 13 us, the backward pass of 16 x 960 by 2 x 2,560 48 and 19; float32
+// 176 and 26, 150 and 32.
+inline int shares_for(int64_t M, int64_t N, int results, int64_t K, int parts, bool rows, int64_t es) {
+    const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64) * results, row = (rows ? 128 : 64) / es;
+    const int64_t stages = (K + row - 1) / row * parts, length = stages * (es == 2 ? 1 : rows ? 4 : 2);
+    if (tiles < 1 || tiles > 192 || length < 32) return 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>({512 / tiles, length / 12, stages, 16}));
+}
+// Bytes of their sums.
+inline size_t part_bytes(int64_t M, int64_t N, int results, int64_t K, int parts, bool rows, int64_t es, int sums) {
+    const int shares = shares_for(M, N, results, K, parts, rows, es);
+    return shares > 1 ? (size_t)shares * sums * M * N * 4 : 0;
 }
 
 // The tile.  A larger one reads its operands less often (256 x 256: 64 bytes of LDS for 8,192 products), but takes a CU
@@ -369,10 +437,15 @@ int launch_product(ProductArgs a, int results, hipStream_t st) {
 // 128: the forward pass of 16,384 x 1,024 by 2 x 4,096, 2,048 tiles, 336 and 378 us; dx, 256 tiles, 265 and 330; but dWg and dWu,
 // 128 tiles, 445 and 315).  Where 128 x 128 leaves CUs idle, 64 x 64 (float32, 1,237 x 333 by 2 x 777: forward 39 to 32
 // us, dx 112 to 42, both weights 96 to 34).
+//
+// Few tiles of a long sum share it (shares_for), each with a join behind.
 template <typename T, int READ, bool GATED = false, bool KEEP = false>
-int product_of(const ProductArgs& a, int results, hipStream_t st) {
+int product_of(ProductArgs a, int results, float* part, hipStream_t st) {
     const auto tiles = [&](int64_t bm, int64_t bn) { return (a.M + bm - 1) / bm * ((a.N + bn - 1) / bn) * results; };
     constexpr int kShare = GATED ? 2 : 1;  // of a tile's columns are one of two sums
+    a.shares = shares_for(a.M, a.N, results, a.K, a.parts, READ == kRowsRows, sizeof(T));
+    a.part = part;
+    if (a.shares > 1) return launch_product<T, READ, 2, 2, 1, kShare, GATED, KEEP, true>(a, results, st);
     if constexpr (sizeof(T) == 2) {
         const int64_t large = tiles(256, 256 / kShare);
         if (large * 4 >= (large + 255) / 256 * 256 * 3)
@@ -587,13 +660,20 @@ size_t forward_bytes(const TridentGated* t) {
     if (t->M <= kFewRows) return 0;
     const int64_t es = size_of(t->dtype);
     return packed_bytes(t->x, t->ld_x, t->M, t->K, es) + packed_bytes(t->gate_weight, t->ld_gate, t->N, t->K, es) +
-           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es);
+           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + part_bytes(t->M, t->N, 1, t->K, 1, true, es, 2);
+}
+
+// Of dx and of the weights' gradients, which come one after the other.
+size_t backward_part(const TridentGated* t) {
+    const int64_t es = size_of(t->dtype);
+    return round_up(std::max(part_bytes(t->M, t->K, 1, t->N, 2, false, es, 1), part_bytes(t->N, t->K, 2, t->M, 1, false, es, 2)),
+                    256);
 }
 
 size_t backward_bytes(const TridentGated* t) {
     const int64_t es = size_of(t->dtype);
     return packed_bytes(t->x, t->ld_x, t->M, t->K, es) + packed_bytes(t->gate_weight, t->ld_gate, t->N, t->K, es) +
-           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + 2 * bytes_of(t->M, pitch_of(t->N, es), es);
+           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + 2 * bytes_of(t->M, pitch_of(t->N, es), es) + backward_part(t);
 }
 
 int check(const TridentGated* t, bool backward) {
@@ -636,13 +716,15 @@ int forward(const TridentGated* t, Scratch s, hipStream_t st) {
     a.K = (int)t->K;
     a.parts = 1;
     a.activation = t->activation;
-    if (keep) return product_of<T, kRowsRows, true, true>(a, 1, st);
-    return product_of<T, kRowsRows, true, false>(a, 1, st);
+    float* part = reinterpret_cast<float*>(s.p);
+    if (keep) return product_of<T, kRowsRows, true, true>(a, 1, part, st);
+    return product_of<T, kRowsRows, true, false>(a, 1, part, st);
 }
 
 template <typename T>
 int backward(const TridentGated* t, Scratch s, hipStream_t st) {
     const int64_t pitch = pitch_of(t->N, sizeof(T));
+    float* part = static_cast<float*>(s.take(backward_part(t)));
     SlopeArgs d{t->grad, t->gate, t->up, s.take(bytes_of(t->M, pitch, sizeof(T))), s.take(bytes_of(t->M, pitch, sizeof(T))),
                 t->ld_grad, t->N, pitch, t->M, (int)t->N, t->activation};
     slope_kernel<T><<<(unsigned)((t->M * (pitch / 8) + kBlock - 1) / kBlock), kBlock, 0, st>>>(d);
@@ -662,7 +744,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->N;
         a.parts = 2;
-        rc = product_of<T, kColumnsRows>(a, 1, st);
+        rc = product_of<T, kColumnsRows>(a, 1, part, st);
     }
     if (rc == TRIDENT_OK && t->dgate_weight) {
         ProductArgs a{};
@@ -677,7 +759,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->M;
         a.parts = 1;
-        rc = product_of<T, kColumnsColumns>(a, 2, st);
+        rc = product_of<T, kColumnsColumns>(a, 2, part, st);
     }
     return rc;
 }
