@@ -6,7 +6,8 @@ one passage.  Both become vectors by the same path,
 
     embedding (scaled rows, padded batches)  ->  layer norm  ->  mean over the tokens  ->  projection
 
-which is trained so that a query is nearest to its passage within the batch: the table's gradient is
+(with ``--layers N``, N transformer layers before that layer norm: attention over each passage's tokens,
+turned by their positions, and a gated feed-forward block), which is trained so that a query is nearest to its passage within the batch: the table's gradient is
 summed by ordered tokens, the table's optimizer keeps its moments in 8 bits, the small tensors' in 32.
 The corpus is then encoded with the projection in 8-bit floating point, indexed (TridentV4Index) and
 searched exactly, as are single queries.
@@ -50,8 +51,31 @@ def make_queries(ids, lengths, rows, tokens, g):
     return ids[rows][torch.arange(rows.numel(), device=ids.device)[:, None], at]
 
 
+class Layer:
+    """Attention and a gated feed-forward block, each on the layer norm of what it adds to."""
+
+    def __init__(self, dim, heads, g, device):
+        rand = lambda *s: (torch.randn(s, generator=g, device=device) / math.sqrt(s[-1])).requires_grad_()  # noqa: E731
+        self.heads, self.head_dim = heads, dim // heads
+        self.norms = [torch.ones(dim, device=device).requires_grad_() for _ in range(2)]
+        self.qkv, self.mix = rand(3 * dim, dim), rand(dim, dim)
+        self.gate, self.up, self.down = rand(2 * dim, dim), rand(2 * dim, dim), rand(dim, 2 * dim)
+        self.frequencies = encoder.rotary_frequencies(self.head_dim, device=device)
+
+    def parameters(self):
+        return [*self.norms, self.qkv, self.mix, self.gate, self.up, self.down]
+
+    def __call__(self, x, lengths):
+        B, L, dim = x.shape
+        qkv = (encoder.layer_norm(x, self.norms[0]) @ self.qkv.t()).view(B, L, 3 * self.heads, self.head_dim)
+        turned = encoder.rotary(qkv[:, :, :2 * self.heads], self.frequencies)  # queries and keys
+        q, k, v = turned[:, :, :self.heads], turned[:, :, self.heads:], qkv[:, :, 2 * self.heads:]
+        x = x + encoder.attention(q, k, v, lengths=lengths).reshape(B, L, dim) @ self.mix.t()
+        return x + encoder.gated_linear(encoder.layer_norm(x, self.norms[1]), self.gate, self.up) @ self.down.t()
+
+
 class TextEncoder:
-    def __init__(self, vocab, dim, out, g, device):
+    def __init__(self, vocab, dim, out, g, device, layers=0, heads=4):
         rand = lambda *s: torch.randn(s, generator=g, device=device)  # noqa: E731
         self.scale = math.sqrt(dim)
         self.table = (rand(vocab, dim) / self.scale).requires_grad_()
@@ -59,11 +83,17 @@ class TextEncoder:
         self.beta = torch.zeros(dim, device=device).requires_grad_()
         self.weight = (rand(out, dim) / self.scale).requires_grad_()
         self.bias = torch.zeros(out, device=device).requires_grad_()
+        self.layers = [Layer(dim, heads, g, device) for _ in range(layers)]
         self.optimizers = [encoder.AdamW([self.table], lr=3e-3, weight_decay=0.0, state_bits=8),
                            encoder.AdamW([self.gamma, self.beta, self.weight, self.bias], lr=3e-3)]
+        if layers:
+            self.optimizers.append(encoder.AdamW([p for layer in self.layers for p in layer.parameters()], lr=1e-3))
 
     def pooled(self, ids):
         x = encoder.embedding(ids, self.table, scale=self.scale)
+        lengths = (ids >= 0).sum(1) if self.layers else None
+        for layer in self.layers:
+            x = layer(x, lengths)
         x = encoder.layer_norm(x, self.gamma, self.beta)
         live = (ids >= 0).unsqueeze(-1).float()
         return (x * live).sum(1) / live.sum(1).clamp(min=1.0)
@@ -94,6 +124,8 @@ def main(argv=None):
     ap.add_argument("--vocab", type=int, default=32768)
     ap.add_argument("--dim", type=int, default=256, help="columns of the table")
     ap.add_argument("--out", type=int, default=128, help="dimensions of the vectors")
+    ap.add_argument("--layers", type=int, default=0, help="transformer layers between the table and the mean")
+    ap.add_argument("--heads", type=int, default=4, help="attention heads of a layer: dim / heads a multiple of 8 up to 128")
     ap.add_argument("--passages", type=int, default=20000)
     ap.add_argument("--length", type=int, default=64, help="tokens of a passage at most")
     ap.add_argument("--steps", type=int, default=200)
@@ -105,7 +137,7 @@ def main(argv=None):
     device = torch.device("cuda:0")
     g = torch.Generator(device=device).manual_seed(a.seed)
     ids, lengths = make_corpus(a.passages, a.vocab, a.length, g, device)
-    model = TextEncoder(a.vocab, a.dim, a.out, g, device)
+    model = TextEncoder(a.vocab, a.dim, a.out, g, device, a.layers, a.heads)
 
     losses, began = [], time.perf_counter()
     for step in range(a.steps):

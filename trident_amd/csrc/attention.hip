@@ -178,7 +178,7 @@ int launch(AttentionArgs a, hipStream_t st) {
         if (e != hipSuccess) return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(attention): %s", hipGetErrorString(e));
     }
     const int64_t tiles = a.slots ? a.count * ((a.slots + BM - 1) / BM) : a.rows / BM + a.count + 2;
-    if (tiles * a.Hq > 0x7fffffff) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention: too many tiles");
+    if (tiles * a.Hq > kMaxGroups) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention: too many tiles");
     a.tiles = (int)tiles;
     kernel<<<(unsigned)(tiles * a.Hq), kWaves * kWave, lds, st>>>(a);
     return capi_check_launch("attention_kernel");

@@ -6,6 +6,7 @@
 namespace trident {
 
 constexpr int kMaxHeadDim = 128;
+constexpr int64_t kMaxGroups = 0xffffff;  // workgroups of 256 threads: a launch has fewer than 2^32 threads
 
 struct AttentionArgs {
     const void *q, *k, *v, *grad;

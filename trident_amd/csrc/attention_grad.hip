@@ -393,7 +393,7 @@ int launch(AttentionArgs a, hipStream_t st) {
                 return capi_fail(TRIDENT_ERR_HIP, "hipFuncSetAttribute(attention_grad): %s", hipGetErrorString(e));
         }
     const int64_t tiles = a.slots ? a.count * ((a.slots + BM - 1) / BM) : a.rows / BM + a.count + 2;
-    if (tiles * std::max(a.Hq, a.Hkv * a.shares) > 0x7fffffff) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention_grad: too many tiles");
+    if (tiles * std::max(a.Hq, a.Hkv * a.shares) > kMaxGroups) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "attention_grad: too many tiles");
     a.tiles = (int)tiles;
     dq<<<(unsigned)(tiles * a.Hq), WAVES * kWave, lds, st>>>(a);
     int rc = capi_check_launch("attention_dq_kernel");

@@ -129,16 +129,19 @@ extern "C" int trident_rotary(const void* x, int32_t dtype, int64_t tokens, int6
                          "rotary: bad sizes tokens=%lld heads=%lld head_dim=%lld pairs=%lld period=%lld",
                          (long long)tokens, (long long)heads, (long long)head_dim, (long long)pairs, (long long)period);
     if (pairs > kAngles) return capi_fail(TRIDENT_ERR_UNSUPPORTED, "rotary: %lld pairs", (long long)pairs);
+    // as many tokens as leave every CU eight workgroups
+    const int64_t most = std::min<int64_t>(kAngles / std::max<int64_t>(pairs, 1), 16);
+    const int64_t tokens_each = std::max<int64_t>(1, std::min(most, tokens / 2048));
+    if (tokens / tokens_each >= 0xffffff)  // a launch has fewer than 2^32 threads
+        return capi_fail(TRIDENT_ERR_UNSUPPORTED, "rotary: %lld tokens of %lld pairs are too many", (long long)tokens,
+                         (long long)pairs);
     if (!(amplitude > -1e30 && amplitude < 1e30))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "rotary: amplitude=%g", amplitude);
     if (tokens == 0 || heads == 0) return TRIDENT_OK;
     if (!x || !out || (pairs && !frequencies)) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "rotary: NULL pointer");
     RotaryArgs a{x, out, frequencies, positions, x_row, x_head, out_row, out_head, tokens, period, (int)heads,
-                 (int)head_dim, (int)pairs, 1, ids64, interleaved != 0, x != out, (float)amplitude,
+                 (int)head_dim, (int)pairs, (int)tokens_each, ids64, interleaved != 0, x != out, (float)amplitude,
                  inverse ? -1.0f : 1.0f};
-    // as many tokens as leave every CU eight workgroups
-    const int64_t most = std::min<int64_t>(kAngles / std::max<int64_t>(pairs, 1), 16);
-    a.tokens_each = (int)std::max<int64_t>(1, std::min(most, tokens / 2048));
     int rc = TRIDENT_OK;
     with_dtype(dtype, [&](auto e) {
         using T = decltype(e);
