@@ -210,3 +210,27 @@ def test_no_forward_mode_derivative(on_gpu):
                      lambda: encoder.gated_linear(d, w, w), lambda: encoder.gated_linear_forward(d, w, w)):
             with pytest.raises(_lib.TridentError, match="forward-mode"):
                 call()
+
+
+def test_outputs_whose_elements_share_places():
+    """_apart against the set of the places themselves."""
+    for D in (1, 3):
+        for heads in (1, 2, 4):
+            for tokens in (2, 5):
+                for head in range(1, 20):
+                    for row in range(1, 20):
+                        places = {t * row + h * head + d for t in range(tokens) for h in range(heads) for d in range(D)}
+                        if encoder._apart(row, head if heads > 1 else D, tokens, heads, D):
+                            assert len(places) == tokens * heads * D, (D, heads, tokens, head, row)
+    for heads_within in (True, False):  # the usual orders are taken
+        row, head = (12, 3) if heads_within else (3, 15)
+        assert encoder._apart(row, head, 5, 4, 3)
+
+
+def test_rotary_refuses_what_it_has_no_gradient_for(on_gpu):
+    x, f = torch.zeros((5, 3, 8)), torch.zeros(4, dtype=torch.float64)
+    with pytest.raises(_lib.TridentError, match="no gradient"):
+        encoder.rotary(x, f.requires_grad_())
+    out = torch.zeros(64).as_strided((5, 3, 8), (8, 8, 1))  # token t + 1 of one head is token t of the next
+    with pytest.raises(_lib.TridentError, match="one place"):
+        encoder.rotary(x, f.detach(), out=out)

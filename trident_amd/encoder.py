@@ -11,8 +11,8 @@
 
 ``embedding``, ``layer_norm``, ``rotary``, ``attention`` and ``gated_linear`` take part in autograd; the
 ``*_forward`` / ``*_grad`` functions are the bare passes; the 8-bit products have no gradient and refuse
-operands that require one.  Tensors with a forward-mode tangent are refused.  Tensors are float32, float16 or bfloat16 on one GPU; sums, statistics
-and states are float32 and every result is rounded once.  Each call runs on the current stream of its
+operands that require one.  Tensors with a forward-mode tangent are refused.  Tensors are float32, float16
+or bfloat16 on one GPU; sums, statistics and states are float32 and every result is rounded once.  Each call runs on the current stream of its
 tensors' device, with the library's workspace of that stream (``trident_amd.ext.workspace``), or, while a
 graph is captured there, with scratch of the graph's own; results are the same bits every time.  Wrong
 arguments raise ``TridentError``.
@@ -687,9 +687,10 @@ def _heads(t: torch.Tensor) -> Tuple[torch.Tensor, int, int]:
     return t, shape[-2] * shape[-1] if row is None else row, stride[-2] if shape[-2] > 1 else shape[-1]
 
 
-def _apart(row: int, head: int, heads: int, D: int) -> bool:
-    """Whether no two elements of a tensor of such strides share their place."""
-    return (head >= D and row >= (heads - 1) * head + D) or (row >= D and head >= row) or heads == 1 and row >= D
+def _apart(row: int, head: int, tokens: int, heads: int, D: int) -> bool:
+    """Whether no two elements of a tensor of such strides share their place: heads lie within tokens, or
+    tokens within heads."""
+    return (head >= D and row >= (heads - 1) * head + D) or (row >= D and head >= (tokens - 1) * row + D)
 
 
 def _rotary(x, frequencies, positions, interleaved, amplitude, inverse, out):
@@ -721,7 +722,7 @@ def _rotary(x, frequencies, positions, interleaved, amplitude, inverse, out):
         if out.dtype is not x.dtype or out.shape != shape or out.get_device() != index:
             _refuse(f"out must be {tuple(shape)} {x.dtype} on cuda:{index}")
         y, out_row, out_head = _heads(out)
-        if y is not out or (tokens > 1 and not _apart(out_row, out_head, H, D)) or (H > 1 and out_head < D):
+        if y is not out or (tokens > 1 and not _apart(out_row, out_head, tokens, H, D)) or (H > 1 and out_head < D):
             _refuse("out must have its tokens one stride apart, and no two elements in one place")
         if out.data_ptr() == x.data_ptr() and (xr is not x or (out_row, out_head) != (row, head)):
             _refuse("out begins where x does: then it must be x, with the same strides")
@@ -763,7 +764,9 @@ def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch
     tensor are one call: ``rotary(qkv[:, :q_heads + k_heads], ...)``.  ``inverse`` turns back, by the same
     amplitude: it is the gradient.  ``out`` may be ``x`` (in place) or not overlap it, and has no gradient."""
     if _forward_ad._current_level >= 0:
-        _no_tangents("rotary", x)
+        _no_tangents("rotary", x, frequencies)
+    if frequencies.requires_grad and torch.is_grad_enabled():
+        _refuse("frequencies have no gradient: pass them detached")
     if out is None and x.requires_grad and torch.is_grad_enabled():
         return _Rotary.apply(x, frequencies, positions, bool(interleaved), float(amplitude), bool(inverse))
     return _rotary(x, frequencies, positions, bool(interleaved), float(amplitude), bool(inverse), out)
