@@ -37,10 +37,10 @@ __device__ __forceinline__ int64_t sequence_value(const void* p, int wide, int64
 }
 
 // The tile with number `tile`; false where there is none.  Padded sequences have a fixed number of tiles.
-// Packed ones begin at tile offset / size + index, which leaves each enough and at most one too many: so
-// no kernel has to lay the tiles out first, and the sequence is found by a search in which a wave's lanes probe 64
-// places at a time.  The rows before the first and after the last offset are sequences without tokens.
-// Values outside [0, rows] are brought inside, so whatever the offsets are, no row outside the tensors is touched.
+// Packed ones begin at tile offset / size + index, which leaves each enough and at most one too many: so no
+// kernel has to lay the tiles out first, and the sequence is found by a search in which a wave's lanes probe 64
+// places at a time.  The rows before the first and after the last offset are sequences without tokens. Values
+// outside [0, rows] are brought inside, so whatever the offsets are, no row outside the tensors is touched.
 __device__ __forceinline__ bool find_tile(const AttentionArgs& a, int tile, int size, SequenceTile* t) {
     if (a.slots) {
         const int each = (a.slots + size - 1) / size, b = tile / each;
@@ -72,14 +72,14 @@ __device__ __forceinline__ bool find_tile(const AttentionArgs& a, int tile, int 
     t->start = (int64_t)__builtin_amdgcn_readfirstlane((int)start);
     t->extent = __builtin_amdgcn_readfirstlane((int)max(end - start, (int64_t)0));
     const int64_t at = tile - (start / size + low);
-    t->first = __builtin_amdgcn_readfirstlane((int)min(max(at, (int64_t)-1), (int64_t)(1 << 24)) * size);
+    t->first = __builtin_amdgcn_readfirstlane((int)min(max(at, (int64_t)-1), (int64_t)(0x7fffffff / size)) * size);
     t->length = low >= 1 && low <= a.count ? t->extent : 0;
     return t->first >= 0 && t->first < t->extent;
 }
 
-// A workgroup's tile of queries and head.  Tiles in the order of their work where they differ (causal: a sequence's last ones
-// first), so that the longest do not begin last; for each the heads, the key heads changing fastest: workgroups go to
-// the eight XCDs in turn, so with eight key heads each XCD's L2 sees one.
+// A workgroup's tile of queries and head.  Tiles in the order of their work where they differ (causal: a
+// sequence's last ones first), so that the longest do not begin last; for each the heads, the key heads
+// changing fastest: workgroups go to the eight XCDs in turn, so with eight key heads each XCD's L2 sees one.
 __device__ __forceinline__ void tile_and_head(const AttentionArgs& a, int* tile, int* h, int* hk) {
     const int at = blockIdx.x / a.Hq, j = blockIdx.x % a.Hq;
     *tile = a.causal ? a.tiles - 1 - at : at;
@@ -149,9 +149,10 @@ __device__ __forceinline__ bool any_not_finite(lds_bytes rows) {
     return __any((seen & ~kMask) != 0);
 }
 
-// The block on the diagonal of causal attention is seen in part by each column, and its product would add zero times
-// infinity where a row that is not finite is not seen.  So there such values are multiplied as zeros (finite_only), and
-// after the loop added to the columns that do see them (add_not_finite), from memory: slow, and rarely taken.
+// The block on the diagonal of causal attention is seen in part by each column, and its product would add zero
+// times infinity where a row that is not finite is not seen.  So there such values are multiplied as zeros
+// (finite_only), and after the loop added to the columns that do see them (add_not_finite), from memory: slow,
+// and rarely taken.
 template <typename T>
 __device__ __forceinline__ frag<T> finite_only(const frag<T>& f) {
     if constexpr (sizeof(T) == 2) {
@@ -171,7 +172,8 @@ __device__ __forceinline__ frag<T> finite_only(const frag<T>& f) {
     }
 }
 
-// The values that are not finite in `rows` rows at p (NANS: a NaN for each) to the columns that `sees(row)` names.
+// The values that are not finite in `rows` rows at p (NANS: a NaN for each) to the columns that `sees(row)`
+// names.
 template <typename T, int DP, bool NANS, typename F>
 __device__ __forceinline__ void add_not_finite(const void* p, int64_t pitch, int rows, int D, f32x16 (&acc)[DP / 32],
                                                F&& sees) {

@@ -2,17 +2,22 @@
 //
 //   dv = P^T do,   dP = do v^T,   dS = P (dP - delta),  delta = rowsum(do out),   dq = scale dS k,   dk = scale dS^T q,
 //
-// dk and dv summed over the query heads of a group.  Two kernels, both without atomics, so results are the
-// same bits every time: one holds a tile of queries and passes over the keys (dq, and delta on the way), the other
-// holds a tile of keys and passes over the queries of every head of the group.  Each makes S and dP for itself: seven
-// products where five are the least, but no sum crosses workgroups.
+// dk and dv summed over the query heads of a group.  Two kernels, both without atomics, so results are the same
+// bits every time: one holds a tile of queries and passes over the keys (dq, and delta on the way), the other
+// holds a tile of keys and passes over the queries of every head of the group.  Each makes S and dP for itself:
+// seven products where five are the least, but no sum crosses workgroups.
+//
+// Bound as the forward pass is, by matrix and vector unit in turns, and by what is held: q, do and dq (or k, v,
+// dk and dv) leave one to three waves a SIMD.  Measured: 12 heads of 64 over 4, float16, 64 sequences of up to
+// 2,048 tokens: dq 600 us, dk and dv 865; 6 heads of 80 over 2, causal, float32, 17 sequences of up to 777
+// tokens: 185 and 266 us, and 9 for the join.
 #include "attention.hpp"
 
 namespace trident {
 namespace {
 
-// dS can be far smaller than float16's least normal number (a gradient of 1e-3 on a row of 10,000 keys), so
-// in float16 it is held times a power of two of its column's own, which follows the largest magnitude so far; the
+// dS can be far smaller than float16's least normal number (a gradient of 1e-3 on a row of 10,000 keys), so in
+// float16 it is held times a power of two of its column's own, which follows the largest magnitude so far; the
 // accumulators are scaled along.  bfloat16 and float32 have the exponents and skip all this.
 template <typename T>
 constexpr bool kFollow = std::is_same<T, f16_t>::value;
@@ -92,8 +97,9 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
     const int last = first + 31, end = CAUSAL ? min(row + 1, t.length) : t.length;
     const TileReader<T, kPitch, DP> reader;
     bool not_finite = false;
-    // One tile of keys; EDGE: with keys that some row of the wave does not see.  What is loaded meanwhile lies elsewhere
-    // than what is read, which __restrict says: else the compiler waits for every load before a transposing read.
+    // One tile of keys; EDGE: with keys that some row of the wave does not see.  What is loaded meanwhile lies
+    // elsewhere than what is read, which __restrict says: else the compiler waits for every load before a
+    // transposing read.
     const auto pass = [&](int n, lds_bytes __restrict from, lds_bytes __restrict to, bool work, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         fetch(n + 1, to);
@@ -237,7 +243,8 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
     Power<DP / 32> power;
     const TileReader<T, kPitch, DP> reader;
     bool not_finite = false;
-    // One tile of queries from row r on; EDGE: causal, with queries before some key of the wave.  For __restrict see above.
+    // One tile of queries from row r on; EDGE: causal, with queries before some key of the wave.  For
+    // __restrict see above.
     const auto pass = [&](int n, int r, lds_bytes __restrict from, lds_bytes __restrict to, bool work, auto edge) {
         constexpr bool EDGE = decltype(edge)::value;
         fetch(n + 1, to);
@@ -365,9 +372,9 @@ __global__ __launch_bounds__(kBlock) void attention_join_kernel(const float* par
 
 size_t delta_bytes(const TridentAttention* t) { return ((size_t)t->rows * t->q_heads * 4 + 255) & ~(size_t)255; }
 
-// Shares of the queries that a tile of keys is cut into, each to a workgroup of its own, where the tiles alone leave CUs idle: then
-// the longest sequence's tile is what the others wait for (17 sequences of up to 777, 2 key heads, float32, three
-// shares: 671 us, with the join 278).
+// Shares of the queries that a tile of keys is cut into, each to a workgroup of its own, where the tiles alone
+// leave CUs idle: then the longest sequence's tile is what the others wait for (17 sequences of up to 777, 2
+// key heads, float32, three shares: 671 us, with the join 278).
 int shares_of(const TridentAttention* t) {
     const int64_t sequences = std::max<int64_t>(t->sequences, 1), length = t->rows / sequences;
     const int64_t tiles = std::max<int64_t>((t->rows + 127) / 128, sequences) * t->kv_heads;
@@ -407,7 +414,8 @@ int launch(AttentionArgs a, hipStream_t st) {
     return capi_check_launch("attention_join_kernel");
 }
 
-// Two waves where sequences are short (1,000 of 16 tokens, 12 heads of 64, bfloat16: 121 us, 166 by four; of 50: 265 and 302).
+// Two waves where sequences are short (1,000 of 16 tokens, 12 heads of 64, bfloat16: 121 us, 166 by four; of
+// 50: 265 and 302).
 template <typename T, int DP, bool CAUSAL>
 int by_length(const AttentionArgs& a, hipStream_t st) {
     const int64_t mean = a.slots ? a.slots : a.rows / std::max<int64_t>(a.count, 1);

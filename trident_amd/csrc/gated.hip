@@ -3,11 +3,16 @@
 //   g = x Wg^T,   u = x Wu^T,   h = act(g) u
 //   dg = dh u act'(g),   du = dh act(g),   dx = dg Wg + du Wu,   dWg = dg^T x,   dWu = du^T x
 //
-// with x [M, K], Wg and Wu [N, K], all row-major.  One kernel of tiles computes every product: an operand's tile is read by
-// rows where the summed axis is its columns (x, Wg, Wu in the forward pass; dg, du in dx) and by columns where it is its
-// rows (Wg, Wu in dx; all of dWg, dWu).  Sums are float32, and g and u are kept so for the backward pass: rounded to 16
-// bits they would add as much error to dg and du as these two's own rounding for their products does, and as much again to
-// the gradients (bfloat16: 3.1e-3 rms with them rounded, 2.4e-3 without, of which the results' own rounding is 1.7e-3).
+// with x [M, K], Wg and Wu [N, K], all row-major.  One kernel of tiles computes every product: an operand's
+// tile is read by rows where the summed axis is its columns (x, Wg, Wu in the forward pass; dg, du in dx) and
+// by columns where it is its rows (Wg, Wu in dx; all of dWg, dWu).  Sums are float32, and g and u are kept so
+// for the backward pass: rounded to 16 bits they would add as much error to dg and du as these two's own
+// rounding for their products does, and as much again to the gradients (bfloat16: 3.1e-3 rms with them rounded,
+// 2.4e-3 without, of which the results' own rounding is 1.7e-3).
+//
+// Many rows are bound by the matrix unit and by LDS, that feeds it: 16,384 x 1,024 by 2 x 4,096, bfloat16, 298
+// us (922 TFLOP/s; 275 GFLOP at the rate of a large square product take 196, a library's product alone of this
+// shape 272), its gradients 250 us of dx and 300 of both weights'.  Few rows are bound by the weights' bytes.
 #include <algorithm>
 
 #include "mfma.hpp"
@@ -17,15 +22,17 @@ namespace {
 
 enum Activation { kSilu = TRIDENT_SILU, kGelu = TRIDENT_GELU, kGeluTanh = TRIDENT_GELU_TANH };
 
-// act(g), and act'(g) where SLOPE.  By the vector unit's own exp2 and reciprocal, off by 1 ulp each: a tile of a
-// short sum is not much longer than its activations (expf, erfcf and divisions are several times as many instructions).
+// act(g), and act'(g) where SLOPE.  By the vector unit's own exp2 and reciprocal, off by 1 ulp each: a tile of
+// a short sum is not much longer than its activations (expf, erfcf and divisions are several times as many
+// instructions).
 template <bool SLOPE>
 __device__ __forceinline__ void activate(int kind, float g, float* value, float* slope) {
     constexpr float kLog2e = 1.4426950408889634f;
     const float g2 = g * g;
     if (kind == kGelu) {
-        // g Phi(g), Phi(-x) = erfc(x / sqrt 2) / 2.  For x >= 0, erfc(x) = t q(t) exp(-x^2) with t = 1 / (1 + x / 2) and q a
-        // polynomial fitted to exp(x^2) erfc(x) / t, off by 5e-8 relative up to x = 14, so small values keep their digits.
+        // g Phi(g), Phi(-x) = erfc(x / sqrt 2) / 2.  For x >= 0, erfc(x) = t q(t) exp(-x^2) with t = 1 / (1 + x
+        // / 2) and q a polynomial fitted to exp(x^2) erfc(x) / t, off by 5e-8 relative up to x = 14, so small
+        // values keep their digits.
         const float x = fabsf(g) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.5f, x, 1.0f));
         constexpr float q[] = {0.282084331f, 0.282412099f, 0.242835108f, 0.203752563f, -0.0291486356f, 0.281733461f, -0.490406549f, 0.286124062f, -0.0593864829f};
         float v = q[8];
@@ -51,8 +58,8 @@ __device__ __forceinline__ void activate(int kind, float g, float* value, float*
 // ------------------------------------------------------------------------------------------------
 // products
 
-// An operand: rows of `pitch` bytes.  By rows, its rows are the tile's and its columns are summed over; by columns the
-// other way round.
+// An operand: rows of `pitch` bytes.  By rows, its rows are the tile's and its columns are summed over; by
+// columns the other way round.
 struct Operand {
     const uint8_t* p;
     int64_t pitch;
@@ -86,8 +93,9 @@ __device__ __forceinline__ void tile_of(int id, int tiles_m, int tiles_n, int* t
 // How the first and the second operand are read.
 enum Reading { kRowsRows, kColumnsRows, kColumnsColumns };
 
-// Of the summed axis, bytes of a stage in LDS; and the stages there at a time.  Operands that are both read by rows come in
-// whole lines of 128 bytes, two stages; else four of 64 (forward pass of 16,384 x 1,024 by 2 x 4,096 bfloat16 307 us, 315 by four of 64; its dx 252 by four, 268 by two).
+// Of the summed axis, bytes of a stage in LDS; and the stages there at a time.  Operands that are both read by
+// rows come in whole lines of 128 bytes, two stages; else four of 64 (forward pass of 16,384 x 1,024 by 2 x
+// 4,096 bfloat16 307 us, 315 by four of 64; its dx 252 by four, 268 by two).
 constexpr int stage_row(int read) { return read == kRowsRows ? 128 : 64; }
 constexpr int stages(int read) { return read == kRowsRows ? 2 : 4; }
 
@@ -145,12 +153,12 @@ struct OperandTile {
     }
 };
 
-// A workgroup of WM x WN waves computes WM MT x WN NT blocks of 32 x 32, a wave MT x NT.  Stages of both operands go
-// straight from memory to LDS, ahead of the one that is multiplied.  The first operand gives the result's columns, so a
-// lane holds four neighbours of a row.
+// A workgroup of WM x WN waves computes WM MT x WN NT blocks of 32 x 32, a wave MT x NT.  Stages of both
+// operands go straight from memory to LDS, ahead of the one that is multiplied.  The first operand gives the
+// result's columns, so a lane holds four neighbours of a row.
 //
-// GATED: the first operand's tile is half gate, half up, and each wave's blocks too, so that a lane holds both sums
-// of the same places: out[0] = act(g) u, and g and u themselves where KEEP.
+// GATED: the first operand's tile is half gate, half up, and each wave's blocks too, so that a lane holds both
+// sums of the same places: out[0] = act(g) u, and g and u themselves where KEEP.
 //
 // SPLIT: a workgroup takes a share of the stages and writes its sums as they are, for the join.
 template <typename T, int READ, int WM, int WN, int MT, int NT, bool GATED, bool KEEP, bool SPLIT>
@@ -215,8 +223,8 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
     };
     constexpr int kFlight = (GATED ? 2 : 1) * First::kLoads + Second::kLoads;  // a wave's loads of one stage
     if constexpr (READ == kRowsRows) {
-        // A stage's next loads are issued as soon as every wave holds its part of it in registers, halfway through its
-        // products, so that they have a stage and a half to arrive.
+        // A stage's next loads are issued as soon as every wave holds its part of it in registers, halfway
+        // through its products, so that they have a stage and a half to arrive.
         for (int n = 0; n < steps; ++n) {
             if (n + 1 < steps) wait_and_meet<kFlight>();
             else wait_and_meet<0>();
@@ -247,9 +255,10 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
             for (int g = G / 2; g < G; ++g) multiply(g);
         }
     } else {
-        // One barrier a stage, past which it has arrived and the one before is no longer read; a group's blocks are read
-        // while the group before is multiplied.  What is loaded and what is read between two barriers lie in different
-        // stages, which __restrict says: else the compiler waits for every load before a transposing read.
+        // One barrier a stage, past which it has arrived and the one before is no longer read; a group's blocks
+        // are read while the group before is multiplied.  What is loaded and what is read between two barriers
+        // lie in different stages, which __restrict says: else the compiler waits for every load before a
+        // transposing read.
         const auto body = [&](int n, lds_bytes __restrict from, lds_bytes __restrict to, int of, bool before) {
             fetch(n + kStages - 1, to);
 #pragma unroll
@@ -416,10 +425,10 @@ int launch_product(ProductArgs a, int results, hipStream_t st) {
     return capi_check_launch("join_product_kernel");
 }
 
-// Workgroups that share the sum of a tile of 64 x 64, where the tiles leave CUs idle and the sum is long: a stage takes 0.3 us
-// (float32 1.2, or 0.6 of half the length) however few the tiles, the join another launch.  bfloat16, whole and shared: the
-// forward pass of 100 x 5,000 by 2 x 333 31 and 13 us, the backward pass of 16 x 960 by 2 x 2,560 48 and 19; float32
-// 176 and 26, 150 and 32.
+// Workgroups that share the sum of a tile of 64 x 64, where the tiles leave CUs idle and the sum is long: a
+// stage takes 0.3 us (float32 1.2, or 0.6 of half the length) however few the tiles, the join another launch.
+// bfloat16, whole and shared: the forward pass of 100 x 5,000 by 2 x 333 31 and 13 us, the backward pass of 16
+// x 960 by 2 x 2,560 48 and 19; float32 176 and 26, 150 and 32.
 inline int shares_for(int64_t M, int64_t N, int results, int64_t K, int parts, bool rows, int64_t es) {
     const int64_t tiles = (M + 63) / 64 * ((N + 63) / 64) * results, row = (rows ? 128 : 64) / es;
     const int64_t stages = (K + row - 1) / row * parts, length = stages * (es == 2 ? 1 : rows ? 4 : 2);
@@ -432,11 +441,11 @@ inline size_t part_bytes(int64_t M, int64_t N, int results, int64_t K, int parts
     return shares > 1 ? (size_t)shares * sums * M * N * 4 : 0;
 }
 
-// The tile.  A larger one reads its operands less often (256 x 256: 64 bytes of LDS for 8,192 products), but takes a CU
-// alone, so its tiles go in rounds of 256: it wins where the rounds are three quarters full (bfloat16, against 128 x
-// 128: the forward pass of 16,384 x 1,024 by 2 x 4,096, 2,048 tiles, 336 and 378 us; dx, 256 tiles, 265 and 330; but dWg and dWu,
-// 128 tiles, 445 and 315).  Where 128 x 128 leaves CUs idle, 64 x 64 (float32, 1,237 x 333 by 2 x 777: forward 39 to 32
-// us, dx 112 to 42, both weights 96 to 34).
+// The tile.  A larger one reads its operands less often (256 x 256: 64 bytes of LDS for 8,192 products), but
+// takes a CU alone, so its tiles go in rounds of 256: it wins where the rounds are three quarters full
+// (bfloat16, against 128 x 128: the forward pass of 16,384 x 1,024 by 2 x 4,096, 2,048 tiles, 336 and 378 us;
+// dx, 256 tiles, 265 and 330; but dWg and dWu, 128 tiles, 445 and 315).  Where 128 x 128 leaves CUs idle, 64 x
+// 64 (float32, 1,237 x 333 by 2 x 777: forward 39 to 32 us, dx 112 to 42, both weights 96 to 34).
 //
 // Few tiles of a long sum share it (shares_for), each with a join behind.
 template <typename T, int READ, bool GATED = false, bool KEEP = false>
@@ -466,7 +475,8 @@ struct SlopeArgs {
     int N, activation;
 };
 
-// dg and du: eight columns a thread, zeros from N up to the pitch.  Bound by bytes: three reads, two writes.
+// dg and du: eight columns a thread, zeros from N up to the pitch.  Bound by bytes: three reads, two writes
+// (16,384 x 4,096 bfloat16, 940 MB, 200 us, 4.7 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
     const int pieces = (int)(a.pitch / 8);
@@ -502,8 +512,8 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
     store_vec<T, 8>(static_cast<T*>(a.dup) + m * a.pitch + col, du);
 }
 
-// Rows copied to a pitch of whole pieces of 16 bytes, zeros behind: for operands whose rows do not begin at such
-// pieces, which LDS cannot take straight.
+// Rows copied to a pitch of whole pieces of 16 bytes, zeros behind: for operands whose rows do not begin at
+// such pieces, which LDS cannot take straight.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void pack_kernel(const T* from, int64_t ld, T* to, int64_t pitch, int64_t rows,
                                                       int cols) {
@@ -560,8 +570,10 @@ __device__ __forceinline__ frag<T> load_eight(const T* p, int left) {
     return f;
 }
 
-// Up to 16 rows, such as a query's: a workgroup takes 16 columns of gate and up, and its waves share K by blocks of 64.
-// Bound by the bytes of the weights, each of which one wave reads once, straight to registers: rows of 16 lanes' pieces.
+// Up to 16 rows, such as a query's: a workgroup takes 16 columns of gate and up, and its waves share K by
+// blocks of 64. Bound by the bytes of the weights, each of which one wave reads once, straight to registers:
+// rows of 16 lanes' pieces (bfloat16: one row of 960 by 2 x 2,560 4.7 us, 16 of 8,192 by 2 x 8,192 49, 5.4
+// TB/s).
 template <typename T, bool KEEP>
 __global__ __launch_bounds__(kFewWaves* kWave) void few_kernel(FewArgs a) {
     __shared__ f32x4v s_acc[2][kFewWaves][kWave];

