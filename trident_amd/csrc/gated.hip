@@ -49,9 +49,12 @@ __device__ __forceinline__ void activate(int kind, float g, float* value, float*
     const float p = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
     *value = g * p;
     if constexpr (SLOPE) {
-        const float dz = kind == kSilu ? 1.0f : 1.5957691216057308f * __builtin_fmaf(3 * 0.044715f, g2, 1.0f);
-        // 1 - p by its own quotient: no digits are lost where p is near 1
-        *slope = __builtin_fmaf(g * p * dz, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kLog2e * z)), p);
+        // dz grows as g^2, and from g = 1e13 on g dz passes float32 where the logistic's own slope p (1 - p) is
+        // zero: so that is multiplied first, and g^2 stops at 1e4, where it is zero for long.  1 - p is its own
+        // quotient: no digits are lost where p is near 1.
+        const float dz = kind == kSilu ? 1.0f : 1.5957691216057308f * __builtin_fmaf(3 * 0.044715f, fminf(g2, 1e4f), 1.0f);
+        const float dp = p * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(kLog2e * z));
+        *slope = __builtin_fmaf(g * dp, dz, p);
     }
 }
 
