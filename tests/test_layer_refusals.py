@@ -1,0 +1,25 @@
+"""Calls of the transformer layer's entry points that have no right answer are refused, and those that have one are not
+(CPU only: nothing is launched)."""
+import ctypes
+
+import pytest
+import torch
+
+from trident_amd import _lib, encoder
+from test_layer_abi import attention, on_gpu, refused  # noqa: F401
+
+
+@pytest.mark.parametrize("scale", [1e-46, 5e-324, 0.0, -1.0, float("inf")])
+def test_scales_that_float32_does_not_hold(on_gpu, scale):  # noqa: F811
+    L = _lib.lib()
+    a = attention(scale=scale)
+    refused(L.trident_attention(ctypes.byref(a), None), 1, "scale")
+    a = attention(scale=scale, lse=256, grad=256, dq=256, dk=256, dv=256)
+    assert L.trident_attention_grad_workspace_bytes(ctypes.byref(a)) == 0
+    refused(L.trident_attention_grad(ctypes.byref(a), 256, 1 << 40, None), 1, "scale")
+    q = torch.zeros((10, 4, 16))
+    for call in (encoder.attention, encoder.attention_forward):
+        with pytest.raises(_lib.TridentError, match="scale"):
+            call(q, q, q, scale=scale)
+    with pytest.raises(_lib.TridentError, match="scale"):
+        encoder.attention_grad(q, q, q, q, q, torch.zeros((4, 10)), scale=scale)

@@ -216,7 +216,8 @@ int attention_check(const TridentAttention* t, bool backward, AttentionArgs* a) 
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT,
                          "%s: %lld rows are not %lld sequences of %lld slots, or offsets and lengths do not go with them",
                          name, (long long)t->rows, (long long)t->sequences, (long long)t->slots);
-    if (!(t->scale > 0.0) || !(t->scale < 1e30))
+    // float32 holds it: a scale that became zero would make NaN of the scores that are not seen
+    if (!(t->scale >= 0x1p-149) || !(t->scale < 1e30))
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: scale=%g", name, t->scale);
     const int64_t es = t->dtype == TRIDENT_F32 ? 4 : 2;
     const int64_t strides[6] = {t->q_row, t->q_head, t->k_row, t->k_head, t->v_row, t->v_head};

@@ -828,8 +828,8 @@ def _attention_args(q, k, v, offsets, lengths, causal, scale):
         else:  # one sequence
             slots = rows
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not 0.0 < scale < 1e30:
-        _refuse(f"scale must be positive, got {scale}")
+    if not 2.0 ** -149 <= scale < 1e30:
+        _refuse(f"scale must be positive in float32 and below 1e30, got {scale}")
     (q, q_row, q_head), (k, k_row, k_head), (v, v_row, v_head) = map(_strided_heads, (q, k, v))
     ids = None if where is None else where.data_ptr()
     a = _lib.TridentAttention(q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, None, None, None, None,
