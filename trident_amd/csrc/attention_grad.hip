@@ -5,7 +5,7 @@
 // dk and dv summed over the query heads of a group.  Two kernels, both without atomics, so results are the same
 // bits every time: one holds a tile of queries and passes over the keys (dq, and delta on the way), the other
 // holds a tile of keys and passes over the queries of every head of the group.  Each makes S and dP for itself:
-// seven products where five are the least, but no sum crosses workgroups.
+// seven products (eight in 16 bits, kMendDelta below) where five are the least, but no sum crosses workgroups.
 //
 // Bound as the forward pass is, by matrix and vector unit in turns, and by what is held: q, do and dq (or k, v,
 // dk and dv) leave one to three waves a SIMD.  Measured: 12 heads of 64 over 4, float16, 64 sequences of up to
@@ -21,6 +21,16 @@ namespace {
 // accumulators are scaled along.  bfloat16 and float32 have the exponents and skip all this.
 template <typename T>
 constexpr bool kFollow = std::is_same<T, f16_t>::value;
+// delta made of an out of 16 bits is off by out's rounding, which can be as large as dP - delta is (values that
+// share a part).  But the rows of P sum to one, so those of dS, made with a delta that is off by e, sum to -e
+// instead of zero: the dq kernel adds them up in float32, takes their sum times that of P k from dq, and keeps the
+// mended delta for dk and dv.  Error of dq in 1e-3, rms, bfloat16, without and with: 2.40 and 2.37 of 2,000
+// rows with flat scores, 3.1 and 2.4 of 4 rows, 4.6 and 2.4 of scores six times as large, 14.4 and 2.4 of values that
+// share 4; dk alike.  It costs a product more, of keys that are in registers already, and its accumulators: of the whole
+// backward pass 7 to 10 % at heads of 64 (sequences of up to 2,048), 2 % at short ones, 23 % at heads of 128, where one wave
+// of a SIMD is left of two.  float32 does without: there out's rounding is no more than the sums' own.
+template <typename T>
+constexpr bool kMendDelta = sizeof(T) == 2;
 // P <= 1 (up to the rounding of lse) in float16 times 2^15: held in full down to 2^-29.
 template <typename T>
 constexpr float kShift = kFollow<T> ? 15.0f : 0.0f;
@@ -89,10 +99,12 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
         delta += other_half(delta);
     }
     const float lse = a.lse[h * a.rows + at];
-    if (row < live && half == 0) a.delta[h * a.rows + at] = delta;
+    const bool keeps = row < live && half == 0;
+    if (!kMendDelta<T> && keeps) a.delta[h * a.rows + at] = delta;
     arrived(q);
     arrived(go);
-    f32x16 acc[DP / 32] = {};
+    f32x16 acc[DP / 32] = {}, pk[kMendDelta<T> ? DP / 32 : 1] = {};
+    float off = 0.0f;  // this half's part of the sum of dS
     Power<DP / 32> power;
     const int last = first + 31, end = CAUSAL ? min(row + 1, t.length) : t.length;
     const TileReader<T, kPitch, DP> reader;
@@ -115,14 +127,25 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
                 s = mma<T>(reader.rows(keys, kb, i), q[i], s);
                 dp = mma<T>(reader.rows(values, kb, i), go[i], dp);
             }
+            frag<T> p[2], ds[2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse)) * (dp[i] - delta);
+            for (int i = 0; i < 16; ++i) {
+                const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], a.scale2, -lse));
+                s[i] = x * (dp[i] - delta);
+                if constexpr (kMendDelta<T>) p[i / 8][i % 8] = (T)x;
+            }
             if constexpr (EDGE) {
                 const int seen_here = end - key - 4 * half;
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
-                    if (8 * (i / 4) + i % 4 >= seen_here) s[i] = 0.0f;
+                    if (8 * (i / 4) + i % 4 >= seen_here) {
+                        s[i] = 0.0f;
+                        if constexpr (kMendDelta<T>) p[i / 8][i % 8] = (T)0.0f;
+                    }
+            }
+            if constexpr (kMendDelta<T>) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) off += s[i];
             }
             if constexpr (kFollow<T>) {
                 float top = 0.0f;
@@ -132,7 +155,6 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
 #pragma unroll
                 for (int i = 0; i < 16; ++i) s[i] *= power.by;
             }
-            frag<T> ds[2];
 #pragma unroll
             for (int i = 0; i < 16; ++i) ds[i / 8][i % 8] = (T)s[i];
             const bool apart = EDGE && CAUSAL && key >= first && any_not_finite<T, kPitch>(keys + kb * 32 * kPitch);
@@ -146,6 +168,7 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
                         if (apart) f = finite_only<T>(f);
                     }
                     acc[j] = mma<T>(f, ds[i], acc[j]);
+                    if constexpr (kMendDelta<T>) pk[j] = mma<T>(f, p[i], pk[j]);
                 }
         }
     };
@@ -160,6 +183,15 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
     for (; n < tiles; ++n) {
         wait_and_meet<0>();
         pass(n, place(n), place(n + 1), n < seen, std::true_type{});
+    }
+    if constexpr (kMendDelta<T>) {
+        off += other_half(off);
+        if (keeps) a.delta[h * a.rows + at] = delta + off;
+        const float by = kFollow<T> ? off * power.by : off;
+#pragma unroll
+        for (int j = 0; j < DP / 32; ++j)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) acc[j][i] = __builtin_fmaf(-by, pk[j][i], acc[j][i]);
     }
     if constexpr (CAUSAL) {
         if (not_finite)
