@@ -99,7 +99,10 @@ template <typename T, int PITCH, int ROWS, int WAVES>
 __device__ __forceinline__ void fetch_tile(lds_bytes to, const void* p, int64_t row, int live, int bytes, int wave) {
     using L = Tile<T, PITCH>;
     constexpr int kLoads = ROWS / L::kRowsAtOnce;
-    const __amdgpu_buffer_rsrc_t buf = buffer_of(p, (uint32_t)(max(min(live, ROWS), 0) * (int)row));
+    // (read from one lane: of min and max the compiler makes a vector instruction, and of a descriptor in vector registers a
+    // loop over the lanes for every load)
+    const int there = __builtin_amdgcn_readfirstlane(max(min(live, ROWS), 0));
+    const __amdgpu_buffer_rsrc_t buf = buffer_of(p, (uint32_t)(there * (int)row));
     const int lane = lane_id(), in = lane / L::kPieces, slot = lane % L::kPieces;
 #pragma unroll
     for (int i = 0; i < (kLoads + WAVES - 1) / WAVES; ++i) {
