@@ -1,5 +1,5 @@
 """Attention's gradients against their formulas in float64 where a looser bound would hide what goes wrong: values that share
-a part, so that dP - delta cancels.
+a part (dP - delta cancels), keys whose infinities keep them from every row.
 
 u = 2^-24 is a float32 operation's rounding, U[dtype] that of P, dS and results.  The bounds have no term for the rounding of
 out: delta is the float32 sum of P dP, made of the rounded out and what the sum of dS shows it to lack.
@@ -100,6 +100,31 @@ def test_scores_that_pick_few_keys(dev, dtype):
     ref = gradients(q, k, v, grad, hidden_keys(200, False, dev), 0.125)
     for n, t in zip(("dq", "dk", "dv"), run(q, k, v, grad, False)):
         within(t, *ref[n], what=n)
+
+
+@pytest.mark.parametrize("m", [31, 64, 70, 100, 129])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_key_that_its_infinity_hides(dev, dtype, causal, m):
+    """A key of -inf in a column where every query is positive has scores of -inf: no row sees it, its gradients are zero and
+    the others those without it, however far the sequence's end is from a tile's.  Only dq's own column has zero times
+    infinity."""
+    g = gen(m)
+    q, k, v, grad = (randn(g, m, H, 64, dtype=dtype) for H in (4, 2, 2, 4))
+    q[..., 0] = q[..., 0].abs() + 0.5
+    hidden = hidden_keys(m, causal, dev)
+    hidden[:, 5] = True
+    ref = gradients(q, k, v, grad, hidden, 0.125)
+    k[5, :, 0] = -math.inf
+    for padded in (0, m + 33):
+        dq, dk, dv = run(q, k, v, grad, causal, padded)
+        assert (dk[5] == 0).all() and (dv[5] == 0).all()
+        within(dk, *ref["dk"], what="dk")
+        within(dv, *ref["dv"], what="dv")
+        within(dq[..., 1:], *(t[..., 1:] for t in ref["dq"]), what="dq")
+        assert dq[5:, :, 0].isnan().all()
+        if causal:
+            within(dq[:5], *(t[:5] for t in ref["dq"]), what="dq")
 
 
 @pytest.mark.parametrize("dtype", TYPES)

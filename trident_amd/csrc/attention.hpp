@@ -133,23 +133,43 @@ __device__ __forceinline__ void arrived(F (&f)[N]) {
     for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
 }
 
+// Magnitudes from infinity on carry into the sign's place.
+template <typename T>
+struct NotFinite {
+    static constexpr uint32_t kMask = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
+    static constexpr uint32_t kCarry = sizeof(T) == 4                          ? 0x00800000u
+                                       : std::is_same<T, bf16_t>::value ? 0x00800080u
+                                                                               : 0x04000400u;
+    uint32_t seen = 0;
+    __device__ __forceinline__ void look(u32x4 w) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) seen |= (w[e] & kMask) + kCarry;
+    }
+    __device__ __forceinline__ bool any() const { return __any((seen & ~kMask) != 0); }  // in the wave
+};
+
 // Whether 32 rows of a tile hold a value that is not finite.
 template <typename T, int PITCH>
 __device__ __forceinline__ bool any_not_finite(lds_bytes rows) {
     typedef const __attribute__((address_space(3))) u32x4* words;
-    // magnitudes from infinity on carry into the sign's place
-    constexpr uint32_t kMask = sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu;
-    constexpr uint32_t kCarry = sizeof(T) == 4                          ? 0x00800000u
-                                : std::is_same<T, bf16_t>::value ? 0x00800080u
-                                                                        : 0x04000400u;
-    uint32_t seen = 0;
+    NotFinite<T> n;
 #pragma unroll
-    for (int i = 0; i < PITCH / 32; ++i) {
-        const u32x4 w = *(words)(rows + i * 1024 + lane_id() * 16);
+    for (int i = 0; i < PITCH / 32; ++i) n.look(*(words)(rows + i * 1024 + lane_id() * 16));
+    return n.any();
+}
+
+// Whether the wave's rows do.
+template <typename T, int N>
+__device__ __forceinline__ bool any_not_finite(const frag<T> (&f)[N]) {
+    NotFinite<T> n;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) seen |= (w[e] & kMask) + kCarry;
+    for (int i = 0; i < N; ++i) {
+        u32x4 w[sizeof(f[i]) / 16];
+        __builtin_memcpy(w, &f[i], sizeof(f[i]));
+#pragma unroll
+        for (const u32x4& part : w) n.look(part);
     }
-    return __any((seen & ~kMask) != 0);
+    return n.any();
 }
 
 // The block on the diagonal of causal attention is seen in part by each column, and its product would add zero

@@ -203,13 +203,13 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
 
 // dk and dv: a wave holds 32 keys and their values; tiles of queries and of their gradients pass through
 // LDS with the rows' lse and delta.  S is queries by keys, so a lane holds one key.  Rows past the
-// sequence's end are zeros in LDS, lse and delta among them, and add nothing.
+// sequence's end have gradients and delta of zero in LDS and add nothing.
 template <typename T, int DP, int WAVES, bool CAUSAL>
 __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 96 ? 2 : 1) void attention_dkv_kernel(AttentionArgs a) {
     constexpr int BM = WAVES * 32, BN = kTileRows<T>, kPitch = kTilePitch<T, DP>, kTile = BN * kPitch;
     constexpr int KB = BN / 32;
     constexpr int kStage = 2 * kTile + 2 * kWave * 4;  // queries, gradients, 64 words of lse and of delta
-    extern __shared__ __align__(16) uint8_t lds[];
+    extern __shared__ __align__(16) uint8_t lds[];     // two of them, and a word a wave
     const int hk = blockIdx.x % a.Hkv, share = blockIdx.x / a.Hkv % a.shares, tile = blockIdx.x / a.Hkv / a.shares;
     const int group = a.Hq / a.Hkv;
     SequenceTile t;
@@ -265,12 +265,17 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
     // from L2, which a float32 product of their size hides.
     constexpr bool kHold = sizeof(T) == 2 || DP <= 64;
     frag<T> k[DP / 16], v[DP / 16];
+    load_row<T, DP>(k_at, a.D, k);
     if constexpr (kHold) {
-        load_row<T, DP>(k_at, a.D, k);
         load_row<T, DP>(v_at, a.D, v);
-        arrived(k);
         arrived(v);
     }
+    arrived(k);
+    typedef __attribute__((address_space(3))) uint32_t* words;
+    const words not_finite_keys = (words)(base + 2 * kStage);  // of each wave
+    not_finite_keys[wave] = any_not_finite<T, DP / 16>(k);
+    meet();
+    const bool infinite = __any(not_finite_keys[lane % WAVES]);
     f32x16 ak[DP / 32] = {}, av[DP / 32] = {};
     Power<DP / 32> power;
     const TileReader<T, kPitch, DP> reader;
@@ -347,6 +352,26 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
         }
     };
     const auto place = [&](int n) { return base + n % 2 * kStage; };
+    // Past this barrier the tile of rows r on is there.  With an infinity among the keys, rows past the sequence's end
+    // get the last one's query and lse: zeros would make a NaN of a key to which every row gives a P of zero.
+    const auto arrive = [&](int r, lds_bytes at) {
+        wait_and_meet<0>();
+        const int rows = t.length - r;
+        if (__builtin_expect(!infinite || rows >= BN, 1)) return;
+        using L = Tile<T, kPitch>;
+        typedef __attribute__((address_space(3))) u32x4* pieces;
+        int id = threadIdx.x;
+        asm volatile("" : "+v"(id));  // nothing of it is made, and held, before the loop
+#pragma unroll 1
+        for (int i = id; i < (BN - rows) * L::kPieces; i += WAVES * kWave) {
+            const int to = rows + i / L::kPieces, piece = i % L::kPieces;
+            *(pieces)(at + to * kPitch + ((piece ^ L::exchange(to)) << 4)) =
+                *(pieces)(at + (rows - 1) * kPitch + ((piece ^ L::exchange(rows - 1)) << 4));
+        }
+        const words lse = (words)(at + 2 * kTile);
+        if (id < BN - rows) lse[rows + id] = lse[rows - 1];
+        meet();
+    };
     // of each head's tiles, those before this wave's last key come first
     const int edges = CAUSAL ? min((first + 32 + BN - 1) / BN - n0, each) : 0;
     for (int n = begin; n < tiles;) {
@@ -355,12 +380,13 @@ __global__ __launch_bounds__(WAVES* kWave, WAVES > 2 && sizeof(T) == 2 && DP <= 
         const int stop = min(tiles - g * each, each);
         for (; m < min(edges, stop); ++m, ++n) {
             const int r = (n0 + m) * BN;
-            wait_and_meet<0>();
+            arrive(r, place(n));
             pass(n, r, place(n), place(n + 1), first < live && r + BN > first, std::true_type{});
         }
         for (; m < stop; ++m, ++n) {
-            wait_and_meet<0>();
-            pass(n, (n0 + m) * BN, place(n), place(n + 1), first < live, std::false_type{});
+            const int r = (n0 + m) * BN;
+            arrive(r, place(n));
+            pass(n, r, place(n), place(n + 1), first < live, std::false_type{});
         }
     }
     if constexpr (CAUSAL) {
@@ -422,7 +448,7 @@ size_t workspace_of(const TridentAttention* t) {
 template <typename T, int DP, int WAVES, bool CAUSAL>
 int launch(AttentionArgs a, hipStream_t st) {
     constexpr int BM = WAVES * 32;
-    constexpr size_t lds = 4 * (size_t)kTileRows<T> * kTilePitch<T, DP> + 4 * kWave * 4;
+    constexpr size_t lds = 4 * (size_t)kTileRows<T> * kTilePitch<T, DP> + 4 * kWave * 4 + WAVES * 4;
     static_assert(lds <= 163840, "LDS of a CU");
     const auto dq = attention_dq_kernel<T, DP, WAVES, CAUSAL>, dkv = attention_dkv_kernel<T, DP, WAVES, CAUSAL>;
     if (lds > 65536)
