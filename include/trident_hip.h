@@ -415,8 +415,9 @@ int trident_attention_grad(const TridentAttention* a, void* workspace, size_t wo
 
 /* The gated half of a feed-forward block: h [M, N] = act(x gate_weight^T) * (x up_weight^T), x [M, K], both weights
  * [N, K], rows of the given pitches in elements.  gate and up [M, N] float32: the two products, kept for the
- * backward pass, or both NULL.  h, gate, up and the results of the backward pass are contiguous.  Rows that begin at 16-byte addresses
- * and hold whole 16 bytes are taken as they are; the workspace is for others, and none for up to 16 rows. */
+ * backward pass, or both NULL.  h, gate, up and the results of the backward pass are contiguous.  Rows that begin at 16-byte addresses,
+ * hold whole 16 bytes and lie at most 2^21 elements apart are taken as they are; the workspace is for others, and none for up to
+ * 16 rows.  N and K are at most 2^21. */
 enum TridentActivation { TRIDENT_SILU = 0, TRIDENT_GELU = 1, TRIDENT_GELU_TANH = 2 };
 
 typedef struct TridentGated {

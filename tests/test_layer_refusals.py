@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from trident_amd import _lib, encoder
-from test_layer_abi import attention, on_gpu, refused  # noqa: F401
+from test_layer_abi import attention, gated, on_gpu, refused  # noqa: F401
 
 
 @pytest.mark.parametrize("scale", [1e-46, 5e-324, 0.0, -1.0, float("inf")])
@@ -23,3 +23,17 @@ def test_scales_that_float32_does_not_hold(on_gpu, scale):  # noqa: F811
             call(q, q, q, scale=scale)
     with pytest.raises(_lib.TridentError, match="scale"):
         encoder.attention_grad(q, q, q, q, q, torch.zeros((4, 10)), scale=scale)
+
+
+def test_rows_far_apart_are_packed():
+    """A pitch past what a tile's offsets reach: such rows go through the workspace, and those of few rows need none."""
+    L, far = _lib.lib(), 1 << 22
+    for name, rows in (("ld_x", 100), ("ld_gate", 64), ("ld_up", 64)):
+        a = gated(**{name: far})
+        need = L.trident_gated_linear_workspace_bytes(ctypes.byref(a))
+        assert need >= rows * 32 * 2
+        refused(L.trident_gated_linear(ctypes.byref(a), 256, need - 1, None), 3, str(need))
+        near = L.trident_gated_linear_grad_workspace_bytes(ctypes.byref(gated()))
+        assert L.trident_gated_linear_grad_workspace_bytes(ctypes.byref(a)) >= near + rows * 32 * 2
+        assert L.trident_gated_linear_workspace_bytes(ctypes.byref(gated(M=16, **{name: far}))) == 0
+        refused(L.trident_gated_linear(ctypes.byref(gated(**{name: 1 << 41})), 256, 1 << 40, None), 1, "bad sizes")

@@ -516,9 +516,9 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
 }
 
 // Rows copied to a pitch of whole pieces of 16 bytes, zeros behind: for operands whose rows do not begin at
-// such pieces, which LDS cannot take straight.  Those of a product in one launch (blockIdx.y): 1,237 x 333 and
-// 2 x 777 in float32 take 3 us each, most of it a launch's own (forward and backward pass 102 us, 95 in one
-// launch each way).
+// such pieces, which LDS cannot take straight, or lie too far apart for a tile's offsets.  Those of a product in one
+// launch (blockIdx.y): 1,237 x 333 and 2 x 777 in float32 take 3 us each, most of it a launch's own (forward and
+// backward pass 102 us, 95 in one launch each way).
 struct PackArgs {
     const void* from[3];
     void* to[3];
@@ -647,8 +647,10 @@ inline int64_t pitch_of(int64_t cols, int64_t es) {
 }
 inline size_t bytes_of(int64_t rows, int64_t pitch, int64_t es) { return (size_t)round_up(rows * pitch * es, 256); }
 
+constexpr int64_t kFarthest = 1 << 21;  // elements from row to row, so that a tile's rows are within 32-bit offsets
+
 inline bool whole(const void* p, int64_t ld, int64_t es) {
-    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0;
+    return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld * es % 16 == 0 && ld <= kFarthest;
 }
 
 struct Scratch {
@@ -722,8 +724,8 @@ int check(const TridentGated* t, bool backward) {
     if (!dtype_ok(t->dtype)) return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: dtype=%d", name, t->dtype);
     if (t->activation < TRIDENT_SILU || t->activation > TRIDENT_GELU_TANH)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: activation=%d", name, t->activation);
-    const int64_t most = 1 << 21;  // so that a tile's rows are within 32-bit offsets
-    if (t->M < 0 || t->N < 0 || t->K < 1 || t->M > (1 << 30) || t->N > most || t->K > most || t->ld_x < t->K ||
+    constexpr int64_t most = (int64_t)1 << 40;
+    if (t->M < 0 || t->N < 0 || t->K < 1 || t->M > (1 << 30) || t->N > kFarthest || t->K > kFarthest || t->ld_x < t->K ||
         t->ld_gate < t->K || t->ld_up < t->K || t->ld_x > most || t->ld_gate > most || t->ld_up > most)
         return capi_fail(TRIDENT_ERR_INVALID_ARGUMENT, "%s: bad sizes M=%lld N=%lld K=%lld pitches %lld, %lld, %lld", name,
                          (long long)t->M, (long long)t->N, (long long)t->K, (long long)t->ld_x, (long long)t->ld_gate,
