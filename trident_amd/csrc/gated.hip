@@ -79,7 +79,12 @@ struct ProductArgs {
     int tiles_m, tiles_n, activation;
     int shares;        // SPLIT: workgroups that share a tile's sum
     float* part;       // [shares][sums of a place: gate and up, or the results][M, N]
+    const float* back; // kScaled: what the sums are multiplied by
 };
+
+// The second operand of the backward products, dg and du, is held in float16 times a power of two (slope_kernel).
+template <typename T>
+constexpr bool kScaled = std::is_same<T, f16_t>::value;
 
 // One of a grid's tiles in an order that keeps neighbours on one XCD: workgroups go to the eight XCDs, each
 // with its own L2, in turn, so each takes a contiguous eighth, in bands of 8 tile rows.
@@ -356,7 +361,8 @@ __device__ __forceinline__ void product(const ProductArgs& a) {
                 put(i, static_cast<float*>(a.out[2]), [&](int j, int e) { return acc[i][j + kBlocks][e]; });
             }
         } else {
-            put(i, static_cast<T*>(a.out[z]), [&](int j, int e) { return acc[i][j][e]; });
+            const float by = kScaled<T> ? *a.back : 1.0f;
+            put(i, static_cast<T*>(a.out[z]), [&](int j, int e) { return kScaled<T> ? acc[i][j][e] * by : acc[i][j][e]; });
         }
     }
 }
@@ -396,6 +402,11 @@ __global__ __launch_bounds__(kBlock) void join_product_kernel(ProductArgs a, int
             store_vec<float, V>(static_cast<float*>(a.out[2]) + at, sum[1]);
         }
     } else {
+        if constexpr (kScaled<T>) {
+            const float by = *a.back;
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum[0][e] *= by;
+        }
         store_vec<T, V>(static_cast<T*>(a.out[blockIdx.y]) + at, sum[0]);
     }
 }
@@ -476,21 +487,17 @@ struct SlopeArgs {
     int64_t ld_grad, ld, pitch;  // of grad, of gate and up, of dgate and dup: elements
     int64_t M;
     int N, activation;
+    float *tops, *back;          // kScaled: the largest values of workgroups, and one over the factor
+    int groups;
 };
 
-// dg and du: eight columns a thread, zeros from N up to the pitch.  Bound by bytes: three reads, two writes
-// (16,384 x 4,096 bfloat16, 940 MB, 200 us, 4.7 TB/s).
+// dg and du of eight columns, zeros from N on.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
-    const int pieces = (int)(a.pitch / 8);
-    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    if (at >= a.M * pieces) return;
-    const int64_t m = at / pieces;
-    const int col = (int)(at - m * pieces) * 8;
+__device__ __forceinline__ void slopes_at(const SlopeArgs& a, int64_t m, int col, float (&dg)[8], float (&du)[8]) {
     const T* dh = static_cast<const T*>(a.grad) + m * a.ld_grad + col;
     const float* g = static_cast<const float*>(a.gate) + m * a.ld + col;
     const float* u = static_cast<const float*>(a.up) + m * a.ld + col;
-    float fh[8], fg[8], fu[8], dg[8], du[8];
+    float fh[8], fg[8], fu[8];
     if (col + 8 <= a.N) {
         load_vec<T, 8>(dh, fh);
         load_vec<float, 8>(g, fg);
@@ -510,6 +517,72 @@ __global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
         activate<true>(a.activation, fg[e], &v, &s);
         dg[e] = fh[e] * fu[e] * s;
         du[e] = fh[e] * v;
+    }
+}
+
+// The largest of a workgroup's values, in every thread.
+__device__ __forceinline__ float block_max(float v) {
+    __shared__ float s_top[kBlock / kWave];
+#pragma unroll
+    for (int by = 1; by < kWave; by *= 2) v = fmaxf(v, __shfl_xor(v, by, kWave));
+    if (lane_id() == 0) s_top[threadIdx.x / kWave] = v;
+    __syncthreads();
+    v = s_top[0];
+#pragma unroll
+    for (int w = 1; w < kBlock / kWave; ++w) v = fmaxf(v, s_top[w]);
+    return v;
+}
+
+// float16: a gradient of 1e-4 by an up of 1e-2 is below its normal numbers, one of 50 by 1e4 above them (errors of
+// some per cent, or infinities, in results that are neither).  So dg and du are held times the power of two that
+// brings the largest finite one of the call to 2^14 .. 2^15, and the products' sums are multiplied by its
+// reciprocal: digits are lost only 2^28 below the largest.  To find that takes a pass of its own over what
+// slope_kernel reads again (the gradients of 16,384 x 1,024 by 2 x 4,096 681 -> 799 us, of 64 x 512 by 2 x 1,024 25 -> 28).
+// The other types have the exponents.
+constexpr int kTops = 1024;
+template <typename T>
+__global__ __launch_bounds__(kBlock) void largest_slope_kernel(SlopeArgs a) {
+    const int pieces = (int)((a.N + 7) / 8);
+    float top = 0.0f;
+    for (int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x; at < a.M * pieces; at += (int64_t)gridDim.x * kBlock) {
+        const int64_t m = at / pieces;
+        float dg[8], du[8];
+        slopes_at<T>(a, m, (int)(at - m * pieces) * 8, dg, du);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float g = fabsf(dg[e]), u = fabsf(du[e]);
+            top = fmaxf(top, fmaxf(g < INFINITY ? g : 0.0f, u < INFINITY ? u : 0.0f));
+        }
+    }
+    top = block_max(top);
+    if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
+}
+
+// dg and du.  Bound by bytes: three reads, two writes (16,384 x 4,096 bfloat16, 940 MB, 200 us, 4.7 TB/s).
+template <typename T>
+__global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
+    float by = 1.0f;
+    if constexpr (kScaled<T>) {
+        float top = 0.0f;
+        for (int i = threadIdx.x; i < a.groups; i += kBlock) top = fmaxf(top, a.tops[i]);
+        const int e = (int)(__float_as_uint(block_max(top)) >> 23);     // 2^(e - 127) <= top
+        const uint32_t exponent = (uint32_t)min(268 - e, 227);          // 2^100 at most
+        by = __uint_as_float(exponent << 23);
+        if (blockIdx.x == 0 && threadIdx.x == 0) *a.back = __uint_as_float((254 - exponent) << 23);
+    }
+    const int pieces = (int)(a.pitch / 8);
+    const int64_t at = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (at >= a.M * pieces) return;
+    const int64_t m = at / pieces;
+    const int col = (int)(at - m * pieces) * 8;
+    float dg[8], du[8];
+    slopes_at<T>(a, m, col, dg, du);
+    if constexpr (kScaled<T>) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            dg[e] *= by;
+            du[e] *= by;
+        }
     }
     store_vec<T, 8>(static_cast<T*>(a.dgate) + m * a.pitch + col, dg);
     store_vec<T, 8>(static_cast<T*>(a.dup) + m * a.pitch + col, du);
@@ -698,6 +771,8 @@ size_t packed_bytes(const void* p, int64_t ld, int64_t rows, int64_t cols, int64
     return whole(p, ld, es) && cols % (16 / es) == 0 ? 0 : bytes_of(rows, pitch_of(cols, es), es);
 }
 
+constexpr size_t kTopsBytes = (kTops + 64) * sizeof(float);  // and the factor back
+
 size_t forward_bytes(const TridentGated* t) {
     if (t->M <= kFewRows) return 0;
     const int64_t es = size_of(t->dtype);
@@ -715,7 +790,8 @@ size_t backward_part(const TridentGated* t) {
 size_t backward_bytes(const TridentGated* t) {
     const int64_t es = size_of(t->dtype);
     return packed_bytes(t->x, t->ld_x, t->M, t->K, es) + packed_bytes(t->gate_weight, t->ld_gate, t->N, t->K, es) +
-           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + 2 * bytes_of(t->M, pitch_of(t->N, es), es) + backward_part(t);
+           packed_bytes(t->up_weight, t->ld_up, t->N, t->K, es) + 2 * bytes_of(t->M, pitch_of(t->N, es), es) + backward_part(t) +
+           (t->dtype == TRIDENT_F16 ? kTopsBytes : 0);
 }
 
 int check(const TridentGated* t, bool backward) {
@@ -770,7 +846,15 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
     const int64_t pitch = pitch_of(t->N, sizeof(T));
     float* part = static_cast<float*>(s.take(backward_part(t)));
     SlopeArgs d{t->grad, t->gate, t->up, s.take(bytes_of(t->M, pitch, sizeof(T))), s.take(bytes_of(t->M, pitch, sizeof(T))),
-                t->ld_grad, t->N, pitch, t->M, (int)t->N, t->activation};
+                t->ld_grad, t->N, pitch, t->M, (int)t->N, t->activation, nullptr, nullptr, 0};
+    if constexpr (kScaled<T>) {
+        d.tops = static_cast<float*>(s.take(kTopsBytes));
+        d.back = d.tops + kTops;
+        d.groups = (int)std::min<int64_t>(kTops, (t->M * ((t->N + 7) / 8) + kBlock - 1) / kBlock);
+        largest_slope_kernel<T><<<(unsigned)d.groups, kBlock, 0, st>>>(d);
+        const int rc = capi_check_launch("largest_slope_kernel");
+        if (rc != TRIDENT_OK) return rc;
+    }
     slope_kernel<T><<<(unsigned)((t->M * (pitch / 8) + kBlock - 1) / kBlock), kBlock, 0, st>>>(d);
     int rc = capi_check_launch("slope_kernel");
     const Operand dg{static_cast<const uint8_t*>(d.dgate), pitch * (int64_t)sizeof(T)},
@@ -796,6 +880,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->N;
         a.parts = 2;
+        a.back = d.back;
         rc = product_of<T, kColumnsRows>(a, 1, part, st);
     }
     if (rc == TRIDENT_OK && t->dgate_weight) {
@@ -810,6 +895,7 @@ int backward(const TridentGated* t, Scratch s, hipStream_t st) {
         a.N = (int)t->K;
         a.K = (int)t->M;
         a.parts = 1;
+        a.back = d.back;
         rc = product_of<T, kColumnsColumns>(a, 2, part, st);
     }
     return rc;

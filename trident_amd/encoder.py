@@ -1020,7 +1020,8 @@ def gated_linear_forward(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tens
 def gated_linear_grad(grad: torch.Tensor, x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor,
                       gate: torch.Tensor, up: torch.Tensor, activation: str = "silu"):
     """(dx, dw_gate, dw_up) from the gradient of h and what ``gated_linear_forward`` took and gave.  The
-    gradients of the two products are rounded to x's type before they are multiplied."""
+    gradients of the two products are rounded to x's type before they are multiplied, in float16 times a power of two that
+    the largest of them calls for."""
     return _gated_grad(grad, x, w_gate, w_up, gate, up, activation, True, True)
 
 
