@@ -1,11 +1,12 @@
-"""Calls of the transformer layer's entry points that have no right answer are refused, and those that have one are not
-(CPU only: nothing is launched)."""
+"""Calls of the transformer layer's entry points that have no right answer are refused, and those that have one are not; a
+kernel's registers (CPU only: nothing is launched)."""
 import ctypes
 
 import pytest
 import torch
 
 from trident_amd import _lib, encoder
+from test_build_guards import code_objects, kernel_resources, pytestmark  # noqa: F401
 from test_layer_abi import attention, gated, on_gpu, refused  # noqa: F401
 
 
@@ -37,3 +38,10 @@ def test_rows_far_apart_are_packed():
         assert L.trident_gated_linear_grad_workspace_bytes(ctypes.byref(a)) >= near + rows * 32 * 2
         assert L.trident_gated_linear_workspace_bytes(ctypes.byref(gated(M=16, **{name: far}))) == 0
         refused(L.trident_gated_linear(ctypes.byref(gated(**{name: 1 << 41})), 256, 1 << 40, None), 1, "bad sizes")
+
+
+def test_no_scratch_in_the_kernel_of_the_largest_slope(code_objects):  # noqa: F811
+    found = {k: r for k, r in kernel_resources(code_objects).items() if "20largest_slope_kernel" in k}
+    assert found
+    for k, r in found.items():
+        assert r["private_segment_fixed_size"] == 0 and r["vgpr_spill_count"] == 0, (k, r)
