@@ -390,8 +390,8 @@ int trident_rotary(const void* x, int32_t dtype, int64_t tokens, int64_t heads, 
  * ids64 is not 0; values outside the rows are brought inside.  q [rows, q_heads, head_dim], k and v [rows,
  * kv_heads, head_dim]: strides in elements, of 16-byte pieces, a row's at least head_dim; query head h takes key and value head
  * h / (q_heads / kv_heads).  out, grad, dq, dk and dv are contiguous.  Every tensor 16-byte aligned.  head_dim: a multiple of
- * 8 up to 128.  lse [q_heads, rows]: the base-2 logarithm of the rows' sums of exp, for the
- * backward pass, or NULL. */
+ * 8 up to 128.  scale: at least 2^-149 (float32 holds it) and below 1e30.  lse [q_heads, rows]: the base-2
+ * logarithm of the rows' sums of exp, for the backward pass, or NULL. */
 typedef struct TridentAttention {
     const void *q, *k, *v;
     void* out;

@@ -7,12 +7,13 @@
 // and values go straight from memory to LDS, the next one while this one is multiplied, and each row keeps a
 // running reference value and sum.
 //
-// Bound by the matrix unit and, with heads of 64, by the vector unit as much: a tile of 32 x 32 scores of such
-// a head is 16 matrix instructions of 8 passes and about as many cycles of exponentials, maxima and roundings,
-// and the waves of a SIMD take turns at both.  Measured: causal, 32 heads of 128 over 8, bfloat16, four
-// sequences of up to 16,384 tokens (5.2 TFLOP) 5.0 ms, 1.04 PFLOP/s; 12 heads of 64, bfloat16, 512 passages
-// padded to 256 tokens 180 us (its bytes take 115); 12 heads of 64 over 4, float16, 64 sequences of up to 2,048
-// tokens 390 us; one query of 16 tokens 3.8 us, a launch and three loads one after another.  A causal kernel is
+// Bound by the vector unit with heads of 64, by both it and the matrix unit with wider ones: 32 x 32 scores of
+// a head of 64 are 8 matrix instructions, 256 cycles, and about 475 of exponentials, multiply-adds, maxima, sums and
+// roundings, and the waves of a SIMD take turns at both.  Measured: causal, 32 heads of 128 over 8, bfloat16,
+// four sequences of up to 16,384 tokens (5.2 TFLOP) 4.8 ms, 1.09 PFLOP/s; 12 heads of 64, bfloat16, 512 passages
+// padded to 256 tokens 177 us (its bytes take 115); 12 heads of 64 over 4, float16, 64 sequences of up to 2,048
+// tokens 371 us; one query of 16 tokens 3.8 us, a launch and three loads one after another (cards differ by up
+// to 7 %).  A causal kernel is
 // apart from the full one: without the diagonal the full one is small enough for four waves of a SIMD in place
 // of three (217 us with it, 185 without).
 #include "attention.hpp"
@@ -30,8 +31,8 @@ constexpr float kShift = std::is_same<T, f16_t>::value ? 7.0f : 0.0f;
 constexpr float kSlack = 8.0f;
 
 // Waves of a workgroup, 32 queries each.  Short sequences leave some without a row, and still four load their
-// keys sooner: 12 heads of 64, bfloat16, one sequence of 16 tokens 3.8 us (one wave 4.5), 1,000 of them 44
-// (50).
+// keys sooner: 12 heads of 64, bfloat16, one sequence of 16 tokens 3.8 us (one wave 4.4), 1,000 of them 44
+// (49).
 constexpr int kWaves = 4;
 
 template <typename T, int DP, bool CAUSAL>

@@ -8,9 +8,10 @@
 // seven products (eight in 16 bits, kMendDelta below) where five are the least, but no sum crosses workgroups.
 //
 // Bound as the forward pass is, by matrix and vector unit in turns, and by what is held: q, do and dq (or k, v,
-// dk and dv) leave one to three waves a SIMD.  Measured: 12 heads of 64 over 4, float16, 64 sequences of up to
-// 2,048 tokens: dq 600 us, dk and dv 865; 6 heads of 80 over 2, causal, float32, 17 sequences of up to 777
-// tokens: 185 and 266 us, and 9 for the join.
+// dk and dv) leave one to four waves a SIMD.  Measured: 12 heads of 64 over 4, float16, 64 sequences of up to
+// 2,048 tokens: dq 708 us, dk and dv 851; 6 heads of 80 over 2, causal, float32, 17 sequences of up to 777
+// tokens: 179 and 266 us, and 9 for the join; 32 heads of 128 over 8, causal, bfloat16, four sequences of up to 16,384: 23.4
+// ms in all, 890 TFLOP/s of the eight products (the five that are the least would take 9.3 ms at the rate of a large one).
 #include "attention.hpp"
 
 namespace trident {
@@ -24,11 +25,12 @@ constexpr bool kFollow = std::is_same<T, f16_t>::value;
 // delta made of an out of 16 bits is off by out's rounding, which can be as large as dP - delta is (values that
 // share a part).  But the rows of P sum to one, so those of dS, made with a delta that is off by e, sum to -e
 // instead of zero: the dq kernel adds them up in float32, takes their sum times that of P k from dq, and keeps the
-// mended delta for dk and dv.  Error of dq in 1e-3, rms, bfloat16, without and with: 2.40 and 2.37 of 2,000
-// rows with flat scores, 3.1 and 2.4 of 4 rows, 4.6 and 2.4 of scores six times as large, 14.4 and 2.4 of values that
-// share 4; dk alike.  It costs a product more, of keys that are in registers already, and its accumulators: of the whole
-// backward pass 7 to 10 % at heads of 64 (sequences of up to 2,048), 2 % at short ones, 23 % at heads of 128, where one wave
-// of a SIMD is left of two.  float32 does without: there out's rounding is no more than the sums' own.
+// mended delta for dk and dv.  Error of dq in 1e-3, rms, bfloat16, without and with (dk alike): 2.40 and 2.37 of
+// 2,000 rows with flat scores, 3.1 and 2.4 of 4 rows, 4.6 and 2.4 of scores six times as large, 14.4 and 2.4 of 500
+// rows whose values share 4, 73 and 2.4 of 20,000.  It costs a product more, of keys that are in registers
+// already, and its accumulators: of the whole backward pass 8 to 11 % at heads of 64 (sequences of up to 2,048), 1
+// to 4 % at short ones, 18 to 23 % at heads of 128, where one wave of a SIMD is left of two.  float32 does without:
+// there out's rounding is no more than the sums' own.
 template <typename T>
 constexpr bool kMendDelta = sizeof(T) == 2;
 // P <= 1 (up to the rounding of lse) in float16 times 2^15: held in full down to 2^-29.
@@ -432,7 +434,7 @@ size_t delta_bytes(const TridentAttention* t) { return ((size_t)t->rows * t->q_h
 
 // Shares of the queries that a tile of keys is cut into, each to a workgroup of its own, where the tiles alone
 // leave CUs idle: then the longest sequence's tile is what the others wait for (17 sequences of up to 777, 2
-// key heads, float32, three shares: 671 us, with the join 278).
+// key heads, float32: the whole backward pass 847 us, with three shares and the join 456).
 int shares_of(const TridentAttention* t) {
     const int64_t sequences = std::max<int64_t>(t->sequences, 1), length = t->rows / sequences;
     const int64_t tiles = std::max<int64_t>((t->rows + 127) / 128, sequences) * t->kv_heads;
@@ -472,8 +474,8 @@ int launch(AttentionArgs a, hipStream_t st) {
     return capi_check_launch("attention_join_kernel");
 }
 
-// Two waves where sequences are short (1,000 of 16 tokens, 12 heads of 64, bfloat16: 121 us, 166 by four; of
-// 50: 265 and 302).
+// Two waves where sequences are short (1,000 of 16 tokens, 12 heads of 64, bfloat16: 124 us, 172 by four; of
+// 50: 268 and 309).
 template <typename T, int DP, bool CAUSAL>
 int by_length(const AttentionArgs& a, hipStream_t st) {
     const int64_t mean = a.slots ? a.slots : a.rows / std::max<int64_t>(a.count, 1);

@@ -10,9 +10,11 @@
 // rounding for their products does, and as much again to the gradients (bfloat16: 3.1e-3 rms with them rounded,
 // 2.4e-3 without, of which the results' own rounding is 1.7e-3).
 //
-// Many rows are bound by the matrix unit and by LDS, that feeds it: 16,384 x 1,024 by 2 x 4,096, bfloat16, 298
-// us (922 TFLOP/s; 275 GFLOP at the rate of a large square product take 196, a library's product alone of this
-// shape 272), its gradients 250 us of dx and 300 of both weights'.  Few rows are bound by the weights' bytes.
+// Many rows are bound by the matrix unit and by LDS, that feeds it, and by the start and end of a tile, which
+// nothing covers where a CU holds one: 16,384 x 1,024 by 2 x 4,096, bfloat16, 298 to 309 us on three cards (890 to
+// 922 TFLOP/s; 275 GFLOP at the rate of a large square product take 196, a library's product alone of this shape
+// 272), 340 to 360 where gate and up are kept; its gradients 240 us of dx and 280 of both weights'.  Few rows are
+// bound by the weights' bytes.
 #include <algorithm>
 
 #include "mfma.hpp"
@@ -558,7 +560,7 @@ __global__ __launch_bounds__(kBlock) void largest_slope_kernel(SlopeArgs a) {
     if (threadIdx.x == 0) a.tops[blockIdx.x] = top;
 }
 
-// dg and du.  Bound by bytes: three reads, two writes (16,384 x 4,096 bfloat16, 940 MB, 200 us, 4.7 TB/s).
+// dg and du.  Bound by bytes: three reads, two writes (16,384 x 4,096 bfloat16, 940 MB, 206 us, 4.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void slope_kernel(SlopeArgs a) {
     float by = 1.0f;

@@ -7,7 +7,7 @@
 // rest is copied.  The inverse turns back, with the same factor a: the gradient.
 //
 // Bound by bytes: one read and one write (131,072 tokens of 24 heads of 64, bfloat16, 157 us, 5.1 TB/s; 16,385
-// of 40 heads of 128, half of each turned, float32, 144 us, 4.7 TB/s).  A token's angles are the same for all
+// of 40 heads of 128, half of each turned, float32, 142 us, 4.7 TB/s).  A token's angles are the same for all
 // of its heads, so a workgroup first makes those of its tokens, in LDS: the turns in float64, since a position
 // of 1e6 leaves a float32 no digits of the angle, and sine and cosine of what is left of a whole turn in
 // float32.

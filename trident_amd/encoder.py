@@ -761,8 +761,9 @@ def rotary(x: torch.Tensor, frequencies: torch.Tensor, positions: Optional[torch
     Pair i is columns i and i + pairs, or 2 i and 2 i + 1 (``interleaved``).  ``positions`` (int32 or int64,
     any value) are the tokens', [...], or those of the last token dimension, shared by the others; without
     them a token's position is its index there.  Angles are made in float64.  Queries and keys that lie in one
-    tensor are one call: ``rotary(qkv[:, :q_heads + k_heads], ...)``.  ``inverse`` turns back, by the same
-    amplitude: it is the gradient.  ``out`` may be ``x`` (in place) or not overlap it, and has no gradient."""
+    tensor are one call: ``rotary(qkv[:, :q_heads + k_heads], ...)``; an ``x`` whose tokens are not one stride apart is
+    copied.  ``inverse`` turns back, by the same amplitude: it is the gradient.  ``out`` may be ``x`` (in place) or not
+    overlap it, and has no gradient."""
     if _forward_ad._current_level >= 0:
         _no_tangents("rotary", x, frequencies)
     if frequencies.requires_grad and torch.is_grad_enabled():
@@ -883,12 +884,16 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: Option
     [sequences, slots, heads, head_dim], sequence i being the first ``lengths[i]`` of its slots (without lengths all).
     Offsets and lengths are int32 or int64 on the device, so no call can check them; values outside the rows are
     brought inside.  Rows without a token, and sequences of no tokens, are allowed: what they hold is never used, and they
-    get zeros.  Within a sequence a value that is not finite shows wherever the formula has it, in causal attention not before its own token.
+    get zeros.  Within a sequence a value that is not finite shows wherever the formula has it, in causal attention not
+    before its own token.
 
     head_dim is a multiple of 8 up to 128; q_heads a multiple of kv_heads (query head h takes key head h //
-    (q_heads // kv_heads)).  ``scale`` is 1 / sqrt(head_dim) if not given.  Strided views, such as parts of one projection's
-    result, are taken as they are where their strides are whole pieces of 16 bytes.  Scores, softmax and sums are
-    float32; probabilities are rounded to the tensors' type for the product with v."""
+    (q_heads // kv_heads)).  ``scale``, at least 2^-149, is 1 / sqrt(head_dim) if not given.  Strided views, such as parts of
+    one projection's result, are taken as they are where their strides are whole pieces of 16 bytes and one stride leads from
+    each token to the next, over the sequences too; others are copied by every call (several padded sequences with their heads
+    before their slots, ``[sequences, heads, slots, head_dim]`` transposed, are such).  Scores, softmax and sums are
+    float32; probabilities are rounded to the tensors' type for the product with v, and in the backward pass they and
+    the gradients of the scores for the products with them."""
     if _forward_ad._current_level >= 0:
         _no_tangents("attention", q, k, v)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
@@ -910,7 +915,9 @@ def attention_grad(grad: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torc
                    lse: torch.Tensor, offsets: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                    causal: bool = False, scale: Optional[float] = None):
     """(dq, dk, dv) from the gradient of ``out``, what ``attention_forward`` took and what it gave.  Those of k
-    and v are sums over the query heads of their group."""
+    and v are sums over the query heads of their group.  The scores' gradients are made in float32, rid of the error
+    that out's rounding would bring them, and rounded to the tensors' type (in float16 times a power of two) for the
+    products with q and k."""
     if _forward_ad._current_level >= 0:
         _no_tangents("attention_grad", grad, q, k, v, out, lse)
     a, kept, index = _attention_args(q, k, v, offsets, lengths, bool(causal), scale)
@@ -1000,8 +1007,9 @@ class _GatedLinear(torch.autograd.Function):
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
     """``act(x @ w_gate.T) * (x @ w_up.T)`` in one kernel: [..., N] in x's type from x [..., K] and weights [N, K] of
-    its type (rows of any pitch, such as the halves of one matrix).  ``activation``: "silu", "gelu", or "gelu_tanh"
-    (gelu by its tanh formula).  The sums, the activation and the product are float32."""
+    its type (rows of any pitch, such as the first token of every passage, or the halves of one matrix; N and K up to
+    2^21).  ``activation``: "silu", "gelu", or "gelu_tanh" (gelu by its tanh formula).  The sums, the activation and the
+    product are float32."""
     if _forward_ad._current_level >= 0:
         _no_tangents("gated_linear", x, w_gate, w_up)
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad):
